@@ -99,6 +99,23 @@ _SIGS = {
     "btvae_masked_scatter": [P, P, P, LL, P],
     "btvae_lse_over_k": [P, P, I, I, P],
     "btvae_pack_lower": [P, P, LL, I, P],
+    "btvae_block_pack": [P, I, LL, P, I, LL, LL, I, I, I, I, P],
+    "btvae_gated_proj_fwd": [P, LL, LL, P, P, LL, LL, P, P, I, P, LL, LL, P, LL, I, I, I, I, I, I, P],
+    "btvae_gated_proj_bwd": [P, LL, LL, P, LL, LL, P, LL, I, P, LL, LL, P, I, I, I, I, I, P],
+    "btvae_block_product": [P, LL, LL, P, LL, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],
+    "btvae_block_wgrad": [P, LL, LL, P, LL, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
+    "btvae_block_colsum": [P, I, LL, P, LL, P, I, I, I, I, P],
+    "btvae_block_strip_sums": [P, I, I, P, P, I, I, P],
+    "btvae_few_rows": [P, LL, P, P, LL, P, P, P, LL, I, I, I, I, I, P],
+    "btvae_fp8_quantize": [P, I, LL, P, LL, P, LL, I, I, P],
+    "btvae_fp8_quantize_blocks": [P, I, LL, P, LL, P, LL, I, I, P],
+    "btvae_fp8_dequantize": [P, LL, P, LL, I, P, I, I, P],
+    "btvae_fp8_expand": [P, LL, P, LL, I, P, LL, I, I, P],
+    "btvae_fp8_product": [P, LL, P, LL, P, LL, P, LL, P, P, LL, I, P, LL, I, I, I, P],
+    "btvae_fp8_gated_proj": [P, LL, P, LL, P, P, P, P, LL, LL, I, P, P, P, LL, P, LL, I, I, I, I, P],
+    "btvae_fp8_few_rows": [P, I, LL, P, P, P, P, LL, LL, P, P, P, LL, I, I, I, I, I, P],
+    "btvae_norm_gate_residual_fwd": [P, P, P, I, F, P, P, P, P, P, I, I, F, P, P, P, I, I, I, P],
+    "btvae_norm_gate_residual_bwd": [P, P, P, P, P, I, F, P, P, P, P, I, I, P, P, P, P, P, P, P, P, P, P, LL, I, I, I, P],
 }
 _RET = {
     "btvae_get_gemm_precision": (c_int, []),
@@ -119,6 +136,14 @@ _RET = {
     "btvae_guard_range_log2": (c_int, [I]),
     "btvae_guard_flags": (ctypes.POINTER(c_int), []),
     "btvae_next_row_pitches": (c_int, [I, I]),
+    "btvae_gated_proj_strips": (c_int, [I, I]),
+    "btvae_block_product_ws": (c_longlong, [I, I, I, I]),
+    "btvae_block_wgrad_ws": (c_longlong, [I, I, I, I]),
+    "btvae_block_colsum_ws": (c_longlong, [I, I]),
+    "btvae_few_rows_max": (c_int, []),
+    "btvae_fp8_product_ws": (c_longlong, [I, I, I]),
+    "btvae_norm_max_columns": (c_int, []),
+    "btvae_norm_gate_residual_ws": (c_longlong, [I, I, I]),
 }
 EXPORTS = sorted(list(_SIGS) + list(_RET))
 PROF_KINDS = ["gemm_fwd", "gemm_dgrad", "gemm_wgrad", "gemm_mvn", "bn", "mvn_rows", "reduce", "optim"]

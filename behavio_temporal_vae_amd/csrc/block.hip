@@ -1,0 +1,817 @@
+// Gated residual block: packing of operands, launches of the products in block_gemm.h, the forms for few rows, 8-bit
+// quantisation and the column sums.
+//
+//   a = x Wg^T + bg,  b = x Wu^T + bu,  h = act(a) b,  y = h Wd^T + bd
+//   dh = dy Wd,  da = dh b act'(a),  db = dh act(a),  dx = [da db] [Wg; Wu],  d[Wg; Wu] = [da db]^T x,  dWd = dy^T h
+#include "block_gemm.h"
+#include <algorithm>
+
+using namespace btvae;
+namespace bk = btvae_block;
+
+namespace btvae_block {
+
+// ---- operands -> bf16 planes ------------------------------------------------------------------------------------------
+// dst[plane][r][c] = piece of src[r][c], zeros for cols <= c < dst_cols; eight columns to a thread.
+template <bool SRC16, int NP>
+__global__ __launch_bounds__(256) void pack_rows(const void* __restrict__ src, long long ld, unsigned short* __restrict__ dst, long long plane, long long dld,
+                                                 int rows, int cols, int groups) {
+    const long long total = (long long)rows * groups;
+    for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < total; g += (long long)gridDim.x * 256) {
+        const long long r = g / groups;
+        const int c = (int)(g - r * groups) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = c + e < cols ? (SRC16 ? bf_load(src, r * ld + c + e) : reinterpret_cast<const float*>(src)[r * ld + c + e]) : 0.f;
+        store_planes8(dst, plane, NP, r * dld + c, v);
+    }
+}
+
+// dst[plane][c][r] = piece of src[r][c] for c < cols, zeros for rows <= r < dst_cols: 64 x 64 tiles through LDS.
+template <bool SRC16, int NP>
+__global__ __launch_bounds__(256) void pack_transposed(const void* __restrict__ src, long long ld, unsigned short* __restrict__ dst, long long plane, long long dld,
+                                                       int rows, int cols, int dst_cols) {
+    __shared__ float t[64][65];
+    const int r0 = (int)blockIdx.x * 64, c0 = (int)blockIdx.y * 64;
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = r0 + (i >> 6), c = c0 + (i & 63);
+        t[i >> 6][i & 63] = r < rows && c < cols ? (SRC16 ? bf_load(src, (long long)r * ld + c) : reinterpret_cast<const float*>(src)[(long long)r * ld + c]) : 0.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int c = i >> 3, rg = (i & 7) * 8;
+        if (c0 + c >= cols || r0 + rg >= dst_cols) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = t[rg + e][c];
+        store_planes8(dst, plane, NP, (long long)(c0 + c) * dld + r0 + rg, v);
+    }
+}
+
+// ---- partial results ------------------------------------------------------------------------------------------------
+// out(m, n) (+)= sum_z slab[z][m][n] (+ bias[n]), in the order of z.  Rows [0, rows0) go to out0, [off1, off1 + rows1) to out1.
+__global__ __launch_bounds__(256) void reduce_slabs(const float* __restrict__ slab, int nz, int M, int N, void* out0, long long ld, int rows0, void* out1, int off1, int rows1,
+                                                    const void* bias, int bias_bf16, int out_bf16, int accumulate) {
+    const long long total = (long long)M * N;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int m = (int)(i / N), n = (int)(i - (long long)m * N);
+        void* out = out0;
+        int row = m;
+        if (m >= rows0) {
+            row = m - off1;
+            if (!out1 || row < 0 || row >= rows1) continue;
+            out = out1;
+        }
+        float v = 0.f;
+        for (int z = 0; z < nz; ++z) v += slab[(long long)z * total + i];
+        if (bias) v += bias_bf16 ? bf_load(bias, n) : reinterpret_cast<const float*>(bias)[n];
+        const long long o = (long long)row * ld + n;
+        if (out_bf16) {
+            unsigned short* d = reinterpret_cast<unsigned short*>(out);
+            d[o] = bf_bits(accumulate ? bf_load(d, o) + v : v);
+        } else {
+            float* d = reinterpret_cast<float*>(out);
+            d[o] = accumulate ? d[o] + v : v;
+        }
+    }
+}
+
+// part[chunk][n] = sum of src[r][n] over the chunk's rows: 64 columns x 4 row lanes to a workgroup
+template <bool SRC16>
+__global__ __launch_bounds__(256) void colsum_chunks(const void* __restrict__ src, long long ld, float* __restrict__ part, int rows, int N, int chunk) {
+    __shared__ float red[4][64];
+    const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
+    const int r0 = (int)blockIdx.y * chunk, r1 = min(rows, r0 + chunk);
+    float s = 0.f;
+    if (c < N) {
+#pragma unroll 8
+        for (int r = r0 + rl; r < r1; r += 4) s += SRC16 ? bf_load(src, (long long)r * ld + c) : reinterpret_cast<const float*>(src)[(long long)r * ld + c];
+    }
+    red[rl][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (rl == 0 && c < N) part[(long long)blockIdx.y * N + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// out0 / out1 [n] (+)= sum over strips of part[strip][0 / 1][n] (halves = 1: part[strip][n], out0 only): 32 columns x 8 strip lanes
+__global__ __launch_bounds__(256) void strip_sums(const float* __restrict__ part, int strips, int N, int halves, void* out0, void* out1, int out_bf16, int accumulate) {
+    __shared__ float red[8][33];
+    const int cols = N * halves;
+    const int c = (int)blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+    float s = 0.f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int r = sl; r < strips; r += 8) s += part[(long long)r * cols + c];
+    }
+    red[sl][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (sl != 0 || c >= cols) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x & 31];
+    void* out = c < N ? out0 : out1;
+    const int o = c < N ? c : c - N;
+    if (!out) return;
+    if (out_bf16) {
+        unsigned short* d = reinterpret_cast<unsigned short*>(out);
+        d[o] = bf_bits(accumulate ? bf_load(d, o) + s : s);
+    } else {
+        float* d = reinterpret_cast<float*>(out);
+        d[o] = accumulate ? d[o] + s : s;
+    }
+}
+
+// ---- 8-bit quantisation -----------------------------------------------------------------------------------------------
+// Rows: one power-of-two scale for each row and 128 columns; 16 lanes x 8 values to a block.  Scaling by a power of two is
+// exact, so the only rounding is the one to e4m3.  A non-finite value becomes NaN and takes no part in its block's maximum.
+template <bool SRC16, bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows(const void* __restrict__ src, long long ld, unsigned char* __restrict__ q, long long ldq,
+                                                     unsigned char* __restrict__ sc, long long scp, int rows, int K, int kb_n) {
+    const long long total = (long long)rows * kb_n;
+    for (long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4; g < total; g += (long long)gridDim.x * 16) {
+        const long long r = g / kb_n;
+        const int kb = (int)(g - r * kb_n), k = kb * 128 + (threadIdx.x & 15) * 8;
+        float v[8];
+        if (VEC) {
+            if (k < K) {
+                if (SRC16) {
+                    const u32x4 u = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(src) + r * ld + k);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[2 * e] = bf_lo(u[e]); v[2 * e + 1] = bf_hi(u[e]); }
+                } else {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + r * ld + k);
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + r * ld + k + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? (SRC16 ? bf_load(src, r * ld + k + e) : reinterpret_cast<const float*>(src)[r * ld + k + e]) : 0.f;
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, finite_abs(v[e]));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 16));
+        const int ex = scale_exp(mx);
+        const float s = pow2i(-ex);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = nan_if_not_finite(v[e]) * s;
+        *reinterpret_cast<u32x2*>(q + r * ldq + k) = u32x2{pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7])};
+        if ((threadIdx.x & 15) == 0) sc[r * scp + kb] = (unsigned char)(ex + 127);
+    }
+}
+
+// Weights: one scale for each 128 x 128 block, one workgroup to a block
+template <bool SRC16>
+__global__ __launch_bounds__(256) void quantize_blocks(const void* __restrict__ src, long long ld, unsigned char* __restrict__ q, long long ldq,
+                                                       unsigned char* __restrict__ sc, long long scp, int N, int K) {
+    __shared__ float red[4];
+    const int n0 = (int)blockIdx.y * 128, k = (int)blockIdx.x * 128 + (threadIdx.x & 15) * 8;
+    auto load = [&](int n, float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = n < N && k + e < K ? (SRC16 ? bf_load(src, (long long)n * ld + k + e) : reinterpret_cast<const float*>(src)[(long long)n * ld + k + e]) : 0.f;
+    };
+    float mx = 0.f, v[8];
+    for (int i = threadIdx.x >> 4; i < 128; i += 16) {
+        load(n0 + i, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, finite_abs(v[e]));
+    }
+    mx = wave_max(mx);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    const int ex = scale_exp(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const float s = pow2i(-ex);
+    for (int i = threadIdx.x >> 4; i < 128 && n0 + i < N; i += 16) {
+        load(n0 + i, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = nan_if_not_finite(v[e]) * s;
+        *reinterpret_cast<u32x2*>(q + (long long)(n0 + i) * ldq + k) = u32x2{pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7])};
+    }
+    if (threadIdx.x == 0) sc[(long long)blockIdx.y * scp + blockIdx.x] = (unsigned char)(ex + 127);
+}
+
+// values of quantised rows or blocks, as fp32
+__global__ __launch_bounds__(256) void dequantize(const unsigned char* __restrict__ q, long long ldq, const unsigned char* __restrict__ sc, long long scp, int row_shift,
+                                                  float* __restrict__ out, int rows, int K) {
+    const long long total = (long long)rows * K;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / K;
+        const int k = (int)(i - r * K);
+        const float v = __builtin_amdgcn_cvt_f32_fp8((int)q[r * ldq + k], 0);
+        out[i] = v * pow2i((int)sc[(r >> row_shift) * scp + (k >> 7)] - 127);
+    }
+}
+
+// the same as bf16, which holds every e4m3 value times a power of two (down to 2^-126): 8 columns to a thread, whole blocks
+__global__ __launch_bounds__(256) void expand_rows(const unsigned char* __restrict__ q, long long ldq, const unsigned char* __restrict__ sc, long long scp, int row_shift,
+                                                   unsigned short* __restrict__ out, long long ldo, int rows, int groups) {
+    const long long total = (long long)rows * groups;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / groups;
+        const int k = (int)(i - r * groups) * 8;
+        const u32x2 b = *reinterpret_cast<const u32x2*>(q + r * ldq + k);
+        const float s = pow2i((int)sc[(r >> row_shift) * scp + (k >> 7)] - 127);
+        u32x4 o;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)b[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)b[h], true);
+            o[2 * h] = pack2(lo[0] * s, lo[1] * s);
+            o[2 * h + 1] = pack2(hi[0] * s, hi[1] * s);
+        }
+        *reinterpret_cast<u32x4*>(out + r * ldo + k) = o;
+    }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+// Up to 32 rows: the weights are read once, straight into the matrix instruction's registers, and the time is theirs.  A
+// workgroup takes 16 weight rows (GATED: 8 gate and the 8 up rows of the same columns), its eight waves share the
+// reduction in interleaved pieces and add up through LDS.  The weight rows are the MFMA's first operand, x its second.
+//   fp32: v_mfma_f32_16x16x4_f32, exact products; bf16: v_mfma_f32_16x16x32_bf16; e4m3: x quantised on the way in (every
+//   workgroup repeats it: 32 values to a lane, the block's maximum over four lanes), both operands expanded to bf16, which
+//   holds every e4m3 value, and multiplied as bf16: the weights' bytes are the time, and the sums are float32's.
+enum { W_F32 = 0, W_BF16 = 1, W_E4M3 = 2 };
+struct FewArgs {
+    const void* X; long long ldx; int x_bf16;
+    const char* B; const char* B2; long long ldb;             // byte pitch
+    const unsigned char* b_sc; const unsigned char* b2_sc; long long b_scp;
+    const void* bias; const void* bias2; int bias_bf16;
+    void* C; long long ldc; int c_bf16;
+    int M, N, K, act;
+};
+
+// 32 e4m3 bytes -> 4 x 8 bf16 of the same values
+__device__ __forceinline__ void expand32(const i32x8 q, bf16x8 (&o)[4]) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        u32x4 u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[2 * g + h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[2 * g + h], true);
+            u[2 * h] = pack2(lo[0], lo[1]);
+            u[2 * h + 1] = pack2(hi[0], hi[1]);
+        }
+        o[g] = __builtin_bit_cast(bf16x8, u);
+    }
+}
+
+template <int WT, bool GATED, int MT, bool VEC>
+__global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
+    constexpr int NWV = 8, COLS = GATED ? 8 : 16;
+    __shared__ float red[NWV][16][16 * MT + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int row = lane & 15, kq = lane >> 4;
+    const int n0 = (int)blockIdx.x * COLS;
+    const int n = min(n0 + (GATED ? (row & 7) : row), p.N - 1);
+    const bool up = GATED && row >= 8;
+    const char* w = (up ? p.B2 : p.B) + (long long)n * p.ldb;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const void* xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const long long o = (long long)min(t * 16 + row, p.M - 1) * p.ldx;
+        xr[t] = p.x_bf16 ? (const void*)(reinterpret_cast<const unsigned short*>(p.X) + o) : (const void*)(reinterpret_cast<const float*>(p.X) + o);
+    }
+
+    if constexpr (WT == W_BF16) {
+        constexpr int U = 4;
+        auto load = [&](const void* base, int k) -> u32x4 {
+            u32x4 v;
+            if constexpr (VEC) {
+                v = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(base) + min(k, p.K - 8));
+                if (k >= p.K) v = u32x4{0, 0, 0, 0};
+            } else {
+                const unsigned short* s = reinterpret_cast<const unsigned short*>(base);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k0 = k + 2 * e, k1 = k0 + 1;
+                    const unsigned lo = s[min(k0, p.K - 1)], hi = s[min(k1, p.K - 1)];
+                    v[e] = (k0 < p.K ? lo : 0u) | (k1 < p.K ? hi << 16 : 0u);
+                }
+            }
+            return v;
+        };
+        for (int kb = wid * 32; kb < p.K; kb += NWV * 32 * U) {
+            u32x4 a[U], b[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kb + u * NWV * 32 + kq * 8;
+                a[u] = load(w, k);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) b[u][t] = load(xr[t], k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u]), __builtin_bit_cast(bf16x8, b[u][t]), acc[t], 0, 0, 0);
+        }
+    } else if constexpr (WT == W_F32) {
+        constexpr int U = 8;
+        auto load = [&](const void* base, int k) -> f32x4 {
+            const float* s = reinterpret_cast<const float*>(base);
+            f32x4 v;
+            if constexpr (VEC) {
+                v = *reinterpret_cast<const f32x4*>(s + min(k, p.K - 4));
+                if (k >= p.K) v = f32x4{0.f, 0.f, 0.f, 0.f};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = s[min(k + e, p.K - 1)];
+                    v[e] = k + e < p.K ? x : 0.f;
+                }
+            }
+            return v;
+        };
+        for (int kb = wid * 16; kb < p.K; kb += NWV * 16 * U) {
+            f32x4 a[U], b[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kb + u * NWV * 16 + kq * 4;
+                a[u] = load(w, k);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) b[u][t] = load(xr[t], k);
+            }
+            // step e of a piece multiplies reduction elements e, 4 + e, 8 + e, 12 + e: any order will do as long as both operands agree
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][e], b[u][t][e], acc[t], 0, 0, 0);
+        }
+    } else {
+        const unsigned char* wsc = (GATED && kq >= 2 ? p.b2_sc : p.b_sc) + (long long)(min(n0, p.N - 1) >> 7) * p.b_scp;      // of this lane's results
+        const int kbn = (p.K + 127) >> 7;
+        for (int kb = wid; kb < kbn; kb += NWV) {
+            const i32x4 a0 = *reinterpret_cast<const i32x4*>(w + kb * 128 + kq * 32), a1 = *reinterpret_cast<const i32x4*>(w + kb * 128 + kq * 32 + 16);
+            const i32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+            const float sw = pow2i((int)wsc[kb] - 127);
+            bf16x8 wa[4];
+            expand32(a, wa);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float v[32];
+                const int k = kb * 128 + kq * 32;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if constexpr (VEC) {
+                        const int kk = min(k + g * 8, p.K - 8);
+                        const bool in = k + g * 8 < p.K;
+                        if (p.x_bf16) {
+                            const u32x4 u = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(xr[t]) + kk);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { v[g * 8 + 2 * e] = in ? bf_lo(u[e]) : 0.f; v[g * 8 + 2 * e + 1] = in ? bf_hi(u[e]) : 0.f; }
+                        } else {
+                            const f32x4 u0 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(xr[t]) + kk);
+                            const f32x4 u1 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(xr[t]) + kk + 4);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { v[g * 8 + e] = in ? u0[e] : 0.f; v[g * 8 + 4 + e] = in ? u1[e] : 0.f; }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int kk = min(k + g * 8 + e, p.K - 1);
+                            const float x = p.x_bf16 ? bf_load(xr[t], kk) : reinterpret_cast<const float*>(xr[t])[kk];
+                            v[g * 8 + e] = k + g * 8 + e < p.K ? x : 0.f;
+                        }
+                    }
+                }
+                float mx = 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, finite_abs(v[e]));
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const int ex = scale_exp(mx);
+                const float s = pow2i(-ex);
+                i32x8 b;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    b[e] = (int)pack_e4m3(nan_if_not_finite(v[4 * e]) * s, nan_if_not_finite(v[4 * e + 1]) * s, nan_if_not_finite(v[4 * e + 2]) * s, nan_if_not_finite(v[4 * e + 3]) * s);
+                bf16x8 xb[4];
+                expand32(b, xb);
+                f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < 4; ++g) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa[g], xb[g], d, 0, 0, 0);
+                // a lane's four results: x row lane & 15, the row it quantised; weight rows of one block (GATED: lanes 0-31 gate, 32-63 up)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] += (d[i] * pow2i(ex)) * sw;
+            }
+        }
+    }
+    // element i of a lane: weight row 4 (lane >> 4) + i, x row lane & 15
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[wid][4 * kq + i][t * 16 + row] = acc[t][i];
+    __syncthreads();
+    for (int i = tid; i < COLS * 16 * MT; i += 512) {
+        const int c = i % COLS, m = i / COLS, nn = n0 + c;
+        if (m >= p.M || nn >= p.N) continue;
+        float v = 0.f, u = 0.f;
+#pragma unroll
+        for (int q = 0; q < NWV; ++q) {
+            v += red[q][c][m];
+            if (GATED) u += red[q][c + 8][m];
+        }
+        if (p.bias) v += p.bias_bf16 ? bf_load(p.bias, nn) : reinterpret_cast<const float*>(p.bias)[nn];
+        if (GATED) {
+            if (p.bias2) u += p.bias_bf16 ? bf_load(p.bias2, nn) : reinterpret_cast<const float*>(p.bias2)[nn];
+            float a, d;
+            act_value<false>(p.act, v, a, d);
+            v = a * u;
+        }
+        const long long o = (long long)m * p.ldc + nn;
+        if (p.c_bf16) reinterpret_cast<unsigned short*>(p.C)[o] = bf_bits(v);
+        else reinterpret_cast<float*>(p.C)[o] = v;
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------
+constexpr int CHIP = 256;                                             // compute units
+
+inline int tiles(int n, int t) { return (n + t - 1) / t; }
+inline bool al16(const void* q) { return ((uintptr_t)q & 15) == 0; }
+
+// Splits of a reduction of `stages` stages over fewer tiles than compute units: as many as fill the chip about once, each at least
+// 12 stages long (the ring's fill and the slab's write and read cost about that much).
+inline int row_splits(int T, int stages, int unit) {
+    if (T >= CHIP * 3 / 4) return 1;
+    int z = std::min(CHIP / T, stages / std::max(12, unit));
+    return std::max(1, std::min(z, 32));
+}
+inline int use_big(int M, int N, int colspan) { return tiles(M, 256) * tiles(N, colspan) >= CHIP * 3 / 4; }
+
+template <int FMT, int EP>
+static int launch_rows(Args& p, int shape, int z, hipStream_t s, const char* what) {
+    // shape 0: 256 x 256, 1: 128 x 128, 2: 128 x 256
+    const int tm = shape == 0 ? 256 : 128, tn = (shape == 1 ? 128 : 256) / (EP == EP_GATED ? 2 : 1);
+    p.tiles_m = tiles(p.M, tm); p.tiles_n = tiles(p.N, tn);
+    const long long T = (long long)p.tiles_m * p.tiles_n;
+    if (T > 0x7fffffffLL) return set_error("%s: too many tiles", what);
+    const dim3 grid((unsigned)T, 1, (unsigned)z);
+    if (shape == 0) hipLaunchKernelGGL((gemm_rows<FMT, EP, 4, 2, 4>), grid, dim3(512), 0, s, p);
+    else if (shape == 1) {
+        if constexpr (!(FMT == FMT_E4M3 && EP == EP_GATED)) hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, 2, 2>), grid, dim3(256), 0, s, p);
+    } else {
+        if constexpr (EP == EP_GATED) hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, 2, 4>), grid, dim3(256), 0, s, p);
+    }
+    return check_launch(what);
+}
+
+struct ProductPlan { int shape, z, kz; };
+// EP_LINEAR: tile shape and splits; `unit`: a split is a multiple of that many stages; `max_stages`: longest split (e4m3: its scales' room)
+static ProductPlan plan_product(int M, int N, int stages, int unit, int max_stages) {
+    ProductPlan r;
+    r.shape = use_big(M, N, 256) ? 0 : 1;
+    const int T = r.shape == 0 ? tiles(M, 256) * tiles(N, 256) : tiles(M, 128) * tiles(N, 128);
+    int z = std::max(row_splits(T, stages, unit), tiles(stages, max_stages));
+    r.kz = tiles(tiles(stages, z), unit) * unit;
+    r.z = tiles(stages, r.kz);
+    return r;
+}
+struct ColPlan { int big, z, rz; };
+static ColPlan plan_cols(int M, int N, int R, int planes) {
+    ColPlan r;
+    r.big = tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
+    const int t = r.big ? 256 : 128;
+    const int T = tiles(M, t) * tiles(N, t);
+    // fill the chip; a split has at least 256 rows, and multiples of eight splits keep one row range on one XCD
+    int z = std::max(1, std::min((T >= CHIP ? 1 : CHIP / T), tiles(R, 256)));
+    if (z > 8) z = z / 8 * 8;
+    const int cap = 1 << 20;                                          // rows of a split
+    z = std::max(z, tiles(R, cap));
+    r.rz = tiles(tiles(std::max(R, 1), z), 32) * 32;
+    r.z = std::max(1, tiles(R, r.rz));
+    return r;
+}
+
+}  // namespace btvae_block
+
+#define BLK_STREAM(s) reinterpret_cast<hipStream_t>(s)
+
+static bool operand_ok(const void* p, long long ld, long long plane, int planes) {
+    return bk::al16(p) && (ld & 7) == 0 && (planes == 1 || (plane & 7) == 0);
+}
+
+// dst[plane][row][0 .. dst_cols) = bf16 pieces of src (planes 1: rounded; 3: exact), zero-padded; transpose: of src^T.
+BTVAE_API int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long plane, long long dst_ld, int rows, int cols, int dst_cols,
+                               int transpose, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_pack: planes must be 1 or 3");
+    BTVAE_REQUIRE(rows >= 0 && cols > 0 && ld >= cols, "block_pack: bad source shape");
+    BTVAE_REQUIRE((dst_cols & 7) == 0 && dst_cols >= (transpose ? rows : cols) && dst_ld >= dst_cols && operand_ok(dst, dst_ld, plane, planes), "block_pack: bad destination layout");
+    if (rows == 0 && !transpose) return 0;
+    hipStream_t s = BLK_STREAM(stream);
+    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+    if (!transpose) {
+        const int groups = dst_cols / 8;
+        const long long need = ((long long)rows * groups + 255) / 256;
+        const unsigned grid = (unsigned)std::min<long long>(need, 16384);
+        if (src_bf16) {
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<true, 1>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+            else hipLaunchKernelGGL((bk::pack_rows<true, 3>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+        } else {
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<false, 1>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+            else hipLaunchKernelGGL((bk::pack_rows<false, 3>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+        }
+    } else {
+        const unsigned gx = (unsigned)bk::tiles(dst_cols, 64), gy = (unsigned)bk::tiles(cols, 64);
+        BTVAE_REQUIRE(gy <= 65535, "block_pack: too many columns");
+        if (src_bf16) {
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<true, 1>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+            else hipLaunchKernelGGL((bk::pack_transposed<true, 3>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+        } else {
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<false, 1>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+            else hipLaunchKernelGGL((bk::pack_transposed<false, 3>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+        }
+    }
+    return check_launch("block_pack");
+}
+
+BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, long long x_plane, const void* Wg, const void* Wu, long long ldw, long long w_plane,
+                                   const void* bg, const void* bu, int bias_bf16, void* H, long long ldh, long long h_plane, void* GU, long long ldgu, int gu_half,
+                                   int planes, int act, int M, int F, int K, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_fwd: planes must be 1 or 3");
+    BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0 && (K & 7) == 0, "gated_proj_fwd: bad sizes (M %d, F %d, K %d)", M, F, K);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_fwd: unknown activation %d", act);
+    const int F8 = (F + 7) / 8 * 8;
+    BTVAE_REQUIRE(operand_ok(X, ldx, x_plane, planes) && ldx >= K && operand_ok(Wg, ldw, w_plane, planes) && operand_ok(Wu, ldw, w_plane, planes) && ldw >= K, "gated_proj_fwd: operand rows must start on 16 bytes");
+    BTVAE_REQUIRE(operand_ok(H, ldh, h_plane, planes) && ldh >= F8, "gated_proj_fwd: bad layout of H");
+    BTVAE_REQUIRE(!GU || (bk::al16(GU) && (ldgu & 7) == 0 && (gu_half & 7) == 0 && gu_half >= F8 && ldgu >= gu_half + F8), "gated_proj_fwd: bad layout of the kept projections");
+    if (M == 0) return 0;
+    bk::Args p = {};
+    p.A = (const char*)X; p.lda = ldx * 2; p.a_plane = x_plane * 2;
+    p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw * 2; p.b_plane = w_plane * 2;
+    p.M = M; p.N = F; p.K = K; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(K, 32); p.kz = p.pairs * p.ks;
+    p.bias = bg; p.bias2 = bu; p.bias_bf16 = bias_bf16;
+    p.C = H; p.ldc = ldh; p.c_plane = h_plane; p.c_type = planes == 3 ? bk::T_PLANES : bk::T_BF16;
+    p.act = act; p.gu = GU; p.ldgu = ldgu; p.gu_half = gu_half; p.gu_f32 = planes == 3;
+    ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
+    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, bk::use_big(M, F, 128) ? 0 : 1, 1, BLK_STREAM(stream), "gated_proj_fwd");
+}
+
+BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, long long dy_plane, const void* WdT, long long ldw, long long w_plane, const void* GU, long long ldgu, int gu_half,
+                                   void* dGU, long long ldd, long long d_plane, float* colpart, int planes, int act, int M, int F, int N, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_bwd: planes must be 1 or 3");
+    BTVAE_REQUIRE(M >= 0 && F > 0 && N > 0 && (N & 7) == 0, "gated_proj_bwd: bad sizes (M %d, F %d, N %d)", M, F, N);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_bwd: unknown activation %d", act);
+    const int F8 = (F + 7) / 8 * 8;
+    BTVAE_REQUIRE(operand_ok(dY, lddy, dy_plane, planes) && lddy >= N && operand_ok(WdT, ldw, w_plane, planes) && ldw >= N, "gated_proj_bwd: operand rows must start on 16 bytes");
+    BTVAE_REQUIRE(bk::al16(GU) && (ldgu & 7) == 0 && (gu_half & 7) == 0 && gu_half >= F8 && ldgu >= gu_half + F8, "gated_proj_bwd: bad layout of the kept projections");
+    BTVAE_REQUIRE(operand_ok(dGU, ldd, d_plane, planes) && ldd >= gu_half + F8, "gated_proj_bwd: bad layout of the gradients");
+    if (M == 0) return 0;
+    bk::Args p = {};
+    p.A = (const char*)dY; p.lda = lddy * 2; p.a_plane = dy_plane * 2;
+    p.B = (const char*)WdT; p.ldb = ldw * 2; p.b_plane = w_plane * 2;
+    p.M = M; p.N = F; p.K = N; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(N, 32); p.kz = p.pairs * p.ks;
+    p.C = dGU; p.ldc = ldd; p.c_plane = d_plane; p.c_type = planes == 3 ? bk::T_PLANES : bk::T_BF16;
+    p.act = act; p.gu = const_cast<void*>(GU); p.ldgu = ldgu; p.gu_half = gu_half; p.gu_f32 = planes == 3; p.colpart = colpart;
+    ProfScope prof(PK_GEMM_DGRAD, BLK_STREAM(stream), 2.0 * M * F * N, 0.0);
+    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED_BWD>(p, bk::use_big(M, F, 256) ? 0 : 1, 1, BLK_STREAM(stream), "gated_proj_bwd");
+}
+// Strips of 64 rows that btvae_gated_proj_bwd leaves column sums for: colpart holds [strips][2][F] floats.
+BTVAE_API int btvae_gated_proj_strips(int M, int F) { return bk::use_big(M, F, 256) ? bk::tiles(M, 256) * 4 : bk::tiles(M, 128) * 2; }
+
+BTVAE_API long long btvae_block_product_ws(int M, int N, int K, int planes) {
+    const bk::ProductPlan r = bk::plan_product(M, N, (planes == 3 ? 6 : 1) * bk::tiles(K, 32), 1, 1 << 30);
+    return r.z > 1 ? (long long)r.z * M * N : 0;
+}
+BTVAE_API int btvae_block_product(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, const void* bias, int bias_bf16,
+                                  void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int planes, int M, int N, int K, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_product: planes must be 1 or 3");
+    BTVAE_REQUIRE(M >= 0 && N > 0 && K > 0 && (K & 7) == 0 && ldc >= N, "block_product: bad sizes (M %d, N %d, K %d)", M, N, K);
+    BTVAE_REQUIRE(operand_ok(A, lda, a_plane, planes) && lda >= K && operand_ok(B, ldb, b_plane, planes) && ldb >= K, "block_product: operand rows must start on 16 bytes");
+    if (M == 0) return 0;
+    hipStream_t s = BLK_STREAM(stream);
+    bk::Args p = {};
+    p.A = (const char*)A; p.lda = lda * 2; p.a_plane = a_plane * 2;
+    p.B = (const char*)B; p.ldb = ldb * 2; p.b_plane = b_plane * 2;
+    p.M = M; p.N = N; p.K = K; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(K, 32);
+    const bk::ProductPlan r = bk::plan_product(M, N, p.pairs * p.ks, 1, 1 << 30);
+    BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "block_product: workspace too small");
+    p.kz = r.kz; p.slab = ws;
+    p.bias = bias; p.bias_bf16 = bias_bf16;
+    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32; p.c_vec = bk::al16(C) && (ldc & (c_bf16 ? 7 : 3)) == 0;
+    ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
+    if (int rc = bk::launch_rows<bk::FMT_BF16, bk::EP_LINEAR>(p, r.shape, r.z, s, "block_product")) return rc;
+    if (r.z == 1) return 0;
+    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0, bias, bias_bf16, c_bf16, 0);
+    return check_launch("block_product reduction");
+}
+
+BTVAE_API long long btvae_block_wgrad_ws(int M, int N, int R, int planes) {
+    const bk::ColPlan r = bk::plan_cols(M, N, R, planes);
+    return (long long)r.z * M * N;
+}
+// out(m, n) (+)= sum_r A[r][m] B[r][n], m < M (rows [0, rows0) -> out0, [off1, off1 + rows1) -> out1), n < N
+BTVAE_API int btvae_block_wgrad(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, float* ws, long long ws_floats,
+                                void* out0, int rows0, void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate, int planes, int M, int N, int R, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_wgrad: planes must be 1 or 3");
+    const int M8 = (M + 7) / 8 * 8, N8 = (N + 7) / 8 * 8;
+    BTVAE_REQUIRE(M > 0 && N > 0 && R >= 0 && rows0 > 0 && rows0 <= M && ldo >= N && out0, "block_wgrad: bad sizes (M %d, N %d, R %d)", M, N, R);
+    BTVAE_REQUIRE(!out1 || (off1 >= rows0 && off1 + rows1 <= M), "block_wgrad: bad row ranges");
+    BTVAE_REQUIRE(R == 0 || (operand_ok(A, lda, a_plane, planes) && lda >= M8 && operand_ok(B, ldb, b_plane, planes) && ldb >= N8), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of 8 columns");
+    hipStream_t s = BLK_STREAM(stream);
+    const bk::ColPlan r = bk::plan_cols(M, N, R, planes);
+    BTVAE_REQUIRE(ws && ws_floats >= (long long)r.z * M * N, "block_wgrad: workspace too small");
+    bk::ColArgs p = {};
+    p.A = (const char*)A; p.lda = lda * 2; p.a_plane = a_plane * 2; p.a_cols = M8;
+    p.B = (const char*)B; p.ldb = ldb * 2; p.b_plane = b_plane * 2; p.b_cols = N8;
+    p.R = R; p.M = M; p.N = N; p.pairs = planes == 3 ? 6 : 1; p.rz = r.rz; p.slab = ws;
+    const int t = r.big ? 256 : 128;
+    p.tiles_m = bk::tiles(M, t); p.tiles_n = bk::tiles(N, t);
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)r.z);
+    {
+        ProfScope prof(PK_GEMM_WGRAD, s, 2.0 * M * N * R, 0.0);
+        if (r.big) hipLaunchKernelGGL((bk::gemm_cols<4, 2, 4>), grid, dim3(512), 0, s, p);
+        else hipLaunchKernelGGL((bk::gemm_cols<2, 2, 2>), grid, dim3(256), 0, s, p);
+    }
+    if (int rc = check_launch("block_wgrad")) return rc;
+    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, out0, ldo, rows0, out1, off1, rows1,
+                       (const void*)nullptr, 0, out_bf16, accumulate);
+    return check_launch("block_wgrad reduction");
+}
+
+// out[n] (+)= sum_r src[r][n]; ws: btvae_block_colsum_ws floats
+static int colsum_chunk(int R) { return std::max(64, bk::tiles(R, 256)); }
+BTVAE_API long long btvae_block_colsum_ws(int R, int N) { return (long long)std::max(1, bk::tiles(R, colsum_chunk(R))) * N; }
+BTVAE_API int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, long long ws_floats, void* out, int out_bf16, int accumulate, int R, int N, void* stream) {
+    BTVAE_REQUIRE(R >= 0 && N > 0 && (R == 0 || ld >= N) && out, "block_colsum: bad sizes (R %d, N %d)", R, N);
+    BTVAE_REQUIRE(ws && ws_floats >= btvae_block_colsum_ws(R, N), "block_colsum: workspace too small");
+    hipStream_t s = BLK_STREAM(stream);
+    const int chunk = colsum_chunk(R), nc = bk::tiles(R, chunk);
+    if (nc > 0) {
+        const dim3 grid((unsigned)bk::tiles(N, 64), (unsigned)nc);
+        if (src_bf16) hipLaunchKernelGGL((bk::colsum_chunks<true>), grid, dim3(256), 0, s, src, ld, ws, R, N, chunk);
+        else hipLaunchKernelGGL((bk::colsum_chunks<false>), grid, dim3(256), 0, s, src, ld, ws, R, N, chunk);
+        if (int rc = check_launch("block_colsum")) return rc;
+    }
+    hipLaunchKernelGGL(bk::strip_sums, dim3((unsigned)bk::tiles(N, 32)), dim3(256), 0, s, (const float*)ws, nc, N, 1, out, (void*)nullptr, out_bf16, accumulate);
+    return check_launch("block_colsum");
+}
+// out0 / out1 [n] (+)= sum over strips of part[strip][0 / 1][n]
+BTVAE_API int btvae_block_strip_sums(const float* part, int strips, int N, void* out0, void* out1, int out_bf16, int accumulate, void* stream) {
+    BTVAE_REQUIRE(strips >= 0 && N > 0 && out0, "block_strip_sums: bad sizes");
+    hipLaunchKernelGGL(bk::strip_sums, dim3((unsigned)bk::tiles(2 * N, 32)), dim3(256), 0, BLK_STREAM(stream), part, strips, N, 2, out0, out1, out_bf16, accumulate);
+    return check_launch("block_strip_sums");
+}
+
+// ---- few rows ----
+BTVAE_API int btvae_few_rows_max(void) { return 32; }
+
+template <int WT, bool GATED>
+static int launch_few(const bk::FewArgs& p, bool vec, hipStream_t s, const char* what) {
+    const dim3 grid((unsigned)bk::tiles(p.N, GATED ? 8 : 16));
+    if (p.M <= 16) {
+        if (vec) hipLaunchKernelGGL((bk::gemm_few<WT, GATED, 1, true>), grid, dim3(512), 0, s, p);
+        else hipLaunchKernelGGL((bk::gemm_few<WT, GATED, 1, false>), grid, dim3(512), 0, s, p);
+    } else {
+        if (vec) hipLaunchKernelGGL((bk::gemm_few<WT, GATED, 2, true>), grid, dim3(512), 0, s, p);
+        else hipLaunchKernelGGL((bk::gemm_few<WT, GATED, 2, false>), grid, dim3(512), 0, s, p);
+    }
+    return check_launch(what);
+}
+// Products with up to btvae_few_rows_max() rows, all matrices fp32 or all bf16 (`bf16`): W2 null: C = X W^T + bias; else C = act(X W^T + bias) (X W2^T + bias2).
+BTVAE_API int btvae_few_rows(const void* X, long long ldx, const void* W, const void* W2, long long ldw, const void* bias, const void* bias2, void* C, long long ldc, int bf16, int act,
+                             int M, int N, int K, void* stream) {
+    BTVAE_REQUIRE(M >= 0 && M <= 32 && N > 0 && K > 0 && ldx >= K && ldw >= K && ldc >= N, "few_rows: bad sizes (M %d, N %d, K %d)", M, N, K);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "few_rows: unknown activation %d", act);
+    if (M == 0) return 0;
+    bk::FewArgs p = {};
+    const int sz = bf16 ? 2 : 4;
+    p.X = X; p.ldx = ldx; p.x_bf16 = bf16; p.B = (const char*)W; p.B2 = (const char*)W2; p.ldb = ldw * sz;
+    p.bias = bias; p.bias2 = bias2; p.bias_bf16 = bf16; p.C = C; p.ldc = ldc; p.c_bf16 = bf16; p.M = M; p.N = N; p.K = K; p.act = act;
+    const int g = 16 / sz;
+    const bool vec = bk::al16(X) && bk::al16(W) && (!W2 || bk::al16(W2)) && K % g == 0 && ldx % g == 0 && ldw % g == 0;
+    hipStream_t s = BLK_STREAM(stream);
+    ProfScope prof(PK_GEMM_FWD, s, (W2 ? 4.0 : 2.0) * M * N * K, 0.0);
+    if (bf16) return W2 ? launch_few<bk::W_BF16, true>(p, vec, s, "few_rows") : launch_few<bk::W_BF16, false>(p, vec, s, "few_rows");
+    return W2 ? launch_few<bk::W_F32, true>(p, vec, s, "few_rows") : launch_few<bk::W_F32, false>(p, vec, s, "few_rows");
+}
+
+// ---- 8-bit products ----
+// q [rows][ldq] (ldq a multiple of 128), scale bytes e + 127 [rows][scp] (scp a multiple of 4), one for each 128 columns
+BTVAE_API int btvae_fp8_quantize(const void* src, int src_bf16, long long ld, void* q, long long ldq, void* sc, long long scp, int rows, int K, void* stream) {
+    const int kb = bk::tiles(K, 128);
+    BTVAE_REQUIRE(rows >= 0 && K > 0 && ld >= K && ldq >= (long long)kb * 128 && (ldq & 15) == 0 && bk::al16(q) && scp >= kb, "fp8_quantize: bad layout");
+    if (rows == 0) return 0;
+    const bool vec = bk::al16(src) && K % 8 == 0 && (ld & (src_bf16 ? 7 : 3)) == 0;
+    const unsigned grid = (unsigned)std::min<long long>(((long long)rows * kb + 15) / 16, 32768);
+    hipStream_t s = BLK_STREAM(stream);
+    unsigned char* qd = (unsigned char*)q;
+    unsigned char* sd = (unsigned char*)sc;
+    if (src_bf16) {
+        if (vec) hipLaunchKernelGGL((bk::quantize_rows<true, true>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
+        else hipLaunchKernelGGL((bk::quantize_rows<true, false>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
+    } else {
+        if (vec) hipLaunchKernelGGL((bk::quantize_rows<false, true>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
+        else hipLaunchKernelGGL((bk::quantize_rows<false, false>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
+    }
+    return check_launch("fp8_quantize");
+}
+// weights: one scale for each 128 x 128 block, scale bytes [ceil(N / 128)][scp]
+BTVAE_API int btvae_fp8_quantize_blocks(const void* src, int src_bf16, long long ld, void* q, long long ldq, void* sc, long long scp, int N, int K, void* stream) {
+    const int kb = bk::tiles(K, 128), nb = bk::tiles(N, 128);
+    BTVAE_REQUIRE(N > 0 && K > 0 && ld >= K && ldq >= (long long)kb * 128 && (ldq & 15) == 0 && bk::al16(q) && scp >= kb && nb <= 65535, "fp8_quantize_blocks: bad layout");
+    hipStream_t s = BLK_STREAM(stream);
+    if (src_bf16) hipLaunchKernelGGL((bk::quantize_blocks<true>), dim3(kb, nb), dim3(256), 0, s, src, ld, (unsigned char*)q, ldq, (unsigned char*)sc, scp, N, K);
+    else hipLaunchKernelGGL((bk::quantize_blocks<false>), dim3(kb, nb), dim3(256), 0, s, src, ld, (unsigned char*)q, ldq, (unsigned char*)sc, scp, N, K);
+    return check_launch("fp8_quantize_blocks");
+}
+// out fp32 [rows][K]: the values that quantised rows (blocks = 0) or weights (blocks = 1) stand for
+BTVAE_API int btvae_fp8_dequantize(const void* q, long long ldq, const void* sc, long long scp, int blocks, float* out, int rows, int K, void* stream) {
+    BTVAE_REQUIRE(rows >= 0 && K > 0 && ldq >= K && scp >= bk::tiles(K, 128), "fp8_dequantize: bad layout");
+    if (rows == 0) return 0;
+    hipLaunchKernelGGL(bk::dequantize, dim3((unsigned)std::min<long long>(((long long)rows * K + 255) / 256, 16384)), dim3(256), 0, BLK_STREAM(stream), (const unsigned char*)q, ldq,
+                       (const unsigned char*)sc, scp, blocks ? 7 : 0, out, rows, K);
+    return check_launch("fp8_dequantize");
+}
+
+// out bf16 [rows][ldo]: the same values, exactly, zeros up to whole blocks of 128 columns
+BTVAE_API int btvae_fp8_expand(const void* q, long long ldq, const void* sc, long long scp, int blocks, void* out, long long ldo, int rows, int K, void* stream) {
+    const int kb = bk::tiles(K, 128);
+    BTVAE_REQUIRE(rows >= 0 && K > 0 && ldq >= kb * 128LL && (ldq & 15) == 0 && bk::al16(q) && scp >= kb && ldo >= kb * 128LL && (ldo & 7) == 0 && bk::al16(out), "fp8_expand: bad layout");
+    if (rows == 0) return 0;
+    hipLaunchKernelGGL(bk::expand_rows, dim3((unsigned)std::min<long long>(((long long)rows * kb * 16 + 255) / 256, 16384)), dim3(256), 0, BLK_STREAM(stream), (const unsigned char*)q, ldq,
+                       (const unsigned char*)sc, scp, blocks ? 7 : 0, (unsigned short*)out, ldo, rows, kb * 16);
+    return check_launch("fp8_expand");
+}
+
+static bool fp8_ok(const void* q, long long ldq, const void* sc, long long scp, int K) {
+    const int kb = bk::tiles(K, 128);
+    return bk::al16(q) && (ldq & 15) == 0 && ldq >= (long long)kb * 128 && ((uintptr_t)sc & 3) == 0 && (scp & 3) == 0 && scp >= kb;
+}
+BTVAE_API long long btvae_fp8_product_ws(int M, int N, int K) {
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tiles(K, 128) * 2, 8, 2 * bk::SC_ROW);
+    return r.z > 1 ? (long long)r.z * M * N : 0;
+}
+BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, long long xsp, const void* W, long long ldw, const void* wsc, long long wscp, const float* bias,
+                                void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int M, int N, int K, void* stream) {
+    BTVAE_REQUIRE(M >= 0 && N > 0 && K > 0 && ldc >= N, "fp8_product: bad sizes (M %d, N %d, K %d)", M, N, K);
+    if (M == 0) return 0;
+    BTVAE_REQUIRE(fp8_ok(X, ldx, xs, xsp, K) && fp8_ok(W, ldw, wsc, wscp, K), "fp8_product: bad operand layout");
+    hipStream_t s = BLK_STREAM(stream);
+    bk::Args p = {};
+    p.A = (const char*)X; p.lda = ldx; p.B = (const char*)W; p.ldb = ldw;
+    p.M = M; p.N = N; p.K = K; p.pairs = 1; p.ks = bk::tiles(K, 128) * 2;
+    p.a_sc = (const unsigned char*)xs; p.a_scp = xsp; p.b_sc = (const unsigned*)wsc; p.b_scp = (int)(wscp / 4);
+    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 8, 2 * bk::SC_ROW);
+    BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "fp8_product: workspace too small");
+    p.kz = r.kz; p.slab = ws; p.bias = bias;
+    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32; p.c_vec = bk::al16(C) && (ldc & (c_bf16 ? 7 : 3)) == 0;
+    ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
+    if (int rc = bk::launch_rows<bk::FMT_E4M3, bk::EP_LINEAR>(p, r.shape, r.z, s, "fp8_product")) return rc;
+    if (r.z == 1) return 0;
+    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0,
+                       (const void*)bias, 0, c_bf16, 0);
+    return check_launch("fp8_product reduction");
+}
+// H = act(x Wg^T + bg) (x Wu^T + bu), quantised again (q [M][ldh], scale bytes [M][hsp]) in the epilogue.  expanded: X, Wg, Wu hold bf16 (pitches in
+// elements, whole blocks of 128 columns) instead of e4m3 and scales.
+BTVAE_API int btvae_fp8_gated_proj(const void* X, long long ldx, const void* xs, long long xsp, const void* Wg, const void* gs, const void* Wu, const void* us, long long ldw, long long wscp,
+                                   int expanded, const float* bg, const float* bu, void* H, long long ldh, void* hs, long long hsp, int act, int M, int F, int K, void* stream) {
+    BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0, "fp8_gated_proj: bad sizes (M %d, F %d, K %d)", M, F, K);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "fp8_gated_proj: unknown activation %d", act);
+    BTVAE_REQUIRE(bk::tiles(K, 128) <= bk::SC_ROW, "fp8_gated_proj: K %d is beyond %d", K, bk::SC_ROW * 128);
+    if (M == 0) return 0;
+    BTVAE_REQUIRE(fp8_ok(H, ldh, hs, hsp, F), "fp8_gated_proj: bad layout of H");
+    bk::Args p = {};
+    const int kp = bk::tiles(K, 128) * 128, sz = expanded ? 2 : 1;
+    p.A = (const char*)X; p.lda = ldx * sz; p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw * sz;
+    p.M = M; p.N = F; p.pairs = 1;
+    p.bias = bg; p.bias2 = bu; p.C = H; p.ldc = ldh; p.c_type = bk::T_E4M3; p.q_sc = (unsigned char*)hs; p.q_scp = hsp; p.act = act;
+    const int shape = bk::use_big(M, F, 128) ? 0 : 2;
+    ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
+    if (expanded) {
+        BTVAE_REQUIRE(operand_ok(X, ldx, 0, 1) && ldx >= kp && operand_ok(Wg, ldw, 0, 1) && operand_ok(Wu, ldw, 0, 1) && ldw >= kp, "fp8_gated_proj: bad operand layout");
+        p.K = kp; p.ks = p.kz = kp / 32;
+        return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, shape, 1, BLK_STREAM(stream), "fp8_gated_proj");
+    }
+    BTVAE_REQUIRE(fp8_ok(X, ldx, xs, xsp, K) && fp8_ok(Wg, ldw, gs, wscp, K) && fp8_ok(Wu, ldw, us, wscp, K), "fp8_gated_proj: bad operand layout");
+    p.K = K; p.ks = p.kz = kp / 64;
+    p.a_sc = (const unsigned char*)xs; p.a_scp = xsp; p.b_sc = (const unsigned*)gs; p.b2_sc = (const unsigned*)us; p.b_scp = (int)(wscp / 4);
+    return bk::launch_rows<bk::FMT_E4M3, bk::EP_GATED>(p, shape, 1, BLK_STREAM(stream), "fp8_gated_proj");
+}
+// Up to btvae_few_rows_max() rows of fp32 / bf16 x, quantised on the way in; W2 null: C = x W^T + bias, else the gated product (C fp32 or bf16).
+BTVAE_API int btvae_fp8_few_rows(const void* X, int x_bf16, long long ldx, const void* W, const void* wsc, const void* W2, const void* wsc2, long long ldw, long long wscp, const float* bias,
+                                 const float* bias2, void* C, long long ldc, int c_bf16, int act, int M, int N, int K, void* stream) {
+    BTVAE_REQUIRE(M >= 0 && M <= 32 && N > 0 && K > 0 && ldx >= K && ldc >= N, "fp8_few_rows: bad sizes (M %d, N %d, K %d)", M, N, K);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "fp8_few_rows: unknown activation %d", act);
+    BTVAE_REQUIRE(fp8_ok(W, ldw, wsc, wscp, K) && (!W2 || fp8_ok(W2, ldw, wsc2, wscp, K)), "fp8_few_rows: bad weight layout");
+    if (M == 0) return 0;
+    bk::FewArgs p = {};
+    p.X = X; p.ldx = ldx; p.x_bf16 = x_bf16; p.B = (const char*)W; p.B2 = (const char*)W2; p.ldb = ldw;
+    p.b_sc = (const unsigned char*)wsc; p.b2_sc = (const unsigned char*)wsc2; p.b_scp = wscp;
+    p.bias = bias; p.bias2 = bias2; p.C = C; p.ldc = ldc; p.c_bf16 = c_bf16; p.M = M; p.N = N; p.K = K; p.act = act;
+    const bool vec = bk::al16(X) && K % 8 == 0 && (ldx & (x_bf16 ? 7 : 3)) == 0;
+    hipStream_t s = BLK_STREAM(stream);
+    ProfScope prof(PK_GEMM_FWD, s, (W2 ? 4.0 : 2.0) * M * N * K, 0.0);
+    return W2 ? launch_few<bk::W_E4M3, true>(p, vec, s, "fp8_few_rows") : launch_few<bk::W_E4M3, false>(p, vec, s, "fp8_few_rows");
+}

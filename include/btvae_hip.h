@@ -381,6 +381,87 @@ int btvae_sample_error_update(const float* xs, const float* x, float* e1, float*
 int btvae_dirichlet_sample(const float* gamma, const long long* rows, float* out, int B, int S, int T, int ldo,
                            int col0, unsigned long long seed, unsigned long long offset, void* stream);
 
+/* ---- gated residual block: h = act(x Wg^T + bg) (x Wu^T + bu), y = h Wd^T + bd, row norms, 8-bit products ----
+ * No counterpart in the reference, whose networks stop at Linear + ReLU + BatchNorm units (src/submodels.py:6-35).
+ * planes: 1 = bf16 operands, 3 = fp32 values as three bf16 planes (x = x0 + x1 + x2, `*_plane` elements apart) and the six
+ * largest of the nine plane products.  Operand matrices start on 16 bytes, pitches (in elements) are multiples of 8; reduction
+ * lengths are multiples of 8, the columns beyond a matrix's own width being zeros.  act: 0 silu, 1 gelu (erf), 2 relu, 3 sigmoid.
+ * Matrices marked with a *_bf16 flag are bf16 when it is set, else fp32. */
+/* dst[plane][row][0 .. dst_cols) = bf16 planes of src [rows, cols] (transpose: of its transpose), zero-padded. */
+int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long plane, long long dst_ld, int rows,
+            int cols, int dst_cols, int transpose, void* stream);
+/* H [planes][M][ldh] = h; GU [M][ldgu] (fp32 with three planes, else bf16; null: not kept): x Wg^T + bg at column 0, x Wu^T + bu at
+ * column gu_half. */
+int btvae_gated_proj_fwd(const void* X, long long ldx, long long x_plane, const void* Wg, const void* Wu, long long ldw,
+            long long w_plane, const void* bg, const void* bu, int bias_bf16, void* H, long long ldh, long long h_plane, void* GU,
+            long long ldgu, int gu_half, int planes, int act, int M, int F, int K, void* stream);
+/* dGU [planes][M][ldd]: da at column 0, db at column gu_half (zeros between F and gu_half) from dh = dY WdT^T, WdT [planes][F][ldw];
+ * colpart: null, or [btvae_gated_proj_strips(M, F)][2][F] column sums of da and db. */
+int btvae_gated_proj_bwd(const void* dY, long long lddy, long long dy_plane, const void* WdT, long long ldw, long long w_plane,
+            const void* GU, long long ldgu, int gu_half, void* dGU, long long ldd, long long d_plane, float* colpart, int planes,
+            int act, int M, int F, int N, void* stream);
+int btvae_gated_proj_strips(int M, int F);
+/* C [M, N] = A B^T + bias; workspace (floats) of btvae_block_product_ws, 0: none. */
+long long btvae_block_product_ws(int M, int N, int K, int planes);
+int btvae_block_product(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane,
+            const void* bias, int bias_bf16, void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int planes, int M,
+            int N, int K, void* stream);
+/* out(m, n) (+)= sum_r A[r][m] B[r][n]: rows m in [0, rows0) to out0, in [off1, off1 + rows1) to out1 (null: dropped); columns of A
+ * and B are read up to the next multiple of 8. */
+long long btvae_block_wgrad_ws(int M, int N, int R, int planes);
+int btvae_block_wgrad(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, float* ws,
+            long long ws_floats, void* out0, int rows0, void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate,
+            int planes, int M, int N, int R, void* stream);
+/* out[n] (+)= column sums of src [R, N]. */
+long long btvae_block_colsum_ws(int R, int N);
+int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, long long ws_floats, void* out, int out_bf16,
+            int accumulate, int R, int N, void* stream);
+/* out0 / out1 [n] (+)= sums over strips of part[strip][0 / 1][n]. */
+int btvae_block_strip_sums(const float* part, int strips, int N, void* out0, void* out1, int out_bf16, int accumulate, void* stream);
+/* Products of up to btvae_few_rows_max() rows, everything fp32 or everything bf16: C = X W^T + bias, or with W2 act(X W^T + bias)
+ * (X W2^T + bias2). */
+int btvae_few_rows_max(void);
+int btvae_few_rows(const void* X, long long ldx, const void* W, const void* W2, long long ldw, const void* bias, const void* bias2,
+            void* C, long long ldc, int bf16, int act, int M, int N, int K, void* stream);
+/* e4m3 with power-of-two scales: q = e4m3(x 2^-e), e the smallest integer >= -126 with the block's largest finite magnitude <= 448 2^e
+ * (0 for zeros), kept as the byte e + 127.  Rows: a block is 128 columns of one row, scales [rows][scp].  Weights: 128 x 128, scales
+ * [ceil(N / 128)][scp].  q's pitch holds whole blocks (zeros beyond K), scp is a multiple of 4.  Non-finite values become NaN. */
+int btvae_fp8_quantize(const void* src, int src_bf16, long long ld, void* q, long long ldq, void* sc, long long scp, int rows, int K,
+            void* stream);
+int btvae_fp8_quantize_blocks(const void* src, int src_bf16, long long ld, void* q, long long ldq, void* sc, long long scp, int N, int K,
+            void* stream);
+int btvae_fp8_dequantize(const void* q, long long ldq, const void* sc, long long scp, int blocks, float* out, int rows, int K,
+            void* stream);
+int btvae_fp8_expand(const void* q, long long ldq, const void* sc, long long scp, int blocks, void* out, long long ldo, int rows, int K,
+            void* stream);
+/* C = X W^T + bias of quantised rows and weights. */
+long long btvae_fp8_product_ws(int M, int N, int K);
+int btvae_fp8_product(const void* X, long long ldx, const void* xs, long long xsp, const void* W, long long ldw, const void* wsc,
+            long long wscp, const float* bias, void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int M, int N, int K,
+            void* stream);
+/* H = act(X Wg^T + bg) (X Wu^T + bu), quantised again row by row.  expanded: X, Wg, Wu are bf16 (btvae_fp8_expand) instead of e4m3 and
+ * scales: sums as exact as float32's, where the 8-bit matrix
+ * instruction's own are off by about 2^-16 of a result. */
+int btvae_fp8_gated_proj(const void* X, long long ldx, const void* xs, long long xsp, const void* Wg, const void* gs, const void* Wu,
+            const void* us, long long ldw, long long wscp, int expanded, const float* bg, const float* bu, void* H, long long ldh,
+            void* hs, long long hsp, int act, int M, int F, int K, void* stream);
+/* Up to btvae_few_rows_max() rows of unquantised x (quantised on the way in); W2 as in btvae_few_rows. */
+int btvae_fp8_few_rows(const void* X, int x_bf16, long long ldx, const void* W, const void* wsc, const void* W2, const void* wsc2,
+            long long ldw, long long wscp, const float* bias, const float* bias2, void* C, long long ldc, int c_bf16, int act, int M,
+            int N, int K, void* stream);
+/* u = post(branch), stream = residual + scale gate u, normed = pre(stream); norms: 0 none, 1 t / sqrt(mean t^2 + eps) w, 2 layer norm.
+ * Gate row of row r: r % G.  types: bit 0 residual / stream bf16, bit 1 branch / gate / normed bf16.  Weights fp32, null: 1 and 0.
+ * stats [4][M] (null: not kept) is what the backward pass reads; gradients that are not wanted are null. */
+int btvae_norm_max_columns(void);
+int btvae_norm_gate_residual_fwd(const void* residual, const void* branch, const void* gate, int G, float scale, const float* scale_vec,
+            const float* post_w, const float* post_b, const float* pre_w, const float* pre_b, int post, int pre, float eps,
+            void* stream_out, void* normed, float* stats, int types, int M, int N, void* stream);
+long long btvae_norm_gate_residual_ws(int M, int N, int G);
+int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* stream_in, const void* branch, const void* gate,
+            int G, float scale, const float* scale_vec, const float* post_w, const float* post_b, const float* pre_w, int post, int pre,
+            const float* stats, void* d_residual, void* d_branch, void* d_gate, float* d_scale, float* d_post_w, float* d_post_b,
+            float* d_pre_w, float* d_pre_b, float* ws, long long ws_floats, int types, int M, int N, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,706 @@
+"""GPU: the gated residual block's operators against their definitions in 64 bits.
+
+Tolerances.  u(t) = finfo(t).eps / 2 is the largest relative error of one rounding to t.  A float32 sum of n products picks up
+about sqrt(n) roundings of the size of its partial sums: its Frobenius error is held to 2^-24 (4 + sqrt(n)) of the result's norm,
+chains of products to the sum of their terms (times the factor by which cancellation shrinks a result, stated where there is one).
+bfloat16 results are held element by element to bounds that count every rounding: with |.| the product of magnitudes,
+an operand rounded to bfloat16 contributes u |.| and the result's own rounding u |result|; float32 sums add n 2^-24 |.|."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from behavio_temporal_vae_amd import _native as nv  # noqa: E402
+from behavio_temporal_vae_amd import block_ops as B  # noqa: E402
+
+BF, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -8          # bfloat16
+E = 2.0 ** -24         # float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    d = torch.device("cuda:0")
+    nv.ensure_device(d)
+    return d
+
+
+def rnd(dev, *shape, seed=0, scale=1.0, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(dev)
+
+
+def d64(t):
+    return None if t is None else t.detach().double()
+
+
+def frob(got, ref, tol, what):
+    assert got.shape == ref.shape, what
+    err, norm = (got.detach().double() - ref).norm().item(), ref.norm().item()
+    assert err <= tol * norm + 1e-300, f"{what}: relative error {err / (norm + 1e-300):.3e} > {tol:.3e}"
+
+
+def within(got, ref, lim, what):
+    err = (got.detach().double() - ref).abs()
+    bad = ~(err <= lim + 1e-300)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst ratio {(err / (lim + 1e-300)).max().item():.2f}"
+
+
+def act64(name, a):
+    if name == "silu":
+        return a * torch.sigmoid(a)
+    if name == "gelu":
+        return 0.5 * a * torch.special.erfc(-a / math.sqrt(2))
+    return torch.relu(a) if name == "relu" else torch.sigmoid(a)
+
+
+def ffn64(t, act):
+    a = t["x"] @ t["wg"].t()
+    b = t["x"] @ t["wu"].t()
+    if t["bg"] is not None:
+        a, b = a + t["bg"], b + t["bu"]
+    h = act64(act, a) * b
+    y = h @ t["wd"].t()
+    return a, b, h, y if t["bd"] is None else y + t["bd"]
+
+
+def ffn_case(dev, M, K, F, N, dtype, bias, seed=1):
+    t = dict(x=rnd(dev, M, K, seed=seed, dtype=dtype), wg=rnd(dev, F, K, seed=seed + 1, scale=1 / math.sqrt(K), dtype=dtype),
+             wu=rnd(dev, F, K, seed=seed + 2, scale=1 / math.sqrt(K), dtype=dtype), wd=rnd(dev, N, F, seed=seed + 3, scale=1 / math.sqrt(F), dtype=dtype))
+    for k, n, s in (("bg", F, 4), ("bu", F, 5), ("bd", N, 6)):
+        t[k] = rnd(dev, n, seed=seed + s, scale=0.3, dtype=dtype) if bias else None
+    return t
+
+
+def call_ffn(t, act):
+    return B.gated_feed_forward(t["x"], t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"], activation=act)
+
+
+def check_ffn_forward(y, t, act):
+    r = {k: d64(v) for k, v in t.items()}
+    a, b, h, ref = ffn64(r, act)
+    K, F = t["x"].shape[1], t["wg"].shape[0]
+    if t["x"].dtype == F32:
+        # two projections meet in h (a 1-Lipschitz-like activation: |act'| <= 1.13), one more product follows
+        frob(y, ref, E * (2.3 * (4 + math.sqrt(K)) + 4 + math.sqrt(F)) * max(1.0, h.norm().item() * r["wd"].norm().item() / math.sqrt(F) / ref.norm().item()), "y")
+        return
+    xs = r["x"].abs()
+    ea = (K + 4) * E * (xs @ r["wg"].abs().t()) + 2 ** -20 * a.abs()          # float32 sums; the fast exp and reciprocal
+    eb = (K + 4) * E * (xs @ r["wu"].abs().t())
+    eh = 1.13 * ea * b.abs() + act64(act, a).abs() * (eb + 2 ** -20 * b.abs()) + U * h.abs()
+    lim = eh @ r["wd"].abs().t() + (F + 4) * E * (h.abs() @ r["wd"].abs().t()) + U * ref.abs()
+    within(y, ref, lim * 1.01, "y")
+
+
+SIZES = [(1, 8, 8, 8), (1, 1000, 2000, 1000), (3, 7, 5, 1), (17, 203, 531, 96), (32, 24, 40, 72), (33, 203, 531, 203), (129, 64, 333, 65), (300, 1000, 264, 48), (700, 40, 1001, 31)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,F,N", SIZES)
+def test_ffn_forward(dev, M, K, F, N, dtype):
+    for i, act in enumerate(B.ACTIVATIONS):
+        t = ffn_case(dev, M, K, F, N, dtype, bias=i % 2 == 0, seed=10 * i)
+        check_ffn_forward(call_ffn(t, act), t, act)
+        y, _ = B.gated_feed_forward_tape(t["x"], t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"], activation=act)
+        check_ffn_forward(y, t, act)
+
+
+def ffn_grads(t, act, dy):
+    leaves = {k: v.detach().clone().requires_grad_(True) for k, v in t.items() if v is not None}
+    y = call_ffn({**{k: None for k in t}, **leaves}, act)
+    return y, dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+
+
+def ffn_grads64(t, act, dy):
+    leaves = {k: d64(v).requires_grad_(True) for k, v in t.items() if v is not None}
+    y = ffn64({**{k: None for k in t}, **leaves}, act)[3]
+    return dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy.double())))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,F,N", [(1, 8, 8, 8), (2, 7, 5, 1), (31, 203, 531, 96), (257, 64, 333, 65), (1037, 200, 264, 200), (2500, 40, 1001, 31)])
+def test_ffn_backward(dev, M, K, F, N, dtype):
+    for i, act in enumerate(B.ACTIVATIONS):
+        t = ffn_case(dev, M, K, F, N, dtype, bias=i % 2 == 1, seed=100 + 10 * i)
+        dy = rnd(dev, M, N, seed=99, dtype=dtype)
+        y, got = ffn_grads(t, act, dy)
+        check_ffn_forward(y, t, act)
+        ref = ffn_grads64(t, act, dy)
+        if dtype == F32:
+            # products in the chain before a gradient: projections (K), dh (N), then its own (2F or M); sums over rows may cancel: times
+            # the ratio of what is added to what is left, at most sqrt(terms) for independent terms of one size
+            for k, v in got.items():
+                n = {"x": 2 * F}.get(k, M)
+                frob(v, ref[k], 3 * E * ((4 + math.sqrt(K)) + (4 + math.sqrt(N)) + (4 + math.sqrt(n))), f"d{k} ({act})")
+            continue
+        r = {k: d64(v) for k, v in t.items()}
+        a, b, h, _ = ffn64(r, act)
+        a = a.detach().requires_grad_(True)
+        v = act64(act, a)
+        d1 = torch.autograd.grad(v.sum(), a, create_graph=act != "relu")[0]
+        d2 = torch.autograd.grad(d1.sum(), a)[0] if act != "relu" else torch.zeros_like(a)
+        a, v, d1 = a.detach(), v.detach(), d1.detach()
+        dy64 = dy.double()
+        dh = dy64 @ r["wd"]
+        s = (K + N + 8) * E * 4 + 2 ** -18                     # float32 sums and the fast exp, generously
+        eh = U * h.abs() + s * (h.abs() + a.abs() * b.abs() + b.abs())
+        # the kept a and b are rounded; act' may move over u |a| by as much as its slope nearby allows (1.2 |a| u covers curvature: |act''| <= 1.2)
+        shift = U * a.abs() + s * (r["x"].abs() @ r["wg"].abs().t())
+        curve = torch.maximum(d2.abs(), torch.full_like(a, 0.1)) * 2 * shift if act != "relu" else (a.abs() <= 2 * shift).double()
+        slope = d1.abs() + curve
+        da, db = dh * b * d1, dh * v
+        dhs = s * (dy64.abs() @ r["wd"].abs())
+        eda = dh.abs() * (U * b.abs() * slope + b.abs() * curve) + dhs * b.abs() * slope + U * da.abs() + s * dh.abs() * (b.abs() + 1)
+        edb = dh.abs() * slope * 2 * shift + dhs * v.abs() + U * db.abs() + s * dh.abs()
+        eda, edb = 1.1 * eda, 1.1 * edb
+        x, wg, wu = r["x"], r["wg"], r["wu"]
+        lim = {"x": eda @ wg.abs() + edb @ wu.abs(), "wg": eda.t() @ x.abs(), "wu": edb.t() @ x.abs(), "wd": dy64.abs().t() @ eh,
+               "bg": eda.sum(0), "bu": edb.sum(0), "bd": (M + 4) * E * dy64.abs().sum(0)}
+        mag = {"x": da.abs() @ wg.abs() + db.abs() @ wu.abs(), "wg": da.abs().t() @ x.abs(), "wu": db.abs().t() @ x.abs(), "wd": dy64.abs().t() @ h.abs(),
+               "bg": da.abs().sum(0), "bu": db.abs().sum(0), "bd": dy64.abs().sum(0)}
+        for k, g in got.items():
+            within(g, ref[k], 1.01 * (lim[k] + (2 * F + M + 8) * E * mag[k] + U * ref[k].abs()), f"d{k} ({act})")
+
+
+def test_ffn_backward_matches_differences(dev):
+    """Directional derivative of the float32 forward, taken in 64 bits from the definition at x +- s v: the gradient's inner product
+    with v is the difference quotient up to O(s^2)."""
+    t = ffn_case(dev, 70, 24, 40, 16, F32, True, seed=7)
+    dy = rnd(dev, 70, 16, seed=8)
+    _, got = ffn_grads(t, "gelu", dy)
+    s = 1e-4
+    for k in got:
+        v = rnd(dev, *t[k].shape, seed=9).double()
+        f = []
+        for sign in (1, -1):
+            r = {q: d64(w) for q, w in t.items()}
+            r[k] = r[k] + sign * s * v
+            f.append((ffn64(r, "gelu")[3] * dy.double()).sum().item())
+        quotient, inner = (f[0] - f[1]) / (2 * s), (got[k].double() * v).sum().item()
+        scale = (got[k].double().abs() * v.abs()).sum().item()
+        assert abs(quotient - inner) <= 2e-6 * scale, (k, quotient, inner)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_ffn_strides_and_shapes(dev, dtype):
+    """Inputs that are views: padded rows, transposed storage, odd offsets, leading dimensions."""
+    t = ffn_case(dev, 96, 40, 56, 24, dtype, True, seed=3)
+    base = call_ffn(t, "silu")
+    wide = torch.full((96, 48), float("nan"), dtype=dtype, device=dev)
+    wide[:, :40] = t["x"]
+    odd = torch.full((96 * 43 + 1,), float("nan"), dtype=dtype, device=dev)[1:].view(96, 43)
+    odd[:, :40] = t["x"]
+    for x in (wide[:, :40], odd[:, :40], t["x"].t().contiguous().t(), t["x"].view(4, 24, 40)):
+        y = call_ffn({**t, "x": x}, "silu")
+        assert y.shape == (*x.shape[:-1], 24) and torch.equal(y.reshape(96, 24), base)
+    wt = {**t, "wg": t["wg"].t().contiguous().t(), "wd": torch.cat([t["wd"], t["wd"]], 1)[:, :56]}
+    assert torch.equal(call_ffn(wt, "silu"), base)
+    few = {**t, "x": odd[:5, :40]}
+    check_ffn_forward(call_ffn(few, "silu"), few, "silu")
+    dy = rnd(dev, 24, 96, dtype=dtype).t()                     # a gradient that is a transposed view
+    _, got = ffn_grads(t, "silu", dy)
+    _, ref = ffn_grads(t, "silu", dy.contiguous())
+    for k in got:
+        assert torch.equal(got[k], ref[k]), k
+
+
+def test_ffn_empty_and_no_grad_paths(dev):
+    t = ffn_case(dev, 0, 40, 56, 24, F32, True)
+    y, got = ffn_grads(t, "silu", torch.empty(0, 24, device=dev))
+    assert y.shape == (0, 24) and got["x"].shape == (0, 40)
+    for k in ("wg", "wu", "wd", "bg", "bu", "bd"):
+        assert not got[k].any(), k
+    t = ffn_case(dev, 50, 40, 56, 24, F32, False)
+    wd = t["wd"].clone().requires_grad_(True)                  # only one gradient asked for
+    call_ffn({**t, "wd": wd}, "silu").sum().backward()
+    assert wd.grad is not None
+    x = t["x"].clone().requires_grad_(True)
+    gx, = torch.autograd.grad(call_ffn({**t, "x": x}, "silu").sum(), x)
+    assert gx.shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M", [20, 200])
+def test_ffn_non_finite_rows_stay_alone(dev, M, dtype):
+    t = ffn_case(dev, M, 72, 96, 40, dtype, True, seed=5)
+    base = call_ffn(t, "silu")
+    x = t["x"].clone()
+    x[3, 71] = float("nan")
+    x[7, 0] = float("inf")
+    y = call_ffn({**t, "x": x}, "silu")
+    keep = [i for i in range(M) if i not in (3, 7)]
+    assert torch.equal(y[keep], base[keep]) and y[3].isnan().all() and not y[7].isfinite().all()
+
+
+def test_ffn_graph_replays_and_streams(dev):
+    """Tapes captured into two graphs, replayed in turn with eager work between: every replay equals the eager result."""
+    t = ffn_case(dev, 300, 64, 96, 64, BF, True, seed=6)
+    dy = rnd(dev, 300, 64, seed=1, dtype=BF)
+    args = (t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])
+
+    def step(x):
+        y, tape = B.gated_feed_forward_tape(x, *args)
+        return (y, *tape.backward(dy))
+
+    xs = [t["x"].clone(), t["x"].clone()]
+    step(xs[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(x))
+        graphs.append(g)
+    for rep in range(4):
+        for i in (0, 1):
+            xs[i].copy_(rnd(dev, 300, 64, seed=20 + 2 * rep + i, dtype=BF))
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for a, b in zip(outs[i], step(xs[i].clone())):
+                assert torch.equal(a, b), (rep, i)
+    side = torch.cuda.Stream()
+    want = step(t["x"])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(t["x"])
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    x = t["x"].clone().requires_grad_(True)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="tape"):
+        with torch.cuda.graph(g):
+            call_ffn({**t, "x": x}, "silu")
+
+
+def test_planes_are_exact(dev):
+    """x times the identity comes back bit for bit from the three-plane product; so does the identity's transposed product."""
+    M, K = 200, 72
+    x = rnd(dev, M, K, seed=4) * torch.exp(rnd(dev, M, K, seed=5) * 8)
+    x[0, 0], x[1, 1], x[2, 2] = 3.4e38, -3.4028234e38, 1e-30
+    eye = torch.eye(K, device=dev)
+    X, I = B._operand(x, 3), B._operand(eye, 3)
+    out = torch.empty(M, K, device=dev)
+    assert torch.equal(B._product(X, I, None, out, 3, M, K, X.width), x)
+    lib = nv.lib()
+    eyem = torch.eye(M, device=dev)
+    Im = B._operand(eyem, 3)
+    ws = torch.empty(lib.btvae_block_wgrad_ws(M, K, M, 3), device=dev)
+    out2 = torch.empty(M, K, device=dev)
+    nv.call("btvae_block_wgrad", Im.ptr(), Im.ld, Im.plane, X.ptr(), X.ld, X.plane, ws.data_ptr(), ws.numel(), out2.data_ptr(), M, None, 0, 0, K, 0, 0, 3, M, K, M)
+    assert torch.equal(out2, x)
+
+
+@pytest.mark.parametrize("planes", [1, 3])
+@pytest.mark.parametrize("M,N,K", [(256, 256, 32), (300, 260, 1000), (1000, 77, 40), (64, 16, 4096), (4100, 2056, 64)])
+def test_block_product(dev, planes, M, N, K):
+    dt = F32 if planes == 3 else BF
+    a, b, bias = rnd(dev, M, K, seed=1, dtype=dt), rnd(dev, N, K, seed=2, dtype=dt), rnd(dev, N, seed=3)
+    A, W = B._operand(a, planes), B._operand(b, planes)
+    ref = a.double() @ b.double().t() + bias.double()
+    frob(B._product(A, W, bias, torch.empty(M, N, device=dev), planes, M, N, A.width), ref, E * (4 + math.sqrt(K)), "fp32 result")
+    got = B._product(A, W, bias, torch.empty(M, N, dtype=BF, device=dev), planes, M, N, A.width)
+    within(got, ref, U * ref.abs() * 1.01 + (K + 4) * E * (a.double().abs() @ b.double().abs().t()) + E, "bf16 result")
+    pad = torch.full((M, N + 3), 7.0, device=dev)
+    B._product(A, W, bias, pad[:, :N], planes, M, N, A.width)
+    assert (pad[:, N:] == 7.0).all()
+
+
+@pytest.mark.parametrize("planes", [1, 3])
+@pytest.mark.parametrize("R", [0, 1, 31, 32, 33, 1000, 5000])
+@pytest.mark.parametrize("M,N", [(8, 8), (130, 264), (333, 65), (1062, 203)])
+def test_block_wgrad(dev, planes, R, M, N):
+    dt = F32 if planes == 3 else BF
+    a, b = rnd(dev, R, M, seed=1, dtype=dt), rnd(dev, R, N, seed=2, dtype=dt)
+    A, X = B._operand(a, planes), B._operand(b, planes)
+    lib = nv.lib()
+    ws = torch.empty(lib.btvae_block_wgrad_ws(M, N, R, planes), device=dev)
+    h = M // 3
+    o0, o1 = torch.full((h, N), 2.0, device=dev), torch.full((M - 2 * h, N), 3.0, device=dev)
+    for acc in (1, 0):
+        nv.call("btvae_block_wgrad", A.ptr(), A.ld, A.plane, X.ptr(), X.ld, X.plane, ws.data_ptr(), ws.numel(), o0.data_ptr(), h, o1.data_ptr(), 2 * h, M - 2 * h, N, 0, acc, planes, M, N, R)
+        ref = a.double().t() @ b.double()
+        tol = E * (4 + math.sqrt(max(R, 1)))
+        frob(o0, ref[:h] + 2.0 * acc, tol + 2 * E, "first rows")
+        frob(o1, ref[2 * h:] + 3.0 * acc, tol + 2 * E, "last rows")
+
+
+# ------------------------------------------------------------------------------------------------ norms
+def norm64(t, kind, w, c, eps):
+    if kind is None:
+        return t
+    if kind == "layer":
+        t = t - t.mean(-1, keepdim=True)
+    t = t / torch.sqrt((t * t).mean(-1, keepdim=True) + eps)
+    t = t if w is None else t * w
+    return t if c is None else t + c
+
+
+def block64(r, post, pre, scale, eps):
+    v = r["residual"]
+    if r["branch"] is not None:
+        u = norm64(r["branch"], post, r["post_weight"], r["post_bias"], eps)
+        if r["gate"] is not None:
+            u = u * r["gate"].repeat(v.shape[0] // r["gate"].shape[0], 1)
+        v = v + (scale if r["scale"] is None else r["scale"]) * u
+    return v, None if pre is None else norm64(v, pre, r["pre_weight"], r["pre_bias"], eps)
+
+
+def norm_case(dev, M, N, G, rt, bt, post, pre, vec_scale, affine, seed=1):
+    t = dict(residual=rnd(dev, M, N, seed=seed, dtype=rt), branch=rnd(dev, M, N, seed=seed + 1, dtype=bt),
+             gate=(1 + rnd(dev, G, N, seed=seed + 2, scale=0.3)).to(bt) if G else None,
+             scale=0.5 + rnd(dev, N, seed=seed + 3, scale=0.1) if vec_scale else None)
+    for k, on in (("post", post), ("pre", pre)):
+        t[k + "_weight"] = 1 + rnd(dev, N, seed=seed + 4, scale=0.2) if affine and on else None
+        t[k + "_bias"] = rnd(dev, N, seed=seed + 5, scale=0.2) if affine and on else None
+    return t
+
+
+def call_norm(t, post, pre, eps=1e-6):
+    return B.norm_gate_residual(t["residual"], t["branch"], gate=t["gate"], scale=0.7 if t["scale"] is None else t["scale"], post_norm=post, post_weight=t["post_weight"],
+                                post_bias=t["post_bias"], pre_norm=pre, pre_weight=t["pre_weight"], pre_bias=t["pre_bias"], eps=eps)
+
+
+def rounding(t):
+    return U if t.dtype == BF else E
+
+
+NORM_CASES = [  # M, N, G, residual type, branch type, post, pre, scale vector, affine
+    (1, 1, 1, F32, F32, "rms", "rms", False, True),
+    (1, 1000, 1, BF, BF, "rms", "rms", False, True),
+    (5, 7, 0, F32, F32, "layer", "layer", True, True),
+    (12, 203, 3, F32, F32, "layer", "rms", True, True),
+    (64, 512, 64, F32, BF, "rms", "layer", False, False),
+    (130, 520, 65, BF, BF, None, "rms", True, True),
+    (96, 1000, 32, BF, BF, "layer", "layer", True, True),
+    (40, 1001, 1, F32, BF, "rms", None, False, True),
+    (4096, 48, 1, F32, F32, "rms", "rms", True, True),
+    (9000, 96, 3000, BF, BF, "rms", "rms", False, True),
+    (33, 2049, 11, F32, F32, "rms", "layer", False, True),
+    (30, 4096, 10, BF, BF, "layer", "rms", True, True),
+    (14, 8192, 7, F32, F32, "layer", "layer", True, True),
+    (6, 5003, 2, F32, BF, "layer", "rms", False, True),
+]
+
+
+@pytest.mark.parametrize("case", NORM_CASES, ids=lambda c: f"{c[0]}x{c[1]}g{c[2]}")
+def test_norm_gate_residual(dev, case):
+    M, N, G, rt, bt, post, pre, vec, affine = case
+    t = norm_case(dev, *case)
+    eps = 1e-6
+    names = [k for k, v in t.items() if v is not None]
+    leaves = {k: v.clone().requires_grad_(True) for k, v in t.items() if v is not None}
+    v, n = call_norm({**{k: None for k in t}, **leaves}, post, pre)
+    with torch.no_grad():
+        v2, n2 = call_norm(t, post, pre)
+    assert torch.equal(v, v2) and (n is None or torch.equal(n, n2))
+    r = {k: (d64(w).requires_grad_(True) if w is not None else None) for k, w in t.items()}
+    rv, rn = block64(r, post, pre, 0.7, eps)
+    # forward: a dozen float32 roundings of terms no larger than these, sums of N in a tree, the result's own rounding
+    f = (16 + math.log2(N)) * E
+    full = None if t["gate"] is None else t["gate"].double().repeat(M // G, 1).abs()
+    su = (rv - r["residual"]).abs().detach()
+    post_out = norm64(r["branch"], post, r["post_weight"], None, eps).abs().detach() * (1 if full is None else full) * (0.7 if t["scale"] is None else t["scale"].double().abs())
+    shift = 1.0
+    if post == "layer":
+        shift = 1 + (t["branch"].double().mean(-1, keepdim=True).abs() / t["branch"].double().std(-1, keepdim=True).clamp(min=1e-3) if N > 1 else 1e3)
+    ev = f * shift * (r["residual"].abs().detach() + 4 * post_out + 4 * su) + f * shift
+    within(v, rv.detach(), ev + rounding(v) * rv.abs().detach(), "stream")
+    if n is not None:
+        q = 1 / torch.sqrt((rv * rv).mean(-1, keepdim=True) + eps) if pre == "rms" else 1 / torch.sqrt(rv.var(-1, correction=0, keepdim=True) + eps)
+        w = 1 if r["pre_weight"] is None else r["pre_weight"].abs()
+        en = (2 * (ev + ev.amax(-1, keepdim=True)) * q * w + 16 * f * rn.abs() + f * (1 + (rv.abs().amax(-1, keepdim=True) * q) * w)).detach()
+        within(n, rn.detach(), en * (1 + (rv.abs().amax(-1, keepdim=True) * q).detach() * 0 + 2) + rounding(n) * rn.abs().detach(), "normed")
+    dv = rnd(dev, M, N, seed=50, dtype=v.dtype)
+    dn = rnd(dev, M, N, seed=51, dtype=n.dtype) if n is not None else None
+    outs = [v] + ([n] if n is not None else [])
+    ups = [dv] + ([dn] if dn is not None else [])
+    got = dict(zip(names, torch.autograd.grad(outs, [leaves[k] for k in names], ups)))
+    routs = [rv] + ([rn] if rn is not None else [])
+    ref = dict(zip(names, torch.autograd.grad(routs, [r[k] for k in names], [u.double() for u in ups])))
+    # gradients: float32 inside; the stream is kept in its type (a rounding of it moves its norm's gradient by as much), the
+    # result is rounded once; column sums add M terms
+    cond = 8.0 if N > 4 else 1e4            # one or a few columns: the norm's gradient cancels to nearly nothing
+    for k in names:
+        tol = rounding(got[k]) + cond * rounding(t["residual"]) + cond * E * (8 + math.sqrt(M) + math.sqrt(N))
+        scale = max(1.0, math.sqrt(M * N) * 0.1 / (ref[k].norm().item() + 1e-30)) if N <= 4 else 1.0
+        frob(got[k], ref[k], tol * scale, f"d{k}")
+
+
+def test_norm_parts(dev):
+    """Pre norm alone, no norm at all, partial gradients, leading dimensions, an infinite row, no rows."""
+    x = rnd(dev, 6, 5, 40, seed=1)
+    s, n = B.norm_gate_residual(x, pre_norm="layer")
+    assert s is x and n.shape == x.shape
+    frob(n, norm64(x.double(), "layer", None, None, 1e-6), 20 * E, "layer norm")
+    y = rnd(dev, 6, 5, 40, seed=2)
+    s, n = B.norm_gate_residual(x, y, scale=2.0, pre_norm=None)
+    assert n is None
+    within(s, x.double() + 2 * y.double(), 2 * E * (x.double().abs() + 2 * y.double().abs()), "sum")
+    xg, yg = x.clone().requires_grad_(True), y.clone().requires_grad_(True)
+    s, n = B.norm_gate_residual(xg, yg, post_norm="rms")
+    gs, = torch.autograd.grad(s.sum(), xg, retain_graph=True)
+    assert torch.equal(gs, torch.ones_like(x))
+    gn, = torch.autograd.grad((n * y).sum(), yg)
+    xr, yr = x.double().requires_grad_(True), y.double().requires_grad_(True)
+    nr = norm64(xr + norm64(yr, "rms", None, None, 1e-6), "rms", None, None, 1e-6)
+    frob(gn, torch.autograd.grad((nr * y.double()).sum(), yr)[0], 200 * E, "gradient through normed alone")
+    xi = x.reshape(30, 40).clone()
+    base = B.norm_gate_residual(xi, y.reshape(30, 40))[1]
+    xi[4, 3], xi[9, 0] = float("inf"), float("nan")
+    out = B.norm_gate_residual(xi, y.reshape(30, 40))[1]
+    keep = [i for i in range(30) if i not in (4, 9)]
+    assert torch.equal(out[keep], base[keep]) and not out[4].isfinite().all() and out[9].isnan().all()
+    w = torch.ones(40, device=dev, requires_grad=True)
+    e = torch.empty(0, 40, device=dev, requires_grad=True)
+    s, n = B.norm_gate_residual(e, torch.empty(0, 40, device=dev), pre_weight=w)
+    ge, gw = torch.autograd.grad(n.sum() + s.sum(), [e, w])
+    assert ge.shape == (0, 40) and not gw.any()
+    z = torch.zeros(3, 40, device=dev)
+    assert not B.norm_gate_residual(z, z, post_norm="rms")[1].any()          # rows of zeros: finite, zero
+
+
+def test_norm_gradients_match_differences(dev):
+    t = norm_case(dev, 24, 40, 8, F32, F32, "layer", "rms", True, True, seed=3)
+    names = list(t)
+    leaves = {k: v.clone().requires_grad_(True) for k, v in t.items()}
+    v, n = call_norm(leaves, "layer", "rms")
+    dv, dn = rnd(dev, 24, 40, seed=5), rnd(dev, 24, 40, seed=6)
+    got = dict(zip(names, torch.autograd.grad([v, n], [leaves[k] for k in names], [dv, dn])))
+    s = 1e-4
+    for k in names:
+        d = rnd(dev, *t[k].shape, seed=7).double()
+        f = []
+        for sign in (1, -1):
+            r = {q: d64(w) for q, w in t.items()}
+            r[k] = r[k] + sign * s * d
+            a, b = block64(r, "layer", "rms", None, 1e-6)
+            f.append((a * dv.double()).sum().item() + (b * dn.double()).sum().item())
+        quotient, inner = (f[0] - f[1]) / (2 * s), (got[k].double() * d).sum().item()
+        assert abs(quotient - inner) <= 5e-6 * (got[k].double().abs() * d.abs()).sum().item() + 1e-6, k
+
+
+def test_norm_graph_replays(dev):
+    t = norm_case(dev, 96, 200, 32, BF, BF, "rms", "rms", True, True, seed=8)
+    dv, dn = rnd(dev, 96, 200, seed=1, dtype=BF), rnd(dev, 96, 200, seed=2, dtype=BF)
+
+    def step(res):
+        v, n, tape = B.norm_gate_residual_tape(res, t["branch"], gate=t["gate"], scale=t["scale"], post_norm="rms", post_weight=t["post_weight"],
+                                               post_bias=t["post_bias"], pre_norm="rms", pre_weight=t["pre_weight"], pre_bias=t["pre_bias"])
+        return (v, n, *tape.backward(dv, dn))
+
+    res = t["residual"].clone()
+    step(res)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(res)
+    for rep in range(4):
+        res.copy_(rnd(dev, 96, 200, seed=30 + rep, dtype=BF))
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step(res.clone())):
+            assert torch.equal(a, b), rep
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit products
+def e4m3_64(t, rows, cols):
+    """Values of t in 64 bits as e4m3 with a power-of-two scale for each rows x cols block, from the definition."""
+    t = t.double()
+    a, b = t.shape
+    p = torch.zeros(-(-a // rows) * rows, -(-b // cols) * cols, dtype=torch.float64, device=t.device)
+    p[:a, :b] = t
+    k = p.view(p.shape[0] // rows, rows, p.shape[1] // cols, cols)
+    amax = k.abs().amax(dim=(1, 3), keepdim=True)
+    e = torch.where(amax > 0, torch.ceil(torch.log2(amax.clamp(min=1e-300) / 448)), torch.zeros_like(amax)).clamp(min=-126)
+    v = k / torch.exp2(e)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    return (torch.round(v / step) * step * torch.exp2(e)).reshape(p.shape)[:a, :b]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 128), (7, 129), (130, 203), (64, 1000), (257, 4100)])
+def test_fp8_quantize(dev, M, K, dtype):
+    x = (rnd(dev, M, K, seed=1) * torch.exp(3 * rnd(dev, M, 1, seed=2))).to(dtype)
+    x[0, 0] = 448.0
+    if K > 130:
+        x[0, 128:] = 0
+        x[-1, :128] *= 2.0 ** -100
+        x[-1, 128:] = (x[-1, 128:].float() * 2.0 ** -124).to(dtype)
+    assert torch.equal(B.fp8_quantize(x).dequantize().double(), e4m3_64(x, 1, 128))
+    assert torch.equal(B.fp8_weight(x).dequantize().double(), e4m3_64(x, 128, 128))
+    assert torch.equal(B.fp8_quantize(x.t().contiguous().t()).dequantize(), B.fp8_quantize(x).dequantize())
+
+
+def test_fp8_quantize_ties_and_non_finite(dev):
+    grid = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()     # every finite value from 0 to 448
+    mid = (grid[:-1] + grid[1:]) / 2
+    x = torch.zeros(4, 256)
+    x[0, :127], x[0, 127] = grid, 448.0
+    x[1, :126], x[1, 127] = mid, 448.0                         # ties: to even
+    x[2, :126], x[2, 127] = -mid, 448.0
+    x[3, :126], x[3, 127] = torch.nextafter(mid, torch.tensor(1e9)), 448.0
+    x = x.to(dev)
+    assert torch.equal(B.fp8_quantize(x).dequantize().double(), e4m3_64(x, 1, 128))
+    y = rnd(dev, 2, 256, seed=1)
+    ref = B.fp8_quantize(torch.where(torch.arange(256, device=dev) == 5, torch.zeros((), device=dev), y)).dequantize()
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        z = y.clone()
+        z[0, 5] = bad
+        got = B.fp8_quantize(z).dequantize()
+        assert got[0, 5].isnan() and got.isnan().sum() == 1
+        got[0, 5] = 0
+        assert torch.equal(got[0], ref[0])
+
+
+FP8_SIZES = [(1, 1, 1), (1, 1000, 2000), (5, 203, 531), (32, 4100, 70), (33, 128, 128), (200, 203, 531), (300, 1000, 264), (64, 20000, 96), (4100, 264, 2056), (1000, 72, 77)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,N", FP8_SIZES)
+def test_fp8_linear(dev, M, K, N, dtype):
+    x = (rnd(dev, M, K, seed=1) * torch.exp(2 * rnd(dev, M, 1, seed=4))).to(dtype)
+    w, bias = rnd(dev, N, K, seed=2, scale=1 / math.sqrt(K), dtype=dtype), rnd(dev, N, seed=3)
+    W = B.fp8_weight(w)
+    xq, wq = e4m3_64(x, 1, 128), e4m3_64(w, 128, 128)
+    ref = xq @ wq.t() + bias.double()
+    lim = (K + 8) * E * (xq.abs() @ wq.abs().t()) + 2 * E * ref.abs()
+    got = B.fp8_linear(x, W, bias, out_dtype=F32)
+    within(got, ref, lim, "fp32 result")
+    frob(got, ref, E * (4 + math.sqrt(K)), "fp32 result")
+    # bfloat16 results of more than 32 rows: the 8-bit pipe cuts each product it adds to a multiple of a unit that follows the largest of its
+    # group.  Over 128 products of normal values its error is 2^-16 of a result (rms): as the result's rms is sqrt(128) times a
+    # product's, and the largest product is about 9 times a product's rms, a cut of at most 2^-15 of the largest product each;
+    # K independent cuts add to sqrt(K) 2^-15 of it, and 4 of those deviations are sqrt(K) 2^-13
+    pipe = math.sqrt(K) * 2.0 ** -13 * xq.abs().amax(1, keepdim=True) * wq.abs().amax(1)
+    within(B.fp8_linear(x, W, bias, out_dtype=BF), ref, lim + pipe * (M > 32) + U * ref.abs() * 1.01, "bf16 result")
+    within(B.fp8_linear(B.fp8_quantize(x), W, bias), ref, lim, "from quantised rows")
+    assert B.fp8_linear(x, W).dtype == dtype
+    within(B.fp8_linear(x, W, out_dtype=F32), xq @ wq.t(), lim, "without a bias")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,F,N", [(1, 1000, 2000, 1000), (4, 7, 5, 3), (32, 203, 531, 96), (33, 203, 531, 96), (300, 1000, 264, 48), (5000, 72, 1001, 40)])
+def test_fp8_gated_feed_forward(dev, M, K, F, N, dtype):
+    for i, act in enumerate(B.ACTIVATIONS):
+        t = ffn_case(dev, M, K, F, N, dtype, bias=i % 2 == 0, seed=40 + i)
+        P = B.fp8_gated_weights(t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])
+        y = B.fp8_gated_feed_forward(t["x"], P, activation=act, out_dtype=F32)
+        r = {k: d64(v) for k, v in t.items()}
+        r["x"], r["wg"], r["wu"] = e4m3_64(t["x"], 1, 128), e4m3_64(t["wg"], 128, 128), e4m3_64(t["wu"], 128, 128)
+        wd = e4m3_64(t["wd"], 128, 128)
+        a, b, h, _ = ffn64({**r, "wd": wd}, act)
+        hq = e4m3_64(h, 1, 128)
+        ref = hq @ wd.t() + (0 if r["bd"] is None else r["bd"])
+        # h comes from float32 sums: where it lies that close to a border between two e4m3 values (or its block's maximum to a
+        # border between two scales) it may take the other one, a step of at most 2^-3 of |h|
+        xs = r["x"].abs()
+        ea = (K + 8) * E * 2 * (xs @ r["wg"].abs().t()) + 2 ** -19 * a.abs()
+        eb = (K + 8) * E * 2 * (xs @ r["wu"].abs().t())
+        eh = 1.13 * ea * b.abs() + act64(act, a).abs() * (eb + 2 ** -19 * b.abs()) + 2 ** -19 * h.abs()
+        lo, hi = e4m3_64(h - eh, 1, 128), e4m3_64(h + eh, 1, 128)
+        step = torch.maximum((lo - hq).abs(), (hi - hq).abs())
+        amax = h.abs().reshape(M, F)
+        for k0 in range(0, F, 128):                            # a block whose maximum is near a border of its scale: every value may move by a step
+            blk, err = amax[:, k0:k0 + 128].amax(1), eh[:, k0:k0 + 128].amax(1)
+            near = torch.ceil(torch.log2((blk + err).clamp(min=1e-300) / 448)) != torch.ceil(torch.log2((blk - err).clamp(min=1e-300) / 448))
+            step[near, k0:k0 + 128] = torch.maximum(step[near, k0:k0 + 128], hq[near, k0:k0 + 128].abs() * 2 ** -3 + blk[near, None] * 2 ** -15)
+        lim = step @ wd.abs().t() + (F + 8) * E * (hq.abs() @ wd.abs().t()) + 2 * E * ref.abs()
+        within(y, ref, lim, f"y ({act})")
+        # bfloat16: projections and result from the 8-bit pipe (its error above), so more of h may move by a step; which, the pipe decides:
+        # every value of h is given a step's chance in proportion to its error over the step, summed in squares (independent), 6 deviations
+        got = B.fp8_gated_feed_forward(t["x"], P, activation=act, out_dtype=BF)
+        if M <= 32:
+            within(got, ref, lim + U * ref.abs() * 1.01, f"bf16 y ({act})")
+            continue
+        pipe = math.sqrt(K) * 2.0 ** -15
+        pa, pb = (pipe * r["x"].abs().amax(1, keepdim=True) * r[k].abs().amax(1) for k in ("wg", "wu"))
+        eh = 1.13 * pa * b.abs() + act64(act, a).abs() * pb + eh
+        st = torch.maximum(hq.abs() * 2 ** -3, h.abs().amax(1, keepdim=True) * 2.0 ** -15)
+        var = (st * torch.minimum(st, eh) + 1e-300) @ (wd * wd).t()
+        pipe = 4 * pipe * math.sqrt(F / K) * hq.abs().amax(1, keepdim=True) * wd.abs().amax(1)
+        frob(got, ref, (var.sqrt().norm() * 3 + pipe.norm()).item() / ref.norm().item() + U, f"bf16 y ({act})")
+
+
+def test_fp8_non_finite_rows_stay_alone(dev):
+    for M in (20, 200):
+        t = ffn_case(dev, M, 200, 96, 40, BF, True, seed=5)
+        P, W = B.fp8_gated_weights(t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"]), B.fp8_weight(t["wg"])
+        x = t["x"].clone()
+        x[3, 71], x[7, 0] = float("nan"), float("inf")
+        keep = [i for i in range(M) if i not in (3, 7)]
+        for f in (lambda z: B.fp8_linear(z, W), lambda z: B.fp8_gated_feed_forward(z, P)):
+            base, y = f(t["x"]), f(x)
+            assert torch.equal(y[keep], base[keep]) and y[3].isnan().all() and y[7].isnan().all()
+
+
+def test_fp8_graph_replays_and_empty(dev):
+    t = ffn_case(dev, 100, 200, 264, 40, BF, True, seed=5)
+    P = B.fp8_gated_weights(t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])
+    x = t["x"].clone()
+    B.fp8_gated_feed_forward(x, P)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = B.fp8_gated_feed_forward(x, P)
+    for rep in range(4):
+        x.copy_(rnd(dev, 100, 200, seed=60 + rep, dtype=BF))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, B.fp8_gated_feed_forward(x.clone(), P)), rep
+    assert B.fp8_gated_feed_forward(x[:0], P).shape == (0, 40) and B.fp8_linear(x[:0], P.gate).shape == (0, 264)
+
+
+def test_block_run_together(dev):
+    """Two residual blocks as they are used: norm, feed-forward, norm + gate + residual + next norm; trained in float32 against
+    64-bit gradients, and evaluated in 8 bits."""
+    M, G, H, F = 192, 48, 72, 136
+    p = {}
+    for i in range(2):
+        t = ffn_case(dev, 1, H, F, H, F32, True, seed=200 + 20 * i)
+        p.update({f"{k}{i}": t[k] for k in ("wg", "wu", "wd", "bg", "bu", "bd")})
+        p[f"post{i}"] = 1 + rnd(dev, H, seed=300 + i, scale=0.1)
+    for i in range(3):
+        p[f"pre{i}"] = 1 + rnd(dev, H, seed=310 + i, scale=0.1)
+    p["x"], p["gate"] = rnd(dev, M, H, seed=320), 1 + rnd(dev, G, H, seed=321, scale=0.2)
+
+    def run(q, ffn, norm):
+        stream, n = norm(q["x"], None, None, 1.0, None, q["pre0"])
+        for i in range(2):
+            stream, n = norm(stream, ffn(n, i), q["gate"], 0.5, q[f"post{i}"], q[f"pre{i + 1}"])
+        return n
+
+    def own(q):
+        def norm(res, y, gate, s, w1, w2):
+            if y is None:
+                return B.norm_gate_residual(res, pre_norm="rms", pre_weight=w2)
+            return B.norm_gate_residual(res, y, gate=gate, scale=s, post_norm="rms", post_weight=w1, pre_norm="rms", pre_weight=w2)
+        return run(q, lambda n, i: B.gated_feed_forward(n, *[q[f"{k}{i}"] for k in ("wg", "wu", "wd", "bg", "bu", "bd")]), norm)
+
+    def ref(q):
+        def norm(res, y, gate, s, w1, w2):
+            v = res if y is None else res + s * gate.repeat(M // G, 1) * norm64(y, "rms", w1, None, 1e-6)
+            return v, norm64(v, "rms", w2, None, 1e-6)
+        return run(q, lambda n, i: ffn64({"x": n, **{k: q[f"{k}{i}"] for k in ("wg", "wu", "wd", "bg", "bu", "bd")}}, "silu")[3], norm)
+
+    leaves = {k: v.clone().requires_grad_(True) for k, v in p.items()}
+    refs = {k: v.double().requires_grad_(True) for k, v in p.items()}
+    d = rnd(dev, M, H, seed=330)
+    y, yr = own(leaves), ref(refs)
+    got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), d)))
+    want = dict(zip(refs, torch.autograd.grad(yr, list(refs.values()), d.double())))
+    depth = 2 * (2 * (4 + math.sqrt(H)) + 4 + math.sqrt(F) + 16) * E
+    frob(y, yr.detach(), depth, "two blocks")
+    for k in got:
+        frob(got[k], want[k], 8 * depth + 4 * E * math.sqrt(M), f"d{k}")
+    with torch.no_grad():
+        packed = [B.fp8_gated_weights(*[p[f"{k}{i}"] for k in ("wg", "wu", "wd", "bg", "bu", "bd")]) for i in range(2)]
+        stream, n = B.norm_gate_residual(p["x"], pre_weight=p["pre0"])
+        for i in range(2):
+            stream, n = B.norm_gate_residual(stream, B.fp8_gated_feed_forward(n, packed[i]), gate=p["gate"], scale=0.5, post_norm="rms", post_weight=p[f"post{i}"], pre_weight=p[f"pre{i + 1}"])
+    # e4m3 rounds to 2^-4 of a value (rms about a third of it): five roundings meet in a unit's result, damped by the residual sum
+    frob(n, yr.detach(), 2 * math.sqrt(5) * 2.0 ** -4, "two blocks in 8 bits")
