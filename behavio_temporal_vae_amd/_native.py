@@ -99,11 +99,11 @@ _SIGS = {
     "btvae_masked_scatter": [P, P, P, LL, P],
     "btvae_lse_over_k": [P, P, I, I, P],
     "btvae_pack_lower": [P, P, LL, I, P],
-    "btvae_block_pack": [P, I, LL, P, I, LL, LL, I, I, I, I, P],
-    "btvae_gated_proj_fwd": [P, LL, LL, P, P, LL, LL, P, P, I, P, LL, LL, P, LL, I, I, I, I, I, I, P],
-    "btvae_gated_proj_bwd": [P, LL, LL, P, LL, LL, P, LL, I, P, LL, LL, P, I, I, I, I, I, P],
-    "btvae_block_product": [P, LL, LL, P, LL, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],
-    "btvae_block_wgrad": [P, LL, LL, P, LL, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
+    "btvae_block_pack": [P, I, LL, P, I, LL, I, I, I, I, P],
+    "btvae_gated_proj_fwd": [P, LL, P, P, LL, P, P, I, P, LL, P, P, LL, I, I, I, I, I, I, P],
+    "btvae_gated_proj_bwd": [P, LL, P, LL, P, P, LL, I, P, LL, P, I, I, I, I, I, P],
+    "btvae_block_product": [P, LL, P, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],
+    "btvae_block_wgrad": [P, LL, P, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
     "btvae_block_colsum": [P, I, LL, P, LL, P, I, I, I, I, P],
     "btvae_block_strip_sums": [P, I, I, P, P, I, I, P],
     "btvae_few_rows": [P, LL, P, P, LL, P, P, P, LL, I, I, I, I, I, P],
@@ -136,7 +136,7 @@ _RET = {
     "btvae_guard_range_log2": (c_int, [I]),
     "btvae_guard_flags": (ctypes.POINTER(c_int), []),
     "btvae_next_row_pitches": (c_int, [I, I]),
-    "btvae_gated_proj_strips": (c_int, [I, I]),
+    "btvae_gated_proj_strips": (c_int, [I]),
     "btvae_block_product_ws": (c_longlong, [I, I, I, I]),
     "btvae_block_wgrad_ws": (c_longlong, [I, I, I, I]),
     "btvae_block_colsum_ws": (c_longlong, [I, I]),

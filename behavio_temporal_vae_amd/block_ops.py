@@ -98,48 +98,60 @@ def _refuse_capture(what):
 
 
 class _Operand:
-    """A matrix as the products read it: ``planes`` bf16 planes, rows on 16 bytes, ``width`` (a multiple of 8) columns of which those
-    beyond the matrix's own are zeros.  A bf16 matrix that is laid out so already is used in place."""
-    __slots__ = ("t", "ld", "plane", "width")
+    """A matrix as the products read it: bf16 (``planes`` 1), or float32 values as three bf16 pieces each, 96 bytes for every 16
+    columns (``planes`` 3); ``ld`` bytes to a row, rows on 16 bytes, ``width`` columns of which those beyond the matrix's own are zeros.  A
+    bf16 matrix that is laid out so already is used in place."""
+    __slots__ = ("t", "ld", "width")
 
-    def __init__(self, t, ld, plane, width):
-        self.t, self.ld, self.plane, self.width = t, ld, plane, width
+    def __init__(self, t, ld, width):
+        self.t, self.ld, self.width = t, ld, width
 
-    def ptr(self, offset=0):
-        return self.t.data_ptr() + 2 * offset
+    def ptr(self):
+        return self.t.data_ptr()
+
+
+def _row_bytes(cols, planes):
+    """Bytes of an operand row of ``cols`` columns (whole groups of 32, so that rows start on 64 bytes)."""
+    return _up(cols, 32) * (6 if planes == 3 else 2)
 
 
 def _fits(t):
     return t.dtype == torch.bfloat16 and t.shape[1] % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0
 
 
-def _pack_into(t, dst, planes, plane, ld, dst_cols, transpose, offset=0):
-    nv.call("btvae_block_pack", _p(t), int(t.dtype == torch.bfloat16), _pitch(t), dst.data_ptr() + 2 * offset, planes, plane, ld,
-            t.shape[0], t.shape[1], dst_cols, int(transpose))
+def _pack_into(t, dst, planes, ld, dst_cols, transpose, offset=0):
+    nv.call("btvae_block_pack", _p(t), int(t.dtype == torch.bfloat16), _pitch(t), dst.data_ptr() + offset, planes, ld, t.shape[0], t.shape[1], dst_cols, int(transpose))
 
 
-def _operand(t, planes) -> _Operand:
+def _packed(t, planes) -> _Operand:
     rows, cols = t.shape
-    if planes == 1 and _fits(t):
-        return _Operand(t, _pitch(t), 0, cols)
-    ld = _up(cols, 32)
-    dst = torch.empty(planes * rows * ld, dtype=torch.bfloat16, device=t.device)
-    _pack_into(t, dst, planes, rows * ld, ld, ld, False)
-    return _Operand(dst, ld, rows * ld, _up(cols, 8))
+    ld = _row_bytes(cols, planes)
+    dst = torch.empty(rows * ld, dtype=torch.uint8, device=t.device)
+    _pack_into(t, dst, planes, ld, _up(cols, 32), False)
+    return _Operand(dst, ld, _up(cols, 8))
 
 
-def _operand_pair(a, b, planes):
-    """Two matrices of one shape with a common pitch and plane distance."""
-    if planes == 1 and _fits(a) and _fits(b) and _pitch(a) == _pitch(b):
-        return _Operand(a, _pitch(a), 0, a.shape[1]), _Operand(b, _pitch(b), 0, b.shape[1])
-    rows, cols = a.shape
-    ld = _up(cols, 32)
-    out = []
-    for t in (a, b):
-        dst = torch.empty(planes * rows * ld, dtype=torch.bfloat16, device=t.device)
-        _pack_into(t, dst, planes, rows * ld, ld, ld, False)
-        out.append(_Operand(dst, ld, rows * ld, _up(cols, 8)))
-    return out
+REPACK_READS = 1024        # rows or columns of a product from which a bf16 matrix with rows off 64-byte boundaries is copied first
+
+
+def _in_place(t, planes, reads):
+    """May a product read ``t`` where it is?  Rows that do not start on 64 bytes cost the copies to LDS twice the requests (measured:
+    65,536 x 1000 times 1000 x 1024, 2000-byte rows 200 us, 2048-byte rows 154; the copy 55), so a matrix that is read against
+    ``reads`` others is laid out anew from ``REPACK_READS`` on."""
+    return planes == 1 and _fits(t) and (reads < REPACK_READS or (2 * _pitch(t) % 64 == 0 and t.data_ptr() % 64 == 0))
+
+
+def _operand(t, planes, reads) -> _Operand:
+    if _in_place(t, planes, reads):
+        return _Operand(t, 2 * _pitch(t), t.shape[1])
+    return _packed(t, planes)
+
+
+def _operand_pair(a, b, planes, reads):
+    """Two matrices of one shape with a common pitch."""
+    if _in_place(a, planes, reads) and _in_place(b, planes, reads) and _pitch(a) == _pitch(b):
+        return _Operand(a, 2 * _pitch(a), a.shape[1]), _Operand(b, 2 * _pitch(b), b.shape[1])
+    return _packed(a, planes), _packed(b, planes)
 
 
 def _workspace(floats, device):
@@ -148,7 +160,7 @@ def _workspace(floats, device):
 
 def _product(a: _Operand, b: _Operand, bias, out, planes, M, N, K):
     ws = _workspace(nv.lib().btvae_block_product_ws(M, N, K, planes) if M else 0, out.device)
-    nv.call("btvae_block_product", a.ptr(), a.ld, a.plane, b.ptr(), b.ld, b.plane, _p(bias), int(bias is not None and bias.dtype == torch.bfloat16),
+    nv.call("btvae_block_product", a.ptr(), a.ld, b.ptr(), b.ld, _p(bias), int(bias is not None and bias.dtype == torch.bfloat16),
             _p(out), _pitch(out), int(out.dtype == torch.bfloat16), _p(ws), ws.numel() if ws is not None else 0, planes, M, N, K)
     return out
 
@@ -157,9 +169,9 @@ def _product(a: _Operand, b: _Operand, bias, out, planes, M, N, K):
 class GatedTape:
     """What the backward pass of one ``gated_feed_forward`` needs: the inputs, both projections, h."""
 
-    def __init__(self, x, weights, biases, act, planes, X, H, GU, half):
+    def __init__(self, x, weights, biases, act, planes, X, H, GU, GU_lo, half):
         self.x, self.weights, self.biases, self.act, self.planes = x, weights, biases, act, planes
-        self.X, self.H, self.GU, self.half = X, H, GU, half
+        self.X, self.H, self.GU, self.GU_lo, self.half = X, H, GU, GU_lo, half
 
     def backward(self, dy, need_input=True, need_weights=True, outs=None, accumulate=False):
         """Gradients (x, w_gate, w_up, w_down, b_gate, b_up, b_down) for the gradient ``dy`` of the result; entries that are
@@ -178,30 +190,28 @@ class GatedTape:
             accumulate = False
         dwg, dwu, dwd, dbg, dbu, dbd = outs
         acc = int(accumulate)
-        DY = _operand(dy, planes)
-        ldt = _up(N, 32)
-        WdT = torch.empty(planes * F * ldt, dtype=torch.bfloat16, device=dev)
-        _pack_into(w_down, WdT, planes, F * ldt, ldt, ldt, True)
-        dGU = torch.empty(planes * M * 2 * half, dtype=torch.bfloat16, device=dev)
-        d_plane = M * 2 * half
+        DY = _operand(dy, planes, F)
+        ldt, ldg = _row_bytes(N, planes), 2 * _row_bytes(F, planes)
+        WdT = torch.empty(F * ldt, dtype=torch.uint8, device=dev)
+        _pack_into(w_down, WdT, planes, ldt, _up(N, 32), True)
+        dGU = _Operand(torch.empty(M * ldg, dtype=torch.uint8, device=dev), ldg, 2 * half)
         want_bias = need_weights and (dbg is not None or dbu is not None)
-        strips = lib.btvae_gated_proj_strips(M, F) if M else 0
+        strips = lib.btvae_gated_proj_strips(M) if M else 0
         colpart = _workspace(strips * 2 * F, dev) if want_bias else None
-        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, DY.plane, _p(WdT), ldt, F * ldt, _p(self.GU), 2 * half, half, _p(dGU), 2 * half, d_plane,
-                _p(colpart), planes, self.act, M, F, DY.width)
+        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, _p(WdT), ldt, _p(self.GU), _p(self.GU_lo), 2 * half, half, dGU.ptr(), ldg, _p(colpart), planes, self.act, M, F, DY.width)
         dx = None
         if need_input:
             dx = torch.empty(M, K, dtype=x.dtype, device=dev)
-            WT = torch.empty(planes * K * 2 * half, dtype=torch.bfloat16, device=dev)
+            WT = torch.empty(K * ldg, dtype=torch.uint8, device=dev)
             for i, w in enumerate((w_gate, w_up)):
-                _pack_into(w, WT, planes, K * 2 * half, 2 * half, half, True, i * half)
-            _product(_Operand(dGU, 2 * half, d_plane, 2 * half), _Operand(WT, 2 * half, K * 2 * half, 2 * half), None, dx, planes, M, K, 2 * half)
+                _pack_into(w, WT, planes, ldg, half, True, i * (ldg // 2))
+            _product(dGU, _Operand(WT, ldg, 2 * half), None, dx, planes, M, K, 2 * half)
         if not need_weights:
             return (dx,) + (None,) * 6
         ws = _workspace(max(lib.btvae_block_wgrad_ws(2 * half, K, M, planes), lib.btvae_block_wgrad_ws(N, F, M, planes)), dev)
-        nv.call("btvae_block_wgrad", _p(dGU), 2 * half, d_plane, self.X.ptr(), self.X.ld, self.X.plane, _p(ws), ws.numel(),
+        nv.call("btvae_block_wgrad", dGU.ptr(), ldg, self.X.ptr(), self.X.ld, _p(ws), ws.numel(),
                 _p(dwg), F, _p(dwu), half, F, K, int(dwg.dtype == torch.bfloat16), acc, planes, 2 * half, K, M)
-        nv.call("btvae_block_wgrad", DY.ptr(), DY.ld, DY.plane, _p(self.H), half, M * half, _p(ws), ws.numel(),
+        nv.call("btvae_block_wgrad", DY.ptr(), DY.ld, self.H.ptr(), self.H.ld, _p(ws), ws.numel(),
                 _p(dwd), N, None, 0, 0, F, int(dwd.dtype == torch.bfloat16), acc, planes, N, F, M)
         if want_bias:
             first, second = (dbg, dbu) if dbg is not None else (torch.empty_like(dbu), dbu)
@@ -240,17 +250,18 @@ def _ffn_forward(x2, weights, biases, act, planes, out_dtype, keep):
     b_gate, b_up, b_down = biases
     dev, (M, K), F, N = x2.device, x2.shape, w_gate.shape[0], w_down.shape[0]
     half = _up(F, 32)
-    X = _operand(x2, planes)
-    Wg, Wu = _operand_pair(w_gate, w_up, planes)
-    H = torch.empty(planes * M * half, dtype=torch.bfloat16, device=dev)
-    GU = torch.empty(M * 2 * half, dtype=torch.float32 if planes == 3 else torch.bfloat16, device=dev) if keep else None
+    X = _operand(x2, planes, 2 * F)
+    Wg, Wu = _operand_pair(w_gate, w_up, planes, M)
+    H = _Operand(torch.empty(M * _row_bytes(F, planes), dtype=torch.uint8, device=dev), _row_bytes(F, planes), _up(F, 8))
+    GU = torch.empty(M * 2 * half, dtype=torch.float32 if planes == 3 else torch.int16, device=dev) if keep else None
+    GU_lo = torch.empty(M * 2 * half, dtype=torch.uint8, device=dev) if keep and planes == 1 else None
     bias16 = int(any(b is not None and b.dtype == torch.bfloat16 for b in (b_gate, b_up)))
-    nv.call("btvae_gated_proj_fwd", X.ptr(), X.ld, X.plane, Wg.ptr(), Wu.ptr(), Wg.ld, Wg.plane, _p(b_gate), _p(b_up), bias16,
-            _p(H), half, M * half, _p(GU), 2 * half, half, planes, act, M, F, X.width)
+    nv.call("btvae_gated_proj_fwd", X.ptr(), X.ld, Wg.ptr(), Wu.ptr(), Wg.ld, _p(b_gate), _p(b_up), bias16,
+            H.ptr(), H.ld, _p(GU), _p(GU_lo), 2 * half, half, planes, act, M, F, X.width)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
-    Wd = _operand(w_down, planes)
-    _product(_Operand(H, half, M * half, Wd.width), Wd, b_down, y, planes, M, N, Wd.width)
-    return y, GatedTape(x2, weights, biases, act, planes, X, H, GU, half) if keep else None
+    Wd = _operand(w_down, planes, M)
+    _product(H, Wd, b_down, y, planes, M, N, Wd.width)
+    return y, GatedTape(x2, weights, biases, act, planes, X, H, GU, GU_lo, half) if keep else None
 
 
 def _ffn_few(x2, weights, biases, act):
@@ -283,7 +294,7 @@ class _GatedNode(torch.autograd.Function):
         x2, w_gate, w_up, w_down, b_gate, b_up, b_down = ctx.saved_tensors
         need = ctx.needs_input_grad
         t = ctx.tape
-        tape = GatedTape(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], t.act, t.planes, t.X, t.H, t.GU, t.half)
+        tape = GatedTape(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], t.act, t.planes, t.X, t.H, t.GU, t.GU_lo, t.half)
         return (None, *tape.backward(dy, need_input=need[1], need_weights=any(need[2:])))
 
 
@@ -318,24 +329,24 @@ def gated_feed_forward_tape(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_d
 class NormTape:
     """What the backward pass of one ``norm_gate_residual`` needs."""
 
-    def __init__(self, stream, branch, gate, scale, scale_vec, vectors, post, pre, stats):
-        self.stream, self.branch, self.gate, self.scale, self.scale_vec = stream, branch, gate, scale, scale_vec
+    def __init__(self, residual, branch, gate, scale, scale_vec, vectors, post, pre, stats):
+        self.residual, self.branch, self.gate, self.scale, self.scale_vec = residual, branch, gate, scale, scale_vec
         self.vectors, self.post, self.pre, self.stats = vectors, post, pre, stats
 
     def backward(self, d_stream=None, d_normed=None, need=(True,) * 8):
         """Gradients (residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias) for the gradients of stream and
         normed (None: zero), rows as [M, N]; entries not wanted or of absent tensors are None."""
-        stream, branch, gate = self.stream, self.branch, self.gate
-        (M, N), dev = stream.shape, stream.device
+        residual, branch, gate = self.residual, self.branch, self.gate
+        (M, N), dev = residual.shape, residual.device
         nv.ensure_device(dev)
         if d_stream is not None:
-            d_stream = _matrix(d_stream.reshape(M, N), "the gradient of stream", (M, N), stream.dtype, dev).contiguous()
-        ntype = branch.dtype if branch is not None else stream.dtype
+            d_stream = _matrix(d_stream.reshape(M, N), "the gradient of stream", (M, N), residual.dtype, dev).contiguous()
+        ntype = branch.dtype if branch is not None else residual.dtype
         if d_normed is not None:
             if not self.pre:
                 raise ValueError("a gradient of normed, which was not asked for")
             d_normed = _matrix(d_normed.reshape(M, N), "the gradient of normed", (M, N), ntype, dev).contiguous()
-        like = (stream, branch, gate, self.scale_vec, *self.vectors)
+        like = (residual, branch, gate, self.scale_vec, *self.vectors)
         outs = [torch.empty_like(t) if t is not None and w else None for t, w in zip(like, need)]
         if d_normed is None:
             for i in (6, 7):
@@ -344,9 +355,9 @@ class NormTape:
         lib, G = nv.lib(), gate.shape[0] if gate is not None else 0
         ws = _workspace(lib.btvae_norm_gate_residual_ws(M, N, G), dev)
         w1, c1, w2, _ = self.vectors
-        nv.call("btvae_norm_gate_residual_bwd", _p(d_stream), _p(d_normed), _p(stream), _p(branch), _p(gate), G, self.scale, _p(self.scale_vec),
+        nv.call("btvae_norm_gate_residual_bwd", _p(d_stream), _p(d_normed), _p(residual), _p(branch), _p(gate), G, self.scale, _p(self.scale_vec),
                 _p(w1), _p(c1), _p(w2), self.post, self.pre, _p(self.stats), *[_p(o) for o in outs], _p(ws), ws.numel() if ws is not None else 0,
-                _types(stream, ntype), M, N)
+                _types(residual, ntype), M, N)
         return tuple(outs)
 
 
@@ -363,7 +374,7 @@ def _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, 
     w1, c1, w2, c2 = vectors
     nv.call("btvae_norm_gate_residual_fwd", _p(residual), _p(branch), _p(gate), gate.shape[0] if gate is not None else 0, scale, _p(scale_vec),
             _p(w1), _p(c1), _p(w2), _p(c2), post, pre, eps, _p(stream), _p(normed), _p(stats), _types(residual, ntype), M, N)
-    tape = NormTape(stream if branch is not None else residual, branch, gate, scale, scale_vec, vectors, post, pre, stats) if keep else None
+    tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, stats) if keep else None
     return stream, normed, tape
 
 
@@ -373,8 +384,7 @@ class _NormNode(torch.autograd.Function):
         stream, normed, tape = _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, eps, True)
         ctx.meta = (scale, post, pre, tape.stats)
         ctx.has = (branch is not None, pre != 0)
-        # (the gradient does not read the residual when there is a branch: the stream stands for both)
-        ctx.save_for_backward(stream if branch is not None else residual, branch, gate, scale_vec, *vectors)
+        ctx.save_for_backward(residual, branch, gate, scale_vec, *vectors)
         ctx.set_materialize_grads(False)
         return tuple(t for t in (stream, normed) if t is not None)
 
@@ -382,14 +392,14 @@ class _NormNode(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *grads):
         _refuse_capture("norm_gate_residual")
-        stream, branch, gate, scale_vec, *vectors = ctx.saved_tensors
+        residual, branch, gate, scale_vec, *vectors = ctx.saved_tensors
         scale, post, pre, stats = ctx.meta
         grads = list(grads)
         d_stream = grads.pop(0) if ctx.has[0] else None
         d_normed = grads.pop(0) if ctx.has[1] else None
         if d_stream is None and d_normed is None:
             return (None,) * 12
-        tape = NormTape(stream, branch, gate, scale, scale_vec, vectors, post, pre, stats)
+        tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, stats)
         return (None, None, None, None, *tape.backward(d_stream, d_normed, need=ctx.needs_input_grad[4:]))
 
 
@@ -492,7 +502,7 @@ class Fp8Rows:
         rows, ld = self.q.shape
         out = torch.empty(rows, ld, dtype=torch.bfloat16, device=self.device)
         nv.call("btvae_fp8_expand", _p(self.q), ld, _p(self.scales), self.scales.shape[1], self.blocks, _p(out), ld, rows, self.shape[-1])
-        return _Operand(out, ld, 0, ld)
+        return _Operand(out, 2 * ld, ld)
 
 
 class Fp8Weight(Fp8Rows):
@@ -607,8 +617,6 @@ def fp8_gated_weights(w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None)
         raise ValueError(f"weights do not fit together: {list(gate.shape)}, {list(up.shape)}, {list(down.shape)}")
     if up.device != gate.device or down.device != gate.device:
         raise RuntimeError("the weights are on different devices")
-    if gate.shape[1] > 128 * FP8_BLOCK:
-        raise ValueError(f"8-bit gated weights support up to {128 * FP8_BLOCK} input columns, got {gate.shape[1]}")
     F, N = gate.shape[0], down.shape[0]
     return Fp8GatedWeights(gate, up, down, _fp8_bias(b_gate, "b_gate", F, gate.device), _fp8_bias(b_up, "b_up", F, gate.device), _fp8_bias(b_down, "b_down", N, gate.device))
 
@@ -644,7 +652,7 @@ def fp8_gated_feed_forward(x, weights: Fp8GatedWeights, activation="silu", out_d
         hq, hs = _fp8_buffers(M, F, M, dev)
         if dtype == torch.float32:
             X, Wg, Wu = xq._expanded(), w.gate._expanded(), w.up._expanded()
-            operands = (X.ptr(), X.ld, None, 0, Wg.ptr(), None, Wu.ptr(), None, Wg.ld, 0, 1)
+            operands = (X.ptr(), X.width, None, 0, Wg.ptr(), None, Wu.ptr(), None, Wg.width, 0, 1)
         else:
             operands = (_p(xq.q), xq.q.shape[1], _p(xq.scales), xq.scales.shape[1], _p(w.gate.q), _p(w.gate.scales), _p(w.up.q), _p(w.up.scales),
                         w.gate.q.shape[1], w.gate.scales.shape[1], 0)

@@ -3,35 +3,59 @@
 //
 //   a = x Wg^T + bg,  b = x Wu^T + bu,  h = act(a) b,  y = h Wd^T + bd
 //   dh = dy Wd,  da = dh b act'(a),  db = dh act(a),  dx = [da db] [Wg; Wu],  d[Wg; Wu] = [da db]^T x,  dWd = dy^T h
-#include "block_gemm.h"
-#include <algorithm>
+#include "block_launch.h"
 
 using namespace btvae;
 namespace bk = btvae_block;
 
 namespace btvae_block {
 
-// ---- operands -> bf16 planes ------------------------------------------------------------------------------------------
-// dst[plane][r][c] = piece of src[r][c], zeros for cols <= c < dst_cols; eight columns to a thread.
-template <bool SRC16, int NP>
-__global__ __launch_bounds__(256) void pack_rows(const void* __restrict__ src, long long ld, unsigned short* __restrict__ dst, long long plane, long long dld,
-                                                 int rows, int cols, int groups) {
+// 8 consecutive values from element offset o, of which `left` exist (zeros behind them); any alignment of whole elements
+template <bool SRC16> __device__ __forceinline__ void load8(const void* src, long long o, int left, float (&v)[8]) {
+    if (left >= 8) {
+        if (SRC16) {
+            const u32x4 u = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<const unsigned short*>(src) + o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[2 * e] = bf_lo(u[e]); v[2 * e + 1] = bf_hi(u[e]); }
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4_any*>(reinterpret_cast<const float*>(src) + o), b = *reinterpret_cast<const f32x4_any*>(reinterpret_cast<const float*>(src) + o + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? (SRC16 ? bf_load(src, o + e) : reinterpret_cast<const float*>(src)[o + e]) : 0.f;
+}
+
+// ---- operands ---------------------------------------------------------------------------------------------------------
+// 8 columns c .. c + 7 of a row, as bf16 or split
+template <bool SPLIT> __device__ __forceinline__ void put_operand(char* row, int c, const float (&v)[8]) {
+    if constexpr (SPLIT) {
+        u32x4 p[3];
+        split8(v, p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4*>(row + split_at(c, k)) = p[k];
+    } else {
+        *reinterpret_cast<u32x4*>(row + 2LL * c) = pack8(v);
+    }
+}
+// dst[r][c] = src[r][c], zeros for cols <= c < dst_cols; eight columns to a thread, `dld` bytes to a row
+template <bool SRC16, bool SPLIT>
+__global__ __launch_bounds__(256) void pack_rows(const void* __restrict__ src, long long ld, char* __restrict__ dst, long long dld, int rows, int cols, int groups) {
     const long long total = (long long)rows * groups;
     for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < total; g += (long long)gridDim.x * 256) {
         const long long r = g / groups;
         const int c = (int)(g - r * groups) * 8;
         float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = c + e < cols ? (SRC16 ? bf_load(src, r * ld + c + e) : reinterpret_cast<const float*>(src)[r * ld + c + e]) : 0.f;
-        store_planes8(dst, plane, NP, r * dld + c, v);
+        load8<SRC16>(src, r * ld + c, cols - c, v);
+        put_operand<SPLIT>(dst + r * dld, c, v);
     }
 }
 
-// dst[plane][c][r] = piece of src[r][c] for c < cols, zeros for rows <= r < dst_cols: 64 x 64 tiles through LDS.
-template <bool SRC16, int NP>
-__global__ __launch_bounds__(256) void pack_transposed(const void* __restrict__ src, long long ld, unsigned short* __restrict__ dst, long long plane, long long dld,
-                                                       int rows, int cols, int dst_cols) {
+// dst[c][r] = src[r][c] for c < cols, zeros for rows <= r < dst_cols: 64 x 64 tiles through LDS.
+template <bool SRC16, bool SPLIT>
+__global__ __launch_bounds__(256) void pack_transposed(const void* __restrict__ src, long long ld, char* __restrict__ dst, long long dld, int rows, int cols, int dst_cols) {
     __shared__ float t[64][65];
     const int r0 = (int)blockIdx.x * 64, c0 = (int)blockIdx.y * 64;
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
@@ -45,7 +69,7 @@ __global__ __launch_bounds__(256) void pack_transposed(const void* __restrict__ 
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = t[rg + e][c];
-        store_planes8(dst, plane, NP, (long long)(c0 + c) * dld + r0 + rg, v);
+        put_operand<SPLIT>(dst + (long long)(c0 + c) * dld, r0 + rg, v);
     }
 }
 
@@ -123,7 +147,7 @@ __global__ __launch_bounds__(256) void strip_sums(const float* __restrict__ part
 // ---- 8-bit quantisation -----------------------------------------------------------------------------------------------
 // Rows: one power-of-two scale for each row and 128 columns; 16 lanes x 8 values to a block.  Scaling by a power of two is
 // exact, so the only rounding is the one to e4m3.  A non-finite value becomes NaN and takes no part in its block's maximum.
-template <bool SRC16, bool VEC>
+template <bool SRC16>
 __global__ __launch_bounds__(256) void quantize_rows(const void* __restrict__ src, long long ld, unsigned char* __restrict__ q, long long ldq,
                                                      unsigned char* __restrict__ sc, long long scp, int rows, int K, int kb_n) {
     const long long total = (long long)rows * kb_n;
@@ -131,26 +155,7 @@ __global__ __launch_bounds__(256) void quantize_rows(const void* __restrict__ sr
         const long long r = g / kb_n;
         const int kb = (int)(g - r * kb_n), k = kb * 128 + (threadIdx.x & 15) * 8;
         float v[8];
-        if (VEC) {
-            if (k < K) {
-                if (SRC16) {
-                    const u32x4 u = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(src) + r * ld + k);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { v[2 * e] = bf_lo(u[e]); v[2 * e + 1] = bf_hi(u[e]); }
-                } else {
-                    const f32x4 a = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + r * ld + k);
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + r * ld + k + 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? (SRC16 ? bf_load(src, r * ld + k + e) : reinterpret_cast<const float*>(src)[r * ld + k + e]) : 0.f;
-        }
+        load8<SRC16>(src, r * ld + k, K - k, v);
         float mx = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, finite_abs(v[e]));
@@ -171,11 +176,7 @@ __global__ __launch_bounds__(256) void quantize_blocks(const void* __restrict__ 
                                                        unsigned char* __restrict__ sc, long long scp, int N, int K) {
     __shared__ float red[4];
     const int n0 = (int)blockIdx.y * 128, k = (int)blockIdx.x * 128 + (threadIdx.x & 15) * 8;
-    auto load = [&](int n, float (&v)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = n < N && k + e < K ? (SRC16 ? bf_load(src, (long long)n * ld + k + e) : reinterpret_cast<const float*>(src)[(long long)n * ld + k + e]) : 0.f;
-    };
+    auto load = [&](int n, float (&v)[8]) { load8<SRC16>(src, (long long)n * ld + k, n < N ? K - k : 0, v); };
     float mx = 0.f, v[8];
     for (int i = threadIdx.x >> 4; i < 128; i += 16) {
         load(n0 + i, v);
@@ -425,7 +426,8 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
         if (GATED) {
             if (p.bias2) u += p.bias_bf16 ? bf_load(p.bias2, nn) : reinterpret_cast<const float*>(p.bias2)[nn];
             float a, d;
-            act_value<false>(p.act, v, a, d);
+            if (p.act == ACT_GELU) act_value<false, true>(p.act, v, a, d);
+            else act_value<false, false>(p.act, v, a, d);
             v = a * u;
         }
         const long long o = (long long)m * p.ldc + nn;
@@ -435,11 +437,6 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
-constexpr int CHIP = 256;                                             // compute units
-
-inline int tiles(int n, int t) { return (n + t - 1) / t; }
-inline bool al16(const void* q) { return ((uintptr_t)q & 15) == 0; }
-
 // Splits of a reduction of `stages` stages over fewer tiles than compute units: as many as fill the chip about once, each at least
 // 12 stages long (the ring's fill and the slab's write and read cost about that much).
 inline int row_splits(int T, int stages, int unit) {
@@ -447,44 +444,25 @@ inline int row_splits(int T, int stages, int unit) {
     int z = std::min(CHIP / T, stages / std::max(12, unit));
     return std::max(1, std::min(z, 32));
 }
-inline int use_big(int M, int N, int colspan) { return tiles(M, 256) * tiles(N, colspan) >= CHIP * 3 / 4; }
 
-template <int FMT, int EP>
-static int launch_rows(Args& p, int shape, int z, hipStream_t s, const char* what) {
-    // shape 0: 256 x 256, 1: 128 x 128, 2: 128 x 256
-    const int tm = shape == 0 ? 256 : 128, tn = (shape == 1 ? 128 : 256) / (EP == EP_GATED ? 2 : 1);
-    p.tiles_m = tiles(p.M, tm); p.tiles_n = tiles(p.N, tn);
-    const long long T = (long long)p.tiles_m * p.tiles_n;
-    if (T > 0x7fffffffLL) return set_error("%s: too many tiles", what);
-    const dim3 grid((unsigned)T, 1, (unsigned)z);
-    if (shape == 0) hipLaunchKernelGGL((gemm_rows<FMT, EP, 4, 2, 4>), grid, dim3(512), 0, s, p);
-    else if (shape == 1) {
-        if constexpr (!(FMT == FMT_E4M3 && EP == EP_GATED)) hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, 2, 2>), grid, dim3(256), 0, s, p);
-    } else {
-        if constexpr (EP == EP_GATED) hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, 2, 4>), grid, dim3(256), 0, s, p);
-    }
-    return check_launch(what);
-}
-
-struct ProductPlan { int shape, z, kz; };
-// EP_LINEAR: tile shape and splits; `unit`: a split is a multiple of that many stages; `max_stages`: longest split (e4m3: its scales' room)
-static ProductPlan plan_product(int M, int N, int stages, int unit, int max_stages) {
+struct ProductPlan { int z, kz; };
+// EP_LINEAR: splits of the reduction, each a multiple of `unit` stages
+static ProductPlan plan_product(int M, int N, int stages, int unit) {
     ProductPlan r;
-    r.shape = use_big(M, N, 256) ? 0 : 1;
-    const int T = r.shape == 0 ? tiles(M, 256) * tiles(N, 256) : tiles(M, 128) * tiles(N, 128);
-    int z = std::max(row_splits(T, stages, unit), tiles(stages, max_stages));
-    r.kz = tiles(tiles(stages, z), unit) * unit;
+    r.kz = tiles(tiles(stages, row_splits(tiles(M, 128) * tiles(N, 128), stages, unit)), unit) * unit;
     r.z = tiles(stages, r.kz);
     return r;
 }
 struct ColPlan { int big, z, rz; };
 static ColPlan plan_cols(int M, int N, int R, int planes) {
     ColPlan r;
+    // 256 x 256 tiles from where their splits fill the chip (measured at 65,536 rows, 4032 x 1000: bf16 773 us against 978 with 128 x 128 tiles)
     r.big = tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
     const int t = r.big ? 256 : 128;
     const int T = tiles(M, t) * tiles(N, t);
     // fill the chip; a split has at least 256 rows, and multiples of eight splits keep one row range on one XCD
-    int z = std::max(1, std::min((T >= CHIP ? 1 : CHIP / T), tiles(R, 256)));
+    const int fill = r.big ? CHIP : 2 * CHIP;
+    int z = std::max(1, std::min((T >= fill ? 1 : fill / T), tiles(R, 256)));
     if (z > 8) z = z / 8 * 8;
     const int cap = 1 << 20;                                          // rows of a split
     z = std::max(z, tiles(R, cap));
@@ -497,111 +475,111 @@ static ColPlan plan_cols(int M, int N, int R, int planes) {
 
 #define BLK_STREAM(s) reinterpret_cast<hipStream_t>(s)
 
-static bool operand_ok(const void* p, long long ld, long long plane, int planes) {
-    return bk::al16(p) && (ld & 7) == 0 && (planes == 1 || (plane & 7) == 0);
+// Operand matrices: bf16 (planes 1), or split (planes 3: 96 bytes for every 16 columns).  `ld` bytes to a row, rows on 16 bytes.
+static bool operand_ok(const void* p, long long ld, int planes, int cols) {
+    return bk::al16(p) && (ld & 15) == 0 && ld >= (planes == 3 ? (long long)bk::tiles(cols, 16) * 96 : 2LL * cols);
 }
+static int stages_of(int K, int planes) { return planes == 3 ? bk::tiles(K, 16) : bk::tiles(K, 64); }
 
-// dst[plane][row][0 .. dst_cols) = bf16 pieces of src (planes 1: rounded; 3: exact), zero-padded; transpose: of src^T.
-BTVAE_API int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long plane, long long dst_ld, int rows, int cols, int dst_cols,
-                               int transpose, void* stream) {
+// dst = src as an operand (transpose: of its transpose), zeros up to dst_cols columns (a multiple of 16)
+BTVAE_API int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long dst_ld, int rows, int cols, int dst_cols, int transpose, void* stream) {
     BTVAE_REQUIRE(planes == 1 || planes == 3, "block_pack: planes must be 1 or 3");
     BTVAE_REQUIRE(rows >= 0 && cols > 0 && ld >= cols, "block_pack: bad source shape");
-    BTVAE_REQUIRE((dst_cols & 7) == 0 && dst_cols >= (transpose ? rows : cols) && dst_ld >= dst_cols && operand_ok(dst, dst_ld, plane, planes), "block_pack: bad destination layout");
+    BTVAE_REQUIRE((dst_cols & 15) == 0 && dst_cols >= (transpose ? rows : cols) && operand_ok(dst, dst_ld, planes, dst_cols), "block_pack: bad destination layout");
     if (rows == 0 && !transpose) return 0;
     hipStream_t s = BLK_STREAM(stream);
-    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+    char* d = (char*)dst;
     if (!transpose) {
         const int groups = dst_cols / 8;
-        const long long need = ((long long)rows * groups + 255) / 256;
-        const unsigned grid = (unsigned)std::min<long long>(need, 16384);
+        const unsigned grid = (unsigned)std::min<long long>(((long long)rows * groups + 255) / 256, 16384);
         if (src_bf16) {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<true, 1>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
-            else hipLaunchKernelGGL((bk::pack_rows<true, 3>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<true, false>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
+            else hipLaunchKernelGGL((bk::pack_rows<true, true>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
         } else {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<false, 1>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
-            else hipLaunchKernelGGL((bk::pack_rows<false, 3>), dim3(grid), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, groups);
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<false, false>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
+            else hipLaunchKernelGGL((bk::pack_rows<false, true>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
         }
     } else {
         const unsigned gx = (unsigned)bk::tiles(dst_cols, 64), gy = (unsigned)bk::tiles(cols, 64);
         BTVAE_REQUIRE(gy <= 65535, "block_pack: too many columns");
         if (src_bf16) {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<true, 1>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
-            else hipLaunchKernelGGL((bk::pack_transposed<true, 3>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<true, false>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
+            else hipLaunchKernelGGL((bk::pack_transposed<true, true>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
         } else {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<false, 1>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
-            else hipLaunchKernelGGL((bk::pack_transposed<false, 3>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, plane, dst_ld, rows, cols, dst_cols);
+            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<false, false>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
+            else hipLaunchKernelGGL((bk::pack_transposed<false, true>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
         }
     }
     return check_launch("block_pack");
 }
 
-BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, long long x_plane, const void* Wg, const void* Wu, long long ldw, long long w_plane,
-                                   const void* bg, const void* bu, int bias_bf16, void* H, long long ldh, long long h_plane, void* GU, long long ldgu, int gu_half,
-                                   int planes, int act, int M, int F, int K, void* stream) {
-    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_fwd: planes must be 1 or 3");
-    BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0 && (K & 7) == 0, "gated_proj_fwd: bad sizes (M %d, F %d, K %d)", M, F, K);
-    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_fwd: unknown activation %d", act);
-    const int F8 = (F + 7) / 8 * 8;
-    BTVAE_REQUIRE(operand_ok(X, ldx, x_plane, planes) && ldx >= K && operand_ok(Wg, ldw, w_plane, planes) && operand_ok(Wu, ldw, w_plane, planes) && ldw >= K, "gated_proj_fwd: operand rows must start on 16 bytes");
-    BTVAE_REQUIRE(operand_ok(H, ldh, h_plane, planes) && ldh >= F8, "gated_proj_fwd: bad layout of H");
-    BTVAE_REQUIRE(!GU || (bk::al16(GU) && (ldgu & 7) == 0 && (gu_half & 7) == 0 && gu_half >= F8 && ldgu >= gu_half + F8), "gated_proj_fwd: bad layout of the kept projections");
-    if (M == 0) return 0;
-    bk::Args p = {};
-    p.A = (const char*)X; p.lda = ldx * 2; p.a_plane = x_plane * 2;
-    p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw * 2; p.b_plane = w_plane * 2;
-    p.M = M; p.N = F; p.K = K; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(K, 32); p.kz = p.pairs * p.ks;
-    p.bias = bg; p.bias2 = bu; p.bias_bf16 = bias_bf16;
-    p.C = H; p.ldc = ldh; p.c_plane = h_plane; p.c_type = planes == 3 ? bk::T_PLANES : bk::T_BF16;
-    p.act = act; p.gu = GU; p.ldgu = ldgu; p.gu_half = gu_half; p.gu_f32 = planes == 3;
-    ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
-    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, bk::use_big(M, F, 128) ? 0 : 1, 1, BLK_STREAM(stream), "gated_proj_fwd");
+static bool kept_ok(const void* GU, const void* GU_lo, long long ldgu, int gu_half, int planes, int F) {
+    return bk::al16(GU) && (planes == 3 || (GU_lo && bk::al16(GU_lo))) && (ldgu & 15) == 0 && (gu_half & 31) == 0 && gu_half >= F && ldgu >= 2LL * gu_half;
 }
 
-BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, long long dy_plane, const void* WdT, long long ldw, long long w_plane, const void* GU, long long ldgu, int gu_half,
-                                   void* dGU, long long ldd, long long d_plane, float* colpart, int planes, int act, int M, int F, int N, void* stream) {
-    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_bwd: planes must be 1 or 3");
-    BTVAE_REQUIRE(M >= 0 && F > 0 && N > 0 && (N & 7) == 0, "gated_proj_bwd: bad sizes (M %d, F %d, N %d)", M, F, N);
-    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_bwd: unknown activation %d", act);
-    const int F8 = (F + 7) / 8 * 8;
-    BTVAE_REQUIRE(operand_ok(dY, lddy, dy_plane, planes) && lddy >= N && operand_ok(WdT, ldw, w_plane, planes) && ldw >= N, "gated_proj_bwd: operand rows must start on 16 bytes");
-    BTVAE_REQUIRE(bk::al16(GU) && (ldgu & 7) == 0 && (gu_half & 7) == 0 && gu_half >= F8 && ldgu >= gu_half + F8, "gated_proj_bwd: bad layout of the kept projections");
-    BTVAE_REQUIRE(operand_ok(dGU, ldd, d_plane, planes) && ldd >= gu_half + F8, "gated_proj_bwd: bad layout of the gradients");
+BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu, int bias_bf16,
+                                   void* H, long long ldh, void* GU, void* GU_lo, long long ldgu, int gu_half, int planes, int act, int M, int F, int K, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_fwd: planes must be 1 or 3");
+    BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0 && (planes == 3 || (K & 7) == 0), "gated_proj_fwd: bad sizes (M %d, F %d, K %d)", M, F, K);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_fwd: unknown activation %d", act);
     if (M == 0) return 0;
+    BTVAE_REQUIRE(operand_ok(X, ldx, planes, K) && operand_ok(Wg, ldw, planes, K) && operand_ok(Wu, ldw, planes, K), "gated_proj_fwd: bad operand layout");
+    BTVAE_REQUIRE(operand_ok(H, ldh, planes, bk::tiles(F, 16) * 16), "gated_proj_fwd: bad layout of H");
+    BTVAE_REQUIRE(!GU || kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_fwd: bad layout of the kept projections");
     bk::Args p = {};
-    p.A = (const char*)dY; p.lda = lddy * 2; p.a_plane = dy_plane * 2;
-    p.B = (const char*)WdT; p.ldb = ldw * 2; p.b_plane = w_plane * 2;
-    p.M = M; p.N = F; p.K = N; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(N, 32); p.kz = p.pairs * p.ks;
-    p.C = dGU; p.ldc = ldd; p.c_plane = d_plane; p.c_type = planes == 3 ? bk::T_PLANES : bk::T_BF16;
-    p.act = act; p.gu = const_cast<void*>(GU); p.ldgu = ldgu; p.gu_half = gu_half; p.gu_f32 = planes == 3; p.colpart = colpart;
-    ProfScope prof(PK_GEMM_DGRAD, BLK_STREAM(stream), 2.0 * M * F * N, 0.0);
-    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED_BWD>(p, bk::use_big(M, F, 256) ? 0 : 1, 1, BLK_STREAM(stream), "gated_proj_bwd");
+    p.A = (const char*)X; p.lda = ldx; p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw;
+    p.M = M; p.N = F; p.K = K; p.ks = p.kz = stages_of(K, planes);
+    p.bias = bg; p.bias2 = bu; p.bias_bf16 = bias_bf16;
+    p.C = H; p.ldc = planes == 3 ? ldh : ldh / 2;
+    p.act = act; p.gu = GU; p.gu_lo = (unsigned char*)GU_lo; p.ldgu = ldgu; p.gu_half = gu_half;
+    ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
+    if (planes == 3) return bk::launch_rows<bk::FMT_SPLIT, bk::EP_GATED_3>(p, 1, BLK_STREAM(stream), "gated_proj_fwd");
+    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, 1, BLK_STREAM(stream), "gated_proj_fwd");
 }
-// Strips of 64 rows that btvae_gated_proj_bwd leaves column sums for: colpart holds [strips][2][F] floats.
-BTVAE_API int btvae_gated_proj_strips(int M, int F) { return bk::use_big(M, F, 256) ? bk::tiles(M, 256) * 4 : bk::tiles(M, 128) * 2; }
+
+BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* GU, const void* GU_lo, long long ldgu, int gu_half,
+                                   void* dGU, long long ldd, float* colpart, int planes, int act, int M, int F, int N, void* stream) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_bwd: planes must be 1 or 3");
+    BTVAE_REQUIRE(M >= 0 && F > 0 && N > 0 && (planes == 3 || (N & 7) == 0), "gated_proj_bwd: bad sizes (M %d, F %d, N %d)", M, F, N);
+    BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_bwd: unknown activation %d", act);
+    if (M == 0) return 0;
+    BTVAE_REQUIRE(operand_ok(dY, lddy, planes, N) && operand_ok(WdT, ldw, planes, N), "gated_proj_bwd: bad operand layout");
+    BTVAE_REQUIRE(kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_bwd: bad layout of the kept projections");
+    BTVAE_REQUIRE(operand_ok(dGU, ldd, planes, 2 * gu_half), "gated_proj_bwd: bad layout of the gradients");
+    bk::Args p = {};
+    p.A = (const char*)dY; p.lda = lddy; p.B = (const char*)WdT; p.ldb = ldw;
+    p.M = M; p.N = F; p.K = N; p.ks = p.kz = stages_of(N, planes);
+    p.C = dGU; p.ldc = planes == 3 ? ldd : ldd / 2;
+    p.act = act; p.gu = const_cast<void*>(GU); p.gu_lo = (unsigned char*)const_cast<void*>(GU_lo); p.ldgu = ldgu; p.gu_half = gu_half; p.colpart = colpart;
+    ProfScope prof(PK_GEMM_DGRAD, BLK_STREAM(stream), 2.0 * M * F * N, 0.0);
+    if (planes == 3) return bk::launch_rows<bk::FMT_SPLIT, bk::EP_GATED_BWD_3>(p, 1, BLK_STREAM(stream), "gated_proj_bwd");
+    return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED_BWD>(p, 1, BLK_STREAM(stream), "gated_proj_bwd");
+}
+// Strips of rows that btvae_gated_proj_bwd leaves column sums for: colpart holds [strips][2][F] floats.
+BTVAE_API int btvae_gated_proj_strips(int M) { return 2 * bk::tiles(M, 128); }
 
 BTVAE_API long long btvae_block_product_ws(int M, int N, int K, int planes) {
-    const bk::ProductPlan r = bk::plan_product(M, N, (planes == 3 ? 6 : 1) * bk::tiles(K, 32), 1, 1 << 30);
+    const bk::ProductPlan r = bk::plan_product(M, N, stages_of(K, planes), 1);
     return r.z > 1 ? (long long)r.z * M * N : 0;
 }
-BTVAE_API int btvae_block_product(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, const void* bias, int bias_bf16,
-                                  void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int planes, int M, int N, int K, void* stream) {
+BTVAE_API int btvae_block_product(const void* A, long long lda, const void* B, long long ldb, const void* bias, int bias_bf16, void* C, long long ldc, int c_bf16,
+                                  float* ws, long long ws_floats, int planes, int M, int N, int K, void* stream) {
     BTVAE_REQUIRE(planes == 1 || planes == 3, "block_product: planes must be 1 or 3");
-    BTVAE_REQUIRE(M >= 0 && N > 0 && K > 0 && (K & 7) == 0 && ldc >= N, "block_product: bad sizes (M %d, N %d, K %d)", M, N, K);
-    BTVAE_REQUIRE(operand_ok(A, lda, a_plane, planes) && lda >= K && operand_ok(B, ldb, b_plane, planes) && ldb >= K, "block_product: operand rows must start on 16 bytes");
+    BTVAE_REQUIRE(M >= 0 && N > 0 && K > 0 && (planes == 3 || (K & 7) == 0) && ldc >= N, "block_product: bad sizes (M %d, N %d, K %d)", M, N, K);
     if (M == 0) return 0;
+    BTVAE_REQUIRE(operand_ok(A, lda, planes, K) && operand_ok(B, ldb, planes, K), "block_product: bad operand layout");
     hipStream_t s = BLK_STREAM(stream);
     bk::Args p = {};
-    p.A = (const char*)A; p.lda = lda * 2; p.a_plane = a_plane * 2;
-    p.B = (const char*)B; p.ldb = ldb * 2; p.b_plane = b_plane * 2;
-    p.M = M; p.N = N; p.K = K; p.pairs = planes == 3 ? 6 : 1; p.ks = bk::tiles(K, 32);
-    const bk::ProductPlan r = bk::plan_product(M, N, p.pairs * p.ks, 1, 1 << 30);
+    p.A = (const char*)A; p.lda = lda; p.B = (const char*)B; p.ldb = ldb;
+    p.M = M; p.N = N; p.K = K; p.ks = stages_of(K, planes);
+    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 1);
     BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "block_product: workspace too small");
     p.kz = r.kz; p.slab = ws;
     p.bias = bias; p.bias_bf16 = bias_bf16;
-    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32; p.c_vec = bk::al16(C) && (ldc & (c_bf16 ? 7 : 3)) == 0;
+    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32;
     ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
-    if (int rc = bk::launch_rows<bk::FMT_BF16, bk::EP_LINEAR>(p, r.shape, r.z, s, "block_product")) return rc;
-    if (r.z == 1) return 0;
+    const int rc = planes == 3 ? bk::launch_rows<bk::FMT_SPLIT, bk::EP_LINEAR>(p, r.z, s, "block_product") : bk::launch_rows<bk::FMT_BF16, bk::EP_LINEAR>(p, r.z, s, "block_product");
+    if (rc || r.z == 1) return rc;
     hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0, bias, bias_bf16, c_bf16, 0);
     return check_launch("block_product reduction");
 }
@@ -611,29 +589,26 @@ BTVAE_API long long btvae_block_wgrad_ws(int M, int N, int R, int planes) {
     return (long long)r.z * M * N;
 }
 // out(m, n) (+)= sum_r A[r][m] B[r][n], m < M (rows [0, rows0) -> out0, [off1, off1 + rows1) -> out1), n < N
-BTVAE_API int btvae_block_wgrad(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, float* ws, long long ws_floats,
+BTVAE_API int btvae_block_wgrad(const void* A, long long lda, const void* B, long long ldb, float* ws, long long ws_floats,
                                 void* out0, int rows0, void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate, int planes, int M, int N, int R, void* stream) {
     BTVAE_REQUIRE(planes == 1 || planes == 3, "block_wgrad: planes must be 1 or 3");
-    const int M8 = (M + 7) / 8 * 8, N8 = (N + 7) / 8 * 8;
+    const int unit = planes == 3 ? 16 : 8, M8 = bk::tiles(M, unit) * unit, N8 = bk::tiles(N, unit) * unit;
     BTVAE_REQUIRE(M > 0 && N > 0 && R >= 0 && rows0 > 0 && rows0 <= M && ldo >= N && out0, "block_wgrad: bad sizes (M %d, N %d, R %d)", M, N, R);
     BTVAE_REQUIRE(!out1 || (off1 >= rows0 && off1 + rows1 <= M), "block_wgrad: bad row ranges");
-    BTVAE_REQUIRE(R == 0 || (operand_ok(A, lda, a_plane, planes) && lda >= M8 && operand_ok(B, ldb, b_plane, planes) && ldb >= N8), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of 8 columns");
+    BTVAE_REQUIRE(R == 0 || (operand_ok(A, lda, planes, M8) && operand_ok(B, ldb, planes, N8)), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of %d columns", unit);
+    BTVAE_REQUIRE(lda < (1 << 23) && ldb < (1 << 23), "block_wgrad: rows of more than 8 MiB");
     hipStream_t s = BLK_STREAM(stream);
     const bk::ColPlan r = bk::plan_cols(M, N, R, planes);
     BTVAE_REQUIRE(ws && ws_floats >= (long long)r.z * M * N, "block_wgrad: workspace too small");
     bk::ColArgs p = {};
-    p.A = (const char*)A; p.lda = lda * 2; p.a_plane = a_plane * 2; p.a_cols = M8;
-    p.B = (const char*)B; p.ldb = ldb * 2; p.b_plane = b_plane * 2; p.b_cols = N8;
-    p.R = R; p.M = M; p.N = N; p.pairs = planes == 3 ? 6 : 1; p.rz = r.rz; p.slab = ws;
+    p.A = (const char*)A; p.lda = lda; p.a_cols = M8; p.B = (const char*)B; p.ldb = ldb; p.b_cols = N8;
+    p.R = R; p.M = M; p.N = N; p.rz = r.rz; p.slab = ws;
     const int t = r.big ? 256 : 128;
     p.tiles_m = bk::tiles(M, t); p.tiles_n = bk::tiles(N, t);
-    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)r.z);
     {
         ProfScope prof(PK_GEMM_WGRAD, s, 2.0 * M * N * R, 0.0);
-        if (r.big) hipLaunchKernelGGL((bk::gemm_cols<4, 2, 4>), grid, dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((bk::gemm_cols<2, 2, 2>), grid, dim3(256), 0, s, p);
+        if (int rc = bk::launch_cols(p, planes == 3, r.big, r.z, s)) return rc;
     }
-    if (int rc = check_launch("block_wgrad")) return rc;
     hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, out0, ldo, rows0, out1, off1, rows1,
                        (const void*)nullptr, 0, out_bf16, accumulate);
     return check_launch("block_wgrad reduction");
@@ -702,18 +677,10 @@ BTVAE_API int btvae_fp8_quantize(const void* src, int src_bf16, long long ld, vo
     const int kb = bk::tiles(K, 128);
     BTVAE_REQUIRE(rows >= 0 && K > 0 && ld >= K && ldq >= (long long)kb * 128 && (ldq & 15) == 0 && bk::al16(q) && scp >= kb, "fp8_quantize: bad layout");
     if (rows == 0) return 0;
-    const bool vec = bk::al16(src) && K % 8 == 0 && (ld & (src_bf16 ? 7 : 3)) == 0;
     const unsigned grid = (unsigned)std::min<long long>(((long long)rows * kb + 15) / 16, 32768);
     hipStream_t s = BLK_STREAM(stream);
-    unsigned char* qd = (unsigned char*)q;
-    unsigned char* sd = (unsigned char*)sc;
-    if (src_bf16) {
-        if (vec) hipLaunchKernelGGL((bk::quantize_rows<true, true>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
-        else hipLaunchKernelGGL((bk::quantize_rows<true, false>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
-    } else {
-        if (vec) hipLaunchKernelGGL((bk::quantize_rows<false, true>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
-        else hipLaunchKernelGGL((bk::quantize_rows<false, false>), dim3(grid), dim3(256), 0, s, src, ld, qd, ldq, sd, scp, rows, K, kb);
-    }
+    if (src_bf16) hipLaunchKernelGGL((bk::quantize_rows<true>), dim3(grid), dim3(256), 0, s, src, ld, (unsigned char*)q, ldq, (unsigned char*)sc, scp, rows, K, kb);
+    else hipLaunchKernelGGL((bk::quantize_rows<false>), dim3(grid), dim3(256), 0, s, src, ld, (unsigned char*)q, ldq, (unsigned char*)sc, scp, rows, K, kb);
     return check_launch("fp8_quantize");
 }
 // weights: one scale for each 128 x 128 block, scale bytes [ceil(N / 128)][scp]
@@ -749,7 +716,7 @@ static bool fp8_ok(const void* q, long long ldq, const void* sc, long long scp, 
     return bk::al16(q) && (ldq & 15) == 0 && ldq >= (long long)kb * 128 && ((uintptr_t)sc & 3) == 0 && (scp & 3) == 0 && scp >= kb;
 }
 BTVAE_API long long btvae_fp8_product_ws(int M, int N, int K) {
-    const bk::ProductPlan r = bk::plan_product(M, N, bk::tiles(K, 128) * 2, 8, 2 * bk::SC_ROW);
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tiles(K, 128), 4);
     return r.z > 1 ? (long long)r.z * M * N : 0;
 }
 BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, long long xsp, const void* W, long long ldw, const void* wsc, long long wscp, const float* bias,
@@ -760,14 +727,14 @@ BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, lo
     hipStream_t s = BLK_STREAM(stream);
     bk::Args p = {};
     p.A = (const char*)X; p.lda = ldx; p.B = (const char*)W; p.ldb = ldw;
-    p.M = M; p.N = N; p.K = K; p.pairs = 1; p.ks = bk::tiles(K, 128) * 2;
+    p.M = M; p.N = N; p.K = K; p.ks = bk::tiles(K, 128);
     p.a_sc = (const unsigned char*)xs; p.a_scp = xsp; p.b_sc = (const unsigned*)wsc; p.b_scp = (int)(wscp / 4);
-    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 8, 2 * bk::SC_ROW);
+    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 4);
     BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "fp8_product: workspace too small");
     p.kz = r.kz; p.slab = ws; p.bias = bias;
-    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32; p.c_vec = bk::al16(C) && (ldc & (c_bf16 ? 7 : 3)) == 0;
+    p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32;
     ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
-    if (int rc = bk::launch_rows<bk::FMT_E4M3, bk::EP_LINEAR>(p, r.shape, r.z, s, "fp8_product")) return rc;
+    if (int rc = bk::launch_rows<bk::FMT_E4M3, bk::EP_LINEAR>(p, r.z, s, "fp8_product")) return rc;
     if (r.z == 1) return 0;
     hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0,
                        (const void*)bias, 0, c_bf16, 0);
@@ -779,25 +746,23 @@ BTVAE_API int btvae_fp8_gated_proj(const void* X, long long ldx, const void* xs,
                                    int expanded, const float* bg, const float* bu, void* H, long long ldh, void* hs, long long hsp, int act, int M, int F, int K, void* stream) {
     BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0, "fp8_gated_proj: bad sizes (M %d, F %d, K %d)", M, F, K);
     BTVAE_REQUIRE(act >= 0 && act <= 3, "fp8_gated_proj: unknown activation %d", act);
-    BTVAE_REQUIRE(bk::tiles(K, 128) <= bk::SC_ROW, "fp8_gated_proj: K %d is beyond %d", K, bk::SC_ROW * 128);
     if (M == 0) return 0;
     BTVAE_REQUIRE(fp8_ok(H, ldh, hs, hsp, F), "fp8_gated_proj: bad layout of H");
     bk::Args p = {};
     const int kp = bk::tiles(K, 128) * 128, sz = expanded ? 2 : 1;
     p.A = (const char*)X; p.lda = ldx * sz; p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw * sz;
-    p.M = M; p.N = F; p.pairs = 1;
-    p.bias = bg; p.bias2 = bu; p.C = H; p.ldc = ldh; p.c_type = bk::T_E4M3; p.q_sc = (unsigned char*)hs; p.q_scp = hsp; p.act = act;
-    const int shape = bk::use_big(M, F, 128) ? 0 : 2;
+    p.M = M; p.N = F;
+    p.bias = bg; p.bias2 = bu; p.C = H; p.ldc = ldh; p.q_sc = (unsigned char*)hs; p.q_scp = hsp; p.act = act;
     ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
     if (expanded) {
-        BTVAE_REQUIRE(operand_ok(X, ldx, 0, 1) && ldx >= kp && operand_ok(Wg, ldw, 0, 1) && operand_ok(Wu, ldw, 0, 1) && ldw >= kp, "fp8_gated_proj: bad operand layout");
-        p.K = kp; p.ks = p.kz = kp / 32;
-        return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, shape, 1, BLK_STREAM(stream), "fp8_gated_proj");
+        BTVAE_REQUIRE(operand_ok(X, ldx * 2, 1, kp) && operand_ok(Wg, ldw * 2, 1, kp) && operand_ok(Wu, ldw * 2, 1, kp), "fp8_gated_proj: bad operand layout");
+        p.K = kp; p.ks = p.kz = kp / 64;
+        return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED_Q>(p, 1, BLK_STREAM(stream), "fp8_gated_proj");
     }
     BTVAE_REQUIRE(fp8_ok(X, ldx, xs, xsp, K) && fp8_ok(Wg, ldw, gs, wscp, K) && fp8_ok(Wu, ldw, us, wscp, K), "fp8_gated_proj: bad operand layout");
-    p.K = K; p.ks = p.kz = kp / 64;
+    p.K = K; p.ks = p.kz = kp / 128;
     p.a_sc = (const unsigned char*)xs; p.a_scp = xsp; p.b_sc = (const unsigned*)gs; p.b2_sc = (const unsigned*)us; p.b_scp = (int)(wscp / 4);
-    return bk::launch_rows<bk::FMT_E4M3, bk::EP_GATED>(p, shape, 1, BLK_STREAM(stream), "fp8_gated_proj");
+    return bk::launch_rows<bk::FMT_E4M3, bk::EP_GATED_Q>(p, 1, BLK_STREAM(stream), "fp8_gated_proj");
 }
 // Up to btvae_few_rows_max() rows of fp32 / bf16 x, quantised on the way in; W2 null: C = x W^T + bias, else the gated product (C fp32 or bf16).
 BTVAE_API int btvae_fp8_few_rows(const void* X, int x_bf16, long long ldx, const void* W, const void* wsc, const void* W2, const void* wsc2, long long ldw, long long wscp, const float* bias,

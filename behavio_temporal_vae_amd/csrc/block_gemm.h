@@ -6,16 +6,28 @@
 //
 // fp32 operands.  A value x is the sum of three bf16 values x0 + x1 + x2 (round to nearest of x, of the rest, of the rest
 // of that: |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, nothing is lost).  Of the nine products of two such sums the six largest
-// are taken; the dropped x1 y2, x2 y1 and x2 y2 are below 2^-26 of x y, four times below an fp32 rounding.  The operands
-// arrive as three planes and the kernel runs its reduction over the six plane pairs one after another, smallest first,
-// into the same fp32 accumulators: the fp32 form is the bf16 kernel with a reduction six times as long.
+// are taken, smallest first, into the same fp32 accumulators; the dropped x1 y2, x2 y1 and x2 y2 are below 2^-26 of x y,
+// four times below an fp32 rounding.  A matrix of such values ("split") keeps, for every 16 columns, 16 x0, 16 x1 and 16 x2: 96
+// bytes in a row.  A stage of 16 reduction steps brings all three pieces of both operands, so that each piece read from LDS is
+// multiplied twice on average: this form waits for the matrix pipe alone.
 //
-// Layout of the loop (both kernels).  A workgroup computes a 256 x 256, 128 x 256 or 128 x 128 tile; the reduction goes in stages
-// of 64 bytes per row (32 bf16, 64 e4m3), copied global -> LDS without passing through registers into a ring of four
-// stages, three of them in flight behind the one being multiplied.  One barrier a stage; the counted waits never drain the
-// queue inside the loop.  Pieces of 16 bytes past the end of a row read from a block of zeros instead, so operands need
-// no padding beyond a multiple of 8 columns; rows past the end repeat the last row (gemm_rows, where they only reach outputs that
-// are not stored) or are zeros (gemm_cols, where rows are the reduction).
+// Layout of the loop (both kernels).  Four waves compute a 256 x 256 tile (128 x 128 each), or 128 x 128 / 128 x 256 where
+// there are too few tiles to fill the chip; the reduction goes in stages of 128 bytes per row (64 bf16, 128 e4m3: whole lines,
+// which is what L2 serves at its full rate), copied global -> LDS without passing through registers, two stages deep.  A wave reads the operands of its next
+// step into a second set of registers while it multiplies the present one; once all waves have read a stage (one barrier a
+// stage) its slot is refilled with the stage after next.  A wave's 128 x 128
+// reads LDS half as often for a multiplication as its 64 x 128 would, which is what bounds the loop; it takes 256
+// accumulators and one wave to a SIMD.  gemm_rows goes through several tiles: the ring keeps filling with
+// the next tile's stages while the results of the last one are computed and stored from registers.  Pieces of 16 bytes past the
+// end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns; rows past
+// the end repeat the last row (gemm_rows, where they only reach outputs that are not stored) or are zeros (gemm_cols, where
+// rows are the reduction).
+//
+// Results.  The weights are the MFMA's first operand, so a lane's 16 results of a 32 x 32 block are 16 columns of ONE row, and the
+// weight rows are laid into LDS with bits 2 and 3 of their index swapped, which makes them two runs of 8 consecutive
+// columns.  Bias, activation, product and rounding happen there; 2 KiB of LDS to a wave then turn each 64 bytes of 32 rows
+// over to four neighbouring lanes a row: stores of 16 bytes a lane whose neighbours do not continue them cost several
+// times as much (measured: 150 cycles a store instruction instead of about 30).
 #pragma once
 #include "common.h"
 #include <type_traits>
@@ -33,34 +45,51 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int ROWB = 64;                 // bytes of a row in one stage
-constexpr int NST = 4;                   // stages in the ring
-constexpr int SC_ROW = 128;              // e4m3: scale bytes kept per row of a tile = the reduction blocks one launch may span
+constexpr int SC_SLOTS = 4;              // e4m3: groups of four 128-blocks whose scale words are in LDS
 
-enum { FMT_BF16 = 0, FMT_E4M3 = 1 };
-enum { EP_LINEAR = 0, EP_GATED = 1, EP_GATED_BWD = 2 };
+enum { FMT_BF16 = 0, FMT_E4M3 = 1, FMT_SPLIT = 2 };
+// EP_GATED / EP_GATED_BWD: bf16 operands, results rounded to bf16; EP_GATED_3 / EP_GATED_BWD_3: fp32 values as planes; EP_GATED_Q: h quantised
+enum { EP_LINEAR = 0, EP_GATED = 1, EP_GATED_BWD = 2, EP_GATED_3 = 3, EP_GATED_BWD_3 = 4, EP_GATED_Q = 5 };
+constexpr bool is_gated(int ep) { return ep == EP_GATED || ep == EP_GATED_3 || ep == EP_GATED_Q; }
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3 };
-enum { T_F32 = 0, T_BF16 = 1, T_PLANES = 2, T_E4M3 = 3 };
+enum { T_F32 = 0, T_BF16 = 1 };
+
+// x / d for 0 <= x < 2^30 by a multiplication: d's reciprocal rounded up to 32 bits behind its leading bit (the error stays below 1 / d)
+struct Div {
+    unsigned d, mul, shift;
+    __host__ __device__ __forceinline__ int of(int x) const {
+        return d == 1 ? x : (int)(((unsigned long long)(unsigned)x * mul) >> 32 >> shift);
+    }
+};
+inline Div div_by(int d) {
+    Div r = {(unsigned)d, 0u, 0u};
+    while ((1u << (r.shift + 1)) < (unsigned)d) ++r.shift;     // 2^shift < d <= 2^(shift + 1)
+    if (d > 1) r.mul = (unsigned)(((1ull << (32 + r.shift)) + d - 1) / d);
+    return r;
+}
+
+constexpr int row_bytes(int fmt) { return fmt == FMT_SPLIT ? 96 : 128; }         // bytes of a row in one stage of gemm_rows
 
 struct Args {
-    const char* A; long long lda, a_plane;          // byte pitch of rows, bytes between planes
-    const char* B; const char* B2; long long ldb, b_plane;      // EP_GATED: B = gate rows, B2 = up rows
-    int M, N, K;                                    // N: output columns (EP_GATED: columns of h); K: reduction elements, a multiple of 8
-    int pairs;                                      // 1, or 6 plane pairs
-    int ks;                                         // stages of one plane pair
-    int kz;                                         // stages of one split of the reduction (gridDim.z splits)
-    int tiles_m, tiles_n;
+    const char* A; long long lda;                   // byte pitch of rows
+    const char* B; const char* B2; long long ldb;   // gated: B = gate rows, B2 = up rows
+    int M, N, K;                                    // N: output columns (gated: columns of h); K: reduction elements (bf16: a multiple of 8)
+    int ks;                                         // stages of the reduction
+    int kz;                                         // stages of one of `splits` splits of it
+    int tiles_m, tiles_n, splits;
+    Div by_tiles, by_band, by_last;                 // x / tiles, x / (8 tiles_n), x / rows of the last band of 8
     const unsigned char* a_sc; long long a_scp;     // e4m3: scale bytes of A [M][a_scp]
     const unsigned* b_sc; const unsigned* b2_sc; int b_scp;     // e4m3: scale bytes of B's 128-row blocks, four to a word [blocks][b_scp words]
-    const void* bias; const void* bias2; int bias_bf16;         // EP_LINEAR: bias; EP_GATED: gate and up
-    void* C; long long ldc; int c_type;             // elements; T_F32, T_BF16 (EP_LINEAR), T_PLANES / T_BF16 (one plane) / T_E4M3 / T_F32 (EP_GATED)
-    long long c_plane;                              // elements between planes of C
-    float* slab;                                    // gridDim.z > 1: fp32 partial results [z][M][N]
-    int c_vec;                                      // rows of C start on 16 bytes and columns up to the next multiple of 8 may be written (zeros)
+    const void* bias; const void* bias2; int bias_bf16;         // plain: bias; gated: gate and up
+    void* C; long long ldc; int c_type;             // EP_LINEAR: T_F32 or T_BF16, pitch in elements; split results: pitch in bytes
+    float* slab;                                    // splits > 1: fp32 partial results [z][M][N]
     int act;
-    void* gu; long long ldgu; int gu_f32; int gu_half;          // EP_GATED: where a, b are kept (null: not); EP_GATED_BWD: read; b starts gu_half columns after a
-    float* colpart;                                 // EP_GATED_BWD: column sums of (da, db) per 64-row strip [strips][2][N], or null
-    unsigned char* q_sc; long long q_scp;           // T_E4M3: scale bytes of the output [M][q_scp]
+    // Gated: where a, b are kept for the backward pass (null: not); backward: read; b starts gu_half columns after a.  fp32, or (bf16
+    // operands) 24 bits: the upper two bytes here, the third in gu_lo -- 2^-17 instead of bf16's 2^-9, since these values are rounded again as part of
+    // the gradients
+    void* gu; unsigned char* gu_lo; long long ldgu; int gu_half;
+    float* colpart;                                 // backward: column sums of (da, db) per wave's strip of rows [strips][2][N], or null
+    unsigned char* q_sc; long long q_scp;           // EP_GATED_Q: scale bytes of the output [M][q_scp]
 };
 
 __device__ __attribute__((aligned(64))) static const unsigned zero_piece[16] = {0};
@@ -68,15 +97,11 @@ __device__ __attribute__((aligned(64))) static const unsigned zero_piece[16] = {
 __device__ __forceinline__ void glds16(const void* g, void* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
-// Within a wave LDS is served in order: only the compiler has to be kept from moving accesses across.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Byte offset of the logical 16-byte piece c of row r in a stage image of 64-byte rows: the XOR spreads the rows that one
-// 16-lane group of a ds_read_b128 touches (the same piece of 16 rows) over all 64 banks.
-__device__ __forceinline__ int st_off(int r, int c) { return r * ROWB + ((c ^ ((r >> 2) & 3)) << 4); }
+// Byte offset of the logical 16-byte piece c of row r in a stage image.  128-byte rows: the XOR spreads the rows that one 16-lane
+// group of a ds_read_b128 touches (the same piece of 16 rows) over all 64 banks.  96-byte rows: eight rows do that by
+// themselves, the next eight take the other piece of a pair.
+template <int FMT> __device__ __forceinline__ int st_swap(int r) { return FMT == FMT_SPLIT ? (r >> 3) & 1 : (r >> 1) & 7; }
+template <int FMT> __device__ __forceinline__ int st_off(int r, int c) { return r * row_bytes(FMT) + ((c ^ st_swap<FMT>(r)) << 4); }
 
 __device__ __forceinline__ unsigned pack2(float a, float b) {
     const f32x2 f = {a, b};
@@ -89,52 +114,58 @@ __device__ __forceinline__ unsigned short bf_bits(float v) { return (unsigned sh
 
 // x = p0 + p1 + p2 in bf16.  A finite x whose first rounding would overflow keeps its truncation; a non-finite x is p0 alone.
 __device__ __forceinline__ void split3(float x, float& p0, float& p1, float& p2) {
+    const bool finite = __builtin_fabsf(x) < __builtin_inff();
     p0 = bf_lo(pack2(x, 0.f));
-    if (!(__builtin_fabsf(p0) < __builtin_inff())) {
-        if (__builtin_fabsf(x) < __builtin_inff()) p0 = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-        else { p1 = 0.f; p2 = 0.f; return; }
-    }
-    const float r = x - p0;
+    const float cut = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    p0 = finite && !(__builtin_fabsf(p0) < __builtin_inff()) ? cut : p0;
+    const float r = finite ? x - p0 : 0.f;
     p1 = bf_lo(pack2(r, 0.f));
     p2 = r - p1;
 }
 
-// 8 consecutive values -> 8 bf16 of each plane at element offset o
-__device__ __forceinline__ void store_planes8(unsigned short* base, long long plane, int np, long long o, const float (&v)[8]) {
-    if (np == 1) {
-        u32x4 q;
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) { return u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])}; }
+__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&p)[3]) {
+    float x[3][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = pack2(v[2 * e], v[2 * e + 1]);
-        *reinterpret_cast<u32x4*>(base + o) = q;
-        return;
-    }
-    u32x4 q0, q1, q2;
+    for (int e = 0; e < 8; ++e) split3(v[e], x[0][e], x[1][e], x[2][e]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float a0, a1, a2, b0, b1, b2;
-        split3(v[2 * e], a0, a1, a2);
-        split3(v[2 * e + 1], b0, b1, b2);
-        q0[e] = pack2(a0, b0); q1[e] = pack2(a1, b1); q2[e] = pack2(a2, b2);
-    }
-    *reinterpret_cast<u32x4*>(base + o) = q0;
-    *reinterpret_cast<u32x4*>(base + plane + o) = q1;
-    *reinterpret_cast<u32x4*>(base + 2 * plane + o) = q2;
+    for (int k = 0; k < 3; ++k) p[k] = pack8(x[k]);
 }
+// byte of column c, piece k, in a row of a split matrix
+__device__ __forceinline__ long long split_at(int c, int k) { return (long long)(c >> 4) * 96 + k * 32 + (c & 15) * 2; }
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 // act(a) and act'(a).  FAST (results that are rounded to bf16 or e4m3): the hardware's exp and reciprocal, each good to
-// about 2^-22, instead of the correctly rounded division.
-template <bool FAST>
+// about 2^-22, and erfc from Abramowitz and Stegun's 7.1.26 (1.5e-7); otherwise the precise exp and division and erfc from the Chebyshev
+// fit t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), of Numerical Recipes (6.2; 1.2e-7 of the value everywhere).
+// GELU is a constant (its code is a path of its own), the others are told apart by `act`.
+template <bool FAST, bool GELU>
 __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) {
-    if (act == ACT_RELU) { v = a > 0.f ? a : (a == a ? 0.f : a); d = a > 0.f ? 1.f : 0.f; return; }
-    if (act == ACT_GELU) {
-        const float phi = 0.5f * erfcf(-0.70710678118654752f * a);
+    if constexpr (GELU) {
+        const float x = __builtin_fabsf(a) * 0.70710678118654752f;
+        float g, half_erfc;                                   // exp(-a^2 / 2), erfc(|a| / sqrt 2) / 2
+        if constexpr (FAST) {
+            const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+            g = __expf(-0.5f * a * a);
+            half_erfc = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * g;
+        } else {
+            const float t = 1.f / (1.f + 0.5f * x);
+            const float P = -1.26551223f + t * (1.00002368f + t * (0.37409196f + t * (0.09678418f + t * (-0.18628806f + t * (0.27886807f +
+                            t * (-1.13520398f + t * (1.48851587f + t * (-0.82215223f + t * 0.17087277f))))))));
+            g = expf(-0.5f * a * a);
+            half_erfc = 0.5f * t * g * expf(P);
+        }
+        const float phi = a < 0.f ? half_erfc : 1.f - half_erfc;
         v = a * phi;
-        d = phi + a * (FAST ? __expf(-0.5f * a * a) : expf(-0.5f * a * a)) * 0.39894228040143268f;
-        return;
+        d = phi + a * g * 0.39894228040143268f;
+    } else {
+        const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-a)) : 1.f / (1.f + expf(-a));
+        const float r = a > 0.f ? a : (a == a ? 0.f : a);
+        v = act == ACT_RELU ? r : (act == ACT_SILU ? a * s : s);
+        d = act == ACT_RELU ? (a > 0.f ? 1.f : 0.f) : (act == ACT_SILU ? s * (1.f + a * (1.f - s)) : s * (1.f - s));
     }
-    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-a)) : 1.f / (1.f + expf(-a));
-    if (act == ACT_SILU) { v = a * s; d = s * (1.f + a * (1.f - s)); }
-    else { v = s; d = s * (1.f - s); }
 }
 
 // Exponent of a block's scale: the smallest e >= -126 with amax <= 448 * 2^e; 0 for a block of zeros.
@@ -160,436 +191,839 @@ __device__ __forceinline__ float finite_abs(float v) {
 }
 __device__ __forceinline__ float nan_if_not_finite(float v) { return __builtin_fabsf(v) < __builtin_inff() ? v : __builtin_nanf(""); }
 
-// Tile of this workgroup.  Workgroups are dealt round-robin over the 8 XCDs; each XCD gets a contiguous run of tiles, and
-// the run goes through bands of 8 tile rows column by column, so that the 32 tiles an XCD works on at a time share 8 row
-// panels and about 4 column panels in its L2.
-__device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& tm, int& tn) {
-    const int T = tiles_m * tiles_n, bid = (int)blockIdx.x;
-    const int q = T >> 3, r = T & 7, xcd = bid & 7, idx = bid >> 3;
-    const int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
-    const int band = t / (8 * tiles_n), in = t - band * 8 * tiles_n;
-    const int rows = min(8, tiles_m - band * 8);
-    tm = band * 8 + in % rows;
-    tn = in / rows;
+// The items (output tiles x splits of the reduction) of this workgroup, one after another.  Workgroups are dealt round-robin over the 8
+// XCDs; each XCD gets a contiguous run of items and its workgroups take them in turn.  Tiles run through bands of 8 tile rows
+// column by column, so that the 32 an XCD works on at a time share 8 row panels and about 4 column panels in its L2.
+struct Items {
+    int next, step, end;
+    __device__ __forceinline__ explicit Items(int total) {
+        const int bid = (int)blockIdx.x, n = (int)gridDim.x, xcd = bid & 7;
+        const int q = total >> 3, r = total & 7;
+        const int start = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
+        next = start + (bid >> 3);
+        step = (n - xcd + 7) >> 3;
+        end = start + q + (xcd < r);
+    }
+};
+__device__ __forceinline__ void tile_of(const Args& p, int t, int& tm, int& tn) {
+    const int band = p.by_band.of(t), in = t - band * 8 * p.tiles_n;
+    const bool last = band * 8 + 8 > p.tiles_m;
+    const int rows = last ? (int)p.by_last.d : 8;
+    tn = last ? p.by_last.of(in) : in >> 3;
+    tm = band * 8 + (in - tn * rows);
 }
 
-__device__ __forceinline__ int plane_a(int pair) { return (0x010120 >> (4 * pair)) & 15; }     // pairs (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-__device__ __forceinline__ int plane_b(int pair) { return (0x001102 >> (4 * pair)) & 15; }
-
-// At most N copies of this wave still in flight, and every LDS read of the stage before done (its slot is about to be refilled).
+// At most N copies of this wave still in flight, and every LDS read before done (its slot is about to be refilled).  Builtins,
+// so that the compiler knows what has been waited for.
 template <int N> __device__ __forceinline__ void wait_vm() {
-    static_assert(N == 0 || N == 4 || N == 6 || N == 8 || N == 12, "");
-    if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
-    else if constexpr (N == 6) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
-    else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));       // vmcnt(N) lgkmcnt(0)
+}
+__device__ __forceinline__ void meet() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// WM x WN waves of 64 x (32 NJ) outputs each.
-template <int FMT, int EP, int WM, int WN, int NJ>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : (NJ == 2 ? 2 : 1)) void gemm_rows(const Args p) {
-    constexpr int NW = WM * WN, TM = WM * 64, CW = NJ * 32, TN = WN * CW;
-    constexpr int STAGE = (TM + TN) * ROWB;
-    constexpr int NA = TM / 16 / NW, NB = TN / 16 / NW, NGL = NA + NB;
-    constexpr int LDP = CW + 4;                                       // floats per row of a wave's epilogue image
-    constexpr int RING = NST * STAGE, EPI_B = NW * 32 * LDP * 4 + (EP == EP_GATED ? TM * WN * 4 : 0);
-    constexpr int MAIN = RING > EPI_B ? RING : EPI_B;
-    constexpr int SCB = FMT == FMT_E4M3 ? TM * SC_ROW : 0;
-    constexpr int SC_AT = RING;                                       // scales sit behind the ring; the epilogue may overwrite them
-    __shared__ __attribute__((aligned(1024))) char smem[(RING + SCB > MAIN) ? RING + SCB : MAIN];
+// Order of a region's instructions: R LDS reads, one behind each of the first matrix instructions (issued in one go they would
+// hold the wave up with its matrix pipe idle; issued late their results would), then V copies the same way, of M matrix instructions.
+template <int M, int R, int V> __device__ __forceinline__ void spread() {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i < M) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (R + i < M) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+}
+
+// A scalar that the compiler knows nothing about: address and edge computations made from it stay inside their block of results instead of
+// being made for all blocks at once and kept, which costs more registers than there are.
+__device__ __forceinline__ int opaque(int x) {
+    x = __builtin_amdgcn_readfirstlane(x);
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// ---- stores and loads of the results' layout ------------------------------------------------------------------------
+// A lane's results of one 32-column block: v[q][e] = column 16 q + 8 (lane >> 5) + e of row lane & 31.  `row0`: matrix row of the
+// block's row 0, `col0`: matrix column of its column 0.
+constexpr int TURN_B = 2048;                                  // bytes of LDS to a wave
+struct Where {
+    int li, lh, r4, p4, r2, p2;                               // result row and half; row and piece of four / two lanes to a row
+    char* lds;
+    __device__ __forceinline__ explicit Where(char* wave_lds) : lds(wave_lds) {
+        const int lane = threadIdx.x & 63;
+        li = lane & 31; lh = lane >> 5; r4 = lane >> 2; p4 = lane & 3; r2 = lane >> 1; p2 = lane & 1;
+    }
+    // The compiler must not move a lane's reads before other lanes' writes (LDS itself serves a wave in order).
+    __device__ __forceinline__ static void fence() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ u32x4* at4(int row, int piece) const { return reinterpret_cast<u32x4*>(lds + row * 64 + ((piece ^ ((row >> 2) & 3)) << 4)); }
+    __device__ __forceinline__ char* at2(int row) const { return lds + row * 32; }
+    __device__ __forceinline__ static int two(int row) { return ((row >> 3) & 1) << 4; }
+    // pieces c0, c1 (16 bytes each) of this lane's row of 64 bytes -> piece p4 of rows r4 and r4 + 16
+    __device__ __forceinline__ void turn(const u32x4 x0, int c0, const u32x4 x1, int c1, u32x4& a, u32x4& b) const {
+        *at4(li, c0) = x0;
+        *at4(li, c1) = x1;
+        fence();
+        a = *at4(r4, p4);
+        b = *at4(r4 + 16, p4);
+        fence();
+    }
+    // ... and back
+    __device__ __forceinline__ void back(const u32x4 a, const u32x4 b, int c0, u32x4& x0, int c1, u32x4& x1) const {
+        *at4(r4, p4) = a;
+        *at4(r4 + 16, p4) = b;
+        fence();
+        x0 = *at4(li, c0);
+        x1 = *at4(li, c1);
+        fence();
+    }
+    // 8-byte pieces lh and 2 + lh of this lane's row of 32 bytes -> 16-byte piece p2 of row r2
+    __device__ __forceinline__ u32x4 turn2(const u32x2 x0, const u32x2 x1) const {
+        *reinterpret_cast<u32x2*>(at2(li) + ((8 * lh) ^ two(li))) = x0;
+        *reinterpret_cast<u32x2*>(at2(li) + ((16 + 8 * lh) ^ two(li))) = x1;
+        fence();
+        const u32x4 a = *reinterpret_cast<const u32x4*>(at2(r2) + ((16 * p2) ^ two(r2)));
+        fence();
+        return a;
+    }
+    __device__ __forceinline__ void back2(const u32x4 a, u32x2& x0, u32x2& x1) const {
+        *reinterpret_cast<u32x4*>(at2(r2) + ((16 * p2) ^ two(r2))) = a;
+        fence();
+        x0 = *reinterpret_cast<const u32x2*>(at2(li) + ((8 * lh) ^ two(li)));
+        x1 = *reinterpret_cast<const u32x2*>(at2(li) + ((16 + 8 * lh) ^ two(li)));
+        fence();
+    }
+};
+// 8 bf16 (a lane's 16 bytes) at columns c .. c + 7 of a row, those below n only
+__device__ __forceinline__ void put_bf16(unsigned short* d, const u32x4 v, int c, int n) {
+    if (c + 8 <= n) { *reinterpret_cast<u32x4_any*>(d) = v; return; }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (c + e < n) d[e] = (unsigned short)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
+}
+__device__ __forceinline__ void put_f32(float* d, const u32x4 u, int c, int n) {
+    if (c + 4 <= n) { *reinterpret_cast<f32x4_any*>(d) = __builtin_bit_cast(f32x4, u); return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (c + e < n) d[e] = __uint_as_float(u[e]);
+}
+__device__ __forceinline__ void store_bf16(unsigned short* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+    u32x4 a, b;
+    w.turn(pack8(v[0]), w.lh, pack8(v[1]), 2 + w.lh, a, b);
+    const int c = col0 + 8 * w.p4, r = row0 + w.r4;
+    if (c >= cols) return;
+    if (r < rows) put_bf16(base + (long long)r * ld + c, a, c, cols);
+    if (r + 16 < rows) put_bf16(base + (long long)(r + 16) * ld + c, b, c, cols);
+}
+__device__ __forceinline__ u32x4 raw4(const float* v) { return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
+__device__ __forceinline__ void store_f32(float* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        u32x4 a, b;
+        w.turn(raw4(v[q]), 2 * w.lh, raw4(v[q] + 4), 2 * w.lh + 1, a, b);
+        const int c = col0 + 16 * q + 4 * w.p4, r = row0 + w.r4;
+        if (c >= cols) continue;
+        if (r < rows) put_f32(base + (long long)r * ld + c, a, c, cols);
+        if (r + 16 < rows) put_f32(base + (long long)(r + 16) * ld + c, b, c, cols);
+    }
+}
+// the block's 192 bytes of each row of a split matrix, 64 at a time (columns are whole groups of 16: `cols` is a multiple of 16)
+__device__ __forceinline__ void store_split(char* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+    u32x4 p[2][3], a, b;
+    split8(v[0], p[0]);
+    split8(v[1], p[1]);
+    const int r = row0 + w.r4;
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {                             // bytes 64 t ..: (run 0: pieces 0, 1), (run 0: piece 2, run 1: piece 0), (run 1: pieces 1, 2)
+        w.turn(t == 0 ? p[0][0] : (t == 1 ? p[0][2] : p[1][1]), w.lh, t == 0 ? p[0][1] : (t == 1 ? p[1][0] : p[1][2]), 2 + w.lh, a, b);
+        const bool in = t == 0 || (t == 1 && w.p4 < 2) || col0 + 16 < cols;
+        if (col0 >= cols || !in) continue;
+        char* d = base + (long long)r * ld + (long long)(col0 >> 4) * 96 + 64 * t + 16 * w.p4;
+        if (r < rows) *reinterpret_cast<u32x4*>(d) = a;
+        if (r + 16 < rows) *reinterpret_cast<u32x4*>(d + 16 * ld) = b;
+    }
+}
+// 24 bits of fp32 values: rounded to the upper three bytes (a value that would round to infinity, infinities and NaN are cut)
+__device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+    u32x4 h[2], a, b;
+    u32x2 l[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        unsigned u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned x = __float_as_uint(v[q][e]), up = x + 0x80u;
+            u[e] = (up & 0x7F800000u) == 0x7F800000u ? x : up;
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) h[q][d] = __builtin_amdgcn_perm(u[2 * d + 1], u[2 * d], 0x07060302u);
+#pragma unroll
+        for (int d = 0; d < 2; ++d)                           // byte 1 of four values
+            l[q][d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0501u), __builtin_amdgcn_perm(u[4 * d + 1], u[4 * d], 0x0C0C0501u), 0x05040100u);
+    }
+    w.turn(h[0], w.lh, h[1], 2 + w.lh, a, b);
+    const u32x4 lv = w.turn2(l[0], l[1]);
+    const int c = col0 + 8 * w.p4, r = row0 + w.r4;           // (cols is a multiple of 16: whole pieces)
+    if (c < cols) {
+        if (r < rows) *reinterpret_cast<u32x4*>(hi + (long long)r * ld + c) = a;
+        if (r + 16 < rows) *reinterpret_cast<u32x4*>(hi + (long long)(r + 16) * ld + c) = b;
+    }
+    const int c2 = col0 + 16 * w.p2, r2 = row0 + w.r2;
+    if (c2 < cols && r2 < rows) *reinterpret_cast<u32x4*>(lo + (long long)r2 * ld + c2) = lv;
+}
+struct Raw24 { u32x4 a, b, l; };
+__device__ __forceinline__ void load_24(const unsigned short* hi, const unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, Raw24& x, const Where& w) {
+    const int c = min(col0 + 8 * w.p4, cols - 8), c2 = min(col0 + 16 * w.p2, cols - 16);
+    x.a = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4, rows - 1) * ld + c);
+    x.b = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
+    x.l = *reinterpret_cast<const u32x4*>(lo + (long long)min(row0 + w.r2, rows - 1) * ld + c2);
+}
+__device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], const Where& w) {
+    u32x4 h[2];
+    u32x2 l[2];
+    w.back(x.a, x.b, w.lh, h[0], 2 + w.lh, h[1]);
+    w.back2(x.l, l[0], l[1]);
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned top = e & 1 ? h[q][e >> 1] & 0xFFFF0000u : h[q][e >> 1] << 16;
+            v[q][e] = __uint_as_float(top | ((l[q][e >> 2] >> (8 * (e & 3))) & 255u) << 8);
+        }
+}
+struct Raw32 { u32x4 a[2], b[2]; };
+__device__ __forceinline__ void load_f32(const float* base, long long ld, int row0, int col0, int rows, int cols, Raw32& x, const Where& w) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int c = min(col0 + 16 * q + 4 * w.p4, cols - 4);
+        x.a[q] = *reinterpret_cast<const u32x4*>(base + (long long)min(row0 + w.r4, rows - 1) * ld + c);
+        x.b[q] = *reinterpret_cast<const u32x4*>(base + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
+    }
+}
+__device__ __forceinline__ void unpack_f32(const Raw32& x, float (&v)[2][8], const Where& w) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        u32x4 p0, p1;
+        w.back(x.a[q], x.b[q], 2 * w.lh, p0, 2 * w.lh + 1, p1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[q][e] = __uint_as_float(p0[e]); v[q][4 + e] = __uint_as_float(p1[e]); }
+    }
+}
+// Biases are loaded once a tile, before its loop, a column to a lane (a load behind the results' stores would wait for them),
+// and read from the lanes: columns c .. c + 31 of what the lanes hold.
+__device__ __forceinline__ float bias_lane(const void* bias, int bf16, int col, int cols) {
+    if (!bias) return 0.f;                                    // (uniform)
+    const int c = min(col, cols - 1);
+    return bf16 ? bf_load(bias, c) : reinterpret_cast<const float*>(bias)[c];
+}
+__device__ __forceinline__ void bias_of(float lanes, int c, float (&v)[2][8], const Where& w) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int k = c + 16 * (r >> 3) + (r & 7);
+        const float lo = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lanes), k)), hi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lanes), k + 8));
+        v[r >> 3][r & 7] = w.lh ? hi : lo;
+    }
+}
+__device__ __forceinline__ void clear_beyond(float (&v)[2][8], int col0, int cols, const Where& w) {
+    if (col0 + 32 <= cols) return;                            // uniform
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (col0 + 16 * (r >> 3) + 8 * w.lh + (r & 7) >= cols) v[r >> 3][r & 7] = 0.f;
+}
+
+// WM x WN waves of (32 MI) x (32 NJ) outputs each.
+template <int FMT, int EP, int WM, int WN, int MI, int NJ>
+__global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows(const Args p) {
+    constexpr bool GATED = is_gated(EP), FAST = EP != EP_GATED_3 && EP != EP_GATED_BWD_3;
+    constexpr bool SPLIT = FMT == FMT_SPLIT;
+    constexpr int ROWB = row_bytes(FMT), SLOTS = SPLIT ? 3 : 2;
+    constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
+    constexpr int STAGE = (TM + TN) * ROWB, RING = SLOTS * STAGE;
+    constexpr int NA = TM * ROWB / 1024 / NW, NB = TN * ROWB / 1024 / NW;      // copies of a wave and stage
+    constexpr int STEPS = FMT == FMT_BF16 ? 4 : 2;            // steps of a stage
+    constexpr int SC_B = FMT == FMT_E4M3 ? SC_SLOTS * TM * 4 : 0;
+    constexpr int MX_B = EP == EP_GATED_Q ? TM * WN * 4 : 0;  // row maxima of the waves (quantised results)
+    __shared__ __attribute__((aligned(1024))) char smem[RING + SC_B + MX_B + NW * TURN_B];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid / WN, wc = wid % WN;
     const int li = lane & 31, lh = lane >> 5;
+    const Where wh(smem + RING + SC_B + MX_B + wid * TURN_B);
 
-    int tile_m, tile_n;
-    tile_of(p.tiles_m, p.tiles_n, tile_m, tile_n);
-    const int m0 = tile_m * TM;
-    const int n0 = tile_n * (EP == EP_GATED ? TN / 2 : TN);
-    const int zz = (int)blockIdx.z;
-    const int s_beg = zz * p.kz, s_end = min(p.pairs * p.ks, s_beg + p.kz);
-    const int nk = s_end - s_beg;
+    const int T = p.tiles_m * p.tiles_n, all_stages = p.ks;
+    const int total_items = T * p.splits;
+    Items feed(total_items);                                  // the item being copied: up to two stages ahead of
+    Items work = feed;                                        // ... the item being multiplied
+    if (feed.next >= feed.end) return;
 
-    // ---- sources of this wave's copies: instruction j fills 16 rows (1 KiB) of the stage image, a lane one piece of 16 bytes
-    const char* asrc[NA];
-    const char* bsrc[NB];
-    const int piece = (lane & 3) ^ ((lane >> 4) & 3);                 // the logical piece that belongs at this lane's place
+    // ---- copies: instruction j fills 1 KiB of the stage image (8 rows of 128 bytes, or 10 2/3 of 96: 32 rows to three), a lane one piece of
+    // 16 bytes; addresses are a base for the tile and stage (scalar) and a lane's offset from the tile's first row
+    constexpr int PR = ROWB / 16;                             // pieces of a row
+    auto row_of = [&](int q) { return (q * 64 + lane) / PR; };
+    auto piece = [&](int q) { return ((q * 64 + lane) % PR) ^ st_swap<FMT>(row_of(q)); };  // the logical piece that belongs at this lane's place of image part q
+    auto up_part = [&](int j) { return GATED && ((wid * NB + j) * 64 / PR) % CW >= CW / 2; };           // (32 rows are whole parts: uniform)
+    unsigned aofs[NA], bofs[NB];
+    const char *abase, *bbase, *bbase2;
+    unsigned sofs = 0;
+    const unsigned char* scbase = nullptr;
+    const bool has_tail = FMT == FMT_BF16 && (p.K & 63) != 0;
+    const bool tail_ok[2] = {(p.ks - 1) * 64 + piece(0) * 8 < p.K, (p.ks - 1) * 64 + piece(1) * 8 < p.K};   // this lane's piece of a last stage lies inside the row
+    int f_kin = 0, f_left = 0, f_slot = 0, f_scslot = 0;
+    long long f_total = 0;                                    // stages still to be copied
+    long long koff = 0;
+    auto open_feed = [&]() {
+        int tm, tn;
+        const int zz = p.by_tiles.of(feed.next);
+        tile_of(p, feed.next - zz * T, tm, tn);
+        const int m0 = tm * TM, n0 = tn * (GATED ? TN / 2 : TN);
+        abase = p.A + (long long)m0 * p.lda;
+        bbase = p.B + (long long)n0 * p.ldb;
+        if constexpr (GATED) bbase2 = p.B2 + (long long)n0 * p.ldb;
 #pragma unroll
-    for (int j = 0; j < NA; ++j) {
-        const int r = (wid * NA + j) * 16 + (lane >> 2);
-        asrc[j] = p.A + (long long)min(m0 + r, p.M - 1) * p.lda + (piece << 4);
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int r = (wid * NB + j) * 16 + (lane >> 2);
-        if constexpr (EP == EP_GATED) {
-            // a wave's columns are CW / 2 gate rows followed by the CW / 2 up rows of the same columns of h
-            const int c = r / CW, q = r % CW;
-            const int f = n0 + c * (CW / 2) + (q % (CW / 2));
-            bsrc[j] = (q < CW / 2 ? p.B : p.B2) + (long long)min(f, p.N - 1) * p.ldb + (piece << 4);
-        } else {
-            bsrc[j] = p.B + (long long)min(n0 + r, p.N - 1) * p.ldb + (piece << 4);
-        }
-    }
-    const bool has_tail = FMT == FMT_BF16 && (p.K & 31) != 0;
-    const bool tail_ok = (p.ks - 1) * 32 + piece * 8 < p.K;           // this lane's piece of a last stage lies inside the row
-    int pair = s_beg / p.ks, kin = s_beg - pair * p.ks;
-    long long aoff = (long long)plane_a(p.pairs == 1 ? 5 : pair) * p.a_plane + (long long)kin * ROWB;
-    long long boff = (long long)plane_b(p.pairs == 1 ? 5 : pair) * p.b_plane + (long long)kin * ROWB;
-    auto issue = [&](int slot) {
-        char* sb = smem + slot * STAGE;
-        const bool cut = has_tail && kin == p.ks - 1;                 // uniform
-#pragma unroll
-        for (int j = 0; j < NA; ++j) {
-            const char* s = asrc[j] + aoff;
-            if (cut) s = tail_ok ? s : reinterpret_cast<const char*>(zero_piece);
-            glds16(s, sb + (wid * NA + j) * 1024);
-        }
+        for (int j = 0; j < NA; ++j)
+            aofs[j] = (unsigned)min(row_of(wid * NA + j), p.M - 1 - m0) * (unsigned)p.lda + (piece(wid * NA + j) << 4);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const char* s = bsrc[j] + boff;
-            if (cut) s = tail_ok ? s : reinterpret_cast<const char*>(zero_piece);
-            glds16(s, sb + TM * ROWB + (wid * NB + j) * 1024);
+            int r = row_of(wid * NB + j);
+            r = (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);  // bits 2 and 3 swapped: see the results' layout
+            if constexpr (GATED) r = (r / CW) * (CW / 2) + r % (CW / 2);       // a wave's columns: CW / 2 gate rows, then the up rows of the same columns of h
+            bofs[j] = (unsigned)min(r, p.N - 1 - n0) * (unsigned)p.ldb + (piece(wid * NB + j) << 4);
         }
-        if (++kin == p.ks) {
-            kin = 0;
-            ++pair;
-            aoff = (long long)plane_a(pair) * p.a_plane;
-            boff = (long long)plane_b(pair) * p.b_plane;
-        } else {
-            aoff += ROWB;
-            boff += ROWB;
+        const int s_beg = zz * p.kz;
+        f_left = min(all_stages, s_beg + p.kz) - s_beg;
+        f_kin = s_beg;
+        koff = (long long)s_beg * ROWB;
+        if constexpr (FMT == FMT_E4M3) {
+            scbase = p.a_sc + (long long)m0 * p.a_scp + s_beg;
+            sofs = (unsigned)min(tid & (TM - 1), p.M - 1 - m0) * (unsigned)p.a_scp;
         }
     };
+    auto next_stage = [&]() {
+        if (--f_left == 0) {
+            feed.next += feed.step;
+            if (feed.next < feed.end) open_feed();
+        } else {
+            ++f_kin;
+            koff += ROWB;
+        }
+    };
+    auto issue = [&]() {
+        char* sb = smem + f_slot * STAGE;
+        const char* ab = abase + koff;
+        const char* bb = bbase + koff;
+        const char* bb2 = GATED ? bbase2 + koff : nullptr;
+        if constexpr (FMT == FMT_E4M3) {
+            if ((f_kin & 3) == 0) {                           // a group of four blocks begins: a scale word of every row (before the stage's own copies)
+                if (wid * 64 < TM)
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(scbase + sofs),
+                                                     (__attribute__((address_space(3))) void*)(smem + RING + f_scslot * TM * 4 + wid * 256), 4, 0, 0);
+                scbase += 4;
+                f_scslot = (f_scslot + 1) & (SC_SLOTS - 1);
+            }
+        }
+        if (has_tail && f_kin == p.ks - 1) {                  // uniform
+#pragma unroll
+            for (int j = 0; j < NA; ++j) glds16(tail_ok[(wid * NA + j) & 1] ? ab + aofs[j] : reinterpret_cast<const char*>(zero_piece), sb + (wid * NA + j) * 1024);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const bool up = up_part(j);
+                glds16(tail_ok[(wid * NB + j) & 1] ? (up ? bb2 : bb) + bofs[j] : reinterpret_cast<const char*>(zero_piece), sb + TM * ROWB + (wid * NB + j) * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const bool up = up_part(j);
+                glds16((up ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+            }
+        }
+        f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
+        --f_total;
+        next_stage();
+    };
+    {   // stages of all items of this workgroup (only the last split of the reduction is shorter)
+        for (int i = feed.next; i < feed.end; i += feed.step) f_total += min(all_stages, (p.by_tiles.of(i) + 1) * p.kz) - p.by_tiles.of(i) * p.kz;
+    }
+    long long w_total = f_total;                              // stages still to be multiplied
 
-    int oa[2], ob[NJ];
+    // operand addresses: piece 2 s + (lane >> 5) of a row at step s (bf16), pieces 4 s + 2 (lane >> 5) and the next (e4m3)
+    int oa[MI], ob[NJ];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) oa[i] = st_off(wr * 64 + i * 32 + li, FMT == FMT_BF16 ? lh : 2 * lh);
+    for (int i = 0; i < MI; ++i) oa[i] = st_off<FMT>(wr * RW + i * 32 + li, FMT == FMT_E4M3 ? 2 * lh : lh);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) ob[j] = TM * ROWB + st_off(wc * CW + j * 32 + li, FMT == FMT_BF16 ? lh : 2 * lh);
-
-    f32x16 acc[2][NJ];
+    for (int j = 0; j < NJ; ++j) ob[j] = TM * ROWB + st_off<FMT>(wc * CW + j * 32 + li, FMT == FMT_E4M3 ? 2 * lh : lh);
+    typedef typename std::conditional<FMT == FMT_E4M3, i32x8, bf16x8>::type Frag;
+    auto frag = [&](const char* sb, int o, int s) -> Frag {
+        if constexpr (SPLIT) return *reinterpret_cast<const bf16x8*>(sb + o + s * 32);        // (pairs of pieces: the swap stays within one)
+        else if constexpr (FMT == FMT_BF16) return *reinterpret_cast<const bf16x8*>(sb + (o ^ (s * 32)));
+        else {
+            const i32x4 lo = *reinterpret_cast<const i32x4*>(sb + (o ^ (s * 64))), hi = *reinterpret_cast<const i32x4*>(sb + (o ^ (s * 64) ^ 16));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    constexpr int READS = (MI + NJ) * (FMT == FMT_E4M3 ? 2 : 1);          // LDS reads of a step
+    // sets of operands: two taken in turn, or (split) the three pieces of A, the three of B and the next stage's first of B
+    Frag fa[SPLIT ? 3 : 2][MI], fb[SPLIT ? 4 : 2][NJ];
+    f32x16 acc[MI][NJ];
+    int sax[MI], sbx[2] = {127, 127};                         // e4m3: the present block's scales
+    unsigned sa4[MI], sb4[2] = {0, 0};                        // ... of four blocks
+    auto load_set = [&](auto set, const char* sb, int s) {
+        constexpr int k = decltype(set)::value & 1;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < MI; ++i) fa[k][i] = frag(sb, oa[i], s);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[k][j] = frag(sb, ob[j], s);
+    };
+    auto product = [&](auto sa, auto sb) {
+        constexpr int ka = decltype(sa)::value, k = decltype(sb)::value;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+            for (int i = 0; i < MI; ++i) {
+                if constexpr (FMT != FMT_E4M3) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[k][j], fa[ka][i], acc[i][j], 0, 0, 0);
+                else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[k][j], fa[ka][i], acc[i][j], 0, 0, 0, (GATED && j >= NJ / 2) ? sbx[1] : sbx[0], 0, sax[i]);
+            }
+    };
+    auto multiply = [&](auto set) { product(std::integral_constant<int, decltype(set)::value & 1>{}, std::integral_constant<int, decltype(set)::value & 1>{}); };
+    auto read_a = [&](auto set, const char* sb) {             // split: piece `set` of A, of B (into register set `to`)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[decltype(set)::value][i] = frag(sb, oa[i], decltype(set)::value);
+    };
+    auto read_b = [&](auto to, auto set, const char* sb) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[decltype(to)::value][j] = frag(sb, ob[j], decltype(set)::value);
+    };
+    // the steps of a stage but the last: multiply one, read the next
+    auto inner = [&](const char* sb) {
+        auto one = [&](auto s) {
+            load_set(std::integral_constant<int, decltype(s)::value + 1>{}, sb, decltype(s)::value + 1);
+            multiply(s);
+            spread<MI * NJ, READS, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        one(std::integral_constant<int, 0>{});
+        if constexpr (STEPS == 4) {
+            one(std::integral_constant<int, 1>{});
+            one(std::integral_constant<int, 2>{});
+        }
+    };
+    std::integral_constant<int, 0> S0;
+    std::integral_constant<int, 1> S1;                        // (the last step's set: STEPS is even)
+    std::integral_constant<int, 2> S2;
+    std::integral_constant<int, 3> S3;
 
-    // e4m3: the scale bytes of this tile's rows, SC_ROW to a row, over the reduction blocks of this split (whole words of four)
-    const unsigned* bs0 = nullptr;
-    const unsigned* bs1 = nullptr;
-    if constexpr (FMT == FMT_E4M3) {
-        const int w0 = s_beg >> 3, nw = (nk + 7) >> 3;                // words of four 128-blocks (eight stages)
-        for (int i = tid; i < TM * nw; i += 64 * NW) {
-            const int r = i / nw, w = i - r * nw;
-            reinterpret_cast<unsigned*>(smem + SC_AT)[r * (SC_ROW / 4) + w] =
-                *reinterpret_cast<const unsigned*>(p.a_sc + (long long)min(m0 + r, p.M - 1) * p.a_scp + 4 * (w0 + w));
-        }
-        if constexpr (EP == EP_GATED) {
-            const int blk = (n0 + wc * (CW / 2)) >> 7;                // a wave's columns of h lie in one 128-row block of the weights
-            bs0 = p.b_sc + (long long)min(blk, (p.N - 1) >> 7) * p.b_scp + w0;
-            bs1 = p.b2_sc + (long long)min(blk, (p.N - 1) >> 7) * p.b_scp + w0;
-        } else {
-            bs0 = p.b_sc + (long long)min((n0 + wc * CW) >> 7, (p.N - 1) >> 7) * p.b_scp + w0;
-        }
-        __syncthreads();
+    open_feed();
+#pragma unroll 1
+    for (int s = 0; s < SLOTS; ++s)
+        if (f_total > 0) issue();
+    if constexpr (SPLIT) f_slot = 0;                          // (also when there were fewer stages than slots)
+    int slot = 0, scslot = 0;
+    wait_vm<0>();
+    meet();
+    if constexpr (SPLIT) {
+        read_a(S2, smem);
+        read_b(S0, S0, smem);
+        read_b(S2, S2, smem);
+        read_a(S1, smem);
+        read_b(S1, S1, smem);
+    } else {
+        load_set(S0, smem, 0);
     }
+    for (; work.next < work.end; work.next += work.step) {
+        int tile_m, tile_n;
+        const int zz = p.by_tiles.of(work.next);
+        tile_of(p, work.next - zz * T, tile_m, tile_n);
+        const int m0 = tile_m * TM, n0 = tile_n * (GATED ? TN / 2 : TN);
+        const int s_beg = zz * p.kz, nk = min(all_stages, s_beg + p.kz) - s_beg;
+        const unsigned* bs0 = nullptr;
+        const unsigned* bs1 = nullptr;
+        if constexpr (FMT == FMT_E4M3) {                      // (a wave's columns lie in one 128-row block of the weights)
+            const int blk = min((n0 + wc * (GATED ? CW / 2 : CW)) >> 7, (p.N - 1) >> 7);
+            bs0 = p.b_sc + (long long)blk * p.b_scp + (s_beg >> 2);
+            if constexpr (GATED) bs1 = p.b2_sc + (long long)blk * p.b_scp + (s_beg >> 2);
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        // biases of this wave's columns, a column to a lane: gated, CW / 2 of each, side by side where they fit one register
+        float bias_a = 0.f, bias_b = 0.f;
+        if constexpr (EP == EP_LINEAR) {
+            static_assert(CW == 64, "");
+            bias_a = bias_lane(p.splits > 1 ? nullptr : p.bias, p.bias_bf16, n0 + wc * CW + lane, p.N);
+        } else if constexpr (GATED) {
+            const int f = n0 + wc * (CW / 2) + lane % (CW / 2);
+            if constexpr (CW == 64) {
+                bias_a = bias_lane(p.bias, p.bias_bf16, f, p.N);
+                const float up = bias_lane(p.bias2, p.bias_bf16, f, p.N);
+                bias_a = lane < 32 ? bias_a : up;
+            } else {
+                bias_a = bias_lane(p.bias, p.bias_bf16, f, p.N);
+                bias_b = bias_lane(p.bias2, p.bias_bf16, f, p.N);
+            }
+        }
+        auto scales = [&](int t) {                            // a stage is one 128-block
+            if constexpr (FMT == FMT_E4M3) {
+                if ((t & 3) == 0) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) sa4[i] = reinterpret_cast<const unsigned*>(smem + RING)[scslot * TM + wr * RW + i * 32 + li];
+                    sb4[0] = bs0[t >> 2];
+                    if constexpr (GATED) sb4[1] = bs1[t >> 2];
+                    scslot = (scslot + 1) & (SC_SLOTS - 1);
+                }
+                const int sh = (t & 3) << 3;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) sax[i] = (int)(sa4[i] >> sh);
+                sbx[0] = (int)(sb4[0] >> sh);
+                sbx[1] = (int)(sb4[1] >> sh);
+            }
+        };
+        // Split operands, products smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).  A piece's registers take the next stage's piece
+        // when its last product has been issued; B's first piece, needed to the end, has a second set.  Behind the first product all
+        // of the stage has been read: the waves meet there, and its slot is refilled three stages ahead.
+        // Past the last stage the copies go on, of the last rows, into slots that are not read again: one straight path.
+        if constexpr (SPLIT) {
+            for (int t = 0; t < nk; ++t) {
+                const char* cb = smem + slot * STAGE;
+                read_a(S0, cb);
+                product(S2, S0);
+                spread<MI * NJ, MI, 0>();
+                __builtin_amdgcn_sched_barrier(0);
+                slot = slot + 1 == SLOTS ? 0 : slot + 1;
+                wait_vm<NA + NB>();                           // the next stage has landed; the one behind it may be on its way
+                meet();
+                const char* nb = smem + slot * STAGE;
+                char* sb = smem + f_slot * STAGE;
+                const char* ab = abase + koff;
+                const char* bb = bbase + koff;
+                const char* bb2 = GATED ? bbase2 + koff : nullptr;
+                read_a(S2, nb);
+                product(S0, S2);
+                spread<MI * NJ, MI, 0>();
+                __builtin_amdgcn_sched_barrier(0);
+                read_b(S3, S0, nb);
+                read_b(S2, S2, nb);
+                product(S1, S1);
+                spread<MI * NJ, 2 * NJ, 0>();
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
+                product(S1, S0);
+                spread<MI * NJ, 0, NA>();
+                __builtin_amdgcn_sched_barrier(0);
+                read_a(S1, nb);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+                product(S0, S1);
+                spread<MI * NJ, MI, NB>();
+                __builtin_amdgcn_sched_barrier(0);
+                read_b(S1, S1, nb);
+                product(S0, S0);
+                spread<MI * NJ, NJ, 0>();
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) fb[0][j] = fb[3][j];
+                f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
+                if (f_total > 0) {
+                    --f_total;
+                    next_stage();
+                }
+            }
+        }
+        if constexpr (!SPLIT) {
+            // one stage; the next one's first operands are read behind its last step
+            auto stage = [&](int t) {
+                scales(t);
+                inner(smem + slot * STAGE);
+                slot ^= 1;
+                if (--w_total > 0) {
+                    wait_vm<0>();                                 // the next stage has landed (and earlier results are stored)
+                    meet();
+                    load_set(S0, smem + slot * STAGE, 0);
+                    if (f_total > 0) issue();                     // into the slot that everyone has just read
+                }
+                multiply(S1);
+            };
+            // the same without the cases: the next stage is this tile's, and the copies are whole pieces of the same rows
+            auto steady = [&](int t, int run) {
+                const char* ab = abase + koff;
+                const char* bb = bbase + koff;
+                const char* bb2 = GATED ? bbase2 + koff : nullptr;
+                for (int left = run; left > 0; --left, ++t) {
+                    scales(t);
+                    char* sb = smem + slot * STAGE;
+                    inner(sb);
+                    slot ^= 1;
+                    wait_vm<0>();
+                    meet();
+                    load_set(S0, smem + slot * STAGE, 0);
+    #pragma unroll
+                    for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
+    #pragma unroll
+                    for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+                    ab += ROWB; bb += ROWB;
+                    if constexpr (GATED) bb2 += ROWB;
+                    multiply(S1);
+                    spread<MI * NJ, READS, NA + NB>();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                koff += (long long)run * ROWB;
+                f_kin += run; f_left -= run; f_total -= run; w_total -= run;
+                f_slot = slot;                                    // (the slot read now is refilled next)
+            };
+            for (int t = 0; t < nk; ++t) {
+                // (a group of scale words begins with a copy of its own, a last stage may end inside the rows)
+                int run = min(nk - 1 - t, f_left - 1);
+                if (FMT == FMT_E4M3) run = min(run, (4 - (f_kin & 3)) & 3);
+                if (f_total > 0 && run > 0) {
+                    steady(t, run);
+                    t += run;
+                }
+                stage(t);
+            }
+        }
 
-#pragma unroll
-    for (int s = 0; s < NST - 1; ++s)
-        if (s < nk) issue(s);
-
-    int slot = 0, islot = NST - 1;
-    unsigned sa4[2] = {0, 0}, sb4[2] = {0, 0};
-    for (int t = 0; t < nk; ++t) {
-        // stage t has landed once at most the two later stages' copies are in flight
-        if (t + 2 < nk) wait_vm<2 * NGL>();
-        else if (t + 1 < nk) wait_vm<NGL>();
-        else wait_vm<0>();
-        __builtin_amdgcn_s_barrier();                                 // everyone's copies of stage t; everyone done with stage t - 1
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + NST - 1 < nk) issue(islot);                           // into the slot that stage t - 1 left
-        const char* sb = smem + slot * STAGE;
-        slot = (slot + 1) & (NST - 1);
-        islot = (islot + 1) & (NST - 1);
-        if constexpr (FMT == FMT_BF16) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                bf16x8 a[2], b[NJ];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) a[i] = *reinterpret_cast<const bf16x8*>(sb + (oa[i] ^ (s * 32)));
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) b[j] = *reinterpret_cast<const bf16x8*>(sb + (ob[j] ^ (s * 32)));
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-            }
-        } else {
-            if ((t & 7) == 0) {                                       // (splits start on a multiple of eight stages)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) sa4[i] = reinterpret_cast<const unsigned*>(smem + SC_AT)[(wr * 64 + i * 32 + li) * (SC_ROW / 4) + (t >> 3)];
-                sb4[0] = bs0[t >> 3];
-                if constexpr (EP == EP_GATED) sb4[1] = bs1[t >> 3];
-            }
-            const int sh = (t & 6) << 2;                              // byte of the word: two stages to a block
-            const int sa[2] = {(int)(sa4[0] >> sh), (int)(sa4[1] >> sh)};
-            const int sbv[2] = {(int)(sb4[0] >> sh), (int)(sb4[1] >> sh)};
-            i32x8 a[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const i32x4 lo = *reinterpret_cast<const i32x4*>(sb + oa[i]), hi = *reinterpret_cast<const i32x4*>(sb + (oa[i] ^ 16));
-                a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+        const int row0 = m0 + wr * RW;
+        if constexpr (EP == EP_LINEAR) {
+            const int col0 = n0 + wc * CW;
+            const bool to_slab = p.splits > 1;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const i32x4 lo = *reinterpret_cast<const i32x4*>(sb + ob[j]), hi = *reinterpret_cast<const i32x4*>(sb + (ob[j] ^ 16));
-                const i32x8 b = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                const int sbj = (EP == EP_GATED && j >= NJ / 2) ? sbv[1] : sbv[0];
+                float b[2][8];
+                bias_of(bias_a, j * 32, b, wh);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b, acc[i][j], 0, 0, 0, sa[i], 0, sbj);
-            }
-        }
-    }
-    __syncthreads();                                                  // all fragments read: the ring becomes the waves' epilogue images
-
-    float* img = reinterpret_cast<float*>(smem) + wid * 32 * LDP;
-    float* rowmax = reinterpret_cast<float*>(smem + NW * 32 * LDP * 4);       // [TM][WN] (EP_GATED)
-    float cs0[8], cs1[8];
+                for (int i = 0; i < MI; ++i) {
+                    float v[2][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) cs0[e] = cs1[e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        wave_lds_fence();
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) img[((r & 3) + 8 * (r >> 2) + 4 * lh) * LDP + j * 32 + li] = acc[i][j][r];
-        wave_lds_fence();
-        const int mrow0 = m0 + wr * 64 + i * 32;
-        if constexpr (EP == EP_LINEAR) {
-            constexpr int LPR = CW / 8, RP = 64 / LPR;                // lanes to a row, rows to a pass
-            const int c = (lane % LPR) * 8, n = n0 + wc * CW + c;
-            const bool to_slab = gridDim.z > 1;
-            float bias[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                bias[e] = (!to_slab && p.bias && n + e < p.N) ? (p.bias_bf16 ? bf_load(p.bias, n + e) : reinterpret_cast<const float*>(p.bias)[n + e]) : 0.f;
-#pragma unroll
-            for (int pass = 0; pass < 32 / RP; ++pass) {
-                const int rr = pass * RP + lane / LPR, m = mrow0 + rr;
-                const f32x4 lo = *reinterpret_cast<const f32x4*>(img + rr * LDP + c), hi = *reinterpret_cast<const f32x4*>(img + rr * LDP + c + 4);
-                if (m >= p.M || n >= p.N) continue;
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) + bias[e];
-                if (to_slab) {
-                    float* d = p.slab + ((long long)zz * p.M + m) * p.N + n;
-                    if ((p.N & 3) == 0 && n + 8 <= p.N) {
-                        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
-                        *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) if (n + e < p.N) d[e] = v[e];
-                    }
-                } else if (p.c_type == T_F32) {
-                    float* d = reinterpret_cast<float*>(p.C) + (long long)m * p.ldc + n;
-                    if (p.c_vec && n + 8 <= p.N) {
-                        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
-                        *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) if (n + e < p.N) d[e] = v[e];
-                    }
-                } else {
-                    unsigned short* d = reinterpret_cast<unsigned short*>(p.C) + (long long)m * p.ldc + n;
-                    if (p.c_vec && n + 8 <= p.N) {
-                        *reinterpret_cast<u32x4*>(d) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) if (n + e < p.N) d[e] = bf_bits(v[e]);
-                    }
+                    for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = acc[i][j][r] + b[r >> 3][r & 7];
+                    const int r0 = opaque(row0 + i * 32), c0 = opaque(col0 + j * 32);
+                    if (to_slab) store_f32(p.slab + (long long)zz * p.M * p.N, p.N, r0, c0, p.M, p.N, v, wh);
+                    else if (p.c_type == T_F32) store_f32(reinterpret_cast<float*>(p.C), p.ldc, r0, c0, p.M, p.N, v, wh);
+                    else store_bf16(reinterpret_cast<unsigned short*>(p.C), p.ldc, r0, c0, p.M, p.N, v, wh);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        } else if constexpr (EP == EP_GATED) {
-            constexpr int HW = CW / 2, LPR = HW / 8, RP = 64 / LPR;
-            const int c = (lane % LPR) * 8, f = n0 + wc * HW + c;
-            float bg[8], bu[8];
+        } else if constexpr (GATED) {
+            constexpr int HJ = NJ / 2;
+            const int col0 = n0 + wc * (CW / 2), N16 = (p.N + 15) & ~15;
+            auto gate = [&](auto gelu) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool in = f + e < p.N;
-                bg[e] = (p.bias && in) ? (p.bias_bf16 ? bf_load(p.bias, f + e) : reinterpret_cast<const float*>(p.bias)[f + e]) : 0.f;
-                bu[e] = (p.bias2 && in) ? (p.bias_bf16 ? bf_load(p.bias2, f + e) : reinterpret_cast<const float*>(p.bias2)[f + e]) : 0.f;
-            }
-            const bool quant = p.c_type == T_E4M3;
+                for (int j = 0; j < HJ; ++j) {
+                    const int c = opaque(col0 + j * 32);
+                    float bg[2][8], bu[2][8];
+                    bias_of(bias_a, j * 32, bg, wh);
+                    bias_of(CW == 64 ? bias_a : bias_b, CW == 64 ? 32 : j * 32, bu, wh);
 #pragma unroll
-            for (int pass = 0; pass < 32 / RP; ++pass) {
-                const int rr = pass * RP + lane / LPR, m = mrow0 + rr;
-                float* src = img + rr * LDP + c;
-                const f32x4 a0 = *reinterpret_cast<const f32x4*>(src), a1 = *reinterpret_cast<const f32x4*>(src + 4);
-                const f32x4 b0 = *reinterpret_cast<const f32x4*>(src + HW), b1 = *reinterpret_cast<const f32x4*>(src + HW + 4);
-                float a[8], b[8], h[8];
+                    for (int i = 0; i < MI; ++i) {
+                        float a[2][8], b[2][8], h[2][8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    a[e] = (e < 4 ? a0[e & 3] : a1[e & 3]) + bg[e];
-                    b[e] = (e < 4 ? b0[e & 3] : b1[e & 3]) + bu[e];
-                    float v, d;
-                    if (p.c_type == T_BF16 || p.c_type == T_E4M3) act_value<true>(p.act, a[e], v, d);
-                    else act_value<false>(p.act, a[e], v, d);
-                    h[e] = f + e < p.N ? v * b[e] : 0.f;              // columns between N and the pitch hold zeros
-                }
-                if (quant) {
-                    float mx = 0.f;
+                        for (int r = 0; r < 16; ++r) {
+                            const int q = r >> 3, e = r & 7;
+                            a[q][e] = acc[i][j][r] + bg[q][e];
+                            b[q][e] = acc[i][j + HJ][r] + bu[q][e];
+                            float v, d;
+                            act_value<FAST, decltype(gelu)::value>(p.act, a[q][e], v, d);
+                            h[q][e] = v * b[q][e];
+                            if (!FAST && (r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
+                        clear_beyond(h, c, p.N, wh);          // columns between N and the pitch hold zeros
+                        const int r0 = opaque(row0 + i * 32);
+                        if constexpr (EP == EP_GATED_Q) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, finite_abs(h[e]));
-#pragma unroll
-                    for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-                    if (lane % LPR == 0) rowmax[(wr * 64 + i * 32 + rr) * WN + wc] = mx;
-                    *reinterpret_cast<f32x4*>(src) = f32x4{h[0], h[1], h[2], h[3]};       // this lane's own places of the image
-                    *reinterpret_cast<f32x4*>(src + 4) = f32x4{h[4], h[5], h[6], h[7]};
-                    continue;
-                }
-                if (m >= p.M || f >= p.N) continue;
-                if (p.c_type == T_F32) {
-                    float* d = reinterpret_cast<float*>(p.C) + (long long)m * p.ldc + f;  // pitch a multiple of 8
-                    *reinterpret_cast<f32x4*>(d) = f32x4{h[0], h[1], h[2], h[3]};
-                    *reinterpret_cast<f32x4*>(d + 4) = f32x4{h[4], h[5], h[6], h[7]};
-                } else {
-                    store_planes8(reinterpret_cast<unsigned short*>(p.C), p.c_plane, p.c_type == T_PLANES ? 3 : 1, (long long)m * p.ldc + f, h);
-                }
-                if (p.gu) {
-                    const long long o = (long long)m * p.ldgu + f;
-                    if (p.gu_f32) {
-                        float* d = reinterpret_cast<float*>(p.gu) + o;
-                        *reinterpret_cast<f32x4*>(d) = f32x4{a[0], a[1], a[2], a[3]};
-                        *reinterpret_cast<f32x4*>(d + 4) = f32x4{a[4], a[5], a[6], a[7]};
-                        *reinterpret_cast<f32x4*>(d + p.gu_half) = f32x4{b[0], b[1], b[2], b[3]};
-                        *reinterpret_cast<f32x4*>(d + p.gu_half + 4) = f32x4{b[4], b[5], b[6], b[7]};
-                    } else {
-                        unsigned short* d = reinterpret_cast<unsigned short*>(p.gu);
-                        store_planes8(d, 0, 1, o, a);
-                        store_planes8(d, 0, 1, o + p.gu_half, b);
+                            for (int r = 0; r < 16; ++r) acc[i][j][r] = h[r >> 3][r & 7];
+                        } else if constexpr (EP == EP_GATED) {
+                            store_bf16(reinterpret_cast<unsigned short*>(p.C), p.ldc, r0, c, p.M, N16, h, wh);
+                            if (p.gu) {
+                                store_24(reinterpret_cast<unsigned short*>(p.gu), p.gu_lo, p.ldgu, r0, c, p.M, N16, a, wh);
+                                store_24(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, p.gu_lo + p.gu_half, p.ldgu, r0, c, p.M, N16, b, wh);
+                            }
+                        } else {
+                            if (p.gu) {
+                                store_f32(reinterpret_cast<float*>(p.gu), p.ldgu, r0, c, p.M, N16, a, wh);
+                                store_f32(reinterpret_cast<float*>(p.gu) + p.gu_half, p.ldgu, r0, c, p.M, N16, b, wh);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                            store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, N16, h, wh);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);    // one block at a time: mixing them costs more registers than there are
                     }
                 }
-            }
-            if (quant) {
-                __syncthreads();                                      // both column waves' row maxima
+            };
+            if (p.act == ACT_GELU) gate(std::true_type{});
+            else gate(std::false_type{});
+            if constexpr (EP == EP_GATED_Q) {                 // the tile's 128 columns of h are one block of every row
+                static_assert(WN * CW == 256, "");
+                float* mx = reinterpret_cast<float*>(smem + RING + SC_B);
 #pragma unroll
-                for (int pass = 0; pass < 32 / RP; ++pass) {
-                    const int rr = pass * RP + lane / LPR, m = mrow0 + rr;
-                    const float* src = img + rr * LDP + c;
-                    const f32x4 h0 = *reinterpret_cast<const f32x4*>(src), h1 = *reinterpret_cast<const f32x4*>(src + 4);
-                    float mx = 0.f;
+                for (int i = 0; i < MI; ++i) {
+                    float m = 0.f;
 #pragma unroll
-                    for (int w = 0; w < WN; ++w) mx = fmaxf(mx, rowmax[(wr * 64 + i * 32 + rr) * WN + w]);
-                    const int e = scale_exp(mx);
+                    for (int j = 0; j < HJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) m = fmaxf(m, finite_abs(acc[i][j][r]));
+                    m = fmaxf(m, __shfl_xor(m, 32, 64));
+                    if (lh == 0) mx[(wr * RW + i * 32 + li) * WN + wc] = m;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WN; ++w) m = fmaxf(m, mx[(wr * RW + i * 32 + li) * WN + w]);
+                    const int r0 = opaque(row0 + i * 32), e = scale_exp(m), row = r0 + li;
                     const float s = pow2i(-e);
-                    if (m >= p.M) continue;
-                    float h[8];
+                    if (wc == 0 && lh == 0 && row < p.M) p.q_sc[(long long)row * p.q_scp + tile_n] = (unsigned char)(e + 127);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) h[q] = nan_if_not_finite((q < 4 ? h0[q & 3] : h1[q & 3])) * s;
-                    // the whole 128-column block is written, zeros beyond N: rows are padded to blocks
-                    *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.C) + (long long)m * p.ldc + f) =
-                        u32x2{pack_e4m3(h[0], h[1], h[2], h[3]), pack_e4m3(h[4], h[5], h[6], h[7])};
-                    if (wc == 0 && lane % LPR == 0) p.q_sc[(long long)m * p.q_scp + tile_n] = (unsigned char)(e + 127);
+                    for (int j = 0; j < HJ; ++j) {
+                        unsigned u[2][2];
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4)
+                            u[r >> 3][(r >> 2) & 1] = pack_e4m3(nan_if_not_finite(acc[i][j][r]) * s, nan_if_not_finite(acc[i][j][r + 1]) * s,
+                                                                nan_if_not_finite(acc[i][j][r + 2]) * s, nan_if_not_finite(acc[i][j][r + 3]) * s);
+                        // the whole 128-column block is written, zeros beyond N: rows are padded to blocks
+                        const u32x4 x = wh.turn2(u32x2{u[0][0], u[0][1]}, u32x2{u[1][0], u[1][1]});
+                        const int c = opaque(col0 + j * 32) + 16 * wh.p2, r = r0 + wh.r2;
+                        if (r < p.M) *reinterpret_cast<u32x4*>(reinterpret_cast<unsigned char*>(p.C) + (long long)r * p.ldc + c) = x;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-                __syncthreads();                                      // the images are read before the next 32 rows replace them
+                __syncthreads();                              // the maxima are read before the next tile's replace them
             }
         } else {
-            constexpr int LPR = CW / 8, RP = 64 / LPR;
-            const int c = (lane % LPR) * 8, f = n0 + wc * CW + c;
+            const int col0 = n0 + wc * CW, strip = tile_m * WM + wr;
+            auto gate = [&](auto gelu) {
 #pragma unroll
-            for (int pass = 0; pass < 32 / RP; ++pass) {
-                const int rr = pass * RP + lane / LPR, m = mrow0 + rr;
-                const f32x4 lo = *reinterpret_cast<const f32x4*>(img + rr * LDP + c), hi = *reinterpret_cast<const f32x4*>(img + rr * LDP + c + 4);
-                if (m >= p.M || f >= p.gu_half) continue;             // zeros from N to gu_half: both halves are one operand of the next product
-                float a[8], b[8], da[8], db[8];
-                const long long o = (long long)m * p.ldgu + f;
-                if (p.gu_f32) {
-                    const float* s = reinterpret_cast<const float*>(p.gu) + o;
-                    const f32x4 a0 = *reinterpret_cast<const f32x4*>(s), a1 = *reinterpret_cast<const f32x4*>(s + 4);
-                    const f32x4 b0 = *reinterpret_cast<const f32x4*>(s + p.gu_half), b1 = *reinterpret_cast<const f32x4*>(s + p.gu_half + 4);
+                for (int j = 0; j < NJ; ++j) {
+                    const int c = opaque(col0 + j * 32);
+                    if (c >= p.gu_half) continue;             // (uniform)
+                    float cs[32];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) { a[e] = e < 4 ? a0[e & 3] : a1[e & 3]; b[e] = e < 4 ? b0[e & 3] : b1[e & 3]; }
-                } else {
-                    const unsigned short* s = reinterpret_cast<const unsigned short*>(p.gu) + o;
-                    const u32x4 qa = *reinterpret_cast<const u32x4*>(s), qb = *reinterpret_cast<const u32x4*>(s + p.gu_half);
+                    for (int k = 0; k < 32; ++k) cs[k] = 0.f;
+                    auto one = [&](int i, float (&a)[2][8], float (&b)[2][8]) {
+                        float da[2][8], db[2][8];
+                        const int r0 = opaque(row0 + i * 32);
+                        const bool row_in = r0 + li < p.M;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[2 * e] = bf_lo(qa[e]); a[2 * e + 1] = bf_hi(qa[e]);
-                        b[2 * e] = bf_lo(qb[e]); b[2 * e + 1] = bf_hi(qb[e]);
+                        for (int r = 0; r < 16; ++r) {
+                            const int q = r >> 3, e = r & 7;
+                            float v, d;
+                            act_value<FAST, decltype(gelu)::value>(p.act, a[q][e], v, d);
+                            const float dh = acc[i][j][r];
+                            da[q][e] = row_in ? dh * b[q][e] * d : 0.f;
+                            db[q][e] = row_in ? dh * v : 0.f;
+                            if (!FAST && (r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
+                        clear_beyond(da, c, p.N, wh);         // zeros from N to gu_half: both halves are one operand of the next product
+                        clear_beyond(db, c, p.N, wh);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            cs[r] += da[r >> 3][r & 7];
+                            cs[16 + r] += db[r >> 3][r & 7];
+                        }
+                        if constexpr (FAST) {
+                            unsigned short* C = reinterpret_cast<unsigned short*>(p.C);
+                            store_bf16(C, p.ldc, r0, c, p.M, p.gu_half, da, wh);
+                            store_bf16(C + p.gu_half, p.ldc, r0, c, p.M, p.gu_half, db, wh);
+                        } else {
+                            store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, p.gu_half, da, wh);
+                            store_split(reinterpret_cast<char*>(p.C) + split_at(p.gu_half, 0), p.ldc, r0, c, p.M, p.gu_half, db, wh);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    if constexpr (FAST) {
+                        const unsigned short* hi = reinterpret_cast<const unsigned short*>(p.gu);
+                        Raw24 ra[MI], rb[MI];
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            load_24(hi, p.gu_lo, p.ldgu, opaque(row0 + i * 32), c, p.M, p.gu_half, ra[i], wh);
+                            load_24(hi + p.gu_half, p.gu_lo + p.gu_half, p.ldgu, opaque(row0 + i * 32), c, p.M, p.gu_half, rb[i], wh);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            float a[2][8], b[2][8];
+                            unpack_24(ra[i], a, wh);
+                            unpack_24(rb[i], b, wh);
+                            one(i, a, b);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            float a[2][8], b[2][8];
+                            Raw32 ra, rb;
+                            const int rl = opaque(row0 + i * 32);
+                            load_f32(reinterpret_cast<const float*>(p.gu), p.ldgu, rl, c, p.M, p.gu_half, ra, wh);
+                            load_f32(reinterpret_cast<const float*>(p.gu) + p.gu_half, p.ldgu, rl, c, p.M, p.gu_half, rb, wh);
+                            unpack_f32(ra, a, wh);
+                            unpack_f32(rb, b, wh);
+                            one(i, a, b);
+                        }
+                    }
+                    if (p.colpart) {
+                        // sums over the 32 rows of a half wave, in a fixed order, halving the values a lane holds with every step: lane
+                        // (li, lh) ends with the sum of value li
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) {
+                            const bool hi = (lane & o) != 0;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (k < o) {
+                                    const float keep = hi ? cs[k + o] : cs[k], give = hi ? cs[k] : cs[k + o];
+                                    cs[k] = keep + __shfl_xor(give, o, 64);
+                                }
+                        }
+                        const int r = li & 15, col = c + 16 * (r >> 3) + 8 * lh + (r & 7);
+                        if (col < p.N) p.colpart[((long long)strip * 2 + (li >> 4)) * p.N + col] = cs[0];
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float dh = e < 4 ? lo[e & 3] : hi[e & 3];
-                    float v, d;
-                    if (p.c_type == T_BF16) act_value<true>(p.act, a[e], v, d);
-                    else act_value<false>(p.act, a[e], v, d);
-                    const bool in = f + e < p.N;
-                    da[e] = in ? dh * b[e] * d : 0.f;
-                    db[e] = in ? dh * v : 0.f;
-                    cs0[e] += da[e];
-                    cs1[e] += db[e];
-                }
-                unsigned short* C = reinterpret_cast<unsigned short*>(p.C);
-                const int np = p.c_type == T_PLANES ? 3 : 1;
-                store_planes8(C, p.c_plane, np, (long long)m * p.ldc + f, da);
-                store_planes8(C, p.c_plane, np, (long long)m * p.ldc + p.gu_half + f, db);
-            }
+            };
+            if (p.act == ACT_GELU) gate(std::true_type{});
+            else gate(std::false_type{});
         }
     }
-    if constexpr (EP == EP_GATED_BWD) {
-        // column sums of this wave's 64 rows, in a fixed order: over a lane's rows above, over the lanes of a column here
-        if (p.colpart) {
-            constexpr int LPR = CW / 8;
-            const int f = n0 + wc * CW + (lane % LPR) * 8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-#pragma unroll
-                for (int o = LPR; o < 64; o <<= 1) { cs0[e] += __shfl_xor(cs0[e], o, 64); cs1[e] += __shfl_xor(cs1[e], o, 64); }
-            }
-            float* d = p.colpart + (long long)(tile_m * WM + wr) * 2 * p.N;
-            if (lane < LPR)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (f + e < p.N) { d[f + e] = cs0[e]; d[p.N + f + e] = cs1[e]; }
-        }
-    }
+    if constexpr (SPLIT) wait_vm<0>();                        // no copy may still be on its way when the LDS passes to others
 }
 
 // ---- reduction across rows -----------------------------------------------------------------------------------------
-// A stage is 32 rows of both operands, TM / TN columns of 2 bytes.  The MFMA wants eight consecutive reduction steps of one
-// column in a lane: two transposing LDS reads (ds_read_b64_tr_b16: a 16-lane group reads 4 rows x 16 columns and lane i gets
-// column i) deliver them.  A row of the image is whole multiples of 256 bytes, so rows collide on the banks; the 32-byte granules
-// of a row are therefore stored at granule ^ 2 (row & 3), which gives the four rows x two granules that 32 lanes read
-// together eight different granules.
+// A stage is 32 rows of both operands, TM / TN columns of 2 bytes (split operands: 16 rows, 6 bytes a column).  The MFMA wants
+// eight consecutive reduction steps of one column in a lane: two transposing LDS reads (ds_read_b64_tr_b16: a 16-lane group
+// reads 4 rows x 16 columns and lane i gets column i) deliver them.  A row of the image is whole multiples of 256 bytes, so
+// rows collide on the banks; the 32-byte granules of a row are therefore stored at granule ^ 2 (row & 3), which gives the four
+// rows x two granules (neighbours, or three apart in a split row) that 32 lanes read together eight different places.
 struct ColArgs {
-    const char* A; long long lda, a_plane; int a_cols;        // byte pitch; columns that may be read (a multiple of 8)
-    const char* B; long long ldb, b_plane; int b_cols;
+    const char* A; long long lda; int a_cols;                 // byte pitch; columns that may be read (a multiple of 8; split: of 16)
+    const char* B; long long ldb; int b_cols;
     int R;                                                    // reduction rows
     int M, N;                                                 // outputs
-    int pairs, rz;                                            // rows of one split (a multiple of 32)
+    int rz;                                                   // rows of one split (a multiple of 32)
     int tiles_m, tiles_n;
     float* slab;                                              // [z][M][N]
 };
 
-template <int WM, int WN, int NJ>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : (NJ == 2 ? 2 : 1)) void gemm_cols(const ColArgs p) {
-    constexpr int NW = WM * WN, TM = WM * 64, CW = NJ * 32, TN = WN * CW;
-    constexpr int ARB = TM * 2, BRB = TN * 2;                 // bytes of an image row
-    constexpr int STAGE = 32 * (ARB + BRB);
-    constexpr int NA = 32 * ARB / 1024 / NW, NB = 32 * BRB / 1024 / NW, NGL = NA + NB;
-    constexpr int LDP = CW + 4;
-    constexpr int RING = NST * STAGE, EPI_B = NW * 32 * LDP * 4;
-    __shared__ __attribute__((aligned(1024))) char smem[RING > EPI_B ? RING : EPI_B];
+template <bool SPLIT, int WM, int WN, int MI, int NJ>
+__global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols(const ColArgs p) {
+    constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
+    constexpr int EB = SPLIT ? 6 : 2, SR = SPLIT ? 16 : 32, SLOTS = SPLIT ? 3 : 4;        // bytes of a column, rows of a stage
+    constexpr int ARB = TM * EB, BRB = TN * EB;               // bytes of an image row
+    constexpr int STAGE = SR * (ARB + BRB), RING = SLOTS * STAGE;
+    constexpr int NA = SR * ARB / 1024 / NW, NB = SR * BRB / 1024 / NW, NGL = NA + NB;
+    __shared__ __attribute__((aligned(1024))) char smem[RING + NW * TURN_B];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid / WN, wc = wid % WN;
-    const int li = lane & 31, lh = lane >> 5;
+    const int lh = lane >> 5;
+    const Where wh(smem + RING + wid * TURN_B);
     // Splits of the reduction first: all output tiles of one row range run together on one XCD and share its rows in L2.
     const int T = p.tiles_m * p.tiles_n, nz = (int)gridDim.z;
     int zz, tile;
@@ -604,67 +1038,64 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : (NJ == 2 ? 2 : 1))
     const int tile_m = tile / p.tiles_n, tile_n = tile % p.tiles_n;
     const int m0 = tile_m * TM, n0 = tile_n * TN;
     const int rbeg = zz * p.rz, rows = max(0, min(p.rz, p.R - rbeg));
-    const int ks = (rows + 31) >> 5, nk = ks * p.pairs;
+    const int nk = (rows + SR - 1) / SR;
 
-    // instruction j of this wave fills 1 KiB = 1024 / ARB rows of the image
-    constexpr int ALR = ARB / 16, BLR = BRB / 16;             // lanes to an image row
-    const char* asrc[NA];
-    const char* bsrc[NB];
+    // instruction j of this wave fills 1 KiB of the image; a piece of 16 bytes past the readable columns reads the row's first instead
+    constexpr int ALR = ARB / 16, BLR = BRB / 16;             // pieces of an image row
+    unsigned aofs[NA], bofs[NB];
     int arow[NA], brow[NB];
+    auto column = [&](int c0, int pc, int cols) -> unsigned {
+        if constexpr (SPLIT) return c0 + (pc / 6) * 16 < cols ? (unsigned)(c0 / 16 * 96 + pc * 16) : 0u;
+        else return c0 + pc * 8 < cols ? 2u * (unsigned)(c0 + pc * 8) : 0u;
+    };
 #pragma unroll
     for (int j = 0; j < NA; ++j) {
-        const int pos = (wid * NA + j) * 64 + lane, r = pos / ALR, pc = (pos % ALR) ^ ((r & 3) << 2);
-        const int col = m0 + pc * 8;
+        const int pos = (wid * NA + j) * 64 + lane, r = pos / ALR;
         arow[j] = r;
-        asrc[j] = p.A + (long long)(rbeg + r) * p.lda + 2LL * (col + 8 <= p.a_cols ? col : 0);
+        aofs[j] = (unsigned)r * (unsigned)p.lda + column(m0, (pos % ALR) ^ ((r & 3) << 2), p.a_cols);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int pos = (wid * NB + j) * 64 + lane, r = pos / BLR, pc = (pos % BLR) ^ ((r & 3) << 2);
-        const int col = n0 + pc * 8;
+        const int pos = (wid * NB + j) * 64 + lane, r = pos / BLR;
         brow[j] = r;
-        bsrc[j] = p.B + (long long)(rbeg + r) * p.ldb + 2LL * (col + 8 <= p.b_cols ? col : 0);
+        bofs[j] = (unsigned)r * (unsigned)p.ldb + column(n0, (pos % BLR) ^ ((r & 3) << 2), p.b_cols);
     }
-    int pair = 0, kin = 0;
-    long long aoff = (long long)plane_a(p.pairs == 1 ? 5 : 0) * p.a_plane, boff = (long long)plane_b(p.pairs == 1 ? 5 : 0) * p.b_plane;
-    auto issue = [&](int slot) {
-        char* sb = smem + slot * STAGE;
-        const int left = rows - kin * 32;                     // uniform
+    const char* ab = p.A + (long long)rbeg * p.lda;
+    const char* bb = p.B + (long long)rbeg * p.ldb;
+    const char* zero = reinterpret_cast<const char*>(zero_piece);
+    int f_slot = 0, left = rows;                              // rows not yet copied
+    // A stage's copies; rows past the end are zeros, and past the last stage all of them are: one straight path
+    auto copy_a = [&]() {
 #pragma unroll
-        for (int j = 0; j < NA; ++j) {
-            const char* s = asrc[j] + aoff;
-            if (left < 32) s = arow[j] < left ? s : reinterpret_cast<const char*>(zero_piece);
-            glds16(s, sb + (wid * NA + j) * 1024);
-        }
+        for (int j = 0; j < NA; ++j) glds16(arow[j] < left ? ab + aofs[j] : zero, smem + f_slot * STAGE + (wid * NA + j) * 1024);
+    };
+    auto copy_b = [&]() {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const char* s = bsrc[j] + boff;
-            if (left < 32) s = brow[j] < left ? s : reinterpret_cast<const char*>(zero_piece);
-            glds16(s, sb + 32 * ARB + (wid * NB + j) * 1024);
-        }
-        if (++kin == ks) {
-            kin = 0;
-            ++pair;
-            aoff = (long long)plane_a(pair) * p.a_plane;
-            boff = (long long)plane_b(pair) * p.b_plane;
-        } else {
-            aoff += 32 * p.lda;
-            boff += 32 * p.ldb;
-        }
+        for (int j = 0; j < NB; ++j) glds16(brow[j] < left ? bb + bofs[j] : zero, smem + f_slot * STAGE + SR * ARB + (wid * NB + j) * 1024);
+    };
+    auto advance = [&]() {
+        ab += SR * p.lda;
+        bb += SR * p.ldb;
+        left -= SR;
+        f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
     };
 
     // a lane's first transposing read of a 32-column block: row 8 (lane >> 5) + ((lane & 15) >> 2), columns 16 ((lane >> 4) & 1) + 4 (lane & 3)
-    const int kr = 8 * lh + ((lane & 15) >> 2), sw = (kr & 3) << 2;
-    const int pc0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in8 = (lane & 1) * 8;
-    int oa[2], ob[NJ];
+    constexpr int PC = SPLIT ? 3 : 1;                         // pieces of a value
+    const int kr = 8 * lh + ((lane & 15) >> 2);
+    auto granule = [&](int c, int k) { return ((((c >> 4) + ((lane >> 4) & 1)) * PC + k) ^ ((kr & 3) << 1)) * 32 + (lane & 3) * 8; };
+    int oa[PC][MI], ob[PC][NJ];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) oa[i] = kr * ARB + ((((wr * 64 + i * 32) / 8 + pc0) ^ sw) << 4) + in8;
+    for (int k = 0; k < PC; ++k) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) ob[j] = 32 * ARB + kr * BRB + ((((wc * CW + j * 32) / 8 + pc0) ^ sw) << 4) + in8;
+        for (int i = 0; i < MI; ++i) oa[k][i] = kr * ARB + granule(wr * RW + i * 32, k);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ob[k][j] = SR * ARB + kr * BRB + granule(wc * CW + j * 32, k);
+    }
 
-    f32x16 acc[2][NJ];
+    f32x16 acc[MI][NJ];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -676,60 +1107,125 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : (NJ == 2 ? 2 : 1))
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * rb));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-
+    bf16x8 fa[SPLIT ? 3 : 2][MI], fb[SPLIT ? 4 : 2][NJ];
+    // register set `to` of A / B: piece k (split), or step s of 16 rows
+    auto read_a = [&](auto to, int k, const char* sb, int s) {
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s)
-        if (s < nk) issue(s);
-    int slot = 0, islot = NST - 1;
-    for (int t = 0; t < nk; ++t) {
-        if (t + 2 < nk) wait_vm<2 * NGL>();
-        else if (t + 1 < nk) wait_vm<NGL>();
-        else wait_vm<0>();
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + NST - 1 < nk) issue(islot);
-        const char* sb = smem + slot * STAGE;
-        slot = (slot + 1) & (NST - 1);
-        islot = (islot + 1) & (NST - 1);
+        for (int i = 0; i < MI; ++i) fa[decltype(to)::value][i] = frag(sb + oa[k][i] + s * 16 * ARB, ARB);
+    };
+    auto read_b = [&](auto to, int k, const char* sb, int s) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 a[2], b[NJ];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) a[i] = frag(sb + oa[i] + s * 16 * ARB, ARB);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) b[j] = frag(sb + ob[j] + s * 16 * BRB, BRB);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-        }
-    }
-    __syncthreads();
-
-    float* img = reinterpret_cast<float*>(smem) + wid * 32 * LDP;
-    constexpr int LPR = CW / 4, RP = 64 / LPR;                // lanes to a row (4 columns each), rows to a pass
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        wave_lds_fence();
+        for (int j = 0; j < NJ; ++j) fb[decltype(to)::value][j] = frag(sb + ob[k][j] + s * 16 * BRB, BRB);
+    };
+    auto product = [&](auto sa, auto sb) {
+        constexpr int x = decltype(sa)::value, y = decltype(sb)::value;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) img[((r & 3) + 8 * (r >> 2) + 4 * lh) * LDP + j * 32 + li] = acc[i][j][r];
-        wave_lds_fence();
-        const int c = (lane % LPR) * 4, n = n0 + wc * CW + c;
+            for (int i = 0; i < MI; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[y][j], fa[x][i], acc[i][j], 0, 0, 0);
+    };
+    std::integral_constant<int, 0> S0;
+    std::integral_constant<int, 1> S1;
+    std::integral_constant<int, 2> S2;
+    std::integral_constant<int, 3> S3;
+#pragma unroll 1
+    for (int s = 0; s < SLOTS; ++s) {
+        copy_a();
+        copy_b();
+        advance();
+    }
+    int slot = 0;
+    wait_vm<0>();
+    meet();
+    if constexpr (SPLIT) {
+        // the loop of gemm_rows' split operands
+        read_a(S2, 2, smem, 0);
+        read_b(S0, 0, smem, 0);
+        read_b(S2, 2, smem, 0);
+        read_a(S1, 1, smem, 0);
+        read_b(S1, 1, smem, 0);
+        for (int t = 0; t < nk; ++t) {
+            read_a(S0, 0, smem + slot * STAGE, 0);
+            product(S2, S0);
+            spread<MI * NJ, 2 * MI, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+            slot = slot + 1 == SLOTS ? 0 : slot + 1;
+            wait_vm<NGL>();
+            meet();
+            const char* nb = smem + slot * STAGE;
+            read_a(S2, 2, nb, 0);
+            product(S0, S2);
+            spread<MI * NJ, 2 * MI, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+            read_b(S3, 0, nb, 0);
+            product(S1, S1);
+            spread<MI * NJ, 2 * NJ, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+            read_b(S2, 2, nb, 0);
+            copy_a();
+            product(S1, S0);
+            spread<MI * NJ, 2 * NJ, NA>();
+            __builtin_amdgcn_sched_barrier(0);
+            read_a(S1, 1, nb, 0);
+            copy_b();
+            product(S0, S1);
+            spread<MI * NJ, 2 * MI, NB>();
+            __builtin_amdgcn_sched_barrier(0);
+            read_b(S1, 1, nb, 0);
+            product(S0, S0);
+            spread<MI * NJ, 2 * NJ, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+            advance();
 #pragma unroll
-        for (int pass = 0; pass < 32 / RP; ++pass) {
-            const int rr = pass * RP + lane / LPR, m = m0 + wr * 64 + i * 32 + rr;
-            const f32x4 v = *reinterpret_cast<const f32x4*>(img + rr * LDP + c);
-            if (m >= p.M || n >= p.N) continue;
-            float* d = p.slab + ((long long)zz * p.M + m) * p.N + n;
-            if ((p.N & 3) == 0 && n + 4 <= p.N) *reinterpret_cast<f32x4*>(d) = v;
-            else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) if (n + e < p.N) d[e] = v[e];
-            }
+            for (int j = 0; j < NJ; ++j) fb[0][j] = fb[3][j];
+        }
+    } else {
+        read_a(S0, 0, smem, 0);
+        read_b(S0, 0, smem, 0);
+        constexpr int READS = 2 * (MI + NJ);
+        for (int t = 0; t < nk; ++t) {
+            const char* cb = smem + slot * STAGE;
+            read_a(S1, 0, cb, 1);
+            read_b(S1, 0, cb, 1);
+            product(S0, S0);
+            spread<MI * NJ, READS, 0>();
+            __builtin_amdgcn_sched_barrier(0);
+            slot = slot + 1 == SLOTS ? 0 : slot + 1;
+            wait_vm<2 * NGL>();                               // the next stage has landed once the two behind it are all that is on its way
+            meet();
+            const char* nb = smem + slot * STAGE;
+            read_a(S0, 0, nb, 0);
+            read_b(S0, 0, nb, 0);
+            copy_a();
+            copy_b();
+            product(S1, S1);
+            spread<MI * NJ, READS, NGL>();
+            __builtin_amdgcn_sched_barrier(0);
+            advance();
         }
     }
+    wait_vm<0>();                                             // no copy may still be on its way when the LDS passes to others
+    // a lane's results of a 32 x 32 block: row lane & 31, element r = column (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
+    float* out = p.slab + (long long)zz * p.M * p.N;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int r0 = opaque(m0 + wr * RW + i * 32) + wh.r4, c0 = opaque(n0 + wc * CW + j * 32) + 4 * wh.p4;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * q + e];
+                u32x4 a, b;
+                wh.turn(raw4(v), wh.lh, raw4(v + 4), 2 + wh.lh, a, b);
+                const int n = c0 + 16 * q;
+                if (n >= p.N) continue;
+                if (r0 < p.M) put_f32(out + (long long)r0 * p.N + n, a, n, p.N);
+                if (r0 + 16 < p.M) put_f32(out + (long long)(r0 + 16) * p.N + n, b, n, p.N);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
 }
 
 }  // namespace btvae_block

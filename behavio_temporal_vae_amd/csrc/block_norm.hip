@@ -232,22 +232,36 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd(const Args p) 
         for (int s = s0; s < s1; ++s) {
             const int row = s * p.G + gr;
             const long long o = (long long)row * p.N;
-            float d[E], y[E];
-            if (p.y) R::template load<BH>(p.y, o, p.N, t, y);
+            float d[E], y[E], u[E];
+            float mean = 0.f, q = 1.f;
+            if (p.y) {                                        // y becomes its normalised self, u what the gate multiplies
+                R::template load<BH>(p.y, o, p.N, t, y);
+                if (p.post != NONE) {
+                    mean = p.stats[row];
+                    q = p.stats[p.M + row];
+                }
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    y[i] = (y[i] - mean) * q;
+                    u[i] = p.post != NONE ? y[i] * w1[i] + c1[i] : y[i];
+                }
+            }
             if (p.dv) R::template load<RH>(p.dv, o, p.N, t, d);
             else {
 #pragma unroll
                 for (int i = 0; i < E; ++i) d[i] = 0.f;
             }
             if (p.dn) {
+                // the stream as the forward pass had it before its rounding
                 float e[E], h[E];
                 R::template load<BH>(p.dn, o, p.N, t, e);
-                R::template load<RH>(p.v, o, p.N, t, h);
-                const float mean = p.stats[2LL * p.M + row], q = p.stats[3LL * p.M + row];
+                R::template load<RH>(p.r, o, p.N, t, h);
+                const float mean2 = p.stats[2LL * p.M + row], q2 = p.stats[3LL * p.M + row];
                 float se = 0.f, seh = 0.f;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    h[i] = (h[i] - mean) * q;                 // past N: finite, and met by e = 0 only
+                    if (p.y) h[i] += sv[i] * (g[i] * u[i]);
+                    h[i] = (h[i] - mean2) * q2;               // past N: finite, and met by e = 0 only
                     aw2[i] += e[i] * h[i];
                     ac2[i] += e[i];
                     e[i] *= w2[i];
@@ -257,29 +271,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd(const Args p) 
                 seh = row_sum<T>(seh, red, turn) * inv_n;
                 se = p.pre == LAYER ? row_sum<T>(se, red, turn) * inv_n : 0.f;
 #pragma unroll
-                for (int i = 0; i < E; ++i) d[i] += q * (e[i] - h[i] * seh - se);
+                for (int i = 0; i < E; ++i) d[i] += q2 * (e[i] - h[i] * seh - se);
             }
             if (p.dr) R::template store<RH>(p.dr, o, p.N, t, d);
             if (p.y) {
-                const float mean = p.post != NONE ? p.stats[row] : 0.f, q = p.post != NONE ? p.stats[p.M + row] : 1.f;
                 float se = 0.f, seh = 0.f;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const float hat = (y[i] - mean) * q;
-                    const float u = p.post != NONE ? hat * w1[i] + c1[i] : y[i];
-                    const float ud = u * d[i];
+                    const float ud = u[i] * d[i];
                     dg[i] += sv[i] * ud;
                     as[i] += g[i] * ud;
-                    const float du = sv[i] * g[i] * d[i];
+                    d[i] *= sv[i] * g[i];
                     if (p.post != NONE) {
-                        aw1[i] += du * hat;
-                        ac1[i] += du;
-                        y[i] = hat;
-                        d[i] = du * w1[i];
+                        aw1[i] += d[i] * y[i];
+                        ac1[i] += d[i];
+                        d[i] *= w1[i];
                         se += d[i];
-                        seh += d[i] * hat;
-                    } else {
-                        d[i] = du;
+                        seh += d[i] * y[i];
                     }
                 }
                 if (p.post != NONE) {
@@ -415,8 +423,8 @@ BTVAE_API long long btvae_norm_gate_residual_ws(int M, int N, int G) {
     return 5LL * b.groups * N + (b.splits > 1 && G > 0 ? (long long)b.splits * g * N : 0);
 }
 
-// Gradients that are not wanted are null.  stats and `stream` as the forward pass left them (stream_in: the residual itself without a branch).
-BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* stream_in, const void* branch, const void* gate, int G, float scale, const float* scale_vec,
+// Gradients that are not wanted are null.  stats as the forward pass left them.
+BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* residual, const void* branch, const void* gate, int G, float scale, const float* scale_vec,
                                            const float* post_w, const float* post_b, const float* pre_w, int post, int pre, const float* stats, void* d_residual, void* d_branch, void* d_gate,
                                            float* d_scale, float* d_post_w, float* d_post_b, float* d_pre_w, float* d_pre_b, float* ws, long long ws_floats, int types, int M, int N, void* stream) {
     BTVAE_REQUIRE(M >= 0 && N > 0 && N <= bn_::MAX_N, "norm_gate_residual_bwd: %d columns (1 to %d)", N, bn_::MAX_N);
@@ -435,12 +443,12 @@ BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_n
     f.part = ws; f.strips = M == 0 ? 0 : b.groups; f.N = N;
     f.out[0] = d_post_w; f.out[1] = d_post_b; f.out[2] = d_normed || M == 0 ? d_pre_w : nullptr; f.out[3] = d_normed || M == 0 ? d_pre_b : nullptr; f.out[4] = d_scale;
     p.y = branch; p.g = gate; p.G = g; p.s = scale; p.sv = scale_vec; p.w1 = post_w; p.c1 = post_b; p.w2 = pre_w; p.post = post; p.pre = pre;
-    p.v = const_cast<void*>(stream_in); p.stats = const_cast<float*>(stats); p.M = M; p.N = N;
+    p.r = residual; p.stats = const_cast<float*>(stats); p.M = M; p.N = N;
     p.dv = d_stream; p.dn = d_normed; p.dr = d_residual; p.dy = d_branch; p.dg = d_gate; p.dg_part = gp ? ws + parts : nullptr;
     p.splits = b.splits; p.share = M / g; p.part = ws;
     for (int k = 0; k < 5; ++k) p.want |= f.out[k] ? 1 << k : 0;
     if (M > 0) {
-        const bool vec = N % 8 == 0 && al(d_stream) && al(d_normed) && al(stream_in) && al(branch) && al(gate) && al(d_residual) && al(d_branch) && al(d_gate) && (!p.dg_part || al(p.dg_part)) && al(ws);
+        const bool vec = N % 8 == 0 && al(d_stream) && al(d_normed) && al(residual) && al(branch) && al(gate) && al(d_residual) && al(d_branch) && al(d_gate) && (!p.dg_part || al(p.dg_part)) && al(ws);
         ProfScope prof(PK_BN, s, 0.0, (types == 3 ? 2.0 : 4.0) * M * N * 6);
         if (types == 0) bn_::launch<false, false, true>(p, vec, b.groups, s);
         else if (types == 2) bn_::launch<false, true, true>(p, vec, b.groups, s);

@@ -383,35 +383,33 @@ int btvae_dirichlet_sample(const float* gamma, const long long* rows, float* out
 
 /* ---- gated residual block: h = act(x Wg^T + bg) (x Wu^T + bu), y = h Wd^T + bd, row norms, 8-bit products ----
  * No counterpart in the reference, whose networks stop at Linear + ReLU + BatchNorm units (src/submodels.py:6-35).
- * planes: 1 = bf16 operands, 3 = fp32 values as three bf16 planes (x = x0 + x1 + x2, `*_plane` elements apart) and the six
- * largest of the nine plane products.  Operand matrices start on 16 bytes, pitches (in elements) are multiples of 8; reduction
- * lengths are multiples of 8, the columns beyond a matrix's own width being zeros.  act: 0 silu, 1 gelu (erf), 2 relu, 3 sigmoid.
+ * planes: 1 = bf16 operands, 3 = fp32 values as three bf16 pieces (x = x0 + x1 + x2; a row holds, for every 16 columns, 16 x0, 16 x1,
+ * 16 x2) and the six largest of the nine products of two.  Operand rows start on 16 bytes, their pitches are in bytes; bf16 reduction
+ * lengths are multiples of 8, the columns beyond a matrix's own width (split operands: up to a multiple of 16) being zeros.  act: 0 silu, 1 gelu (erf), 2 relu, 3 sigmoid.
  * Matrices marked with a *_bf16 flag are bf16 when it is set, else fp32. */
-/* dst[plane][row][0 .. dst_cols) = bf16 planes of src [rows, cols] (transpose: of its transpose), zero-padded. */
-int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long plane, long long dst_ld, int rows,
-            int cols, int dst_cols, int transpose, void* stream);
-/* H [planes][M][ldh] = h; GU [M][ldgu] (fp32 with three planes, else bf16; null: not kept): x Wg^T + bg at column 0, x Wu^T + bu at
- * column gu_half. */
-int btvae_gated_proj_fwd(const void* X, long long ldx, long long x_plane, const void* Wg, const void* Wu, long long ldw,
-            long long w_plane, const void* bg, const void* bu, int bias_bf16, void* H, long long ldh, long long h_plane, void* GU,
-            long long ldgu, int gu_half, int planes, int act, int M, int F, int K, void* stream);
-/* dGU [planes][M][ldd]: da at column 0, db at column gu_half (zeros between F and gu_half) from dh = dY WdT^T, WdT [planes][F][ldw];
- * colpart: null, or [btvae_gated_proj_strips(M, F)][2][F] column sums of da and db. */
-int btvae_gated_proj_bwd(const void* dY, long long lddy, long long dy_plane, const void* WdT, long long ldw, long long w_plane,
-            const void* GU, long long ldgu, int gu_half, void* dGU, long long ldd, long long d_plane, float* colpart, int planes,
-            int act, int M, int F, int N, void* stream);
-int btvae_gated_proj_strips(int M, int F);
+/* dst = src [rows, cols] (transpose: its transpose) as an operand, zeros up to dst_cols columns (a multiple of 16). */
+int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long dst_ld, int rows, int cols,
+            int dst_cols, int transpose, void* stream);
+/* H [M] = h, an operand (zeros up to a multiple of 16 columns); GU [M][ldgu] (null: not kept): x Wg^T + bg at column 0, x Wu^T + bu at column gu_half, fp32 with three
+ * planes, else the upper two bytes of fp32 there and the third in GU_lo [M][ldgu]. */
+int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu,
+            int bias_bf16, void* H, long long ldh, void* GU, void* GU_lo, long long ldgu, int gu_half, int planes, int act, int M, int F,
+            int K, void* stream);
+/* dGU [M], an operand of 2 gu_half columns: da at column 0, db at column gu_half (zeros between F and gu_half) from dh = dY WdT^T;
+ * colpart: null, or [btvae_gated_proj_strips(M)][2][F] column sums of da and db. */
+int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* GU, const void* GU_lo,
+            long long ldgu, int gu_half, void* dGU, long long ldd, float* colpart, int planes, int act, int M, int F, int N,
+            void* stream);
+int btvae_gated_proj_strips(int M);
 /* C [M, N] = A B^T + bias; workspace (floats) of btvae_block_product_ws, 0: none. */
 long long btvae_block_product_ws(int M, int N, int K, int planes);
-int btvae_block_product(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane,
-            const void* bias, int bias_bf16, void* C, long long ldc, int c_bf16, float* ws, long long ws_floats, int planes, int M,
-            int N, int K, void* stream);
+int btvae_block_product(const void* A, long long lda, const void* B, long long ldb, const void* bias, int bias_bf16, void* C,
+            long long ldc, int c_bf16, float* ws, long long ws_floats, int planes, int M, int N, int K, void* stream);
 /* out(m, n) (+)= sum_r A[r][m] B[r][n]: rows m in [0, rows0) to out0, in [off1, off1 + rows1) to out1 (null: dropped); columns of A
- * and B are read up to the next multiple of 8. */
+ * and B are read up to the next multiple of 8 (split: 16). */
 long long btvae_block_wgrad_ws(int M, int N, int R, int planes);
-int btvae_block_wgrad(const void* A, long long lda, long long a_plane, const void* B, long long ldb, long long b_plane, float* ws,
-            long long ws_floats, void* out0, int rows0, void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate,
-            int planes, int M, int N, int R, void* stream);
+int btvae_block_wgrad(const void* A, long long lda, const void* B, long long ldb, float* ws, long long ws_floats, void* out0, int rows0,
+            void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate, int planes, int M, int N, int R, void* stream);
 /* out[n] (+)= column sums of src [R, N]. */
 long long btvae_block_colsum_ws(int R, int N);
 int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, long long ws_floats, void* out, int out_bf16,
@@ -457,7 +455,7 @@ int btvae_norm_gate_residual_fwd(const void* residual, const void* branch, const
             const float* post_w, const float* post_b, const float* pre_w, const float* pre_b, int post, int pre, float eps,
             void* stream_out, void* normed, float* stats, int types, int M, int N, void* stream);
 long long btvae_norm_gate_residual_ws(int M, int N, int G);
-int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* stream_in, const void* branch, const void* gate,
+int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* residual, const void* branch, const void* gate,
             int G, float scale, const float* scale_vec, const float* post_w, const float* post_b, const float* pre_w, int post, int pre,
             const float* stats, void* d_residual, void* d_branch, void* d_gate, float* d_scale, float* d_post_w, float* d_post_b,
             float* d_pre_w, float* d_pre_b, float* ws, long long ws_floats, int types, int M, int N, void* stream);

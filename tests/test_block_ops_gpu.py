@@ -283,15 +283,15 @@ def test_planes_are_exact(dev):
     x = rnd(dev, M, K, seed=4) * torch.exp(rnd(dev, M, K, seed=5) * 8)
     x[0, 0], x[1, 1], x[2, 2] = 3.4e38, -3.4028234e38, 1e-30
     eye = torch.eye(K, device=dev)
-    X, I = B._operand(x, 3), B._operand(eye, 3)
+    X, I = B._operand(x, 3, K), B._operand(eye, 3, M)
     out = torch.empty(M, K, device=dev)
     assert torch.equal(B._product(X, I, None, out, 3, M, K, X.width), x)
     lib = nv.lib()
     eyem = torch.eye(M, device=dev)
-    Im = B._operand(eyem, 3)
+    Im = B._operand(eyem, 3, K)
     ws = torch.empty(lib.btvae_block_wgrad_ws(M, K, M, 3), device=dev)
     out2 = torch.empty(M, K, device=dev)
-    nv.call("btvae_block_wgrad", Im.ptr(), Im.ld, Im.plane, X.ptr(), X.ld, X.plane, ws.data_ptr(), ws.numel(), out2.data_ptr(), M, None, 0, 0, K, 0, 0, 3, M, K, M)
+    nv.call("btvae_block_wgrad", Im.ptr(), Im.ld, X.ptr(), X.ld, ws.data_ptr(), ws.numel(), out2.data_ptr(), M, None, 0, 0, K, 0, 0, 3, M, K, M)
     assert torch.equal(out2, x)
 
 
@@ -300,7 +300,7 @@ def test_planes_are_exact(dev):
 def test_block_product(dev, planes, M, N, K):
     dt = F32 if planes == 3 else BF
     a, b, bias = rnd(dev, M, K, seed=1, dtype=dt), rnd(dev, N, K, seed=2, dtype=dt), rnd(dev, N, seed=3)
-    A, W = B._operand(a, planes), B._operand(b, planes)
+    A, W = B._operand(a, planes, N), B._operand(b, planes, M)
     ref = a.double() @ b.double().t() + bias.double()
     frob(B._product(A, W, bias, torch.empty(M, N, device=dev), planes, M, N, A.width), ref, E * (4 + math.sqrt(K)), "fp32 result")
     got = B._product(A, W, bias, torch.empty(M, N, dtype=BF, device=dev), planes, M, N, A.width)
@@ -316,13 +316,13 @@ def test_block_product(dev, planes, M, N, K):
 def test_block_wgrad(dev, planes, R, M, N):
     dt = F32 if planes == 3 else BF
     a, b = rnd(dev, R, M, seed=1, dtype=dt), rnd(dev, R, N, seed=2, dtype=dt)
-    A, X = B._operand(a, planes), B._operand(b, planes)
+    A, X = B._operand(a, planes, N), B._operand(b, planes, M)
     lib = nv.lib()
     ws = torch.empty(lib.btvae_block_wgrad_ws(M, N, R, planes), device=dev)
     h = M // 3
     o0, o1 = torch.full((h, N), 2.0, device=dev), torch.full((M - 2 * h, N), 3.0, device=dev)
     for acc in (1, 0):
-        nv.call("btvae_block_wgrad", A.ptr(), A.ld, A.plane, X.ptr(), X.ld, X.plane, ws.data_ptr(), ws.numel(), o0.data_ptr(), h, o1.data_ptr(), 2 * h, M - 2 * h, N, 0, acc, planes, M, N, R)
+        nv.call("btvae_block_wgrad", A.ptr(), A.ld, X.ptr(), X.ld, ws.data_ptr(), ws.numel(), o0.data_ptr(), h, o1.data_ptr(), 2 * h, M - 2 * h, N, 0, acc, planes, M, N, R)
         ref = a.double().t() @ b.double()
         tol = E * (4 + math.sqrt(max(R, 1)))
         frob(o0, ref[:h] + 2.0 * acc, tol + 2 * E, "first rows")
