@@ -99,7 +99,7 @@ _SIGS = {
     "btvae_masked_scatter": [P, P, P, LL, P],
     "btvae_lse_over_k": [P, P, I, I, P],
     "btvae_pack_lower": [P, P, LL, I, P],
-    "btvae_block_pack": [P, I, LL, P, I, LL, I, I, I, I, P],
+    "btvae_block_pack": [P, I, P],
     "btvae_gated_proj_fwd": [P, LL, P, P, LL, P, P, I, P, LL, P, P, LL, I, I, I, I, I, I, P],
     "btvae_gated_proj_bwd": [P, LL, P, LL, P, P, LL, I, P, LL, P, I, I, I, I, I, P],
     "btvae_block_product": [P, LL, P, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],

@@ -14,6 +14,7 @@ Autograd nodes are not captured into graphs: inside one, use the tapes (``gated_
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -74,10 +75,15 @@ def _rows(t, what):
         rows *= n
     if rows >= 2 ** 31 or t.shape[-1] >= 2 ** 30:
         raise ValueError(f"{what} is too large: {list(t.shape)}")
-    t = t.reshape(rows, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(rows, t.shape[-1])
     if t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
+
+
+def _shaped(t, shape):
+    return t if t.shape == shape else t.view(shape)          # a view is one more autograd node
 
 
 def _pitch(t):
@@ -101,13 +107,18 @@ class _Operand:
     """A matrix as the products read it: bf16 (``planes`` 1), or float32 values as three bf16 pieces each, 96 bytes for every 16
     columns (``planes`` 3); ``ld`` bytes to a row, rows on 16 bytes, ``width`` columns of which those beyond the matrix's own are zeros.  A
     bf16 matrix that is laid out so already is used in place."""
-    __slots__ = ("t", "ld", "width")
+    __slots__ = ("at", "ld", "width", "t")
 
-    def __init__(self, t, ld, width):
-        self.t, self.ld, self.width = t, ld, width
+    def __init__(self, at, ld, width, t=None):
+        self.at, self.ld, self.width, self.t = at, ld, width, t      # `t` holds the memory at address `at`
 
     def ptr(self):
-        return self.t.data_ptr()
+        return self.at
+
+
+def _operand_buffer(rows, ld, width, device) -> _Operand:
+    t = torch.empty(rows * ld, dtype=torch.uint8, device=device)
+    return _Operand(t.data_ptr(), ld, width, t)
 
 
 def _row_bytes(cols, planes):
@@ -119,16 +130,43 @@ def _fits(t):
     return t.dtype == torch.bfloat16 and t.shape[1] % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0
 
 
-def _pack_into(t, dst, planes, ld, dst_cols, transpose, offset=0):
-    nv.call("btvae_block_pack", _p(t), int(t.dtype == torch.bfloat16), _pitch(t), dst.data_ptr() + offset, planes, ld, t.shape[0], t.shape[1], dst_cols, int(transpose))
+class _Packer:
+    """Matrices to be laid out as operands: noted one by one, written by one launch into one buffer."""
 
+    def __init__(self, planes, device):
+        self.planes, self.device, self.todo, self.bytes = planes, device, [], 0
 
-def _packed(t, planes) -> _Operand:
-    rows, cols = t.shape
-    ld = _row_bytes(cols, planes)
-    dst = torch.empty(rows * ld, dtype=torch.uint8, device=t.device)
-    _pack_into(t, dst, planes, ld, _up(cols, 32), False)
-    return _Operand(dst, ld, _up(cols, 8))
+    def add(self, t, apart=False) -> _Operand:
+        """``apart``: in a buffer of its own, for what outlives the others."""
+        rows, cols = t.shape
+        ld = _row_bytes(cols, self.planes)
+        op = _operand_buffer(rows, ld, _up(cols, 8), self.device) if apart else _Operand(self.bytes, ld, _up(cols, 8))
+        self._job(t, op, 0, 0 if apart else rows * ld, _up(cols, 32), 0)
+        return op
+
+    def add_transposed(self, *ts, width) -> _Operand:
+        """[t0^T t1^T ..], ``width`` columns to each."""
+        cols, piece = ts[0].shape[1], _row_bytes(width, self.planes)
+        ld = piece * len(ts)
+        op = _Operand(self.bytes, ld, width * len(ts))
+        for i, t in enumerate(ts):
+            self._job(t, op, i * piece, cols * ld if i == 0 else 0, width, 1)
+        return op
+
+    def _job(self, t, op, offset, size, dst_cols, transpose):
+        self.todo.append((op, offset, t, dst_cols, transpose))
+        self.bytes += _up(size, 256)
+
+    def run(self):
+        if not self.todo:
+            return
+        buf = torch.empty(self.bytes, dtype=torch.uint8, device=self.device)
+        base, jobs = buf.data_ptr(), []
+        for op, offset, t, dst_cols, transpose in self.todo:
+            if op.t is None:
+                op.at, op.t = base + op.at, buf
+            jobs += (t.data_ptr(), t.dtype == torch.bfloat16, _pitch(t), op.at + offset, self.planes, op.ld, *t.shape, dst_cols, transpose)
+        nv.call("btvae_block_pack", (ctypes.c_longlong * len(jobs))(*jobs), len(self.todo))
 
 
 REPACK_READS = 1024        # rows or columns of a product from which a bf16 matrix with rows off 64-byte boundaries is copied first
@@ -141,17 +179,23 @@ def _in_place(t, planes, reads):
     return planes == 1 and _fits(t) and (reads < REPACK_READS or (2 * _pitch(t) % 64 == 0 and t.data_ptr() % 64 == 0))
 
 
-def _operand(t, planes, reads) -> _Operand:
+def _operand(t, planes, reads, packer=None, apart=False) -> _Operand:
+    """``t`` where it is, or laid out by ``packer`` (its ``run`` has to come before the operand is used; absent: at once)."""
     if _in_place(t, planes, reads):
-        return _Operand(t, 2 * _pitch(t), t.shape[1])
-    return _packed(t, planes)
+        return _Operand(t.data_ptr(), 2 * _pitch(t), t.shape[1], t)
+    if packer is not None:
+        return packer.add(t, apart)
+    packer = _Packer(planes, t.device)
+    op = packer.add(t)
+    packer.run()
+    return op
 
 
-def _operand_pair(a, b, planes, reads):
+def _operand_pair(a, b, planes, reads, packer):
     """Two matrices of one shape with a common pitch."""
     if _in_place(a, planes, reads) and _in_place(b, planes, reads) and _pitch(a) == _pitch(b):
-        return _Operand(a, 2 * _pitch(a), a.shape[1]), _Operand(b, 2 * _pitch(b), b.shape[1])
-    return _packed(a, planes), _packed(b, planes)
+        return _operand(a, planes, reads), _operand(b, planes, reads)
+    return packer.add(a), packer.add(b)
 
 
 def _workspace(floats, device):
@@ -190,26 +234,23 @@ class GatedTape:
             accumulate = False
         dwg, dwu, dwd, dbg, dbu, dbd = outs
         acc = int(accumulate)
-        DY = _operand(dy, planes, F)
-        ldt, ldg = _row_bytes(N, planes), 2 * _row_bytes(F, planes)
-        WdT = torch.empty(F * ldt, dtype=torch.uint8, device=dev)
-        _pack_into(w_down, WdT, planes, ldt, _up(N, 32), True)
-        dGU = _Operand(torch.empty(M * ldg, dtype=torch.uint8, device=dev), ldg, 2 * half)
+        packer = _Packer(planes, dev)
+        DY, WdT = _operand(dy, planes, F, packer), packer.add_transposed(w_down, width=_up(N, 32))
+        WT = packer.add_transposed(w_gate, w_up, width=half) if need_input else None
+        packer.run()
+        dGU = _operand_buffer(M, 2 * _row_bytes(F, planes), 2 * half, dev)
         want_bias = need_weights and (dbg is not None or dbu is not None)
         strips = lib.btvae_gated_proj_strips(M) if M else 0
         colpart = _workspace(strips * 2 * F, dev) if want_bias else None
-        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, _p(WdT), ldt, _p(self.GU), _p(self.GU_lo), 2 * half, half, dGU.ptr(), ldg, _p(colpart), planes, self.act, M, F, DY.width)
+        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, WdT.ptr(), WdT.ld, _p(self.GU), _p(self.GU_lo), 2 * half, half, dGU.ptr(), dGU.ld, _p(colpart), planes, self.act, M, F, DY.width)
         dx = None
         if need_input:
             dx = torch.empty(M, K, dtype=x.dtype, device=dev)
-            WT = torch.empty(K * ldg, dtype=torch.uint8, device=dev)
-            for i, w in enumerate((w_gate, w_up)):
-                _pack_into(w, WT, planes, ldg, half, True, i * (ldg // 2))
-            _product(dGU, _Operand(WT, ldg, 2 * half), None, dx, planes, M, K, 2 * half)
+            _product(dGU, WT, None, dx, planes, M, K, 2 * half)
         if not need_weights:
             return (dx,) + (None,) * 6
         ws = _workspace(max(lib.btvae_block_wgrad_ws(2 * half, K, M, planes), lib.btvae_block_wgrad_ws(N, F, M, planes)), dev)
-        nv.call("btvae_block_wgrad", dGU.ptr(), ldg, self.X.ptr(), self.X.ld, _p(ws), ws.numel(),
+        nv.call("btvae_block_wgrad", dGU.ptr(), dGU.ld, self.X.ptr(), self.X.ld, _p(ws), ws.numel(),
                 _p(dwg), F, _p(dwu), half, F, K, int(dwg.dtype == torch.bfloat16), acc, planes, 2 * half, K, M)
         nv.call("btvae_block_wgrad", DY.ptr(), DY.ld, self.H.ptr(), self.H.ld, _p(ws), ws.numel(),
                 _p(dwd), N, None, 0, 0, F, int(dwd.dtype == torch.bfloat16), acc, planes, N, F, M)
@@ -250,16 +291,18 @@ def _ffn_forward(x2, weights, biases, act, planes, out_dtype, keep):
     b_gate, b_up, b_down = biases
     dev, (M, K), F, N = x2.device, x2.shape, w_gate.shape[0], w_down.shape[0]
     half = _up(F, 32)
-    X = _operand(x2, planes, 2 * F)
-    Wg, Wu = _operand_pair(w_gate, w_up, planes, M)
-    H = _Operand(torch.empty(M * _row_bytes(F, planes), dtype=torch.uint8, device=dev), _row_bytes(F, planes), _up(F, 8))
+    packer = _Packer(planes, dev)
+    X = _operand(x2, planes, 2 * F, packer, apart=keep)
+    Wg, Wu = _operand_pair(w_gate, w_up, planes, M, packer)
+    Wd = _operand(w_down, planes, M, packer)
+    packer.run()
+    H = _operand_buffer(M, _row_bytes(F, planes), _up(F, 8), dev)
     GU = torch.empty(M * 2 * half, dtype=torch.float32 if planes == 3 else torch.int16, device=dev) if keep else None
     GU_lo = torch.empty(M * 2 * half, dtype=torch.uint8, device=dev) if keep and planes == 1 else None
     bias16 = int(any(b is not None and b.dtype == torch.bfloat16 for b in (b_gate, b_up)))
     nv.call("btvae_gated_proj_fwd", X.ptr(), X.ld, Wg.ptr(), Wu.ptr(), Wg.ld, _p(b_gate), _p(b_up), bias16,
             H.ptr(), H.ld, _p(GU), _p(GU_lo), 2 * half, half, planes, act, M, F, X.width)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
-    Wd = _operand(w_down, planes, M)
     _product(H, Wd, b_down, y, planes, M, N, Wd.width)
     return y, GatedTape(x2, weights, biases, act, planes, X, H, GU, GU_lo, half) if keep else None
 
@@ -314,7 +357,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
         y = _ffn_few(x2, weights, biases, act)
     else:
         y, _ = _ffn_forward(x2, weights, biases, act, 3 if x.dtype == torch.float32 else 1, x.dtype, False)
-    return y.view(*x.shape[:-1], y.shape[1])
+    return _shaped(y, (*x.shape[:-1], y.shape[1]))
 
 
 @torch.no_grad()
@@ -322,7 +365,7 @@ def gated_feed_forward_tape(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_d
     """``gated_feed_forward`` without autograd: (y, tape), ``tape.backward(dy)`` returns the gradients.  May be captured into a graph."""
     x2, weights, biases, act = _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
     y, tape = _ffn_forward(x2, weights, biases, act, 3 if x.dtype == torch.float32 else 1, x.dtype, True)
-    return y.view(*x.shape[:-1], y.shape[1]), tape
+    return _shaped(y, (*x.shape[:-1], y.shape[1])), tape
 
 
 # ------------------------------------------------------------------------------------------------ norms, gate, residual
@@ -461,7 +504,7 @@ def norm_gate_residual(residual, branch=None, gate=None, scale=1.0, post_norm=No
         normed = out.pop(0) if pre else None
     else:
         stream, normed, _ = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, False)
-    return residual if stream is None else stream.view(residual.shape), None if normed is None else normed.view(residual.shape)
+    return residual if stream is None else _shaped(stream, residual.shape), None if normed is None else _shaped(normed, residual.shape)
 
 
 @torch.no_grad()
@@ -471,7 +514,7 @@ def norm_gate_residual_tape(residual, branch=None, gate=None, scale=1.0, post_no
     May be captured into a graph."""
     r2, b2, g2, number, vec, vectors, post, pre, eps = _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps)
     stream, normed, tape = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, True)
-    return residual if stream is None else stream.view(residual.shape), None if normed is None else normed.view(residual.shape), tape
+    return residual if stream is None else _shaped(stream, residual.shape), None if normed is None else _shaped(normed, residual.shape), tape
 
 
 # ------------------------------------------------------------------------------------------------ 8-bit products
@@ -502,7 +545,7 @@ class Fp8Rows:
         rows, ld = self.q.shape
         out = torch.empty(rows, ld, dtype=torch.bfloat16, device=self.device)
         nv.call("btvae_fp8_expand", _p(self.q), ld, _p(self.scales), self.scales.shape[1], self.blocks, _p(out), ld, rows, self.shape[-1])
-        return _Operand(out, 2 * ld, ld)
+        return _Operand(out.data_ptr(), 2 * ld, ld, out)
 
 
 class Fp8Weight(Fp8Rows):

@@ -40,36 +40,61 @@ template <bool SPLIT> __device__ __forceinline__ void put_operand(char* row, int
         *reinterpret_cast<u32x4*>(row + 2LL * c) = pack8(v);
     }
 }
+// Up to four matrices become operands in one launch (a small unit's time is its launches): each takes a run of workgroups.
+struct PackJob {
+    const void* src; char* dst; long long ld, dld;
+    int src16, planes, rows, cols, dst_cols, transpose;
+    unsigned first, blocks;
+};
+struct PackJobs { PackJob j[4]; int n; };
+
 // dst[r][c] = src[r][c], zeros for cols <= c < dst_cols; eight columns to a thread, `dld` bytes to a row
 template <bool SRC16, bool SPLIT>
-__global__ __launch_bounds__(256) void pack_rows(const void* __restrict__ src, long long ld, char* __restrict__ dst, long long dld, int rows, int cols, int groups) {
-    const long long total = (long long)rows * groups;
-    for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < total; g += (long long)gridDim.x * 256) {
+__device__ __forceinline__ void pack_rows(const PackJob& p, unsigned block) {
+    const int groups = p.dst_cols / 8;
+    const long long total = (long long)p.rows * groups;
+    for (long long g = (long long)block * 256 + threadIdx.x; g < total; g += (long long)p.blocks * 256) {
         const long long r = g / groups;
         const int c = (int)(g - r * groups) * 8;
         float v[8];
-        load8<SRC16>(src, r * ld + c, cols - c, v);
-        put_operand<SPLIT>(dst + r * dld, c, v);
+        load8<SRC16>(p.src, r * p.ld + c, p.cols - c, v);
+        put_operand<SPLIT>(p.dst + r * p.dld, c, v);
     }
 }
-
-// dst[c][r] = src[r][c] for c < cols, zeros for rows <= r < dst_cols: 64 x 64 tiles through LDS.
+// dst[c][r] = src[r][c] for c < cols, zeros for rows <= r < dst_cols: a 64 x 64 tile through LDS
 template <bool SRC16, bool SPLIT>
-__global__ __launch_bounds__(256) void pack_transposed(const void* __restrict__ src, long long ld, char* __restrict__ dst, long long dld, int rows, int cols, int dst_cols) {
-    __shared__ float t[64][65];
-    const int r0 = (int)blockIdx.x * 64, c0 = (int)blockIdx.y * 64;
+__device__ __forceinline__ void pack_transposed(const PackJob& p, unsigned block, float (*t)[65]) {
+    const unsigned across = (unsigned)(p.dst_cols + 63) / 64;
+    const int r0 = (int)(block % across) * 64, c0 = (int)(block / across) * 64;
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
         const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        t[i >> 6][i & 63] = r < rows && c < cols ? (SRC16 ? bf_load(src, (long long)r * ld + c) : reinterpret_cast<const float*>(src)[(long long)r * ld + c]) : 0.f;
+        t[i >> 6][i & 63] = r < p.rows && c < p.cols ? (SRC16 ? bf_load(p.src, (long long)r * p.ld + c) : reinterpret_cast<const float*>(p.src)[(long long)r * p.ld + c]) : 0.f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
         const int c = i >> 3, rg = (i & 7) * 8;
-        if (c0 + c >= cols || r0 + rg >= dst_cols) continue;
+        if (c0 + c >= p.cols || r0 + rg >= p.dst_cols) continue;
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = t[rg + e][c];
-        put_operand<SPLIT>(dst + (long long)(c0 + c) * dld, r0 + rg, v);
+        put_operand<SPLIT>(p.dst + (long long)(c0 + c) * p.dld, r0 + rg, v);
+    }
+}
+__global__ __launch_bounds__(256) void pack(const PackJobs jobs) {
+    __shared__ float t[64][65];
+    int i = 0;
+    while (i + 1 < jobs.n && blockIdx.x >= jobs.j[i + 1].first) ++i;
+    const PackJob p = jobs.j[i];
+    const unsigned block = blockIdx.x - p.first;
+    switch ((p.transpose ? 4 : 0) | (p.src16 ? 2 : 0) | (p.planes == 3 ? 1 : 0)) {
+        case 0: pack_rows<false, false>(p, block); break;
+        case 1: pack_rows<false, true>(p, block); break;
+        case 2: pack_rows<true, false>(p, block); break;
+        case 3: pack_rows<true, true>(p, block); break;
+        case 4: pack_transposed<false, false>(p, block, t); break;
+        case 5: pack_transposed<false, true>(p, block, t); break;
+        case 6: pack_transposed<true, false>(p, block, t); break;
+        default: pack_transposed<true, true>(p, block, t); break;
     }
 }
 
@@ -481,35 +506,31 @@ static bool operand_ok(const void* p, long long ld, int planes, int cols) {
 }
 static int stages_of(int K, int planes) { return planes == 3 ? bk::tiles(K, 16) : bk::tiles(K, 64); }
 
-// dst = src as an operand (transpose: of its transpose), zeros up to dst_cols columns (a multiple of 16)
-BTVAE_API int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long dst_ld, int rows, int cols, int dst_cols, int transpose, void* stream) {
-    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_pack: planes must be 1 or 3");
-    BTVAE_REQUIRE(rows >= 0 && cols > 0 && ld >= cols, "block_pack: bad source shape");
-    BTVAE_REQUIRE((dst_cols & 15) == 0 && dst_cols >= (transpose ? rows : cols) && operand_ok(dst, dst_ld, planes, dst_cols), "block_pack: bad destination layout");
-    if (rows == 0 && !transpose) return 0;
-    hipStream_t s = BLK_STREAM(stream);
-    char* d = (char*)dst;
-    if (!transpose) {
-        const int groups = dst_cols / 8;
-        const unsigned grid = (unsigned)std::min<long long>(((long long)rows * groups + 255) / 256, 16384);
-        if (src_bf16) {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<true, false>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
-            else hipLaunchKernelGGL((bk::pack_rows<true, true>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
-        } else {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_rows<false, false>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
-            else hipLaunchKernelGGL((bk::pack_rows<false, true>), dim3(grid), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, groups);
-        }
-    } else {
-        const unsigned gx = (unsigned)bk::tiles(dst_cols, 64), gy = (unsigned)bk::tiles(cols, 64);
-        BTVAE_REQUIRE(gy <= 65535, "block_pack: too many columns");
-        if (src_bf16) {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<true, false>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
-            else hipLaunchKernelGGL((bk::pack_transposed<true, true>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
-        } else {
-            if (planes == 1) hipLaunchKernelGGL((bk::pack_transposed<false, false>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
-            else hipLaunchKernelGGL((bk::pack_transposed<false, true>), dim3(gx, gy), dim3(256), 0, s, src, ld, d, dst_ld, rows, cols, dst_cols);
-        }
+// n <= 4 jobs of ten numbers: src, src_bf16, ld, dst, planes, dst_ld, rows, cols, dst_cols, transpose
+BTVAE_API int btvae_block_pack(const long long* jobs, int n, void* stream) {
+    BTVAE_REQUIRE(jobs && n >= 0 && n <= 4, "block_pack: up to four matrices");
+    bk::PackJobs q;
+    q.n = 0;
+    long long blocks = 0;
+    for (int i = 0; i < n; ++i) {
+        const long long* a = jobs + 10 * i;
+        bk::PackJob p;
+        p.src = reinterpret_cast<const void*>(a[0]); p.src16 = a[1] != 0; p.ld = a[2];
+        p.dst = reinterpret_cast<char*>(a[3]); p.planes = (int)a[4]; p.dld = a[5];
+        BTVAE_REQUIRE(a[6] >= 0 && a[7] > 0 && a[8] > 0 && a[6] < (1LL << 31) && a[7] < (1LL << 31) && a[8] < (1LL << 31) && p.ld >= a[7], "block_pack: bad source shape");
+        p.rows = (int)a[6]; p.cols = (int)a[7]; p.dst_cols = (int)a[8]; p.transpose = a[9] != 0;
+        BTVAE_REQUIRE(p.planes == 1 || p.planes == 3, "block_pack: planes must be 1 or 3");
+        BTVAE_REQUIRE((p.dst_cols & 15) == 0 && p.dst_cols >= (p.transpose ? p.rows : p.cols) && operand_ok(p.dst, p.dld, p.planes, p.dst_cols), "block_pack: bad destination layout");
+        if (p.rows == 0 && !p.transpose) continue;
+        BTVAE_REQUIRE((p.src || p.rows == 0) && p.dst, "block_pack: null matrix");
+        const long long b = p.transpose ? (long long)bk::tiles(p.dst_cols, 64) * bk::tiles(p.cols, 64) : std::min<long long>(((long long)p.rows * (p.dst_cols / 8) + 255) / 256, 16384);
+        p.first = (unsigned)blocks; p.blocks = (unsigned)b;
+        blocks += b;
+        BTVAE_REQUIRE(blocks < (1LL << 31), "block_pack: too large");
+        q.j[q.n++] = p;
     }
+    if (q.n == 0) return 0;
+    hipLaunchKernelGGL(bk::pack, dim3((unsigned)blocks), dim3(256), 0, BLK_STREAM(stream), q);
     return check_launch("block_pack");
 }
 

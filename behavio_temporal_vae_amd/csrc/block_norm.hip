@@ -6,8 +6,8 @@
 //   du = s g dv,  dy = post'(du);   norm'(d) = q (e - hat mean(e hat) [- mean(e)]),  e = d w,  q = 1 / deviation
 //
 // Memory bound: every matrix is read once and written once; a row stays in registers between its two norms.  A row belongs to
-// 1, 4 or 8 waves (up to 1024, 4096, 8192 columns), eight or sixteen values to a lane; the two moments and every sum are fp32.  Row weights
-// stay in registers over the rows a group of waves goes through.  Gate row of row r: r % G, the order of the framework's
+// 1, 2, 4 or 8 waves (up to 512, 1024, 2048, 8192 columns), eight values to a lane (sixteen beyond 4096 columns); the two moments and every sum are fp32.  The next
+// row is on its way while one is worked on.  Gate row of row r: r % G, the order of the framework's
 // draws (draw s of profile b is row s B + b).  In the backward pass a group takes all (or one stretch) of the rows of one
 // gate row, so that gate row's gradient is a running sum in registers; the gradients of the row weights are running
 // sums too, joined over a workgroup's rows through LDS and over workgroups by a second launch, always in the same order.
@@ -48,37 +48,41 @@ template <bool H> __device__ __forceinline__ void st1(void* p, long long i, floa
 }
 
 // A thread's 8 NV values of a row.  VEC: NV runs of 8 consecutive columns (N a multiple of 8, rows on 16 bytes); else column
-// (8 j + e) T + t, whole lines to a wave whatever N is.  Columns past N read as zero.
+// (8 j + e) T + t, whole lines to a wave whatever N is.  Columns past N read as zero.  `Raw` is what a row looks like on its way: the
+// next row's loads are issued before the present row is worked on.
 template <int T, int NV, bool VEC> struct Row {
     __device__ __forceinline__ static int col(int t, int j, int e) { return VEC ? (j * T + t) * 8 + e : (j * 8 + e) * T + t; }
-    template <bool H> __device__ __forceinline__ static void load(const void* p, long long row0, int N, int t, float (&v)[8 * NV]) {
+    template <bool H> struct Raw { u32x4 v[NV][H ? 1 : 2]; };
+    template <bool H> __device__ __forceinline__ static void fetch(const void* p, long long row0, int N, int t, Raw<H>& x) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (VEC) {
                 const int c = col(t, j, 0);
-                if (c < N) {
-                    if (H) {
-                        const u32x4 u = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(p) + row0 + c);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] = bf_lo(u[e]); v[8 * j + 2 * e + 1] = bf_hi(u[e]); }
-                    } else {
-                        const f32x4 a = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + row0 + c);
-                        const f32x4 b = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + row0 + c + 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { v[8 * j + e] = a[e]; v[8 * j + 4 + e] = b[e]; }
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[8 * j + e] = 0.f;
-                }
+                const u32x4* s = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p) + (row0 + min(c, N - 8)) * (H ? 2 : 4));
+                x.v[j][0] = s[0];
+                if constexpr (!H) x.v[j][1] = s[1];
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int c = col(t, j, e);
-                    v[8 * j + e] = c < N ? ld1<H>(p, row0 + c) : 0.f;
+                    const long long i = row0 + min(col(t, j, e), N - 1);
+                    if constexpr (H) {
+                        const unsigned u = reinterpret_cast<const unsigned short*>(p)[i];
+                        x.v[j][0][e >> 1] = e & 1 ? x.v[j][0][e >> 1] | (u << 16) : u;
+                    } else {
+                        x.v[j][e >> 2][e & 3] = reinterpret_cast<const unsigned*>(p)[i];
+                    }
                 }
             }
         }
+    }
+    template <bool H> __device__ __forceinline__ static void unpack(const Raw<H>& x, int N, int t, float (&v)[8 * NV]) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = H ? (e & 1 ? bf_hi(x.v[j][0][e >> 1]) : bf_lo(x.v[j][0][e >> 1])) : __uint_as_float(x.v[j][H ? 0 : e >> 2][e & 3]);
+                v[8 * j + e] = col(t, j, VEC ? 0 : e) < N ? f : 0.f;
+            }
     }
     template <bool H> __device__ __forceinline__ static void store(void* p, long long row0, int N, int t, const float (&v)[8 * NV]) {
 #pragma unroll
@@ -105,15 +109,56 @@ template <int T, int NV, bool VEC> struct Row {
             }
         }
     }
-    // fp32 vectors that may be absent; read element by element (they need no alignment)
-    __device__ __forceinline__ static void vec(const float* p, float absent, int N, int t, float (&v)[8 * NV]) {
+};
+
+// A weight vector over the rows of a workgroup.  Rows of one wave share it in LDS (a wave then needs few enough registers for two
+// to four waves a SIMD); longer rows, one to a workgroup, keep their part in registers.  Absent: a constant, zero past N.
+template <int T, int NV, bool VEC> struct Vec {
+    static constexpr bool LDS = T == 64;
+    float reg[LDS ? 1 : 8 * NV];
+    float* lds;
+    bool present;
+    float absent;
+    __device__ __forceinline__ void init(const float* p, float other, int N, int t, float* room) {
+        present = p != nullptr;
+        absent = other;
+        lds = room;
+        if constexpr (LDS) {
+            if (present)
+                for (int i = threadIdx.x; i < 8 * NV * T; i += blockDim.x) lds[i] = i < N ? p[i] : 0.f;
+        } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = col(t, j, e);
-                v[8 * j + e] = c < N ? (p ? p[c] : absent) : 0.f;
+                for (int e = 0; e < 8; ++e) {
+                    const int c = Row<T, NV, VEC>::col(t, j, e);
+                    reg[8 * j + e] = c < N ? (present ? p[c] : other) : 0.f;
+                }
+        }
+    }
+    __device__ __forceinline__ void get(int N, int t, float (&v)[8 * NV]) const {
+        if constexpr (!LDS) {
+#pragma unroll
+            for (int i = 0; i < 8 * NV; ++i) v[i] = reg[i];
+        } else if (present) {
+            asm volatile("" ::: "memory");                    // read again for every row: kept over rows it would be registers after all
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if (VEC) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(lds + (j * T + t) * 8), b = *reinterpret_cast<const f32x4*>(lds + (j * T + t) * 8 + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[8 * j + e] = a[e]; v[8 * j + 4 + e] = b[e]; }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[8 * j + e] = lds[(j * 8 + e) * T + t];
+                }
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * j + e] = Row<T, NV, VEC>::col(t, j, e) < N ? absent : 0.f;
+        }
     }
 };
 
@@ -161,166 +206,284 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd(const Args p) 
     constexpr int T = 64 * W, RPB = W == 1 ? 4 : 1, E = 8 * NV;
     typedef Row<T, NV, VEC> R;
     __shared__ float red[2 * W];
+    __shared__ __attribute__((aligned(16))) float room[W == 1 ? 5 * 64 * E : 1];
     int turn = 0;
     const int t = threadIdx.x % T;
-    float w1[E], w2[E], c1[E], c2[E], sv[E];
-    if (p.y) {
-        R::vec(p.w1, 1.f, p.N, t, w1);
-        R::vec(p.c1, 0.f, p.N, t, c1);
-        R::vec(p.sv, p.s, p.N, t, sv);
-    }
-    if (p.n) {
-        R::vec(p.w2, 1.f, p.N, t, w2);
-        R::vec(p.c2, 0.f, p.N, t, c2);
-    }
-    for (int row = (int)blockIdx.x * RPB + threadIdx.x / T; row < p.M; row += (int)gridDim.x * RPB) {
+    Vec<T, NV, VEC> w1, c1, w2, c2, sv;
+    w1.init(p.w1, 1.f, p.N, t, room);
+    c1.init(p.c1, 0.f, p.N, t, room + 64 * E);
+    sv.init(p.sv, p.s, p.N, t, room + 2 * 64 * E);
+    w2.init(p.w2, 1.f, p.N, t, room + 3 * 64 * E);
+    c2.init(p.c2, 0.f, p.N, t, room + 4 * 64 * E);
+    if (W == 1) __syncthreads();
+    typename R::template Raw<RH> rr;
+    typename R::template Raw<BH> ry, rg;
+    auto fetch = [&](int row) {
         const long long o = (long long)row * p.N;
-        float v[E];
-        R::template load<RH>(p.r, o, p.N, t, v);
+        R::template fetch<RH>(p.r, o, p.N, t, rr);
         if (p.y) {
-            float y[E], g[E];
-            R::template load<BH>(p.y, o, p.N, t, y);
-            if (p.g) R::template load<BH>(p.g, (long long)(row % p.G) * p.N, p.N, t, g);
-            float mean = 0.f, q = 1.f;
-            if (p.post != NONE) moments<T, NV, VEC>(y, p.post, p.eps, p.N, t, red, turn, mean, q);
+            R::template fetch<BH>(p.y, o, p.N, t, ry);
+            if (p.g) R::template fetch<BH>(p.g, (long long)(row % p.G) * p.N, p.N, t, rg);
+        }
+    };
+    int row = (int)blockIdx.x * RPB + threadIdx.x / T;
+    if (row < p.M) fetch(row);
+    for (; row < p.M; row += (int)gridDim.x * RPB) {
+        const long long o = (long long)row * p.N;
+        float v[E], x[E], f[E];
+        R::template unpack<RH>(rr, p.N, t, v);
+        float mean = 0.f, q = 1.f;
+        if (p.y) {
+            R::template unpack<BH>(ry, p.N, t, x);
+            if (p.g) R::template unpack<BH>(rg, p.N, t, f);
+            else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float u = p.post != NONE ? (y[i] - mean) * q * w1[i] + c1[i] : y[i];
-                v[i] += sv[i] * (p.g ? g[i] * u : u);
+                for (int i = 0; i < E; ++i) f[i] = 1.f;
             }
+        }
+        if (row + (int)gridDim.x * RPB < p.M) fetch(row + (int)gridDim.x * RPB);
+        if (p.y) {
+            if (p.post != NONE) moments<T, NV, VEC>(x, p.post, p.eps, p.N, t, red, turn, mean, q);
+            float w[E];
+            sv.get(p.N, t, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] *= w[i];         // scale times gate
+            if (p.post != NONE) {
+                w1.get(p.N, t, w);
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[i] = (x[i] - mean) * q * w[i];
+                if (p.c1) {
+                    c1.get(p.N, t, w);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) x[i] += w[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] += f[i] * x[i];
             R::template store<RH>(p.v, o, p.N, t, v);
             if (p.stats && t == 0) { p.stats[row] = mean; p.stats[p.M + row] = q; }
         }
         if (p.n) {
-            float mean, q;
             moments<T, NV, VEC>(v, p.pre, p.eps, p.N, t, red, turn, mean, q);
+            float w[E];
+            w2.get(p.N, t, w);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = (v[i] - mean) * q * w2[i] + c2[i];
+            for (int i = 0; i < E; ++i) v[i] = (v[i] - mean) * q * w[i];
+            if (p.c2) {
+                c2.get(p.N, t, w);
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i] += w[i];
+            }
             R::template store<BH>(p.n, o, p.N, t, v);
             if (p.stats && t == 0) { p.stats[2LL * p.M + row] = mean; p.stats[3LL * p.M + row] = q; }
         }
     }
 }
 
-template <bool RH, bool BH, int W, int NV, bool VEC>
+// FULL: column sums of the biases and of the scale are wanted too.
+template <bool RH, bool BH, int W, int NV, bool VEC, bool FULL>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd(const Args p) {
     constexpr int T = 64 * W, RPB = W == 1 ? 4 : 1, E = 8 * NV;
     typedef Row<T, NV, VEC> R;
     __shared__ float red[2 * W];
-    __shared__ float join[W == 1 ? 3 * 64 * E : 1];
+    __shared__ __attribute__((aligned(16))) float room[W == 1 ? 4 * 64 * E : 1];
     int turn = 0;
     const int t = threadIdx.x % T;
     const float inv_n = 1.f / (float)p.N;
-    float w1[E], c1[E], w2[E], sv[E];
-    float aw1[E], ac1[E], aw2[E], ac2[E], as[E];
+    Vec<T, NV, VEC> w1, c1, w2, sv;
+    w1.init(p.w1, 1.f, p.N, t, room);
+    c1.init(p.c1, 0.f, p.N, t, room + 64 * E);
+    sv.init(p.sv, p.s, p.N, t, room + 2 * 64 * E);
+    w2.init(p.w2, 1.f, p.N, t, room + 3 * 64 * E);
+    if (W == 1) __syncthreads();
+    float aw1[E], aw2[E], ac1[FULL ? E : 1], ac2[FULL ? E : 1], as[FULL ? E : 1], dg[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) aw1[i] = ac1[i] = aw2[i] = ac2[i] = as[i] = 0.f;
-    if (p.y) {
-        R::vec(p.w1, 1.f, p.N, t, w1);
-        R::vec(p.c1, 0.f, p.N, t, c1);
-        R::vec(p.sv, p.s, p.N, t, sv);
+    for (int i = 0; i < E; ++i) aw1[i] = aw2[i] = dg[i] = 0.f;
+    if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) ac1[i] = ac2[i] = as[i] = 0.f;
     }
-    R::vec(p.w2, 1.f, p.N, t, w2);
+    // rows in the order this group takes them: the rows of a stretch of one gate row, then the next stretch
     const int units = p.G * p.splits;
-    for (int unit = (int)blockIdx.x * RPB + threadIdx.x / T; unit < units; unit += (int)gridDim.x * RPB) {
-        const int split = unit / p.G, gr = unit - split * p.G;
-        const int s0 = (int)((long long)p.share * split / p.splits), s1 = (int)((long long)p.share * (split + 1) / p.splits);
-        float g[E], dg[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) { g[i] = 1.f; dg[i] = 0.f; }
-        if (p.y && p.g) R::template load<BH>(p.g, (long long)gr * p.N, p.N, t, g);
-        for (int s = s0; s < s1; ++s) {
-            const int row = s * p.G + gr;
-            const long long o = (long long)row * p.N;
-            float d[E], y[E], u[E];
-            float mean = 0.f, q = 1.f;
-            if (p.y) {                                        // y becomes its normalised self, u what the gate multiplies
-                R::template load<BH>(p.y, o, p.N, t, y);
-                if (p.post != NONE) {
-                    mean = p.stats[row];
-                    q = p.stats[p.M + row];
-                }
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    y[i] = (y[i] - mean) * q;
-                    u[i] = p.post != NONE ? y[i] * w1[i] + c1[i] : y[i];
-                }
-            }
-            if (p.dv) R::template load<RH>(p.dv, o, p.N, t, d);
+    struct At { int unit, s, end, gr; };
+    auto open = [&](int unit) {
+        At a;
+        a.unit = unit;
+        const int split = unit / p.G;
+        a.gr = unit - split * p.G;
+        a.s = (int)((long long)p.share * split / p.splits);
+        a.end = (int)((long long)p.share * (split + 1) / p.splits);
+        return a;
+    };
+    typename R::template Raw<RH> rr, rd;
+    typename R::template Raw<BH> ry, rn, rg;
+    auto fetch = [&](const At& a) {
+        const long long o = (long long)(a.s * p.G + a.gr) * p.N;
+        if (p.y) R::template fetch<BH>(p.y, o, p.N, t, ry);
+        if (p.dv) R::template fetch<RH>(p.dv, o, p.N, t, rd);
+        if (p.dn) {
+            R::template fetch<BH>(p.dn, o, p.N, t, rn);
+            R::template fetch<RH>(p.r, o, p.N, t, rr);
+        }
+        if (p.y && p.g) R::template fetch<BH>(p.g, (long long)a.gr * p.N, p.N, t, rg);
+    };
+    At at = {0, 0, 0, 0};
+    int unit = (int)blockIdx.x * RPB + threadIdx.x / T;
+    const bool any = unit < units;                            // (every stretch has rows)
+    if (any) {
+        at = open(unit);
+        fetch(at);
+    }
+    for (bool more = any; more;) {
+        const int row = at.s * p.G + at.gr, gr = at.gr, split = at.unit / p.G;
+        const long long o = (long long)row * p.N;
+        float y[E], g[E], d[E], e[E], h[E], w[E];
+        if (p.y) {
+            R::template unpack<BH>(ry, p.N, t, y);
+            if (p.g) R::template unpack<BH>(rg, p.N, t, g);
             else {
 #pragma unroll
-                for (int i = 0; i < E; ++i) d[i] = 0.f;
+                for (int i = 0; i < E; ++i) g[i] = 1.f;
             }
-            if (p.dn) {
-                // the stream as the forward pass had it before its rounding
-                float e[E], h[E];
-                R::template load<BH>(p.dn, o, p.N, t, e);
-                R::template load<RH>(p.r, o, p.N, t, h);
-                const float mean2 = p.stats[2LL * p.M + row], q2 = p.stats[3LL * p.M + row];
-                float se = 0.f, seh = 0.f;
+        }
+        if (p.dv) R::template unpack<RH>(rd, p.N, t, d);
+        else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) d[i] = 0.f;
+        }
+        if (p.dn) {
+            R::template unpack<BH>(rn, p.N, t, e);
+            R::template unpack<RH>(rr, p.N, t, h);
+        }
+        const float mean = p.post != NONE ? p.stats[row] : 0.f, q = p.post != NONE ? p.stats[p.M + row] : 1.f;
+        const float mean2 = p.dn ? p.stats[2LL * p.M + row] : 0.f, q2 = p.dn ? p.stats[3LL * p.M + row] : 0.f;
+        bool last = ++at.s == at.end;                         // of its stretch
+        if (last) {
+            const int next = at.unit + (int)gridDim.x * RPB;
+            more = next < units;
+            if (more) at = open(next);
+        }
+        if (more) fetch(at);
+        if (p.y) {                                            // y becomes its normalised self, g scale times gate
+            sv.get(p.N, t, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                y[i] = (y[i] - mean) * q;
+                if constexpr (!FULL) g[i] *= w[i];
+            }
+        }
+        auto branch = [&](float (&u)[E]) {                    // what the gate multiplies
+            if (p.post == NONE) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) u[i] = y[i];
+                return;
+            }
+            w1.get(p.N, t, u);
+#pragma unroll
+            for (int i = 0; i < E; ++i) u[i] *= y[i];
+            if (p.c1) {
+                float c[E];
+                c1.get(p.N, t, c);
+#pragma unroll
+                for (int i = 0; i < E; ++i) u[i] += c[i];
+            }
+        };
+        if (p.dn) {
+            // the stream as the forward pass had it before its rounding
+            if (p.y) {
+                float u[E];
+                branch(u);
+                if constexpr (FULL) sv.get(p.N, t, w);
+#pragma unroll
+                for (int i = 0; i < E; ++i) h[i] += (FULL ? w[i] * g[i] : g[i]) * u[i];
+            }
+            w2.get(p.N, t, w);
+            float se = 0.f, seh = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                h[i] = (h[i] - mean2) * q2;                   // past N: finite, and met by e = 0 only
+                aw2[i] += e[i] * h[i];
+                if constexpr (FULL) ac2[i] += e[i];
+                e[i] *= w[i];
+                se += e[i];
+                seh += e[i] * h[i];
+            }
+            seh = row_sum<T>(seh, red, turn) * inv_n;
+            se = p.pre == LAYER ? row_sum<T>(se, red, turn) * inv_n : 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) d[i] += q2 * (e[i] - h[i] * seh - se);
+        }
+        if (p.dr) R::template store<RH>(p.dr, o, p.N, t, d);
+        if (p.y) {
+            float se = 0.f, seh = 0.f;
+            branch(e);
+            if constexpr (FULL) {
+                sv.get(p.N, t, w);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    if (p.y) h[i] += sv[i] * (g[i] * u[i]);
-                    h[i] = (h[i] - mean2) * q2;               // past N: finite, and met by e = 0 only
-                    aw2[i] += e[i] * h[i];
-                    ac2[i] += e[i];
-                    e[i] *= w2[i];
-                    se += e[i];
-                    seh += e[i] * h[i];
+                    const float ud = e[i] * d[i];
+                    dg[i] += w[i] * ud;
+                    as[i] += g[i] * ud;
+                    d[i] *= w[i] * g[i];
+                }
+            } else {
+                sv.get(p.N, t, w);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    dg[i] += w[i] * (e[i] * d[i]);
+                    d[i] *= g[i];
+                }
+            }
+            if (p.post != NONE) {
+                w1.get(p.N, t, w);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    aw1[i] += d[i] * y[i];
+                    if constexpr (FULL) ac1[i] += d[i];
+                    d[i] *= w[i];
+                    se += d[i];
+                    seh += d[i] * y[i];
                 }
                 seh = row_sum<T>(seh, red, turn) * inv_n;
-                se = p.pre == LAYER ? row_sum<T>(se, red, turn) * inv_n : 0.f;
+                se = p.post == LAYER ? row_sum<T>(se, red, turn) * inv_n : 0.f;
 #pragma unroll
-                for (int i = 0; i < E; ++i) d[i] += q2 * (e[i] - h[i] * seh - se);
+                for (int i = 0; i < E; ++i) d[i] = q * (d[i] - y[i] * seh - se);
             }
-            if (p.dr) R::template store<RH>(p.dr, o, p.N, t, d);
-            if (p.y) {
-                float se = 0.f, seh = 0.f;
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const float ud = u[i] * d[i];
-                    dg[i] += sv[i] * ud;
-                    as[i] += g[i] * ud;
-                    d[i] *= sv[i] * g[i];
-                    if (p.post != NONE) {
-                        aw1[i] += d[i] * y[i];
-                        ac1[i] += d[i];
-                        d[i] *= w1[i];
-                        se += d[i];
-                        seh += d[i] * y[i];
-                    }
-                }
-                if (p.post != NONE) {
-                    seh = row_sum<T>(seh, red, turn) * inv_n;
-                    se = p.post == LAYER ? row_sum<T>(se, red, turn) * inv_n : 0.f;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) d[i] = q * (d[i] - y[i] * seh - se);
-                }
-                if (p.dy) R::template store<BH>(p.dy, o, p.N, t, d);
-            }
+            if (p.dy) R::template store<BH>(p.dy, o, p.N, t, d);
         }
-        if (p.y && p.g) {
-            if (p.dg_part) R::template store<false>(p.dg_part, ((long long)split * p.G + gr) * p.N, p.N, t, dg);
-            else if (p.dg) R::template store<BH>(p.dg, (long long)gr * p.N, p.N, t, dg);
+        if (last) {
+            if (p.y && p.g) {
+                if (p.dg_part) R::template store<false>(p.dg_part, ((long long)split * p.G + gr) * p.N, p.N, t, dg);
+                else if (p.dg) R::template store<BH>(p.dg, (long long)gr * p.N, p.N, t, dg);
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) dg[i] = 0.f;
         }
     }
-    auto finish = [&](int k, float (&a)[E]) {
+    if (W == 1) __syncthreads();                              // the vectors' room becomes the meeting place of the rows' sums
+    auto finish = [&](int k, auto& a) {
         if (!((p.want >> k) & 1)) return;                     // uniform
         if constexpr (W == 1) {
             const int wv = threadIdx.x >> 6;
             __syncthreads();
             if (wv > 0) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) join[((wv - 1) * E + i) * 64 + t] = a[i];
+                for (int i = 0; i < E; ++i) room[((wv - 1) * E + i) * 64 + t] = a[i];
             }
             __syncthreads();
             if (wv > 0) return;
 #pragma unroll
-            for (int i = 0; i < E; ++i) a[i] += (join[i * 64 + t] + join[(E + i) * 64 + t]) + join[(2 * E + i) * 64 + t];
+            for (int i = 0; i < E; ++i) a[i] += (room[i * 64 + t] + room[(E + i) * 64 + t]) + room[(2 * E + i) * 64 + t];
         }
         R::template store<false>(p.part, ((long long)k * gridDim.x + blockIdx.x) * p.N, p.N, t, a);
     };
-    finish(0, aw1); finish(1, ac1); finish(2, aw2); finish(3, ac2); finish(4, as);
+    finish(0, aw1);
+    finish(2, aw2);
+    if constexpr (FULL) {
+        finish(1, ac1);
+        finish(3, ac2);
+        finish(4, as);
+    }
 }
 
 struct FinishArgs { const float* part; int strips, N; float* out[5]; };
@@ -354,13 +517,15 @@ __global__ __launch_bounds__(256) void norm_gate_sum(const float* __restrict__ p
 }
 
 constexpr int MAX_N = 8192;
-inline int waves_for(int N) { return N <= 1024 ? 1 : N <= 4096 ? 4 : 8; }
+inline int waves_for(int N) { return N <= 512 ? 1 : N <= 1024 ? 2 : N <= 2048 ? 4 : 8; }
 
 // workgroups of the backward pass (their column sums are joined by a second launch) and stretches of a gate row
 struct BwdPlan { int groups, splits; };
 static BwdPlan bwd_plan(int M, int N, int G) {
     const int W = waves_for(N), rpb = W == 1 ? 4 : 1;
-    const int units = W == 1 ? 2048 : W == 4 ? 512 : 256;      // row groups in flight that fill the chip
+    // row groups in flight: a few waves to a SIMD, fewer and each column sum is shorter (65,536 x 1000 bf16: 1024 groups 217 us with the sums,
+    // 1366 202, 2048 241)
+    const int units = W == 1 ? 2048 : W == 2 ? 1366 : W == 4 ? 768 : 384;
     const int share = M / std::max(G, 1);
     BwdPlan b;
     b.splits = G >= units ? 1 : std::max(1, std::min(share, units / std::max(G, 1)));
@@ -371,15 +536,16 @@ static BwdPlan bwd_plan(int M, int N, int G) {
 
 template <bool RH, bool BH, bool BWD>
 static void launch(const Args& p, bool vec, int grid, hipStream_t s) {
-    const int W = waves_for(p.N), nv = p.N <= 512 * W ? 1 : 2;
+    const int W = waves_for(p.N);
 #define BTVAE_NORM_GO(WW, VV, XX) \
-    do { if constexpr (BWD) hipLaunchKernelGGL((norm_bwd<RH, BH, WW, VV, XX>), dim3(grid), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p); \
+    do { if constexpr (BWD) { \
+            if (p.want & 26) hipLaunchKernelGGL((norm_bwd<RH, BH, WW, VV, XX, true>), dim3(grid), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p); \
+            else hipLaunchKernelGGL((norm_bwd<RH, BH, WW, VV, XX, false>), dim3(grid), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p); } \
          else hipLaunchKernelGGL((norm_fwd<RH, BH, WW, VV, XX>), dim3(grid), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p); } while (0)
-#define BTVAE_NORM_NV(WW, XX) do { if (nv == 1) BTVAE_NORM_GO(WW, 1, XX); else BTVAE_NORM_GO(WW, 2, XX); } while (0)
-#define BTVAE_NORM_W(XX) do { if (W == 1) BTVAE_NORM_NV(1, XX); else if (W == 4) BTVAE_NORM_NV(4, XX); else BTVAE_NORM_NV(8, XX); } while (0)
+#define BTVAE_NORM_W(XX) do { if (W == 1) BTVAE_NORM_GO(1, 1, XX); else if (W == 2) BTVAE_NORM_GO(2, 1, XX); else if (W == 4) BTVAE_NORM_GO(4, 1, XX); \
+        else if (p.N <= 4096) BTVAE_NORM_GO(8, 1, XX); else BTVAE_NORM_GO(8, 2, XX); } while (0)
     if (vec) BTVAE_NORM_W(true); else BTVAE_NORM_W(false);
 #undef BTVAE_NORM_W
-#undef BTVAE_NORM_NV
 #undef BTVAE_NORM_GO
 }
 
@@ -406,7 +572,7 @@ BTVAE_API int btvae_norm_gate_residual_fwd(const void* residual, const void* bra
     p.post = post; p.pre = pre; p.eps = eps; p.v = stream_out; p.n = normed; p.stats = stats; p.M = M; p.N = N;
     const bool vec = N % 8 == 0 && al(residual) && al(branch) && al(gate) && al(stream_out) && al(normed);
     const int rpb = bn_::waves_for(N) == 1 ? 4 : 1;
-    const int grid = (int)std::min<long long>(((long long)M + rpb - 1) / rpb, rpb == 4 ? 2048 : bn_::waves_for(N) == 4 ? 2048 : 512);
+    const int grid = (int)std::min<long long>(((long long)M + rpb - 1) / rpb, 2048);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     ProfScope prof(PK_BN, s, 0.0, (types == 3 ? 2.0 : 4.0) * M * N * 4);
     if (types == 0) bn_::launch<false, false, false>(p, vec, grid, s);

@@ -387,9 +387,9 @@ int btvae_dirichlet_sample(const float* gamma, const long long* rows, float* out
  * 16 x2) and the six largest of the nine products of two.  Operand rows start on 16 bytes, their pitches are in bytes; bf16 reduction
  * lengths are multiples of 8, the columns beyond a matrix's own width (split operands: up to a multiple of 16) being zeros.  act: 0 silu, 1 gelu (erf), 2 relu, 3 sigmoid.
  * Matrices marked with a *_bf16 flag are bf16 when it is set, else fp32. */
-/* dst = src [rows, cols] (transpose: its transpose) as an operand, zeros up to dst_cols columns (a multiple of 16). */
-int btvae_block_pack(const void* src, int src_bf16, long long ld, void* dst, int planes, long long dst_ld, int rows, int cols,
-            int dst_cols, int transpose, void* stream);
+/* n <= 4 operands in one launch, each described by ten numbers: src [rows, cols] (pointer), src_bf16, ld, dst (pointer), planes,
+ * dst_ld, rows, cols, dst_cols, transpose.  dst = src (transpose: its transpose), zeros up to dst_cols columns (a multiple of 16). */
+int btvae_block_pack(const long long* jobs, int n, void* stream);
 /* H [M] = h, an operand (zeros up to a multiple of 16 columns); GU [M][ldgu] (null: not kept): x Wg^T + bg at column 0, x Wu^T + bu at column gu_half, fp32 with three
  * planes, else the upper two bytes of fp32 there and the third in GU_lo [M][ldgu]. */
 int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu,
