@@ -106,7 +106,7 @@ _SIGS = {
     "btvae_block_wgrad": [P, LL, P, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
     "btvae_block_colsum": [P, I, LL, P, LL, P, I, I, I, I, P],
     "btvae_block_strip_sums": [P, I, I, P, P, I, I, P],
-    "btvae_few_rows": [P, LL, P, P, LL, P, P, P, LL, I, I, I, I, I, P],
+    "btvae_few_rows": [P, I, LL, P, P, I, LL, P, P, P, I, LL, I, I, I, I, P],
     "btvae_fp8_quantize": [P, I, LL, P, LL, P, LL, I, I, P],
     "btvae_fp8_quantize_blocks": [P, I, LL, P, LL, P, LL, I, I, P],
     "btvae_fp8_dequantize": [P, LL, P, LL, I, P, I, I, P],

@@ -313,10 +313,10 @@ def _ffn_few(x2, weights, biases, act):
     if _pitch(w_up) != _pitch(w_gate):
         w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     bf = int(x2.dtype == torch.bfloat16)
-    h = torch.empty(M, F, dtype=x2.dtype, device=x2.device)
+    h = torch.empty(M, F, device=x2.device)                  # float32: few rows cost nothing to keep unrounded
     y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
-    nv.call("btvae_few_rows", _p(x2), _pitch(x2), _p(w_gate), _p(w_up), _pitch(w_gate), _p(biases[0]), _p(biases[1]), _p(h), F, bf, act, M, F, K)
-    nv.call("btvae_few_rows", _p(h), F, _p(w_down), None, _pitch(w_down), _p(biases[2]), None, _p(y), N, bf, act, M, N, F)
+    nv.call("btvae_few_rows", _p(x2), bf, _pitch(x2), _p(w_gate), _p(w_up), bf, _pitch(w_gate), _p(biases[0]), _p(biases[1]), _p(h), 0, F, act, M, F, K)
+    nv.call("btvae_few_rows", _p(h), 0, F, _p(w_down), None, bf, _pitch(w_down), _p(biases[2]), None, _p(y), bf, N, act, M, N, F)
     return y
 
 

@@ -258,10 +258,11 @@ __global__ __launch_bounds__(256) void expand_rows(const unsigned char* __restri
 // Up to 32 rows: the weights are read once, straight into the matrix instruction's registers, and the time is theirs.  A
 // workgroup takes 16 weight rows (GATED: 8 gate and the 8 up rows of the same columns), its eight waves share the
 // reduction in interleaved pieces and add up through LDS.  The weight rows are the MFMA's first operand, x its second.
-//   fp32: v_mfma_f32_16x16x4_f32, exact products; bf16: v_mfma_f32_16x16x32_bf16; e4m3: x quantised on the way in (every
+//   fp32: v_mfma_f32_16x16x4_f32, exact products; bf16: v_mfma_f32_16x16x32_bf16, with fp32 rows x (the hidden layer of a unit, which is
+//   not rounded on its way) as two bf16 pieces, off by 2^-17 of a value at most; e4m3: x quantised on the way in (every
 //   workgroup repeats it: 32 values to a lane, the block's maximum over four lanes), both operands expanded to bf16, which
 //   holds every e4m3 value, and multiplied as bf16: the weights' bytes are the time, and the sums are float32's.
-enum { W_F32 = 0, W_BF16 = 1, W_E4M3 = 2 };
+enum { W_F32 = 0, W_BF16 = 1, W_E4M3 = 2, W_BF16_X32 = 3 };
 struct FewArgs {
     const void* X; long long ldx; int x_bf16;
     const char* B; const char* B2; long long ldb;             // byte pitch
@@ -338,6 +339,42 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
                     acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u]), __builtin_bit_cast(bf16x8, b[u][t]), acc[t], 0, 0, 0);
+        }
+    } else if constexpr (WT == W_BF16_X32) {
+        constexpr int U = 2;
+        for (int kb = wid * 32; kb < p.K; kb += NWV * 32 * U) {
+            u32x4 a[U];
+            float b[U][MT][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kb + u * NWV * 32 + kq * 8;
+                float wv[8];
+                if constexpr (VEC) {
+                    a[u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned short*>(w) + min(k, p.K - 8));
+                    if (k >= p.K) a[u] = u32x4{0, 0, 0, 0};
+                } else {
+                    load8<true>(w, k, p.K - k, wv);
+                    a[u] = pack8(wv);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) load8<false>(xr[t], k, p.K - k, b[u][t]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    float lo[8];
+                    const u32x4 hi = pack8(b[u][t]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // a value that is infinite as bf16 has no second piece
+                        const float h0 = bf_lo(hi[e]), h1 = bf_hi(hi[e]);
+                        lo[2 * e] = __builtin_fabsf(h0) < __builtin_inff() ? b[u][t][2 * e] - h0 : 0.f;
+                        lo[2 * e + 1] = __builtin_fabsf(h1) < __builtin_inff() ? b[u][t][2 * e + 1] - h1 : 0.f;
+                    }
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u]), __builtin_bit_cast(bf16x8, hi), acc[t], 0, 0, 0);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u]), __builtin_bit_cast(bf16x8, pack8(lo)), acc[t], 0, 0, 0);
+                }
         }
     } else if constexpr (WT == W_F32) {
         constexpr int U = 8;
@@ -674,21 +711,23 @@ static int launch_few(const bk::FewArgs& p, bool vec, hipStream_t s, const char*
     }
     return check_launch(what);
 }
-// Products with up to btvae_few_rows_max() rows, all matrices fp32 or all bf16 (`bf16`): W2 null: C = X W^T + bias; else C = act(X W^T + bias) (X W2^T + bias2).
-BTVAE_API int btvae_few_rows(const void* X, long long ldx, const void* W, const void* W2, long long ldw, const void* bias, const void* bias2, void* C, long long ldc, int bf16, int act,
-                             int M, int N, int K, void* stream) {
+// Products with up to btvae_few_rows_max() rows; W2 null: C = X W^T + bias; else C = act(X W^T + bias) (X W2^T + bias2).  `w_bf16`: the
+// weights and biases; X of their type, or (without W2) fp32; C of either.
+BTVAE_API int btvae_few_rows(const void* X, int x_bf16, long long ldx, const void* W, const void* W2, int w_bf16, long long ldw, const void* bias, const void* bias2, void* C, int c_bf16, long long ldc,
+                             int act, int M, int N, int K, void* stream) {
     BTVAE_REQUIRE(M >= 0 && M <= 32 && N > 0 && K > 0 && ldx >= K && ldw >= K && ldc >= N, "few_rows: bad sizes (M %d, N %d, K %d)", M, N, K);
     BTVAE_REQUIRE(act >= 0 && act <= 3, "few_rows: unknown activation %d", act);
+    BTVAE_REQUIRE(!x_bf16 == !w_bf16 || (w_bf16 && !W2), "few_rows: unsupported pair of types");
     if (M == 0) return 0;
     bk::FewArgs p = {};
-    const int sz = bf16 ? 2 : 4;
-    p.X = X; p.ldx = ldx; p.x_bf16 = bf16; p.B = (const char*)W; p.B2 = (const char*)W2; p.ldb = ldw * sz;
-    p.bias = bias; p.bias2 = bias2; p.bias_bf16 = bf16; p.C = C; p.ldc = ldc; p.c_bf16 = bf16; p.M = M; p.N = N; p.K = K; p.act = act;
-    const int g = 16 / sz;
-    const bool vec = bk::al16(X) && bk::al16(W) && (!W2 || bk::al16(W2)) && K % g == 0 && ldx % g == 0 && ldw % g == 0;
+    const int sw = w_bf16 ? 2 : 4, gw = 16 / sw, gx = x_bf16 ? 8 : 4;
+    p.X = X; p.ldx = ldx; p.x_bf16 = x_bf16; p.B = (const char*)W; p.B2 = (const char*)W2; p.ldb = ldw * sw;
+    p.bias = bias; p.bias2 = bias2; p.bias_bf16 = w_bf16; p.C = C; p.ldc = ldc; p.c_bf16 = c_bf16; p.M = M; p.N = N; p.K = K; p.act = act;
+    const bool vec = bk::al16(X) && bk::al16(W) && (!W2 || bk::al16(W2)) && K % gw == 0 && ldx % gx == 0 && ldw % gw == 0;
     hipStream_t s = BLK_STREAM(stream);
     ProfScope prof(PK_GEMM_FWD, s, (W2 ? 4.0 : 2.0) * M * N * K, 0.0);
-    if (bf16) return W2 ? launch_few<bk::W_BF16, true>(p, vec, s, "few_rows") : launch_few<bk::W_BF16, false>(p, vec, s, "few_rows");
+    if (w_bf16 && !x_bf16) return launch_few<bk::W_BF16_X32, false>(p, vec, s, "few_rows");
+    if (w_bf16) return W2 ? launch_few<bk::W_BF16, true>(p, vec, s, "few_rows") : launch_few<bk::W_BF16, false>(p, vec, s, "few_rows");
     return W2 ? launch_few<bk::W_F32, true>(p, vec, s, "few_rows") : launch_few<bk::W_F32, false>(p, vec, s, "few_rows");
 }
 

@@ -573,7 +573,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
     constexpr int READS = (MI + NJ) * (FMT == FMT_E4M3 ? 2 : 1);          // LDS reads of a step
     // sets of operands: two taken in turn, or (split) the three pieces of A, the three of B and the next stage's first of B
     Frag fa[SPLIT ? 3 : 2][MI], fb[SPLIT ? 4 : 2][NJ];
-    f32x16 acc[MI][NJ];
+    f32x16 acc[MI][NJ], low[SPLIT ? MI : 1][SPLIT ? NJ : 1];  // split: sums of the products of first pieces, and of the others
     int sax[MI], sbx[2] = {127, 127};                         // e4m3: the present block's scales
     unsigned sa4[MI], sb4[2] = {0, 0};                        // ... of four blocks
     auto load_set = [&](auto set, const char* sb, int s) {
@@ -589,7 +589,10 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                if constexpr (FMT != FMT_E4M3) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[k][j], fa[ka][i], acc[i][j], 0, 0, 0);
+                if constexpr (SPLIT) {
+                    f32x16& sum = ka || k ? low[i][j] : acc[i][j];
+                    sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[k][j], fa[ka][i], sum, 0, 0, 0);
+                } else if constexpr (FMT == FMT_BF16) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[k][j], fa[ka][i], acc[i][j], 0, 0, 0);
                 else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[k][j], fa[ka][i], acc[i][j], 0, 0, 0, (GATED && j >= NJ / 2) ? sbx[1] : sbx[0], 0, sax[i]);
             }
     };
@@ -656,7 +659,10 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+                for (int r = 0; r < 16; ++r) {
+                    acc[i][j][r] = 0.f;
+                    if constexpr (SPLIT) low[i][j][r] = 0.f;
+                }
         // biases of this wave's columns, a column to a lane: gated, CW / 2 of each, side by side where they fit one register
         float bias_a = 0.f, bias_b = 0.f;
         if constexpr (EP == EP_LINEAR) {
@@ -689,7 +695,8 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                 sbx[1] = (int)(sb4[1] >> sh);
             }
         };
-        // Split operands, products smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).  A piece's registers take the next stage's piece
+        // Split operands: products (2,0) (0,2) (1,1) (1,0) (0,1) into one sum, 2^-8 of a result, and (0,0) into another, which so is rounded
+        // once in 16 columns and not six times.  A piece's registers take the next stage's piece
         // when its last product has been issued; B's first piece, needed to the end, has a second set.  Behind the first product all
         // of the stage has been read: the waves meet there, and its slot is refilled three stages ahead.
         // Past the last stage the copies go on, of the last rows, into slots that are not read again: one straight path.
@@ -740,6 +747,12 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                     next_stage();
                 }
             }
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] += low[i][j][r];
         }
         if constexpr (!SPLIT) {
             // one stage; the next one's first operands are read behind its last step

@@ -416,11 +416,11 @@ int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, l
             int accumulate, int R, int N, void* stream);
 /* out0 / out1 [n] (+)= sums over strips of part[strip][0 / 1][n]. */
 int btvae_block_strip_sums(const float* part, int strips, int N, void* out0, void* out1, int out_bf16, int accumulate, void* stream);
-/* Products of up to btvae_few_rows_max() rows, everything fp32 or everything bf16: C = X W^T + bias, or with W2 act(X W^T + bias)
- * (X W2^T + bias2). */
+/* Products of up to btvae_few_rows_max() rows: C = X W^T + bias, or with W2 act(X W^T + bias) (X W2^T + bias2).  Weights and biases are of
+ * one type; X is of theirs, or (without W2) fp32. */
 int btvae_few_rows_max(void);
-int btvae_few_rows(const void* X, long long ldx, const void* W, const void* W2, long long ldw, const void* bias, const void* bias2,
-            void* C, long long ldc, int bf16, int act, int M, int N, int K, void* stream);
+int btvae_few_rows(const void* X, int x_bf16, long long ldx, const void* W, const void* W2, int w_bf16, long long ldw, const void* bias,
+            const void* bias2, void* C, int c_bf16, long long ldc, int act, int M, int N, int K, void* stream);
 /* e4m3 with power-of-two scales: q = e4m3(x 2^-e), e the smallest integer >= -126 with the block's largest finite magnitude <= 448 2^e
  * (0 for zeros), kept as the byte e + 127.  Rows: a block is 128 columns of one row, scales [rows][scp].  Weights: 128 x 128, scales
  * [ceil(N / 128)][scp].  q's pitch holds whole blocks (zeros beyond K), scp is a multiple of 4.  Non-finite values become NaN. */
