@@ -267,7 +267,6 @@ def _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
     act = _name(ACTIVATIONS, activation, "activation")
     _tensor(x, "x")
     _tensor(w_gate, "w_gate")
-    nv.ensure_device(x.device)
     if w_gate.dim() != 2 or w_gate.shape[0] == 0:
         raise ValueError(f"w_gate must be a matrix [hidden, {x.shape[-1] if x.dim() else '?'}], got {list(w_gate.shape)}")
     x2 = _rows(x, "x")
@@ -280,6 +279,7 @@ def _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
     _matrix(w_down, "w_down", (w_down.shape[0], F), x.dtype, x.device)
     for b, n, what in ((b_gate, F, "b_gate"), (b_up, F, "b_up"), (b_down, w_down.shape[0], "b_down")):
         _vector(b, what, n, (x.dtype,), x.device)
+    nv.ensure_device(x.device)
     weights = [_rows(w, "weight") for w in (w_gate, w_up, w_down)]
     biases = [None if b is None else b.contiguous() for b in (b_gate, b_up, b_down)]
     return x2, weights, biases, act
@@ -372,7 +372,8 @@ def gated_feed_forward_tape(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_d
 class NormTape:
     """What the backward pass of one ``norm_gate_residual`` needs."""
 
-    def __init__(self, residual, branch, gate, scale, scale_vec, vectors, post, pre, stats):
+    def __init__(self, residual, branch, gate, scale, scale_vec, vectors, post, pre, ntype, stats):
+        self.ntype = ntype
         self.residual, self.branch, self.gate, self.scale, self.scale_vec = residual, branch, gate, scale, scale_vec
         self.vectors, self.post, self.pre, self.stats = vectors, post, pre, stats
 
@@ -384,7 +385,7 @@ class NormTape:
         nv.ensure_device(dev)
         if d_stream is not None:
             d_stream = _matrix(d_stream.reshape(M, N), "the gradient of stream", (M, N), residual.dtype, dev).contiguous()
-        ntype = branch.dtype if branch is not None else residual.dtype
+        ntype = self.ntype
         if d_normed is not None:
             if not self.pre:
                 raise ValueError("a gradient of normed, which was not asked for")
@@ -408,24 +409,23 @@ def _types(residual, branch_type):
     return int(residual.dtype == torch.bfloat16) | (2 if branch_type == torch.bfloat16 else 0)
 
 
-def _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, eps, keep):
+def _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, eps, ntype, keep):
     (M, N), dev = residual.shape, residual.device
-    ntype = branch.dtype if branch is not None else residual.dtype
     stream = torch.empty_like(residual) if branch is not None else None
     normed = torch.empty(M, N, dtype=ntype, device=dev) if pre else None
     stats = torch.empty(4 * M, dtype=torch.float32, device=dev) if keep else None
     w1, c1, w2, c2 = vectors
     nv.call("btvae_norm_gate_residual_fwd", _p(residual), _p(branch), _p(gate), gate.shape[0] if gate is not None else 0, scale, _p(scale_vec),
             _p(w1), _p(c1), _p(w2), _p(c2), post, pre, eps, _p(stream), _p(normed), _p(stats), _types(residual, ntype), M, N)
-    tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, stats) if keep else None
+    tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, ntype, stats) if keep else None
     return stream, normed, tape
 
 
 class _NormNode(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, scale, post, pre, eps, residual, branch, gate, scale_vec, *vectors):
-        stream, normed, tape = _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, eps, True)
-        ctx.meta = (scale, post, pre, tape.stats)
+    def forward(ctx, scale, post, pre, eps, ntype, residual, branch, gate, scale_vec, *vectors):
+        stream, normed, tape = _norm_forward(residual, branch, gate, scale, scale_vec, vectors, post, pre, eps, ntype, True)
+        ctx.meta = (scale, post, pre, ntype, tape.stats)
         ctx.has = (branch is not None, pre != 0)
         ctx.save_for_backward(residual, branch, gate, scale_vec, *vectors)
         ctx.set_materialize_grads(False)
@@ -436,20 +436,19 @@ class _NormNode(torch.autograd.Function):
     def backward(ctx, *grads):
         _refuse_capture("norm_gate_residual")
         residual, branch, gate, scale_vec, *vectors = ctx.saved_tensors
-        scale, post, pre, stats = ctx.meta
+        scale, post, pre, ntype, stats = ctx.meta
         grads = list(grads)
         d_stream = grads.pop(0) if ctx.has[0] else None
         d_normed = grads.pop(0) if ctx.has[1] else None
         if d_stream is None and d_normed is None:
-            return (None,) * 12
-        tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, stats)
-        return (None, None, None, None, *tape.backward(d_stream, d_normed, need=ctx.needs_input_grad[4:]))
+            return (None,) * 13
+        tape = NormTape(residual, branch, gate, scale, scale_vec, vectors, post, pre, ntype, stats)
+        return (None, None, None, None, None, *tape.backward(d_stream, d_normed, need=ctx.needs_input_grad[5:]))
 
 
-def _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps):
+def _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps, normed_dtype):
     post, pre = _name(NORMS, post_norm, "norm"), _name(NORMS, pre_norm, "norm")
     _tensor(residual, "residual")
-    nv.ensure_device(residual.device)
     dev = residual.device
     r2 = _rows(residual, "residual").contiguous()
     M, N = r2.shape
@@ -482,38 +481,45 @@ def _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bia
         raise ValueError("pre_weight and pre_bias need a pre norm")
     vectors = [v if v is None else v.contiguous() for v in (_vector(post_weight, "post_weight", N, f32, dev), _vector(post_bias, "post_bias", N, f32, dev),
                                                             _vector(pre_weight, "pre_weight", N, f32, dev), _vector(pre_bias, "pre_bias", N, f32, dev))]
-    return r2, b2, g2, float(scale), vec, vectors, post, pre, float(eps)
+    ntype = branch.dtype if branch is not None else residual.dtype
+    if normed_dtype is not None and normed_dtype != ntype:
+        if branch is not None or normed_dtype != torch.bfloat16:
+            raise TypeError(f"normed_dtype must be {str(ntype)[6:]}" + ("" if branch is not None or residual.dtype == torch.bfloat16 else " or bfloat16"))
+        ntype = normed_dtype
+    nv.ensure_device(dev)
+    return r2, b2, g2, float(scale), vec, vectors, post, pre, float(eps), ntype
 
 
 def norm_gate_residual(residual, branch=None, gate=None, scale=1.0, post_norm=None, post_weight=None, post_bias=None, pre_norm="rms",
-                       pre_weight=None, pre_bias=None, eps=1e-6):
+                       pre_weight=None, pre_bias=None, eps=1e-6, normed_dtype=None):
     """(stream, normed): stream = residual + scale * gate * post(branch), normed = pre(stream), in one pass.
 
     ``residual``, ``branch`` [..., N] float32 or bfloat16 (a bfloat16 residual needs a bfloat16 branch; normed has the branch's
     type, stream the residual's); ``gate`` [G, N] of the branch's type multiplies row r with its row r % G (draw s of profile b
     is row s * B + b); ``scale`` a number or a float32 [N]; norms "rms", "layer" or None with float32 weights and biases
     (absent: 1 and 0).  Without a branch the stream is the residual itself; without a pre norm normed is None.  Up to 8192 columns.
-    Statistics and sums are float32; normed is computed from the stream before its rounding.  Differentiable in every tensor."""
-    args = _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps)
-    r2, b2, g2, number, vec, vectors, post, pre, eps = args
+    ``normed_dtype``: without a branch, bfloat16 gives a bfloat16 normed of a float32 residual.  Statistics and sums are float32; normed is computed from the stream before its rounding.  Differentiable in every tensor."""
+    args = _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps, normed_dtype)
+    r2, b2, g2, number, vec, vectors, post, pre, eps, ntype = args
     tensors = [t for t in (r2, b2, g2, vec, *vectors) if t is not None]
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         _refuse_capture("norm_gate_residual")
-        out = list(_NormNode.apply(number, post, pre, eps, r2, b2, g2, vec, *vectors))
+        out = list(_NormNode.apply(number, post, pre, eps, ntype, r2, b2, g2, vec, *vectors))
         stream = out.pop(0) if b2 is not None else None
         normed = out.pop(0) if pre else None
     else:
-        stream, normed, _ = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, False)
+        stream, normed, _ = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, ntype, False)
     return residual if stream is None else _shaped(stream, residual.shape), None if normed is None else _shaped(normed, residual.shape)
 
 
 @torch.no_grad()
 def norm_gate_residual_tape(residual, branch=None, gate=None, scale=1.0, post_norm=None, post_weight=None, post_bias=None, pre_norm="rms",
-                            pre_weight=None, pre_bias=None, eps=1e-6):
+                            pre_weight=None, pre_bias=None, eps=1e-6, normed_dtype=None):
     """``norm_gate_residual`` without autograd: (stream, normed, tape), ``tape.backward(d_stream, d_normed)`` returns the gradients.
     May be captured into a graph."""
-    r2, b2, g2, number, vec, vectors, post, pre, eps = _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm, pre_weight, pre_bias, eps)
-    stream, normed, tape = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, True)
+    r2, b2, g2, number, vec, vectors, post, pre, eps, ntype = _norm_inputs(residual, branch, gate, scale, post_norm, post_weight, post_bias, pre_norm,
+                                                                          pre_weight, pre_bias, eps, normed_dtype)
+    stream, normed, tape = _norm_forward(r2, b2, g2, number, vec, vectors, post, pre, eps, ntype, True)
     return residual if stream is None else _shaped(stream, residual.shape), None if normed is None else _shaped(normed, residual.shape), tape
 
 
@@ -569,9 +575,9 @@ def fp8_quantize(x) -> Fp8Rows:
     max |x| <= 448 * 2^e, and the value x * 2^-e is rounded to the nearest e4m3, ties to even.  Non-finite values become NaN and
     take no part in their block's maximum."""
     _tensor(x, "x")
-    nv.ensure_device(x.device)
     _no_graph("fp8_quantize", x)
     x2 = _rows(x, "x")
+    nv.ensure_device(x.device)
     M, K = x2.shape
     q, sc = _fp8_buffers(M, K, M, x.device)
     nv.call("btvae_fp8_quantize", _p(x2), int(x.dtype == torch.bfloat16), _pitch(x2), _p(q), q.shape[1], _p(sc), sc.shape[1], M, K)
@@ -582,10 +588,10 @@ def fp8_quantize(x) -> Fp8Rows:
 def fp8_weight(w) -> Fp8Weight:
     """A weight [N, K] as e4m3 with the scales of 128 x 128 blocks; a copy of ``w`` as it is now."""
     _tensor(w, "the weight")
-    nv.ensure_device(w.device)
     if w.dim() != 2 or w.shape[0] == 0:
         raise ValueError(f"the weight must be a matrix, got {list(w.shape)}")
     w2 = _rows(w, "the weight")
+    nv.ensure_device(w.device)
     N, K = w2.shape
     q, sc = _fp8_buffers(N, K, -(-N // FP8_BLOCK), w.device)
     nv.call("btvae_fp8_quantize_blocks", _p(w2), int(w.dtype == torch.bfloat16), _pitch(w2), _p(q), q.shape[1], _p(sc), sc.shape[1], N, K)
@@ -621,7 +627,6 @@ def fp8_linear(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype]
     if not packed:
         _tensor(x, "x")
         _no_graph("fp8_linear", x, bias)
-    nv.ensure_device(x.device)
     N, K = weight.shape
     if len(x.shape) < 1 or x.shape[-1] != K:
         raise ValueError(f"x must have {K} columns, got {list(x.shape)}")
@@ -631,6 +636,7 @@ def fp8_linear(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype]
     if dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32 or bfloat16, got {dtype}")
     b = _fp8_bias(bias, "bias", N, x.device)
+    nv.ensure_device(x.device)
     shape = x.shape
     if not packed:
         x2 = _rows(x, "x")
@@ -672,7 +678,6 @@ def fp8_gated_feed_forward(x, weights: Fp8GatedWeights, activation="silu", out_d
         raise TypeError("weights must come from fp8_gated_weights")
     _tensor(x, "x")
     _no_graph("fp8_gated_feed_forward", x)
-    nv.ensure_device(x.device)
     w, dev = weights, x.device
     if w.gate.device != dev:
         raise RuntimeError(f"the weights are on {w.gate.device}, the input on {dev}")
@@ -683,6 +688,7 @@ def fp8_gated_feed_forward(x, weights: Fp8GatedWeights, activation="silu", out_d
     dtype = out_dtype or x.dtype
     if dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32 or bfloat16, got {dtype}")
+    nv.ensure_device(dev)
     y = torch.empty(M, N, dtype=dtype, device=dev)
     if M <= nv.lib().btvae_few_rows_max():
         h = torch.empty(M, F, device=dev)

@@ -21,6 +21,7 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _native as nv
+from . import block_ops as B
 
 P = nv.ptr
 PR = nv.ptr_rows
@@ -93,6 +94,18 @@ class Saved:
     synced: bool = False                     # the statistics were merged over a process group: the backward sums are too
 
 
+@dataclass
+class GatedUnit:
+    """The gated residual layers of a trunk (``submodels.GatedLayer``), run as one unit between Linear units.  It reads and
+    returns a materialised fp32 matrix."""
+    layers: List[torch.nn.Module]
+    bn = None
+    act = True
+    residual = True      # (its input is kept whole)
+    dropout_p = 0.0
+    lin = None
+
+
 class NetPlan:
     """Ordered units of one distribution network and its output non-linearities."""
 
@@ -101,6 +114,8 @@ class NetPlan:
         self.dist = dist
         self.trunk = [self._unit(blocks["input"].input_layer, False)]
         self.trunk += [self._unit(seq, True) for seq in blocks["input"].middle_layers]
+        if hasattr(blocks["input"], "gated_layers"):
+            self.trunk.append(GatedUnit(list(blocks["input"].gated_layers)))
         self.trunk.append(self._unit(blocks["input"].output_layer, False))
         self.heads: Dict[str, List[Unit]] = {}
         for name in dist.parameterizer.dist_params:
@@ -438,7 +453,7 @@ def _plan_planes(plan: "NetPlan", backward: bool) -> Dict[torch.nn.Linear, torch
     bf = _hidden_bf16()
     if not bf and (not PRESPLIT_WEIGHTS or not mode):
         return {}
-    items = [(u.lin, PLANES_FWD | (PLANES_DX if backward else 0)) for u in plan.trunk]
+    items = [(u.lin, PLANES_FWD | (PLANES_DX if backward else 0)) for u in plan.trunk if u.lin is not None]
     for units in plan.heads.values():
         items += [(u.lin, PLANES_FWD | (PLANES_DX if backward else 0)) for u in units[:-1]]
         if backward:
@@ -793,6 +808,63 @@ def unit_forward(u: Unit, x, train: bool, saved: Optional[List[Saved]], keep_nor
     return out
 
 
+def _block_precision():
+    """(operand planes, branch type) of the gated layers: bf16 operands and branches in bf16 mode, else float32 accuracy."""
+    return (1, torch.bfloat16) if nv.lib().btvae_get_gemm_precision() == 1 else (3, torch.float32)
+
+
+def gated_forward(u: GatedUnit, x: torch.Tensor, saved: Optional[list]):
+    """x -> x + sum of the layers' branches; the stream between the layers is fp32, every addition and the next layer's norm
+    are one pass.  ``saved``: receives the layers' tapes as one entry."""
+    planes, btype = _block_precision()
+    stream = x.detach()
+    stream = (stream if stream.dtype == torch.float32 else stream.float()).contiguous()
+    M = stream.shape[0]
+    few = saved is None and M <= nv.lib().btvae_few_rows_max()
+    if few:
+        btype = torch.float32
+    branch, scale, tapes = None, None, []
+    for layer in u.layers:
+        add = dict(branch=branch, scale=scale) if branch is not None else dict(normed_dtype=btype)
+        stream, n, ntape = B.norm_gate_residual_tape(stream, pre_weight=layer.norm.detach(), **add)
+        weights, biases = [m.weight.detach() for m in (layer.gate, layer.up, layer.down)], [m.bias.detach() for m in (layer.gate, layer.up, layer.down)]
+        act, ftape = B.ACTIVATIONS[layer.activation], None
+        if saved is None and layer.eval_fp8:
+            # a copy of the weights as they are now, made per pass like the other products' images
+            branch = B.fp8_gated_feed_forward(n, B.fp8_gated_weights(*weights, *biases), layer.activation)
+        elif few:
+            branch = B._ffn_few(n, weights, biases, act)
+        else:
+            branch, ftape = B._ffn_forward(n, weights, biases, act, planes, btype, saved is not None)
+        scale = layer.scale.detach()
+        if saved is not None:
+            tapes.append((ntape, ftape))
+    stream, _, ntape = B.norm_gate_residual_tape(stream, branch=branch, scale=scale, pre_norm=None)
+    if saved is not None:
+        saved.append((tapes, ntape))
+    return stream
+
+
+def gated_backward(u: GatedUnit, sv, g: torch.Tensor, accumulate: bool):
+    """Gradient of the unit's input; parameter gradients into their ``.grad``."""
+    def put(p, value):
+        view = _grad_view(p)
+        view.add_(value) if accumulate else view.copy_(value)
+
+    tapes, last = sv
+    g = (g if g.dtype == torch.float32 else g.float()).contiguous()
+    need = (True, True, False, True, False, False, True, False)
+    g, dbranch, _, dscale, *_ = last.backward(g, None, need)
+    for i in range(len(u.layers) - 1, -1, -1):
+        layer, (ntape, ftape) = u.layers[i], tapes[i]
+        put(layer.scale, dscale)
+        linears = (layer.gate, layer.up, layer.down)
+        dn = ftape.backward(dbranch, outs=[_grad_view(m.weight) for m in linears] + [_grad_view(m.bias) for m in linears], accumulate=accumulate)[0]
+        g, dbranch, _, dscale, _, _, dnorm, _ = ntape.backward(g, dn, need)
+        put(layer.norm, dnorm)
+    return g
+
+
 def head_forward(u: Unit, x, act: int, lo: float, hi: float, want_dfac: bool, want_sq: bool,
                  planes: Optional[Dict[torch.nn.Linear, torch.Tensor]] = None):
     """Head output Linear fused with its clamp / softplus / relu non-linearity
@@ -848,7 +920,12 @@ def net_forward(plan: NetPlan, x: torch.Tensor, train: bool, tape: Optional[NetT
         # eval mode: the result may stay in the pair format when everything that reads it is a hidden unit (a residual one
         # adds it in that format)
         pairs_ok = not train and (i + 1 < nt or all(len(units) > 1 for units in plan.heads.values()))
-        if train:
+        if isinstance(u, GatedUnit):
+            h = gated_forward(u, h, tape.trunk if tape is not None else None)
+            continue
+        if i + 1 < nt and isinstance(plan.trunk[i + 1], GatedUnit):
+            pairs_ok = False
+        elif train:
             # train mode: a materialised result may be in the pair format when every reader is the Linear of a BatchNorm unit
             readers = [plan.trunk[i + 1]] if i + 1 < nt else [units[0] for units in plan.heads.values() if len(units) > 1]
             pairs_ok = (i + 1 < nt or all(len(units) > 1 for units in plan.heads.values())) and all(r.bn is not None and r.act for r in readers)
@@ -1087,6 +1164,9 @@ def net_backward(plan: NetPlan, tape: NetTape, draw: Dict[str, torch.Tensor], ne
         after_heads()
     g = g_trunk
     for i in range(len(plan.trunk) - 1, -1, -1):
+        if isinstance(plan.trunk[i], GatedUnit):
+            g = gated_backward(plan.trunk[i], tape.trunk[i], g, accumulate)
+            continue
         g = _unit_backward(plan.trunk[i], tape.trunk[i], g, None, need_input_grad or i > 0, accumulate)
     return g
 

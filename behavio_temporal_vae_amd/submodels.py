@@ -15,6 +15,7 @@ import torch
 from . import _native as nv
 from . import engine as E
 from .autograd_ops import apply_net, dict_log_likelihood
+from .block_ops import ACTIVATIONS
 from .utils import kl_divergence, log_prob, matrix_normalizer  # noqa: F401  (re-exported like the reference does)
 
 ACTIVATION = torch.nn.ReLU()
@@ -28,19 +29,40 @@ def _stack(n_in, n_out, relu, bn, dropout, rate):
     return mods, bn, dropout, rate
 
 
+class GatedLayer(torch.nn.Module):
+    """Parameters of one gated residual layer, ``x + scale * down(act(gate(n)) * up(n))`` with ``n`` the RMS norm of ``x``
+    (``block_ops.norm_gate_residual``, ``block_ops.gated_feed_forward``).  ``scale`` starts at 0.1: the layer starts
+    near the identity.  It has neither BatchNorm nor Dropout."""
+
+    def __init__(self, width, hidden, activation, eval_fp8):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown gated_activation {activation!r}; choose from {list(ACTIVATIONS)}")
+        self.activation, self.eval_fp8 = activation, bool(eval_fp8)
+        self.norm = torch.nn.Parameter(torch.ones(width))
+        self.gate, self.up, self.down = torch.nn.Linear(width, hidden), torch.nn.Linear(width, hidden), torch.nn.Linear(hidden, width)
+        self.scale = torch.nn.Parameter(torch.full((width,), 0.1))
+
+
 class NNBlock(torch.nn.Module):
     """Input Linear+ReLU, ``num_hidden_layers`` residual Linear+ReLU units, output Linear; BatchNorm and
     Dropout are appended to the ReLU units when enabled (reference: src/submodels.py:6-35).  Construction
-    order matches the reference so that a given torch seed produces the same initial weights."""
+    order matches the reference so that a given torch seed produces the same initial weights.
+
+    ``gated_layers`` gated residual layers of ``gated_hidden`` units (default: twice ``num_neurons``) may follow the
+    residual units; with ``gated_eval_fp8`` their products run on 8-bit operands in eval mode."""
 
     def __init__(self, input_dim, output_dim, num_neurons=50, num_hidden_layers=2, dropout=False, dropout_rate=0.5,
-                 batch_normalization=False, resnet=True, **_):
+                 batch_normalization=False, resnet=True, gated_layers=0, gated_hidden=None, gated_activation="silu", gated_eval_fp8=False, **_):
         super().__init__()
         self.input_dim, self.output_dim = input_dim, output_dim
         self.num_neurons, self.num_layers, self.resnet = num_neurons, num_hidden_layers, resnet
         S, L = torch.nn.Sequential, torch.nn.Linear
         self.input_layer = S(L(input_dim, num_neurons), ACTIVATION)
         self.middle_layers = torch.nn.ModuleList(S(L(num_neurons, num_neurons), ACTIVATION) for _ in range(num_hidden_layers))
+        if gated_layers:
+            self.gated_layers = torch.nn.ModuleList(GatedLayer(num_neurons, gated_hidden or 2 * num_neurons, gated_activation, gated_eval_fp8)
+                                                    for _ in range(gated_layers))
         self.output_layer = S(L(num_neurons, output_dim))
         relu_units = [self.input_layer, *self.middle_layers]
         if batch_normalization:
@@ -58,12 +80,13 @@ class ParameterizerNN(torch.nn.Module):
     """Shared trunk + one two-layer head per distribution parameter (reference: src/submodels.py:41-69)."""
 
     def __init__(self, input_dim, output_dim, dist_params=["mu"], num_hidden_layers=2, num_neurons=50, dropout=False,
-                 dropout_rate=0.5, batch_normalization=False, **_):
+                 dropout_rate=0.5, batch_normalization=False, gated_layers=0, gated_hidden=None, gated_activation="silu", gated_eval_fp8=False, **_):
         super().__init__()
         self.dist_params = dist_params
         self.block_dict = torch.nn.ModuleDict()
         common = dict(num_neurons=num_neurons, dropout=dropout, dropout_rate=dropout_rate, batch_normalization=batch_normalization)
-        trunk = NNBlock(input_dim, num_neurons, num_hidden_layers=num_hidden_layers, **common)
+        trunk = NNBlock(input_dim, num_neurons, num_hidden_layers=num_hidden_layers, gated_layers=gated_layers, gated_hidden=gated_hidden,
+                        gated_activation=gated_activation, gated_eval_fp8=gated_eval_fp8, **common)
         trunk.output_layer.append(ACTIVATION)
         if batch_normalization:
             trunk.output_layer.append(torch.nn.BatchNorm1d(num_neurons))
@@ -135,7 +158,7 @@ class GaussianNN(torch.nn.Module):
 
     def __init__(self, input_dim, output_dim, sigma_fixed=1.0, sigma_lim=0.1, marginal_std_lim=None, average_max_std=1.0,
                  mu_upper_lim=5.0, mu_lower_lim=-3.0, learn_sigma=True, num_hidden_layers=2, num_neurons=50, dropout=True,
-                 dropout_rate=0.5, batch_normalization=True, **_):
+                 dropout_rate=0.5, batch_normalization=True, gated_layers=0, gated_hidden=None, gated_activation="silu", gated_eval_fp8=False, **_):
         super().__init__()
         self.input_dim, self.output_dim = input_dim, output_dim
         self.learn_sigma, self.sigma_fixed = learn_sigma, sigma_fixed
@@ -149,7 +172,8 @@ class GaussianNN(torch.nn.Module):
         self.mu_upper_lim, self.mu_lower_lim = mu_upper_lim, mu_lower_lim
         self.parameterizer = ParameterizerNN(input_dim, output_dim, dist_params=["mu", "sigma"] if learn_sigma else ["mu"],
                                              num_hidden_layers=num_hidden_layers, num_neurons=num_neurons, dropout=dropout,
-                                             dropout_rate=dropout_rate, batch_normalization=batch_normalization)
+                                             dropout_rate=dropout_rate, batch_normalization=batch_normalization, gated_layers=gated_layers,
+                                             gated_hidden=gated_hidden, gated_activation=gated_activation, gated_eval_fp8=gated_eval_fp8)
         self._plan = None
 
     def plan(self) -> E.NetPlan:
@@ -215,7 +239,7 @@ class DictionaryGaussian(torch.nn.Module):
 
     def __init__(self, input_dim, output_dim, vocab_size=100, sigma_lim=0.1, marginal_std_lim=0.01, average_max_std=1.0,
                  mu_upper_lim=5.0, mu_lower_lim=-3.0, num_hidden_layers=2, num_neurons=50, dropout=True, dropout_rate=0.5,
-                 batch_normalization=True, **_):
+                 batch_normalization=True, gated_layers=0, gated_hidden=None, gated_activation="silu", gated_eval_fp8=False, **_):
         super().__init__()
         if vocab_size <= output_dim:
             raise ValueError("Vocabulary size should be larger than the output dimension. Please increase the vocabulary size.")
@@ -230,7 +254,8 @@ class DictionaryGaussian(torch.nn.Module):
             raise ValueError("Sigma upper limit is smaller than sigma lower limit. Please decresase the vocabulary size or the sigma lower limit.")
         self.parameterizer = ParameterizerNN(input_dim, {"mu": output_dim, "sigma": vocab_size}, dist_params=["mu", "sigma"],
                                              num_hidden_layers=num_hidden_layers, num_neurons=num_neurons, dropout=dropout,
-                                             dropout_rate=dropout_rate, batch_normalization=batch_normalization)
+                                             dropout_rate=dropout_rate, batch_normalization=batch_normalization, gated_layers=gated_layers,
+                                             gated_hidden=gated_hidden, gated_activation=gated_activation, gated_eval_fp8=gated_eval_fp8)
         self.SigmaMapper = torch.nn.Parameter(torch.randn(output_dim, vocab_size), requires_grad=True)
         self._plan = None
 

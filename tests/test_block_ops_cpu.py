@@ -1,0 +1,202 @@
+"""What the gated residual block's operators refuse, without a GPU: every case ends in an exception (Python) or a non-zero status
+with a message (C entry points) before anything could be launched."""
+import ctypes
+
+import pytest
+import torch
+
+from behavio_temporal_vae_amd import _native as nv
+from behavio_temporal_vae_amd import block_ops as B
+
+BF = torch.bfloat16
+M, K, F, N = 5, 8, 12, 6
+
+
+def ffn(**kw):
+    t = dict(x=torch.zeros(M, K), w_gate=torch.zeros(F, K), w_up=torch.zeros(F, K), w_down=torch.zeros(N, F), b_gate=None, b_up=None, b_down=None)
+    act = kw.pop("activation", "silu")
+    t.update(kw)
+    return lambda fn: fn(*t.values(), activation=act)
+
+
+@pytest.mark.parametrize("fn", [B.gated_feed_forward, B.gated_feed_forward_tape])
+@pytest.mark.parametrize("call,error,words", [
+    (ffn(), RuntimeError, "MI355X only"),
+    (ffn(activation="tanh"), ValueError, "unknown activation"),
+    (ffn(activation=["silu"]), ValueError, "unknown activation"),
+    (ffn(x=[[0.0]]), TypeError, "x must be a tensor"),
+    (ffn(x=torch.zeros(M, K, dtype=torch.float16)), TypeError, "x must be float32 or bfloat16"),
+    (ffn(x=torch.zeros(M, K, dtype=torch.float64)), TypeError, "x must be"),
+    (ffn(x=torch.tensor(1.0)), ValueError, "at least one dimension"),
+    (ffn(x=torch.zeros(M, 0), w_gate=torch.zeros(F, 0), w_up=torch.zeros(F, 0)), ValueError, "no columns"),
+    (ffn(x=torch.zeros(M, K + 1)), ValueError, "w_gate must have shape"),
+    (ffn(x=torch.zeros(M, K, dtype=BF)), TypeError, "w_gate must be bfloat16"),
+    (ffn(w_gate=torch.zeros(0, K), w_up=torch.zeros(0, K), w_down=torch.zeros(N, 0)), ValueError, "w_gate must be a matrix"),
+    (ffn(w_gate=torch.zeros(F)), ValueError, "w_gate must be a matrix"),
+    (ffn(w_up=torch.zeros(F + 1, K)), ValueError, "w_up must have shape"),
+    (ffn(w_down=torch.zeros(N, F + 1)), ValueError, "w_down must have shape"),
+    (ffn(w_down=torch.zeros(0, F)), ValueError, "w_down must be a matrix"),
+    (ffn(w_down=torch.zeros(N, F, dtype=BF)), TypeError, "w_down must be float32"),
+    (ffn(w_up=torch.zeros(F, K, device="meta")), RuntimeError, "w_up is on meta"),
+    (ffn(b_gate=torch.zeros(F + 1)), ValueError, "b_gate must have shape"),
+    (ffn(b_up=torch.zeros(1, F)), ValueError, "b_up must have shape"),
+    (ffn(b_down=torch.zeros(N, dtype=BF)), TypeError, "b_down must be float32"),
+    (ffn(x=torch.zeros(M, K, requires_grad=True)), RuntimeError, "MI355X only"),
+])
+def test_ffn_refusals(fn, call, error, words):
+    with pytest.raises(error, match=words):
+        call(fn)
+
+
+def norm(**kw):
+    t = dict(residual=torch.zeros(M, N), branch=torch.zeros(M, N))
+    t.update(kw)
+    return lambda fn: fn(**t)
+
+
+@pytest.mark.parametrize("fn", [B.norm_gate_residual, B.norm_gate_residual_tape])
+@pytest.mark.parametrize("call,error,words", [
+    (norm(), RuntimeError, "MI355X only"),
+    (norm(post_norm="batch"), ValueError, "unknown norm"),
+    (norm(pre_norm=3), ValueError, "unknown norm"),
+    (norm(residual=torch.zeros(M, N, dtype=torch.float16)), TypeError, "residual must be"),
+    (norm(residual=torch.zeros(M, N, dtype=BF)), TypeError, "bfloat16 residual needs a bfloat16 branch"),
+    (norm(residual=torch.zeros(M, 0), branch=torch.zeros(M, 0)), ValueError, "no columns"),
+    (norm(residual=torch.zeros(1, 8193), branch=torch.zeros(1, 8193)), ValueError, "up to 8192 columns"),
+    (norm(eps=-1.0), ValueError, "eps"),
+    (norm(eps=float("nan")), ValueError, "eps"),
+    (norm(branch=torch.zeros(M, N + 1)), ValueError, "branch must have shape"),
+    (norm(branch=torch.zeros(M + 1, N)), ValueError, "branch must have shape"),
+    (norm(branch=None, scale=2.0), ValueError, "need a branch"),
+    (norm(branch=None, gate=torch.zeros(1, N)), ValueError, "need a branch"),
+    (norm(branch=None, post_norm="rms"), ValueError, "need a branch"),
+    (norm(branch=None, pre_norm=None), ValueError, "nothing to compute"),
+    (norm(gate=torch.zeros(2, N)), ValueError, "a multiple of G"),
+    (norm(gate=torch.zeros(0, N)), ValueError, "a multiple of G"),
+    (norm(gate=torch.zeros(M, N - 1)), ValueError, "gate must be"),
+    (norm(gate=torch.zeros(M, N, dtype=BF)), TypeError, "gate must be float32"),
+    (norm(scale=torch.zeros(N + 1)), ValueError, "scale must have shape"),
+    (norm(scale=torch.zeros(N, dtype=BF)), TypeError, "scale must be float32"),
+    (norm(post_weight=torch.ones(N)), ValueError, "need a post norm"),
+    (norm(pre_norm=None, pre_bias=torch.ones(N)), ValueError, "need a pre norm"),
+    (norm(pre_weight=torch.ones(N - 1)), ValueError, "pre_weight must have shape"),
+    (norm(post_norm="layer", post_bias=torch.ones(N, dtype=BF)), TypeError, "post_bias must be float32"),
+    (norm(normed_dtype=BF), TypeError, "normed_dtype must be float32"),
+    (norm(branch=None, normed_dtype=torch.float16), TypeError, "normed_dtype must be float32 or bfloat16"),
+    (norm(residual=torch.zeros(M, N, dtype=BF), branch=None, normed_dtype=torch.float32), TypeError, "normed_dtype must be bfloat16"),
+    (norm(branch=torch.zeros(M, N, device="meta")), RuntimeError, "branch is on meta"),
+])
+def test_norm_refusals(fn, call, error, words):
+    with pytest.raises(error, match=words):
+        call(fn)
+
+
+def weight(n=N, k=K):
+    kb = -(-k // 128)
+    return B.Fp8Weight(torch.zeros(n, kb * 128, dtype=torch.uint8), torch.zeros(-(-n // 128), 4 * (-(-kb // 4)), dtype=torch.uint8), (n, k))
+
+
+@pytest.mark.parametrize("call,error,words", [
+    (lambda: B.fp8_quantize(torch.zeros(M, K)), RuntimeError, "MI355X only"),
+    (lambda: B.fp8_quantize(torch.zeros(M, K, dtype=torch.float16)), TypeError, "x must be"),
+    (lambda: B.fp8_quantize(torch.zeros(M, 0)), ValueError, "no columns"),
+    (lambda: B.fp8_quantize(torch.zeros(M, K, requires_grad=True)), RuntimeError, "no backward pass"),
+    (lambda: B.fp8_weight(torch.zeros(N, K)), RuntimeError, "MI355X only"),
+    (lambda: B.fp8_weight(torch.zeros(N)), ValueError, "must be a matrix"),
+    (lambda: B.fp8_weight(torch.zeros(0, K)), ValueError, "must be a matrix"),
+    (lambda: B.fp8_weight(torch.zeros(N, K, dtype=torch.int8)), TypeError, "the weight must be"),
+    (lambda: B.fp8_linear(torch.zeros(M, K), torch.zeros(N, K)), TypeError, "fp8_weight"),
+    (lambda: B.fp8_linear(torch.zeros(M, K + 1), weight()), ValueError, "x must have 8 columns"),
+    (lambda: B.fp8_linear(torch.tensor(0.0), weight()), ValueError, "x must have 8 columns"),
+    (lambda: B.fp8_linear(weight(), weight()), TypeError, "x must be a tensor"),
+    (lambda: B.fp8_linear(torch.zeros(M, K), weight(), torch.zeros(N + 1)), ValueError, "bias must have shape"),
+    (lambda: B.fp8_linear(torch.zeros(M, K), weight(), torch.zeros(N, requires_grad=True)), RuntimeError, "no backward pass"),
+    (lambda: B.fp8_linear(torch.zeros(M, K, requires_grad=True), weight()), RuntimeError, "no backward pass"),
+    (lambda: B.fp8_linear(torch.zeros(M, K), weight(), out_dtype=torch.float16), TypeError, "out_dtype"),
+    (lambda: B.fp8_linear(torch.zeros(M, K, device="meta"), weight()), RuntimeError, "the weight is on cpu"),
+    (lambda: B.fp8_linear(torch.zeros(M, K), weight()), RuntimeError, "MI355X only"),
+    (lambda: B.fp8_gated_weights(torch.zeros(F, K), torch.zeros(F, K), torch.zeros(N, F)), RuntimeError, "MI355X only"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K), weight()), TypeError, "fp8_gated_weights"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K), gated(), "softplus"), ValueError, "unknown activation"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K + 1), gated()), ValueError, "x must have 8 columns"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K), gated(), out_dtype=torch.int8), TypeError, "out_dtype"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K, requires_grad=True), gated()), RuntimeError, "no backward pass"),
+    (lambda: B.fp8_gated_feed_forward(torch.zeros(M, K), gated()), RuntimeError, "MI355X only"),
+])
+def test_fp8_refusals(call, error, words):
+    with pytest.raises(error, match=words):
+        call()
+
+
+def gated():
+    return B.Fp8GatedWeights(weight(F, K), weight(F, K), weight(N, F), None, None, None)
+
+
+def test_c_entry_points_refuse():
+    """Sizes, layouts and workspaces that the kernels do not take come back as a status, with a message."""
+    lib = nv.lib()
+    a = 1 << 20                                    # an address that is never followed: every call is refused first
+
+    def refused(name, words, *args):
+        assert getattr(lib, name)(*args, None) != 0, (name, args)
+        assert words in nv.last_error(), (words, nv.last_error())
+
+    def pack(words, **kw):
+        j = dict(src=a, bf16=0, ld=64, dst=a, planes=1, dld=128, rows=4, cols=64, dst_cols=64, t=0)
+        j.update(kw)
+        refused("btvae_block_pack", words, (ctypes.c_longlong * 10)(*j.values()), 1)
+
+    pack("planes", planes=2)
+    pack("source", cols=0)
+    pack("source", rows=-1)
+    pack("source", ld=63)
+    pack("source", rows=1 << 31)
+    pack("destination", dst_cols=60)
+    pack("destination", dst=a + 8)
+    pack("destination", dld=120)
+    pack("destination", planes=3)                  # a row of 64 columns is 384 bytes
+    pack("destination", t=1, rows=80)              # 80 columns do not fit in 64
+    pack("null", src=0)
+    refused("btvae_block_pack", "four", None, 1)
+    refused("btvae_block_pack", "four", (ctypes.c_longlong * 50)(), 5)
+
+    refused("btvae_gated_proj_fwd", "planes", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 2, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "sizes", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 0, 4, 64, 60)
+    refused("btvae_gated_proj_fwd", "activation", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 4, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "operand", a, 112, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "layout of H", a, 128, a, a, 128, None, None, 0, a, 112, None, None, 0, 0, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "kept", a, 128, a, a, 128, None, None, 0, a, 128, a, None, 128, 64, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "kept", a, 128, a, a, 128, None, None, 0, a, 128, a, a, 128, 32, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_bwd", "kept", a, 128, a, 128, None, None, 128, 64, a, 256, None, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_bwd", "gradients", a, 128, a, 128, a, a, 128, 64, a, 128, None, 1, 0, 4, 64, 64)
+    refused("btvae_block_product", "sizes", a, 128, a, 128, None, 0, a, 60, 0, None, 0, 1, 4, 64, 64)
+    refused("btvae_block_product", "operand", a, 128, a + 4, 128, None, 0, a, 64, 0, None, 0, 1, 4, 64, 64)
+    need = lib.btvae_block_product_ws(64, 64, 4096, 1)
+    assert need > 0
+    refused("btvae_block_product", "workspace", a, 8192, a, 8192, None, 0, a, 64, 0, a, need - 1, 1, 64, 64, 4096)
+    refused("btvae_block_wgrad", "sizes", a, 128, a, 128, a, 1, a, 65, None, 0, 0, 64, 0, 0, 1, 64, 64, 4)
+    refused("btvae_block_wgrad", "row ranges", a, 128, a, 128, a, 1, a, 32, a, 16, 32, 64, 0, 0, 1, 64, 64, 4)
+    refused("btvae_block_wgrad", "workspace", a, 128, a, 128, a, 0, a, 64, None, 0, 0, 64, 0, 0, 1, 64, 64, 4)
+    refused("btvae_block_colsum", "workspace", a, 0, 64, None, 0, a, 0, 0, 4, 64)
+    refused("btvae_block_strip_sums", "sizes", a, -1, 64, a, a, 0, 0)
+    rows = lib.btvae_few_rows_max()
+    refused("btvae_few_rows", "sizes", a, 0, 64, a, None, 0, 64, None, None, a, 0, 64, 0, rows + 1, 64, 64)
+    refused("btvae_few_rows", "types", a, 1, 64, a, None, 0, 64, None, None, a, 0, 64, 0, 1, 64, 64)
+    refused("btvae_few_rows", "types", a, 0, 64, a, a, 1, 64, None, None, a, 0, 64, 0, 1, 64, 64)
+    refused("btvae_fp8_few_rows", "layout", a, 0, 64, a, a, None, None, 64, 4, None, None, a, 64, 0, 0, 1, 64, 64)
+    refused("btvae_fp8_quantize", "layout", a, 0, 64, a, 64, a, 4, 4, 64)
+    refused("btvae_fp8_product", "operand", a, 128, a, 3, a, 128, a, 4, None, a, 64, 0, None, 0, 4, 64, 64)
+    limit = lib.btvae_norm_max_columns()
+    none = [None] * 3
+
+    def nfwd(words, M=4, N=64, types=0, post=0, pre=1, eps=1e-6, branch=a, gate=None, G=0, out=a, normed=a):
+        refused("btvae_norm_gate_residual_fwd", words, a, branch, gate, G, 1.0, None, *none, None, post, pre, eps, out, normed, None, types, M, N)
+
+    nfwd("columns", N=limit + 1)
+    nfwd("columns", N=0)
+    nfwd("bf16 branch", types=1)
+    nfwd("bad norm", post=3)
+    nfwd("bad norm", eps=-1.0)
+    nfwd("outputs", out=None)
+    nfwd("outputs", normed=None)
+    nfwd("gate rows", gate=a, G=3)

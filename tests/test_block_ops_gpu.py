@@ -704,3 +704,172 @@ def test_block_run_together(dev):
             stream, n = B.norm_gate_residual(stream, B.fp8_gated_feed_forward(n, packed[i]), gate=p["gate"], scale=0.5, post_norm="rms", post_weight=p[f"post{i}"], pre_weight=p[f"pre{i + 1}"])
     # e4m3 rounds to 2^-4 of a value (rms about a third of it): five roundings meet in a unit's result, damped by the residual sum
     frob(n, yr.detach(), 2 * math.sqrt(5) * 2.0 ** -4, "two blocks in 8 bits")
+
+
+def test_norm_normed_dtype(dev):
+    """A bfloat16 normed of a float32 residual without a branch: the float32 result rounded once; gradients from a bfloat16 one."""
+    M, N = 37, 72
+    x, w = rnd(dev, M, N, seed=91).requires_grad_(), rnd(dev, N, seed=92).requires_grad_()
+    s, n = B.norm_gate_residual(x, pre_weight=w, normed_dtype=BF)
+    assert s is x and n.dtype == BF
+    assert torch.equal(n, B.norm_gate_residual(x, pre_weight=w)[1].to(BF))
+    d = rnd(dev, M, N, seed=93, dtype=BF)
+    got = torch.autograd.grad(n, [x, w], d)
+    want = torch.autograd.grad(B.norm_gate_residual(x, pre_weight=w)[1], [x, w], d.float())
+    for g, r in zip(got, want):
+        assert torch.equal(g, r)
+
+
+# ---- the gated layers of a network -----------------------------------------------------------------------------------------
+class Cdim:
+    def __init__(self, c):
+        self.cond_dim = c
+
+
+def conditions(prec):
+    """Width of the conditions: bf16 mode wants network inputs of whole groups of four columns."""
+    return 4 if prec == "bf16" else 5
+
+
+def gated_model(dev, prec, hidden, gated, bn=True, eval_fp8=False, act="silu", width=40):
+    from behavio_temporal_vae_amd.vae_models import CVAE
+    common = dict(num_neurons=width, num_hidden_layers=hidden, dropout=False, batch_normalization=bn, gated_layers=gated, gated_hidden=72, gated_activation=act,
+                  gated_eval_fp8=eval_fp8)
+    cfg = {"latent_dim": 8, "gemm_precision": prec, "distribution_dict": {
+        "posterior": {"dist_type": "normal", "sigma_lim": 0.05, "mu_upper_lim": 5.0, "mu_lower_lim": -5.0, **common},
+        "likelihood": {"dist_type": "normal", "sigma_lim": 0.05, "mu_upper_lim": 5.0, "mu_lower_lim": -5.0, **common}}}
+    torch.manual_seed(17)
+    return CVAE(input_dim=24, conditioner=Cdim(conditions(prec)), **cfg).to(dev)
+
+
+def net64(net, x, train, wide=None):
+    """A network's raw head outputs in 64 bits from its parameters ``wide`` (name -> tensor) by plain formulas."""
+    blocks = net.parameterizer.block_dict
+    names = {id(p): k for k, p in net.named_parameters()}
+    P = lambda p: wide[names[id(p)]]
+
+    def unit(seq, h, residual):
+        y = torch.relu(h @ P(seq[0].weight).t() + P(seq[0].bias))
+        for m in list(seq)[1:]:
+            if isinstance(m, torch.nn.BatchNorm1d):
+                mean, var = (y.mean(0), y.var(0, unbiased=False)) if train else (m.running_mean.double(), m.running_var.double())
+                y = (y - mean) / torch.sqrt(var + m.eps) * P(m.weight) + P(m.bias)
+        return y + h if residual else y
+
+    t = blocks["input"]
+    h = unit(t.input_layer, x, False)
+    for seq in t.middle_layers:
+        h = unit(seq, h, True)
+    for g in getattr(t, "gated_layers", []):
+        n = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6) * P(g.norm)
+        y = act64(g.activation, n @ P(g.gate.weight).t() + P(g.gate.bias)) * (n @ P(g.up.weight).t() + P(g.up.bias))
+        h = h + P(g.scale) * (y @ P(g.down.weight).t() + P(g.down.bias))
+    h = unit(t.output_layer, h, False)
+    out = {}
+    for name in ("mu", "sigma"):
+        b = blocks[name]
+        v = unit(b.input_layer, h, False)
+        out[name] = v @ P(b.output_layer[0].weight).t() + P(b.output_layer[0].bias)
+    lo, hi = net.head_specs()["mu"][1:]
+    lo2, hi2 = net.head_specs()["sigma"][1:]
+    return {"mu": out["mu"].clamp(lo, hi), "sigma": torch.nn.functional.softplus(out["sigma"]).clamp(lo2, hi2)}
+
+
+# Tolerances of a whole network.  Its products, six to nine of them one behind another, each add the operators' own errors (float32:
+# 2^-24 (4 + sqrt(K)) with K <= 72, 13 2^-24) times the amplification of the layers behind, which for these widths and initial weights
+# stays under 10, and BatchNorm's division by a column's deviation: float32 modes are held to 2000 2^-24 = 1.2e-4 of a tensor's norm.
+# bf16 mode rounds every product's operands (2^-8 relative each, in Frobenius norm sqrt(2) 2^-9 a product at least): 40 2^-8 of the norm
+# over all gradients together.
+@pytest.mark.parametrize("prec,hidden,gated,bn,act", [("fp32", 1, 1, True, "silu"), ("fp32_split", 0, 2, True, "gelu"), ("fp32_split2", 2, 1, False, "relu"),
+                                                      ("bf16", 1, 2, True, "silu")])
+@pytest.mark.parametrize("M", [20, 130])
+def test_network_with_gated_layers(dev, prec, hidden, gated, bn, act, M):
+    """Head outputs and every parameter's gradient of a decoder with gated layers against formulas in 64 bits."""
+    m = gated_model(dev, prec, hidden, gated, bn, act=act).train()
+    m._check_arena()
+    net = m.decoder
+    x = rnd(dev, M, 8 + conditions(prec), seed=51).requires_grad_()
+    wmu, wsg = rnd(dev, M, 24, seed=52), rnd(dev, M, 24, seed=53)
+    try:
+        for p in net.parameters():
+            p.grad.zero_()
+        out = net(x)
+        ((out["mu"] * wmu).sum() + (out["sigma"] * wsg).sum()).backward()
+        wide = {k: p.detach().double().requires_grad_() for k, p in net.named_parameters()}
+        x64 = x.detach().double().requires_grad_()
+        ref = net64(net, x64, True, wide)
+        ((ref["mu"] * wmu.double()).sum() + (ref["sigma"] * wsg.double()).sum()).backward()
+        tol = 40 * U if prec == "bf16" else 2000 * E
+        for k in ("mu", "sigma"):
+            frob(out[k], ref[k].detach(), tol, k)
+        whole = math.sqrt(sum(float(w.grad.norm()) ** 2 for w in wide.values()))
+        for k, p in net.named_parameters():
+            assert ((p.grad.double() - wide[k].grad).norm().item()) <= tol * whole, k
+        frob(x.grad, x64.grad, tol, "input gradient") if prec != "bf16" else None
+        assert any("gated_layers" in k for k, _ in net.named_parameters())
+    finally:
+        nv.set_gemm_precision("fp32")
+
+
+@pytest.mark.parametrize("prec", ["fp32_split2", "bf16"])
+@pytest.mark.parametrize("M", [1, 20, 300])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_network_with_gated_layers_eval(dev, prec, M, fp8):
+    """Eval mode: few rows and many, float32 and bf16, and the 8-bit form (which differs from the plain one by the e4m3 roundings
+    of both operands, 2^-4 each, in the branches that the scale 0.1 adds: an order below them)."""
+    m = gated_model(dev, prec, 1, 2, eval_fp8=fp8).eval()
+    net = m.decoder
+    x = rnd(dev, M, 8 + conditions(prec), seed=61)
+    try:
+        m._check_arena()
+        with torch.no_grad():
+            out = net(x)
+        wide = {k: p.detach().double() for k, p in net.named_parameters()}
+        ref = net64(net, x.double(), False, wide)
+        tol = 2.0 ** -4 if fp8 else 40 * U if prec == "bf16" else 2000 * E
+        for k in ("mu", "sigma"):
+            frob(out[k], ref[k], tol, k)
+        if fp8:
+            for g in net.parameterizer.block_dict["input"].gated_layers:
+                g.eval_fp8 = False
+            with torch.no_grad():
+                plain = net(x)
+            assert not torch.equal(plain["mu"], out["mu"])            # the 8-bit form ran
+    finally:
+        nv.set_gemm_precision("fp32")
+
+
+@pytest.mark.parametrize("prec", ["fp32_split2", "bf16"])
+def test_training_steps_with_gated_layers_captured(dev, monkeypatch, prec):
+    """Training steps replayed from captured graphs change the weights bit for bit as eager steps do; a state dict goes round."""
+    x, c, eps = rnd(dev, 60, 24, seed=71), rnd(dev, 60, conditions(prec), seed=72), rnd(dev, 2, 60, 8, seed=73)
+    runs = []
+    try:
+        for mode in ("0", "1"):
+            monkeypatch.setenv("BTVAE_STEP_GRAPH", mode)
+            m = gated_model(dev, prec, 1, 1).train()
+            m.train_kwargs = {"num_mc_samples": 2, "beta": 0.8, "gradient_clipping": True, "gradient_clipping_kwargs": {"max_norm": 1.0}}
+            opt = m.get_optimizer(lr=1e-3, weight_decay=1e-5)
+            for i in range(7):
+                out = m._train_step(x, c, opt, eps=eps)
+                out["loss"].item()
+                (x * 2).sum().item()                                   # eager work between the replays
+            runs.append({k: v.detach().clone() for k, v in m.state_dict().items()})
+            assert bool(m.__dict__.get("_step_graphs")) == (mode == "1")
+        for k, v in runs[0].items():
+            assert torch.equal(v, runs[1][k]), k
+        fresh = gated_model(dev, prec, 1, 1)
+        before = {k: v.clone() for k, v in fresh.state_dict().items()}
+        assert any(not torch.equal(before[k], runs[0][k]) for k in before if "gated_layers" in k and "scale" in k)
+        fresh.load_state_dict(runs[0])
+        m.eval(), fresh.eval()
+        z = x[:, :8 + conditions(prec)].contiguous()
+        with torch.no_grad():
+            assert torch.equal(fresh.decoder(z)["mu"], m.decoder(z)["mu"])
+    finally:
+        nv.set_gemm_precision("fp32")
+
+
+def test_gated_layers_argument_checks(dev):
+    with pytest.raises(ValueError, match="gated_activation"):
+        gated_model(dev, "fp32", 1, 1, act="tanh")
