@@ -225,6 +225,12 @@ __device__ __forceinline__ void meet() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// copies of `per` that belong to step q of `steps`
+constexpr int share(int per, int steps, int q) {
+    int n = 0;
+    for (int j = 0; j < per; ++j) n += j * steps / per == q;
+    return n;
+}
 // Order of a region's instructions: R LDS reads, one behind each of the first matrix instructions (issued in one go they would
 // hold the wave up with its matrix pipe idle; issued late their results would), then V copies the same way, of M matrix instructions.
 template <int M, int R, int V> __device__ __forceinline__ void spread() {
@@ -241,6 +247,21 @@ template <int M, int R, int V> __device__ __forceinline__ void spread() {
     __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
 }
 
+// The same with R LDS reads, W LDS writes and V loads, a third of the matrix instructions' worth at a time
+template <int M, int R, int V, int W = V> __device__ __forceinline__ void refill() {
+    constexpr int ALL = R + V + W;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+        for (int k = i * ALL / M; k < (i + 1) * ALL / M; ++k) {
+            if (k < R) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            else if (k < R + W) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            else __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+    }
+}
+__device__ __forceinline__ void wait_lds() { wait_vm<63>(); }
 // A scalar that the compiler knows nothing about: address and edge computations made from it stay inside their block of results instead of
 // being made for all blocks at once and kept, which costs more registers than there are.
 __device__ __forceinline__ int opaque(int x) {
@@ -444,7 +465,8 @@ template <int FMT, int EP, int WM, int WN, int MI, int NJ>
 __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows(const Args p) {
     constexpr bool GATED = is_gated(EP), FAST = EP != EP_GATED_3 && EP != EP_GATED_BWD_3;
     constexpr bool SPLIT = FMT == FMT_SPLIT;
-    constexpr int ROWB = row_bytes(FMT), SLOTS = SPLIT ? 3 : 2;
+    constexpr int ROWB = row_bytes(FMT), SLOTS = SPLIT || WM * WN == 8 ? 3 : 2;
+    constexpr bool EARLY = !SPLIT && SLOTS == 3;              // copies go into the slot of the stage before
     constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
     constexpr int STAGE = (TM + TN) * ROWB, RING = SLOTS * STAGE;
     constexpr int NA = TM * ROWB / 1024 / NW, NB = TN * ROWB / 1024 / NW;      // copies of a wave and stage
@@ -606,11 +628,24 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         for (int j = 0; j < NJ; ++j) fb[decltype(to)::value][j] = frag(sb, ob[j], decltype(set)::value);
     };
     // the steps of a stage but the last: multiply one, read the next
-    auto inner = [&](const char* sb) {
+    // (EARLY: with the copies of the stage behind the next, a share to each step)
+    constexpr int PER = NA + NB;
+    auto copy = [&](auto step, const char* ab, const char* bb, const char* bb2, char* to) {
+        constexpr int q = decltype(step)::value;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (j * STEPS / PER == q) {
+                if (j < NA) glds16(ab + aofs[j < NA ? j : 0], to + (wid * NA + j) * 1024);
+                else glds16((up_part(j - NA) ? bb2 : bb) + bofs[j < NA ? 0 : j - NA], to + TM * ROWB + (wid * NB + j - NA) * 1024);
+            }
+    };
+    auto inner = [&](const char* sb, auto copies, const char* ab, const char* bb, const char* bb2, char* to) {
+        constexpr bool C = decltype(copies)::value;
         auto one = [&](auto s) {
             load_set(std::integral_constant<int, decltype(s)::value + 1>{}, sb, decltype(s)::value + 1);
+            if constexpr (C) copy(s, ab, bb, bb2, to);
             multiply(s);
-            spread<MI * NJ, READS, 0>();
+            spread<MI * NJ, READS, C ? share(PER, STEPS, decltype(s)::value) : 0>();
             __builtin_amdgcn_sched_barrier(0);
         };
         one(std::integral_constant<int, 0>{});
@@ -626,7 +661,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
 
     open_feed();
 #pragma unroll 1
-    for (int s = 0; s < SLOTS; ++s)
+    for (int s = 0; s < (EARLY ? 2 : SLOTS); ++s)
         if (f_total > 0) issue();
     if constexpr (SPLIT) f_slot = 0;                          // (also when there were fewer stages than slots)
     int slot = 0, scslot = 0;
@@ -757,14 +792,18 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         if constexpr (!SPLIT) {
             // one stage; the next one's first operands are read behind its last step
             auto stage = [&](int t) {
+                if constexpr (EARLY)
+                    if (f_total > 0) issue();
                 scales(t);
-                inner(smem + slot * STAGE);
-                slot ^= 1;
+                inner(smem + slot * STAGE, std::false_type{}, nullptr, nullptr, nullptr, nullptr);
+                slot = slot + 1 == SLOTS ? 0 : slot + 1;
                 if (--w_total > 0) {
-                    wait_vm<0>();                                 // the next stage has landed (and earlier results are stored)
+                    if (EARLY && w_total - f_total >= 2) wait_vm<PER>();      // the next stage has landed; the one behind it may be on its way
+                    else wait_vm<0>();                        // (and earlier results are stored)
                     meet();
                     load_set(S0, smem + slot * STAGE, 0);
-                    if (f_total > 0) issue();                     // into the slot that everyone has just read
+                    if constexpr (!EARLY)
+                        if (f_total > 0) issue();             // into the slot that everyone has just read
                 }
                 multiply(S1);
             };
@@ -776,24 +815,30 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                 for (int left = run; left > 0; --left, ++t) {
                     scales(t);
                     char* sb = smem + slot * STAGE;
-                    inner(sb);
-                    slot ^= 1;
-                    wait_vm<0>();
+                    char* to = EARLY ? smem + f_slot * STAGE : sb;
+                    inner(sb, std::integral_constant<bool, EARLY>{}, ab, bb, bb2, to);
+                    slot = slot + 1 == SLOTS ? 0 : slot + 1;
+                    wait_vm<EARLY ? PER - share(PER, STEPS, STEPS - 1) : 0>();
                     meet();
                     load_set(S0, smem + slot * STAGE, 0);
-    #pragma unroll
-                    for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
-    #pragma unroll
-                    for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+                    if constexpr (EARLY) {
+                        copy(std::integral_constant<int, STEPS - 1>{}, ab, bb, bb2, to);
+                        f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
+#pragma unroll
+                        for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+                    }
                     ab += ROWB; bb += ROWB;
                     if constexpr (GATED) bb2 += ROWB;
                     multiply(S1);
-                    spread<MI * NJ, READS, NA + NB>();
+                    spread<MI * NJ, READS, EARLY ? share(PER, STEPS, STEPS - 1) : PER>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 koff += (long long)run * ROWB;
                 f_kin += run; f_left -= run; f_total -= run; w_total -= run;
-                f_slot = slot;                                    // (the slot read now is refilled next)
+                if constexpr (!EARLY) f_slot = slot;          // (the slot read now is refilled next)
             };
             for (int t = 0; t < nk; ++t) {
                 // (a group of scale words begins with a copy of its own, a last stage may end inside the rows)
@@ -1027,7 +1072,7 @@ struct ColArgs {
 template <bool SPLIT, int WM, int WN, int MI, int NJ>
 __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols(const ColArgs p) {
     constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
-    constexpr int EB = SPLIT ? 6 : 2, SR = SPLIT ? 16 : 32, SLOTS = SPLIT ? 3 : 4;        // bytes of a column, rows of a stage
+    constexpr int EB = SPLIT ? 6 : 2, SR = SPLIT ? 16 : 32, SLOTS = 3, SETS = SPLIT ? 1 : 2;        // bytes of a column, rows of a stage, stages in LDS and in registers
     constexpr int ARB = TM * EB, BRB = TN * EB;               // bytes of an image row
     constexpr int STAGE = SR * (ARB + BRB), RING = SLOTS * STAGE;
     constexpr int NA = SR * ARB / 1024 / NW, NB = SR * BRB / 1024 / NW, NGL = NA + NB;
@@ -1076,20 +1121,28 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
     const char* ab = p.A + (long long)rbeg * p.lda;
     const char* bb = p.B + (long long)rbeg * p.ldb;
     const char* zero = reinterpret_cast<const char*>(zero_piece);
-    int f_slot = 0, left = rows;                              // rows not yet copied
-    // A stage's copies; rows past the end are zeros, and past the last stage all of them are: one straight path
-    auto copy_a = [&]() {
+    int f_slot = 0, left = rows;                              // rows not yet loaded
+    typedef __attribute__((address_space(1))) u32x4 global_u32x4;
+    u32x4 regs[SETS][NGL];
+    // One stage's loads; rows past the end are zeros, and past the last stage all of them are: one straight path
+    auto fetch_a = [&](auto set) {
 #pragma unroll
-        for (int j = 0; j < NA; ++j) glds16(arow[j] < left ? ab + aofs[j] : zero, smem + f_slot * STAGE + (wid * NA + j) * 1024);
+        for (int j = 0; j < NA; ++j) regs[decltype(set)::value][j] = *(const global_u32x4*)(arow[j] < left ? ab + aofs[j] : zero);
     };
-    auto copy_b = [&]() {
+    auto fetch_b = [&](auto set) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) glds16(brow[j] < left ? bb + bofs[j] : zero, smem + f_slot * STAGE + SR * ARB + (wid * NB + j) * 1024);
-    };
-    auto advance = [&]() {
+        for (int j = 0; j < NB; ++j) regs[decltype(set)::value][NA + j] = *(const global_u32x4*)(brow[j] < left ? bb + bofs[j] : zero);
         ab += SR * p.lda;
         bb += SR * p.ldb;
         left -= SR;
+    };
+    auto put_a = [&](auto set) {
+#pragma unroll
+        for (int j = 0; j < NA; ++j) *reinterpret_cast<u32x4*>(smem + f_slot * STAGE + (wid * NA + j) * 1024 + lane * 16) = regs[decltype(set)::value][j];
+    };
+    auto put_b = [&](auto set) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<u32x4*>(smem + f_slot * STAGE + SR * ARB + (wid * NB + j) * 1024 + lane * 16) = regs[decltype(set)::value][NA + j];
         f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
     };
 
@@ -1142,13 +1195,20 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
     std::integral_constant<int, 2> S2;
     std::integral_constant<int, 3> S3;
 #pragma unroll 1
-    for (int s = 0; s < SLOTS; ++s) {
-        copy_a();
-        copy_b();
-        advance();
+    for (int s = 0; s < 2; ++s) {
+        fetch_a(S0);
+        fetch_b(S0);
+        put_a(S0);
+        put_b(S0);
+    }
+    fetch_a(S0);
+    fetch_b(S0);
+    if constexpr (SETS == 2) {
+        fetch_a(S1);
+        fetch_b(S1);
     }
     int slot = 0;
-    wait_vm<0>();
+    wait_lds();
     meet();
     if constexpr (SPLIT) {
         // the loop of gemm_rows' split operands
@@ -1163,7 +1223,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
             spread<MI * NJ, 2 * MI, 0>();
             __builtin_amdgcn_sched_barrier(0);
             slot = slot + 1 == SLOTS ? 0 : slot + 1;
-            wait_vm<NGL>();
+            wait_lds();                                       // this stage is read, and the next one written
             meet();
             const char* nb = smem + slot * STAGE;
             read_a(S2, 2, nb, 0);
@@ -1175,20 +1235,21 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
             spread<MI * NJ, 2 * NJ, 0>();
             __builtin_amdgcn_sched_barrier(0);
             read_b(S2, 2, nb, 0);
-            copy_a();
+            put_a(S0);
+            fetch_a(S0);
             product(S1, S0);
-            spread<MI * NJ, 2 * NJ, NA>();
+            refill<MI * NJ, 2 * NJ, NA>();
             __builtin_amdgcn_sched_barrier(0);
             read_a(S1, 1, nb, 0);
-            copy_b();
+            put_b(S0);
+            fetch_b(S0);
             product(S0, S1);
-            spread<MI * NJ, 2 * MI, NB>();
+            refill<MI * NJ, 2 * MI, NB>();
             __builtin_amdgcn_sched_barrier(0);
             read_b(S1, 1, nb, 0);
             product(S0, S0);
             spread<MI * NJ, 2 * NJ, 0>();
             __builtin_amdgcn_sched_barrier(0);
-            advance();
 #pragma unroll
             for (int j = 0; j < NJ; ++j) fb[0][j] = fb[3][j];
         }
@@ -1196,28 +1257,32 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
         read_a(S0, 0, smem, 0);
         read_b(S0, 0, smem, 0);
         constexpr int READS = 2 * (MI + NJ);
-        for (int t = 0; t < nk; ++t) {
+        auto stage = [&](auto set) {
             const char* cb = smem + slot * STAGE;
             read_a(S1, 0, cb, 1);
             read_b(S1, 0, cb, 1);
+            put_a(set);
+            put_b(set);
             product(S0, S0);
-            spread<MI * NJ, READS, 0>();
+            refill<MI * NJ, READS, 0, NGL>();
             __builtin_amdgcn_sched_barrier(0);
             slot = slot + 1 == SLOTS ? 0 : slot + 1;
-            wait_vm<2 * NGL>();                               // the next stage has landed once the two behind it are all that is on its way
+            wait_lds();                                       // this stage is read, and the next one written
             meet();
             const char* nb = smem + slot * STAGE;
             read_a(S0, 0, nb, 0);
             read_b(S0, 0, nb, 0);
-            copy_a();
-            copy_b();
+            fetch_a(set);
+            fetch_b(set);
             product(S1, S1);
-            spread<MI * NJ, READS, NGL>();
+            refill<MI * NJ, READS, NGL, 0>();
             __builtin_amdgcn_sched_barrier(0);
-            advance();
+        };
+        for (int t = 0; t < nk; t += 2) {                     // (an odd one out is followed by a stage of zeros)
+            stage(S0);
+            stage(S1);
         }
     }
-    wait_vm<0>();                                             // no copy may still be on its way when the LDS passes to others
     // a lane's results of a 32 x 32 block: row lane & 31, element r = column (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
     float* out = p.slab + (long long)zz * p.M * p.N;
 #pragma unroll
