@@ -97,6 +97,13 @@ __device__ __attribute__((aligned(64))) static const unsigned zero_piece[16] = {
 __device__ __forceinline__ void glds16(const void* g, void* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
+// The same through a buffer descriptor (a scalar base), at a lane's offset and a scalar one: no address arithmetic, and no wait for every
+// LDS read on its way, which the compiler inserts behind the form above.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_at(const void* base) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, -1, 0x00020000); }
+__device__ __forceinline__ void blds16(Buffer g, unsigned lane_offset, unsigned offset, void* l) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(g, (__attribute__((address_space(3))) void*)l, 16, lane_offset, offset, 0, 0);
+}
 // Byte offset of the logical 16-byte piece c of row r in a stage image.  128-byte rows: the XOR spreads the rows that one 16-lane
 // group of a ds_read_b128 touches (the same piece of 16 rows) over all 64 banks.  96-byte rows: eight rows do that by
 // themselves, the next eight take the other piece of a pair.
@@ -233,15 +240,16 @@ constexpr int share(int per, int steps, int q) {
 }
 // Order of a region's instructions: R LDS reads, one behind each of the first matrix instructions (issued in one go they would
 // hold the wave up with its matrix pipe idle; issued late their results would), then V copies the same way, of M matrix instructions.
-template <int M, int R, int V> __device__ __forceinline__ void spread() {
+template <int M, int R, int V, int P = 1> __device__ __forceinline__ void spread() {
+    constexpr int G = (R + P - 1) / P;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < G; ++i) {
         if (i < M) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, P, 0);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (R + i < M) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (G + i < M) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
@@ -273,8 +281,9 @@ __device__ __forceinline__ int opaque(int x) {
 // ---- stores and loads of the results' layout ------------------------------------------------------------------------
 // A lane's results of one 32-column block: v[q][e] = column 16 q + 8 (lane >> 5) + e of row lane & 31.  `row0`: matrix row of the
 // block's row 0, `col0`: matrix column of its column 0.
-constexpr int TURN_B = 2048;                                  // bytes of LDS to a wave
-struct Where {
+// HALF: in 1 KiB of LDS to a wave, 16 rows at a time, where the stages leave no more.
+template <bool HALF> struct Where {
+    static constexpr int LDS_B = HALF ? 1024 : 2048;
     int li, lh, r4, p4, r2, p2;                               // result row and half; row and piece of four / two lanes to a row
     char* lds;
     __device__ __forceinline__ explicit Where(char* wave_lds) : lds(wave_lds) {
@@ -291,15 +300,26 @@ struct Where {
     __device__ __forceinline__ static int two(int row) { return ((row >> 3) & 1) << 4; }
     // pieces c0, c1 (16 bytes each) of this lane's row of 64 bytes -> piece p4 of rows r4 and r4 + 16
     __device__ __forceinline__ void turn(const u32x4 x0, int c0, const u32x4 x1, int c1, u32x4& a, u32x4& b) const {
-        *at4(li, c0) = x0;
-        *at4(li, c1) = x1;
-        fence();
-        a = *at4(r4, p4);
-        b = *at4(r4 + 16, p4);
+        if constexpr (HALF) {
+            if (li < 16) { *at4(li, c0) = x0; *at4(li, c1) = x1; }
+            fence();
+            a = *at4(r4, p4);
+            fence();
+            if (li >= 16) { *at4(li - 16, c0) = x0; *at4(li - 16, c1) = x1; }
+            fence();
+            b = *at4(r4, p4);
+        } else {
+            *at4(li, c0) = x0;
+            *at4(li, c1) = x1;
+            fence();
+            a = *at4(r4, p4);
+            b = *at4(r4 + 16, p4);
+        }
         fence();
     }
     // ... and back
     __device__ __forceinline__ void back(const u32x4 a, const u32x4 b, int c0, u32x4& x0, int c1, u32x4& x1) const {
+        static_assert(!HALF, "");
         *at4(r4, p4) = a;
         *at4(r4 + 16, p4) = b;
         fence();
@@ -336,7 +356,7 @@ __device__ __forceinline__ void put_f32(float* d, const u32x4 u, int c, int n) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) if (c + e < n) d[e] = __uint_as_float(u[e]);
 }
-__device__ __forceinline__ void store_bf16(unsigned short* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void store_bf16(unsigned short* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
     u32x4 a, b;
     w.turn(pack8(v[0]), w.lh, pack8(v[1]), 2 + w.lh, a, b);
     const int c = col0 + 8 * w.p4, r = row0 + w.r4;
@@ -345,7 +365,7 @@ __device__ __forceinline__ void store_bf16(unsigned short* base, long long ld, i
     if (r + 16 < rows) put_bf16(base + (long long)(r + 16) * ld + c, b, c, cols);
 }
 __device__ __forceinline__ u32x4 raw4(const float* v) { return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
-__device__ __forceinline__ void store_f32(float* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void store_f32(float* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         u32x4 a, b;
@@ -357,7 +377,7 @@ __device__ __forceinline__ void store_f32(float* base, long long ld, int row0, i
     }
 }
 // the block's 192 bytes of each row of a split matrix, 64 at a time (columns are whole groups of 16: `cols` is a multiple of 16)
-__device__ __forceinline__ void store_split(char* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void store_split(char* base, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
     u32x4 p[2][3], a, b;
     split8(v[0], p[0]);
     split8(v[1], p[1]);
@@ -373,7 +393,7 @@ __device__ __forceinline__ void store_split(char* base, long long ld, int row0, 
     }
 }
 // 24 bits of fp32 values: rounded to the upper three bytes (a value that would round to infinity, infinities and NaN are cut)
-__device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
     u32x4 h[2], a, b;
     u32x2 l[2];
 #pragma unroll
@@ -401,13 +421,13 @@ __device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, 
     if (c2 < cols && r2 < rows) *reinterpret_cast<u32x4*>(lo + (long long)r2 * ld + c2) = lv;
 }
 struct Raw24 { u32x4 a, b, l; };
-__device__ __forceinline__ void load_24(const unsigned short* hi, const unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, Raw24& x, const Where& w) {
+template <class W> __device__ __forceinline__ void load_24(const unsigned short* hi, const unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, Raw24& x, const W& w) {
     const int c = min(col0 + 8 * w.p4, cols - 8), c2 = min(col0 + 16 * w.p2, cols - 16);
     x.a = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4, rows - 1) * ld + c);
     x.b = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
     x.l = *reinterpret_cast<const u32x4*>(lo + (long long)min(row0 + w.r2, rows - 1) * ld + c2);
 }
-__device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], const W& w) {
     u32x4 h[2];
     u32x2 l[2];
     w.back(x.a, x.b, w.lh, h[0], 2 + w.lh, h[1]);
@@ -421,7 +441,7 @@ __device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], cons
         }
 }
 struct Raw32 { u32x4 a[2], b[2]; };
-__device__ __forceinline__ void load_f32(const float* base, long long ld, int row0, int col0, int rows, int cols, Raw32& x, const Where& w) {
+template <class W> __device__ __forceinline__ void load_f32(const float* base, long long ld, int row0, int col0, int rows, int cols, Raw32& x, const W& w) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int c = min(col0 + 16 * q + 4 * w.p4, cols - 4);
@@ -429,7 +449,7 @@ __device__ __forceinline__ void load_f32(const float* base, long long ld, int ro
         x.b[q] = *reinterpret_cast<const u32x4*>(base + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
     }
 }
-__device__ __forceinline__ void unpack_f32(const Raw32& x, float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void unpack_f32(const Raw32& x, float (&v)[2][8], const W& w) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         u32x4 p0, p1;
@@ -445,7 +465,7 @@ __device__ __forceinline__ float bias_lane(const void* bias, int bf16, int col, 
     const int c = min(col, cols - 1);
     return bf16 ? bf_load(bias, c) : reinterpret_cast<const float*>(bias)[c];
 }
-__device__ __forceinline__ void bias_of(float lanes, int c, float (&v)[2][8], const Where& w) {
+template <class W> __device__ __forceinline__ void bias_of(float lanes, int c, float (&v)[2][8], const W& w) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int k = c + 16 * (r >> 3) + (r & 7);
@@ -453,7 +473,7 @@ __device__ __forceinline__ void bias_of(float lanes, int c, float (&v)[2][8], co
         v[r >> 3][r & 7] = w.lh ? hi : lo;
     }
 }
-__device__ __forceinline__ void clear_beyond(float (&v)[2][8], int col0, int cols, const Where& w) {
+template <class W> __device__ __forceinline__ void clear_beyond(float (&v)[2][8], int col0, int cols, const W& w) {
     if (col0 + 32 <= cols) return;                            // uniform
 #pragma unroll
     for (int r = 0; r < 16; ++r)
@@ -462,23 +482,23 @@ __device__ __forceinline__ void clear_beyond(float (&v)[2][8], int col0, int col
 
 // WM x WN waves of (32 MI) x (32 NJ) outputs each.
 template <int FMT, int EP, int WM, int WN, int MI, int NJ>
-__global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows(const Args p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
     constexpr bool GATED = is_gated(EP), FAST = EP != EP_GATED_3 && EP != EP_GATED_BWD_3;
     constexpr bool SPLIT = FMT == FMT_SPLIT;
-    constexpr int ROWB = row_bytes(FMT), SLOTS = SPLIT || WM * WN == 8 ? 3 : 2;
-    constexpr bool EARLY = !SPLIT && SLOTS == 3;              // copies go into the slot of the stage before
+    constexpr int ROWB = row_bytes(FMT), SLOTS = 3;
     constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
     constexpr int STAGE = (TM + TN) * ROWB, RING = SLOTS * STAGE;
     constexpr int NA = TM * ROWB / 1024 / NW, NB = TN * ROWB / 1024 / NW;      // copies of a wave and stage
     constexpr int STEPS = FMT == FMT_BF16 ? 4 : 2;            // steps of a stage
     constexpr int SC_B = FMT == FMT_E4M3 ? SC_SLOTS * TM * 4 : 0;
     constexpr int MX_B = EP == EP_GATED_Q ? TM * WN * 4 : 0;  // row maxima of the waves (quantised results)
-    __shared__ __attribute__((aligned(1024))) char smem[RING + SC_B + MX_B + NW * TURN_B];
+    typedef Where<FMT == FMT_E4M3 || EP == EP_GATED_Q> Turn;
+    __shared__ __attribute__((aligned(1024))) char smem[RING + SC_B + MX_B + NW * Turn::LDS_B];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid / WN, wc = wid % WN;
     const int li = lane & 31, lh = lane >> 5;
-    const Where wh(smem + RING + SC_B + MX_B + wid * TURN_B);
+    const Turn wh(smem + RING + SC_B + MX_B + wid * Turn::LDS_B);
 
     const int T = p.tiles_m * p.tiles_n, all_stages = p.ks;
     const int total_items = T * p.splits;
@@ -491,9 +511,10 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
     constexpr int PR = ROWB / 16;                             // pieces of a row
     auto row_of = [&](int q) { return (q * 64 + lane) / PR; };
     auto piece = [&](int q) { return ((q * 64 + lane) % PR) ^ st_swap<FMT>(row_of(q)); };  // the logical piece that belongs at this lane's place of image part q
-    auto up_part = [&](int j) { return GATED && ((wid * NB + j) * 64 / PR) % CW >= CW / 2; };           // (32 rows are whole parts: uniform)
+    static_assert(!GATED || WM == 2, "");
+    const char* const wave_b = GATED && (wid & 1) ? p.B2 : p.B;         // (a wave copies CW / 2 rows, all gate or all up)
     unsigned aofs[NA], bofs[NB];
-    const char *abase, *bbase, *bbase2;
+    const char *abase, *bbase;
     unsigned sofs = 0;
     const unsigned char* scbase = nullptr;
     const bool has_tail = FMT == FMT_BF16 && (p.K & 63) != 0;
@@ -507,8 +528,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         tile_of(p, feed.next - zz * T, tm, tn);
         const int m0 = tm * TM, n0 = tn * (GATED ? TN / 2 : TN);
         abase = p.A + (long long)m0 * p.lda;
-        bbase = p.B + (long long)n0 * p.ldb;
-        if constexpr (GATED) bbase2 = p.B2 + (long long)n0 * p.ldb;
+        bbase = wave_b + (long long)n0 * p.ldb;
 #pragma unroll
         for (int j = 0; j < NA; ++j)
             aofs[j] = (unsigned)min(row_of(wid * NA + j), p.M - 1 - m0) * (unsigned)p.lda + (piece(wid * NA + j) << 4);
@@ -537,11 +557,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
             koff += ROWB;
         }
     };
-    auto issue = [&]() {
-        char* sb = smem + f_slot * STAGE;
-        const char* ab = abase + koff;
-        const char* bb = bbase + koff;
-        const char* bb2 = GATED ? bbase2 + koff : nullptr;
+    auto copy_scales = [&]() {
         if constexpr (FMT == FMT_E4M3) {
             if ((f_kin & 3) == 0) {                           // a group of four blocks begins: a scale word of every row (before the stage's own copies)
                 if (wid * 64 < TM)
@@ -551,22 +567,22 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                 f_scslot = (f_scslot + 1) & (SC_SLOTS - 1);
             }
         }
+    };
+    auto issue = [&]() {
+        char* sb = smem + f_slot * STAGE;
+        const char* ab = abase + koff;
+        const char* bb = bbase + koff;
+        copy_scales();
         if (has_tail && f_kin == p.ks - 1) {                  // uniform
 #pragma unroll
             for (int j = 0; j < NA; ++j) glds16(tail_ok[(wid * NA + j) & 1] ? ab + aofs[j] : reinterpret_cast<const char*>(zero_piece), sb + (wid * NA + j) * 1024);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const bool up = up_part(j);
-                glds16(tail_ok[(wid * NB + j) & 1] ? (up ? bb2 : bb) + bofs[j] : reinterpret_cast<const char*>(zero_piece), sb + TM * ROWB + (wid * NB + j) * 1024);
-            }
+            for (int j = 0; j < NB; ++j) glds16(tail_ok[(wid * NB + j) & 1] ? bb + bofs[j] : reinterpret_cast<const char*>(zero_piece), sb + TM * ROWB + (wid * NB + j) * 1024);
         } else {
 #pragma unroll
             for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const bool up = up_part(j);
-                glds16((up ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
-            }
+            for (int j = 0; j < NB; ++j) glds16(bb + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
         }
         f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
         --f_total;
@@ -628,24 +644,24 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         for (int j = 0; j < NJ; ++j) fb[decltype(to)::value][j] = frag(sb, ob[j], decltype(set)::value);
     };
     // the steps of a stage but the last: multiply one, read the next
-    // (EARLY: with the copies of the stage behind the next, a share to each step)
+    // (and, in the steady loop, copies of the stage behind the next, a share to each step)
     constexpr int PER = NA + NB;
-    auto copy = [&](auto step, const char* ab, const char* bb, const char* bb2, char* to) {
+    auto copy = [&](auto step, Buffer ab, Buffer bb, unsigned at, char* to) {
         constexpr int q = decltype(step)::value;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (j * STEPS / PER == q) {
-                if (j < NA) glds16(ab + aofs[j < NA ? j : 0], to + (wid * NA + j) * 1024);
-                else glds16((up_part(j - NA) ? bb2 : bb) + bofs[j < NA ? 0 : j - NA], to + TM * ROWB + (wid * NB + j - NA) * 1024);
+                if (j < NA) blds16(ab, aofs[j < NA ? j : 0], at, to + (wid * NA + j) * 1024);
+                else blds16(bb, bofs[j < NA ? 0 : j - NA], at, to + TM * ROWB + (wid * NB + j - NA) * 1024);
             }
     };
-    auto inner = [&](const char* sb, auto copies, const char* ab, const char* bb, const char* bb2, char* to) {
+    auto inner = [&](const char* sb, auto copies, Buffer ab, Buffer bb, unsigned at, char* to) {
         constexpr bool C = decltype(copies)::value;
         auto one = [&](auto s) {
             load_set(std::integral_constant<int, decltype(s)::value + 1>{}, sb, decltype(s)::value + 1);
-            if constexpr (C) copy(s, ab, bb, bb2, to);
+            if constexpr (C) copy(s, ab, bb, at, to);
             multiply(s);
-            spread<MI * NJ, READS, C ? share(PER, STEPS, decltype(s)::value) : 0>();
+            spread<MI * NJ, READS, C ? share(PER, STEPS, decltype(s)::value) : 0, 2>();
             __builtin_amdgcn_sched_barrier(0);
         };
         one(std::integral_constant<int, 0>{});
@@ -661,7 +677,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
 
     open_feed();
 #pragma unroll 1
-    for (int s = 0; s < (EARLY ? 2 : SLOTS); ++s)
+    for (int s = 0; s < (SPLIT ? 3 : 2); ++s)
         if (f_total > 0) issue();
     if constexpr (SPLIT) f_slot = 0;                          // (also when there were fewer stages than slots)
     int slot = 0, scslot = 0;
@@ -699,28 +715,24 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                     if constexpr (SPLIT) low[i][j][r] = 0.f;
                 }
         // biases of this wave's columns, a column to a lane: gated, CW / 2 of each, side by side where they fit one register
-        float bias_a = 0.f, bias_b = 0.f;
+        float bias_a = 0.f;
+        static_assert(CW == 64, "");
         if constexpr (EP == EP_LINEAR) {
-            static_assert(CW == 64, "");
             bias_a = bias_lane(p.splits > 1 ? nullptr : p.bias, p.bias_bf16, n0 + wc * CW + lane, p.N);
         } else if constexpr (GATED) {
             const int f = n0 + wc * (CW / 2) + lane % (CW / 2);
-            if constexpr (CW == 64) {
-                bias_a = bias_lane(p.bias, p.bias_bf16, f, p.N);
-                const float up = bias_lane(p.bias2, p.bias_bf16, f, p.N);
-                bias_a = lane < 32 ? bias_a : up;
-            } else {
-                bias_a = bias_lane(p.bias, p.bias_bf16, f, p.N);
-                bias_b = bias_lane(p.bias2, p.bias_bf16, f, p.N);
-            }
+            bias_a = bias_lane(p.bias, p.bias_bf16, f, p.N);
+            const float up = bias_lane(p.bias2, p.bias_bf16, f, p.N);
+            bias_a = lane < 32 ? bias_a : up;
         }
+        typedef __attribute__((address_space(4))) unsigned uniform_word;
         auto scales = [&](int t) {                            // a stage is one 128-block
             if constexpr (FMT == FMT_E4M3) {
                 if ((t & 3) == 0) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i) sa4[i] = reinterpret_cast<const unsigned*>(smem + RING)[scslot * TM + wr * RW + i * 32 + li];
-                    sb4[0] = bs0[t >> 2];
-                    if constexpr (GATED) sb4[1] = bs1[t >> 2];
+                    sb4[0] = ((const uniform_word*)bs0)[t >> 2];          // (a vector load would wait for every copy on its way)
+                    if constexpr (GATED) sb4[1] = ((const uniform_word*)bs1)[t >> 2];
                     scslot = (scslot + 1) & (SC_SLOTS - 1);
                 }
                 const int sh = (t & 3) << 3;
@@ -747,9 +759,8 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                 meet();
                 const char* nb = smem + slot * STAGE;
                 char* sb = smem + f_slot * STAGE;
-                const char* ab = abase + koff;
-                const char* bb = bbase + koff;
-                const char* bb2 = GATED ? bbase2 + koff : nullptr;
+                const Buffer ab = buffer_at(abase), bb = buffer_at(bbase);
+                const unsigned at = (unsigned)koff;
                 read_a(S2, nb);
                 product(S0, S2);
                 spread<MI * NJ, MI, 0>();
@@ -760,13 +771,13 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                 spread<MI * NJ, 2 * NJ, 0>();
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
+                for (int j = 0; j < NA; ++j) blds16(ab, aofs[j], at, sb + (wid * NA + j) * 1024);
                 product(S1, S0);
                 spread<MI * NJ, 0, NA>();
                 __builtin_amdgcn_sched_barrier(0);
                 read_a(S1, nb);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
+                for (int j = 0; j < NB; ++j) blds16(bb, bofs[j], at, sb + TM * ROWB + (wid * NB + j) * 1024);
                 product(S0, S1);
                 spread<MI * NJ, MI, NB>();
                 __builtin_amdgcn_sched_barrier(0);
@@ -792,58 +803,44 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
         if constexpr (!SPLIT) {
             // one stage; the next one's first operands are read behind its last step
             auto stage = [&](int t) {
-                if constexpr (EARLY)
-                    if (f_total > 0) issue();
+                if (f_total > 0) issue();                     // into the slot of the stage before
                 scales(t);
-                inner(smem + slot * STAGE, std::false_type{}, nullptr, nullptr, nullptr, nullptr);
+                inner(smem + slot * STAGE, std::false_type{}, buffer_at(nullptr), buffer_at(nullptr), 0, nullptr);
                 slot = slot + 1 == SLOTS ? 0 : slot + 1;
                 if (--w_total > 0) {
-                    if (EARLY && w_total - f_total >= 2) wait_vm<PER>();      // the next stage has landed; the one behind it may be on its way
+                    if (w_total - f_total >= 2) wait_vm<PER>();      // the next stage has landed; the one behind it may be on its way
                     else wait_vm<0>();                        // (and earlier results are stored)
                     meet();
                     load_set(S0, smem + slot * STAGE, 0);
-                    if constexpr (!EARLY)
-                        if (f_total > 0) issue();             // into the slot that everyone has just read
                 }
                 multiply(S1);
             };
             // the same without the cases: the next stage is this tile's, and the copies are whole pieces of the same rows
             auto steady = [&](int t, int run) {
-                const char* ab = abase + koff;
-                const char* bb = bbase + koff;
-                const char* bb2 = GATED ? bbase2 + koff : nullptr;
+                const Buffer ab = buffer_at(abase), bb = buffer_at(bbase);
+                unsigned at = (unsigned)koff;
                 for (int left = run; left > 0; --left, ++t) {
+                    copy_scales();
+                    ++f_kin;
                     scales(t);
-                    char* sb = smem + slot * STAGE;
-                    char* to = EARLY ? smem + f_slot * STAGE : sb;
-                    inner(sb, std::integral_constant<bool, EARLY>{}, ab, bb, bb2, to);
+                    char* to = smem + f_slot * STAGE;
+                    inner(smem + slot * STAGE, std::true_type{}, ab, bb, at, to);
                     slot = slot + 1 == SLOTS ? 0 : slot + 1;
-                    wait_vm<EARLY ? PER - share(PER, STEPS, STEPS - 1) : 0>();
+                    f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
+                    wait_vm<PER - share(PER, STEPS, STEPS - 1)>();
                     meet();
                     load_set(S0, smem + slot * STAGE, 0);
-                    if constexpr (EARLY) {
-                        copy(std::integral_constant<int, STEPS - 1>{}, ab, bb, bb2, to);
-                        f_slot = f_slot + 1 == SLOTS ? 0 : f_slot + 1;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < NA; ++j) glds16(ab + aofs[j], sb + (wid * NA + j) * 1024);
-#pragma unroll
-                        for (int j = 0; j < NB; ++j) glds16((up_part(j) ? bb2 : bb) + bofs[j], sb + TM * ROWB + (wid * NB + j) * 1024);
-                    }
-                    ab += ROWB; bb += ROWB;
-                    if constexpr (GATED) bb2 += ROWB;
+                    copy(std::integral_constant<int, STEPS - 1>{}, ab, bb, at, to);
+                    at += ROWB;
                     multiply(S1);
-                    spread<MI * NJ, READS, EARLY ? share(PER, STEPS, STEPS - 1) : PER>();
+                    spread<MI * NJ, READS, share(PER, STEPS, STEPS - 1), 2>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 koff += (long long)run * ROWB;
-                f_kin += run; f_left -= run; f_total -= run; w_total -= run;
-                if constexpr (!EARLY) f_slot = slot;          // (the slot read now is refilled next)
+                f_left -= run; f_total -= run; w_total -= run;
             };
             for (int t = 0; t < nk; ++t) {
-                // (a group of scale words begins with a copy of its own, a last stage may end inside the rows)
-                int run = min(nk - 1 - t, f_left - 1);
-                if (FMT == FMT_E4M3) run = min(run, (4 - (f_kin & 3)) & 3);
+                const int run = min(nk - 1 - t, f_left - 1);  // (a last stage may end inside the rows)
                 if (f_total > 0 && run > 0) {
                     steady(t, run);
                     t += run;
@@ -881,7 +878,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_rows
                     const int c = opaque(col0 + j * 32);
                     float bg[2][8], bu[2][8];
                     bias_of(bias_a, j * 32, bg, wh);
-                    bias_of(CW == 64 ? bias_a : bias_b, CW == 64 ? 32 : j * 32, bu, wh);
+                    bias_of(bias_a, 32, bu, wh);
 #pragma unroll
                     for (int i = 0; i < MI; ++i) {
                         float a[2][8], b[2][8], h[2][8];
@@ -1076,12 +1073,12 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
     constexpr int ARB = TM * EB, BRB = TN * EB;               // bytes of an image row
     constexpr int STAGE = SR * (ARB + BRB), RING = SLOTS * STAGE;
     constexpr int NA = SR * ARB / 1024 / NW, NB = SR * BRB / 1024 / NW, NGL = NA + NB;
-    __shared__ __attribute__((aligned(1024))) char smem[RING + NW * TURN_B];
+    __shared__ __attribute__((aligned(1024))) char smem[RING + NW * Where<false>::LDS_B];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid / WN, wc = wid % WN;
     const int lh = lane >> 5;
-    const Where wh(smem + RING + wid * TURN_B);
+    const Where<false> wh(smem + RING + wid * Where<false>::LDS_B);
     // Splits of the reduction first: all output tiles of one row range run together on one XCD and share its rows in L2.
     const int T = p.tiles_m * p.tiles_n, nz = (int)gridDim.z;
     int zz, tile;

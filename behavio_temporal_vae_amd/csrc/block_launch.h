@@ -18,14 +18,14 @@ int launch_cols(const ColArgs& p, int split, int big, int z, hipStream_t s);
 // quantised results: 128 x 256 and one, since a row's block of 128 columns of h has to lie in one workgroup.
 template <int FMT, int EP>
 int launch_rows(Args& p, int z, hipStream_t s, const char* what) {
-    constexpr int NJ = EP == EP_GATED_Q ? 4 : 2, WN = FMT == FMT_BF16 && EP != EP_GATED_Q ? 4 : 2;
-    p.tiles_m = tiles(p.M, 128); p.tiles_n = tiles(p.N, 32 * WN * NJ / (is_gated(EP) ? 2 : 1)); p.splits = z;
+    constexpr int WN = FMT == FMT_SPLIT ? 2 : 4;
+    p.tiles_m = tiles(p.M, 128); p.tiles_n = tiles(p.N, 64 * WN / (is_gated(EP) ? 2 : 1)); p.splits = z;
     const long long items = (long long)p.tiles_m * p.tiles_n * z;
     if (items >= (1 << 29)) return btvae::set_error("%s: too many tiles", what);
     if (p.lda >= (1 << 23) || p.ldb >= (1 << 23)) return btvae::set_error("%s: rows of more than 8 MiB", what);
     p.by_tiles = div_by(p.tiles_m * p.tiles_n); p.by_band = div_by(8 * p.tiles_n); p.by_last = div_by(p.tiles_m % 8 ? p.tiles_m % 8 : 8);
-    const dim3 grid((unsigned)std::min<long long>(items, WN * NJ == 4 ? 2 * CHIP : CHIP));
-    hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, WN, 2, NJ>), grid, dim3(128 * WN), 0, s, p);
+    const dim3 grid((unsigned)std::min<long long>(items, FMT == FMT_SPLIT ? 2 * CHIP : CHIP));
+    hipLaunchKernelGGL((gemm_rows<FMT, EP, 2, WN, 2, 2>), grid, dim3(128 * WN), 0, s, p);
     return btvae::check_launch(what);
 }
 #endif
