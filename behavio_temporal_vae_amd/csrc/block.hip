@@ -488,8 +488,7 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
         if (GATED) {
             if (p.bias2) u += p.bias_bf16 ? bf_load(p.bias2, nn) : reinterpret_cast<const float*>(p.bias2)[nn];
             float a, d;
-            if (p.act == ACT_GELU) act_value<false, true>(p.act, v, a, d);
-            else act_value<false, false>(p.act, v, a, d);
+            with_act(p.act, [&](auto act) { act_value<false, decltype(act)::value>(p.act, v, a, d); });
             v = a * u;
         }
         const long long o = (long long)m * p.ldc + nn;

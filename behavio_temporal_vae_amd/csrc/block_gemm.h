@@ -85,7 +85,7 @@ struct Args {
     float* slab;                                    // splits > 1: fp32 partial results [z][M][N]
     int act;
     // Gated: where a, b are kept for the backward pass (null: not); backward: read; b starts gu_half columns after a.  fp32, or (bf16
-    // operands) 24 bits: the upper two bytes here, the third in gu_lo -- 2^-17 instead of bf16's 2^-9, since these values are rounded again as part of
+    // operands) 24 bits: the upper two bytes here, the third in gu_lo -- 2^-15 instead of bf16's 2^-8, since these values are rounded again as part of
     // the gradients
     void* gu; unsigned char* gu_lo; long long ldgu; int gu_half;
     float* colpart;                                 // backward: column sums of (da, db) per wave's strip of rows [strips][2][N], or null
@@ -147,10 +147,10 @@ typedef f32x4 f32x4_any __attribute__((aligned(4)));
 // act(a) and act'(a).  FAST (results that are rounded to bf16 or e4m3): the hardware's exp and reciprocal, each good to
 // about 2^-22, and erfc from Abramowitz and Stegun's 7.1.26 (1.5e-7); otherwise the precise exp and division and erfc from the Chebyshev
 // fit t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), of Numerical Recipes (6.2; 1.2e-7 of the value everywhere).
-// GELU is a constant (its code is a path of its own), the others are told apart by `act`.
-template <bool FAST, bool GELU>
+// Code of its own for SiLU and GELU (ACT), the others are told apart by `act`: a choice made for every value would cost as much as the value.
+template <bool FAST, int ACT>
 __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) {
-    if constexpr (GELU) {
+    if constexpr (ACT == ACT_GELU) {
         const float x = __builtin_fabsf(a) * 0.70710678118654752f;
         float g, half_erfc;                                   // exp(-a^2 / 2), erfc(|a| / sqrt 2) / 2
         if constexpr (FAST) {
@@ -168,11 +168,27 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
         v = a * phi;
         d = phi + a * g * 0.39894228040143268f;
     } else {
-        const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-a)) : 1.f / (1.f + expf(-a));
-        const float r = a > 0.f ? a : (a == a ? 0.f : a);
-        v = act == ACT_RELU ? r : (act == ACT_SILU ? a * s : s);
-        d = act == ACT_RELU ? (a > 0.f ? 1.f : 0.f) : (act == ACT_SILU ? s * (1.f + a * (1.f - s)) : s * (1.f - s));
+        float s;
+        if constexpr (FAST) {
+            s = __builtin_amdgcn_rcpf(1.f + __expf(-a));
+        } else {                                              // one Newton step from the approximate reciprocal, of a finite number
+            const float x = fminf(1.f + expf(-a), 3e38f), y = __builtin_amdgcn_rcpf(x);
+            s = a == a ? __builtin_fmaf(__builtin_fmaf(-x, y, 1.f), y, y) : a;
+        }
+        if constexpr (ACT == ACT_SILU) {
+            v = a * s;
+            d = s * (1.f + a * (1.f - s));
+        } else {
+            v = act == ACT_RELU ? (a > 0.f ? a : (a == a ? 0.f : a)) : s;
+            d = act == ACT_RELU ? (a > 0.f ? 1.f : 0.f) : s * (1.f - s);
+        }
     }
+}
+// f(the activation as a constant: SiLU, GELU or -1)
+template <class F> __device__ __forceinline__ void with_act(int act, F f) {
+    if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+    else if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
+    else f(std::integral_constant<int, -1>{});
 }
 
 // Exponent of a block's scale: the smallest e >= -126 with amax <= 448 * 2^e; 0 for a block of zeros.
@@ -392,7 +408,8 @@ template <class W> __device__ __forceinline__ void store_split(char* base, long 
         if (r + 16 < rows) *reinterpret_cast<u32x4*>(d + 16 * ld) = b;
     }
 }
-// 24 bits of fp32 values: rounded to the upper three bytes (a value that would round to infinity, infinities and NaN are cut)
+// 24 bits of fp32 values: the upper three bytes, cut (off by 2^-15 of a value at most, where the gradients made from
+// them are rounded to bf16, 2^-8; rounding took four more instructions a value)
 template <class W> __device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
     u32x4 h[2], a, b;
     u32x2 l[2];
@@ -400,10 +417,7 @@ template <class W> __device__ __forceinline__ void store_24(unsigned short* hi, 
     for (int q = 0; q < 2; ++q) {
         unsigned u[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const unsigned x = __float_as_uint(v[q][e]), up = x + 0x80u;
-            u[e] = (up & 0x7F800000u) == 0x7F800000u ? x : up;
-        }
+        for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[q][e]);
 #pragma unroll
         for (int d = 0; d < 4; ++d) h[q][d] = __builtin_amdgcn_perm(u[2 * d + 1], u[2 * d], 0x07060302u);
 #pragma unroll
@@ -436,8 +450,9 @@ template <class W> __device__ __forceinline__ void unpack_24(const Raw24& x, flo
     for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const unsigned top = e & 1 ? h[q][e >> 1] & 0xFFFF0000u : h[q][e >> 1] << 16;
-            v[q][e] = __uint_as_float(top | ((l[q][e >> 2] >> (8 * (e & 3))) & 255u) << 8);
+            // bytes 3, 2: the half word, byte 1: the low byte, byte 0: zero
+            const unsigned sel = (e & 1 ? 0x07060000u : 0x05040000u) | (unsigned)(e & 3) << 8 | 0x0Cu;
+            v[q][e] = __uint_as_float(__builtin_amdgcn_perm(h[q][e >> 1], l[q][e >> 2], sel));
         }
 }
 struct Raw32 { u32x4 a[2], b[2]; };
@@ -465,13 +480,20 @@ __device__ __forceinline__ float bias_lane(const void* bias, int bf16, int col, 
     const int c = min(col, cols - 1);
     return bf16 ? bf_load(bias, c) : reinterpret_cast<const float*>(bias)[c];
 }
-template <class W> __device__ __forceinline__ void bias_of(float lanes, int c, float (&v)[2][8], const W& w) {
+// (through the wave's LDS: a lane's sixteen values in four reads)
+template <class W> __device__ __forceinline__ void put_biases(float lanes, const W& w) {
+    reinterpret_cast<float*>(w.lds)[threadIdx.x & 63] = lanes;
+    W::fence();
+}
+template <class W> __device__ __forceinline__ void bias_of(int c, float (&v)[2][8], const W& w) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int k = c + 16 * (r >> 3) + (r & 7);
-        const float lo = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lanes), k)), hi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lanes), k + 8));
-        v[r >> 3][r & 7] = w.lh ? hi : lo;
-    }
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(w.lds + (c + 16 * q + 8 * w.lh + 4 * k) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][4 * k + e] = x[e];
+        }
 }
 template <class W> __device__ __forceinline__ void clear_beyond(float (&v)[2][8], int col0, int cols, const W& w) {
     if (col0 + 32 <= cols) return;                            // uniform
@@ -853,15 +875,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
         if constexpr (EP == EP_LINEAR) {
             const int col0 = n0 + wc * CW;
             const bool to_slab = p.splits > 1;
+            float b[NJ][2][8];
+            put_biases(bias_a, wh);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) bias_of(j * 32, b[j], wh);
+            Turn::fence();
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                float b[2][8];
-                bias_of(bias_a, j * 32, b, wh);
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
                     float v[2][8];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = acc[i][j][r] + b[r >> 3][r & 7];
+                    for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = acc[i][j][r] + b[j][r >> 3][r & 7];
                     const int r0 = opaque(row0 + i * 32), c0 = opaque(col0 + j * 32);
                     if (to_slab) store_f32(p.slab + (long long)zz * p.M * p.N, p.N, r0, c0, p.M, p.N, v, wh);
                     else if (p.c_type == T_F32) store_f32(reinterpret_cast<float*>(p.C), p.ldc, r0, c0, p.M, p.N, v, wh);
@@ -871,14 +896,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
             }
         } else if constexpr (GATED) {
             constexpr int HJ = NJ / 2;
+            static_assert(HJ == 1, "");
+            float bg[2][8], bu[2][8];
+            put_biases(bias_a, wh);
+            bias_of(0, bg, wh);
+            bias_of(32, bu, wh);
+            Turn::fence();
             const int col0 = n0 + wc * (CW / 2), N16 = (p.N + 15) & ~15;
-            auto gate = [&](auto gelu) {
+            auto gate = [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < HJ; ++j) {
                     const int c = opaque(col0 + j * 32);
-                    float bg[2][8], bu[2][8];
-                    bias_of(bias_a, j * 32, bg, wh);
-                    bias_of(bias_a, 32, bu, wh);
 #pragma unroll
                     for (int i = 0; i < MI; ++i) {
                         float a[2][8], b[2][8], h[2][8];
@@ -888,7 +916,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             a[q][e] = acc[i][j][r] + bg[q][e];
                             b[q][e] = acc[i][j + HJ][r] + bu[q][e];
                             float v, d;
-                            act_value<FAST, decltype(gelu)::value>(p.act, a[q][e], v, d);
+                            act_value<FAST, decltype(act)::value>(p.act, a[q][e], v, d);
                             h[q][e] = v * b[q][e];
                             if (!FAST && (r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
                         }
@@ -915,8 +943,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                     }
                 }
             };
-            if (p.act == ACT_GELU) gate(std::true_type{});
-            else gate(std::false_type{});
+            with_act(p.act, gate);
             if constexpr (EP == EP_GATED_Q) {                 // the tile's 128 columns of h are one block of every row
                 static_assert(WN * CW == 256, "");
                 float* mx = reinterpret_cast<float*>(smem + RING + SC_B);
@@ -957,7 +984,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
             }
         } else {
             const int col0 = n0 + wc * CW, strip = tile_m * WM + wr;
-            auto gate = [&](auto gelu) {
+            auto gate = [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const int c = opaque(col0 + j * 32);
@@ -968,16 +995,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                     auto one = [&](int i, float (&a)[2][8], float (&b)[2][8]) {
                         float da[2][8], db[2][8];
                         const int r0 = opaque(row0 + i * 32);
-                        const bool row_in = r0 + li < p.M;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int q = r >> 3, e = r & 7;
                             float v, d;
-                            act_value<FAST, decltype(gelu)::value>(p.act, a[q][e], v, d);
+                            act_value<FAST, decltype(act)::value>(p.act, a[q][e], v, d);
                             const float dh = acc[i][j][r];
-                            da[q][e] = row_in ? dh * b[q][e] * d : 0.f;
-                            db[q][e] = row_in ? dh * v : 0.f;
+                            da[q][e] = dh * b[q][e] * d;
+                            db[q][e] = dh * v;
                             if (!FAST && (r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
+                        if (r0 + 32 > p.M && r0 + li >= p.M) {      // (rows behind the last take no part in the sums)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) da[r >> 3][r & 7] = db[r >> 3][r & 7] = 0.f;
                         }
                         clear_beyond(da, c, p.N, wh);         // zeros from N to gu_half: both halves are one operand of the next product
                         clear_beyond(db, c, p.N, wh);
@@ -1043,8 +1073,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                     }
                 }
             };
-            if (p.act == ACT_GELU) gate(std::true_type{});
-            else gate(std::false_type{});
+            with_act(p.act, gate);
         }
     }
     if constexpr (SPLIT) wait_vm<0>();                        // no copy may still be on its way when the LDS passes to others
