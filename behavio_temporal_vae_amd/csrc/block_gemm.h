@@ -155,7 +155,7 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
         float g, half_erfc;                                   // exp(-a^2 / 2), erfc(|a| / sqrt 2) / 2
         if constexpr (FAST) {
             const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-            g = __expf(-0.5f * a * a);
+            g = __builtin_amdgcn_exp2f(-0.72134752f * a * a);
             half_erfc = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * g;
         } else {
             const float t = 1.f / (1.f + 0.5f * x);
@@ -170,7 +170,7 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
     } else {
         float s;
         if constexpr (FAST) {
-            s = __builtin_amdgcn_rcpf(1.f + __expf(-a));
+            s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * a));
         } else {                                              // one Newton step from the approximate reciprocal, of a finite number
             const float x = fminf(1.f + expf(-a), 3e38f), y = __builtin_amdgcn_rcpf(x);
             s = a == a ? __builtin_fmaf(__builtin_fmaf(-x, y, 1.f), y, y) : a;
