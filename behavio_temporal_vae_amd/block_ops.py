@@ -217,21 +217,38 @@ class GatedTape:
         self.x, self.weights, self.biases, self.act, self.planes = x, weights, biases, act, planes
         self.X, self.H, self.GU, self.GU_lo, self.half = X, H, GU, GU_lo, half
 
+    def _check_outs(self, outs):
+        if len(outs) != 6:
+            raise ValueError(f"outs must be six tensors, got {len(outs)}")
+        names = ("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
+        for o, t, what in zip(outs, self.weights + self.biases, names):
+            if t is None or o is None:
+                if o is not None or what[0] == "w":
+                    raise ValueError(f"outs: {what} " + ("is absent" if t is None else "is missing"))
+                continue
+            _matrix(_tensor(o, f"outs: {what}"), f"outs: {what}", t.shape, o.dtype, self.x.device)
+            if not o.is_contiguous():
+                raise ValueError(f"outs: {what} must be contiguous")
+        for a, b in ((0, 1), (3, 4)):
+            if outs[a] is not None and outs[b] is not None and outs[a].dtype != outs[b].dtype:
+                raise TypeError(f"outs: {names[a]} and {names[b]} must be of one type")
+
     def backward(self, dy, need_input=True, need_weights=True, outs=None, accumulate=False):
         """Gradients (x, w_gate, w_up, w_down, b_gate, b_up, b_down) for the gradient ``dy`` of the result; entries that are
-        not wanted, or belong to an absent bias, are None.  ``outs``: six tensors (float32 or bfloat16, contiguous) that the
-        weights' and biases' gradients are written to, or added to with ``accumulate``."""
+        not wanted, or belong to an absent bias, are None.  ``outs``: six tensors (float32 or bfloat16, contiguous, None for
+        biases that are absent or not wanted) that the weights' and biases' gradients are written to, or added to with ``accumulate``."""
         x, (w_gate, w_up, w_down), planes = self.x, self.weights, self.planes
         dev, (M, K), (F, _), N = x.device, x.shape, w_gate.shape, w_down.shape[0]
         nv.ensure_device(dev)
-        dy = _rows(_matrix(dy, "the gradient", dy.shape, dy.dtype, dev), "the gradient")
-        if tuple(dy.shape) != (M, N):
-            raise ValueError(f"the gradient must have {M} rows of {N}, got {list(dy.shape)}")
+        dy = _rows(_tensor(dy, "the gradient"), "the gradient")
+        _matrix(dy, "the gradient", (M, N), dy.dtype, dev)
         lib, half = nv.lib(), self.half
         if outs is None:
             outs = [torch.empty_like(w, memory_format=torch.contiguous_format) for w in self.weights] + \
                    [None if b is None else torch.empty_like(b, memory_format=torch.contiguous_format) for b in self.biases]
             accumulate = False
+        else:
+            self._check_outs(outs)
         dwg, dwu, dwd, dbg, dbu, dbd = outs
         acc = int(accumulate)
         packer = _Packer(planes, dev)

@@ -873,3 +873,56 @@ def test_training_steps_with_gated_layers_captured(dev, monkeypatch, prec):
 def test_gated_layers_argument_checks(dev):
     with pytest.raises(ValueError, match="gated_activation"):
         gated_model(dev, "fp32", 1, 1, act="tanh")
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF, F32), (BF, BF)])
+def test_ffn_tape_outs(dev, dtype, out):
+    """Gradients written to, and added to, given tensors: the first pass is the tape's own result (rounded once more where that was
+    float32), the second one twice that, exactly, in float32.  What does not fit is refused before anything is launched."""
+    M, K, F, N = 150, 40, 72, 24
+    t = ffn_case(dev, M, K, F, N, dtype, True, seed=31)
+    dy = rnd(dev, M, N, seed=33, dtype=dtype)
+    args = [t[k] for k in ("x", "wg", "wu", "wd", "bg", "bu", "bd")]
+    y, tape = B.gated_feed_forward_tape(*args)
+    own = tape.backward(dy)
+    outs = [torch.full(a.shape, float("nan"), dtype=out, device=dev) for a in args[1:]]
+    got = tape.backward(dy, outs=outs)
+    for g, o, w in zip(got[1:], outs, own[1:]):
+        assert g is o
+        assert torch.equal(o, w) if out == dtype else torch.equal(o.to(dtype), w)
+    once = [o.clone() for o in outs]
+    tape.backward(dy, outs=outs, accumulate=True)
+    for o, w in zip(outs, once):
+        if out == F32:
+            assert torch.equal(o, 2 * w)
+        else:                                      # the sum of a rounded value and an unrounded one, rounded: two roundings of 2^-8
+            within(o, 2 * d64(w), (2 * U + U) * 2 * d64(w).abs() + 2.0 ** -130, "accumulated")
+    dx = tape.backward(dy, need_weights=False)
+    assert dx[1:] == (None,) * 6 and torch.equal(dx[0], own[0])
+    bad = lambda i, o: [o if k == i else v for k, v in enumerate(outs)]
+    for wrong, error, words in ((outs[:5], ValueError, "six"), (bad(0, None), ValueError, "w_gate is missing"), (bad(2, outs[0]), ValueError, "w_down must have shape"),
+                                (bad(1, torch.empty(K, F, dtype=out, device=dev).t()), ValueError, "contiguous"), (bad(3, outs[3].half()), TypeError, "b_gate"),
+                                (bad(4, outs[4].to(BF if out == F32 else F32)), TypeError, "one type"), (bad(5, outs[5].cpu()), RuntimeError, "on cpu")):
+        with pytest.raises(error, match=words):
+            tape.backward(dy, outs=wrong)
+    for wrong, error in ((dy.half(), TypeError), (dy[:-1], ValueError), (dy[:, :-1], ValueError), (dy.cpu(), RuntimeError)):
+        with pytest.raises(error):
+            tape.backward(wrong)
+    assert tape.backward(dy, outs=bad(3, None))[4] is None
+
+
+def test_networks_gradients_accumulate(dev):
+    """Two backward passes through a network with gated layers add up in its parameters' gradients, exactly."""
+    m = gated_model(dev, "fp32", 1, 1).train()
+    m._check_arena()
+    net, x, w = m.decoder, rnd(dev, 40, 13, seed=81), rnd(dev, 40, 24, seed=82)
+    grads = []
+    for passes in (1, 2):
+        for p in net.parameters():
+            p.grad.zero_()
+        for _ in range(passes):
+            (net(x)["mu"] * w).sum().backward()
+        grads.append({k: p.grad.clone() for k, p in net.named_parameters() if "gated_layers" in k})
+    assert grads[0]
+    for k, g in grads[0].items():
+        assert torch.equal(grads[1][k], 2 * g), k
