@@ -571,7 +571,7 @@ BTVAE_API int btvae_block_pack(const long long* jobs, int n, void* stream) {
 }
 
 static bool kept_ok(const void* GU, const void* GU_lo, long long ldgu, int gu_half, int planes, int F) {
-    return bk::al16(GU) && (planes == 3 || (GU_lo && bk::al16(GU_lo))) && (ldgu & 15) == 0 && (gu_half & 31) == 0 && gu_half >= F && ldgu >= 2LL * gu_half;
+    return bk::al16(GU) && (planes == 3 || (GU_lo && bk::al16(GU_lo))) && (ldgu & 15) == 0 && (gu_half & 31) == 0 && gu_half >= F && ldgu >= 2LL * gu_half && ldgu < (1 << 24);
 }
 
 BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu, int bias_bf16,
@@ -581,7 +581,7 @@ BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg,
     BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_fwd: unknown activation %d", act);
     if (M == 0) return 0;
     BTVAE_REQUIRE(operand_ok(X, ldx, planes, K) && operand_ok(Wg, ldw, planes, K) && operand_ok(Wu, ldw, planes, K), "gated_proj_fwd: bad operand layout");
-    BTVAE_REQUIRE(operand_ok(H, ldh, planes, bk::tiles(F, 16) * 16), "gated_proj_fwd: bad layout of H");
+    BTVAE_REQUIRE(operand_ok(H, ldh, planes, bk::tiles(F, 16) * 16) && ldh < (1 << 24), "gated_proj_fwd: bad layout of H");
     BTVAE_REQUIRE(!GU || kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_fwd: bad layout of the kept projections");
     bk::Args p = {};
     p.A = (const char*)X; p.lda = ldx; p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw;
@@ -602,7 +602,7 @@ BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* W
     if (M == 0) return 0;
     BTVAE_REQUIRE(operand_ok(dY, lddy, planes, N) && operand_ok(WdT, ldw, planes, N), "gated_proj_bwd: bad operand layout");
     BTVAE_REQUIRE(kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_bwd: bad layout of the kept projections");
-    BTVAE_REQUIRE(operand_ok(dGU, ldd, planes, 2 * gu_half), "gated_proj_bwd: bad layout of the gradients");
+    BTVAE_REQUIRE(operand_ok(dGU, ldd, planes, 2 * gu_half) && ldd < (1 << 26), "gated_proj_bwd: bad layout of the gradients");
     bk::Args p = {};
     p.A = (const char*)dY; p.lda = lddy; p.B = (const char*)WdT; p.ldb = ldw;
     p.M = M; p.N = F; p.K = N; p.ks = p.kz = stages_of(N, planes);

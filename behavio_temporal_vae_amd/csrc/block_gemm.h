@@ -147,6 +147,19 @@ typedef f32x4 f32x4_any __attribute__((aligned(4)));
 // act(a) and act'(a).  FAST (results that are rounded to bf16 or e4m3): the hardware's exp and reciprocal, each good to
 // about 2^-22, and erfc from Abramowitz and Stegun's 7.1.26 (1.5e-7); otherwise the precise exp and division and erfc from the Chebyshev
 // fit t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), of Numerical Recipes (6.2; 1.2e-7 of the value everywhere).
+// e^x to about a unit in the last place, for x in [-87, 88] and clamped to it (the product with log2 e in two pieces)
+__device__ __forceinline__ float exp_clamped(float x) {
+    x = __builtin_amdgcn_fmed3f(x, -87.f, 88.f);
+    const float t = x * 1.44269504f, r = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269504f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, r * 0.69314718f, e);
+}
+// 1 / x for 1 <= x (an infinity as 3e38): the approximate reciprocal and one Newton step
+__device__ __forceinline__ float reciprocal(float x) {
+    x = fminf(x, 3e38f);
+    const float y = __builtin_amdgcn_rcpf(x);
+    return __builtin_fmaf(__builtin_fmaf(-x, y, 1.f), y, y);
+}
 // Code of its own for SiLU and GELU (ACT), the others are told apart by `act`: a choice made for every value would cost as much as the value.
 template <bool FAST, int ACT>
 __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) {
@@ -158,11 +171,11 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
             g = __builtin_amdgcn_exp2f(-0.72134752f * a * a);
             half_erfc = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * g;
         } else {
-            const float t = 1.f / (1.f + 0.5f * x);
+            const float t = reciprocal(1.f + 0.5f * x);
             const float P = -1.26551223f + t * (1.00002368f + t * (0.37409196f + t * (0.09678418f + t * (-0.18628806f + t * (0.27886807f +
                             t * (-1.13520398f + t * (1.48851587f + t * (-0.82215223f + t * 0.17087277f))))))));
-            g = expf(-0.5f * a * a);
-            half_erfc = 0.5f * t * g * expf(P);
+            g = exp_clamped(-0.5f * a * a);
+            half_erfc = 0.5f * t * g * exp_clamped(P);
         }
         const float phi = a < 0.f ? half_erfc : 1.f - half_erfc;
         v = a * phi;
@@ -171,9 +184,9 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
         float s;
         if constexpr (FAST) {
             s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * a));
-        } else {                                              // one Newton step from the approximate reciprocal, of a finite number
-            const float x = fminf(1.f + expf(-a), 3e38f), y = __builtin_amdgcn_rcpf(x);
-            s = a == a ? __builtin_fmaf(__builtin_fmaf(-x, y, 1.f), y, y) : a;
+        } else {
+            s = reciprocal(1.f + exp_clamped(-a));
+            if constexpr (ACT != ACT_SILU) s = a == a ? s : a;
         }
         if constexpr (ACT == ACT_SILU) {
             v = a * s;
@@ -408,9 +421,31 @@ template <class W> __device__ __forceinline__ void store_split(char* base, long 
         if (r + 16 < rows) *reinterpret_cast<u32x4*>(d + 16 * ld) = b;
     }
 }
+// A wave's rows of a matrix of whole 16-byte pieces, through a buffer descriptor that ends behind the last row: pieces outside are loaded as
+// zeros and not stored.  No lane is masked, so that no wait has to allow for stores that were skipped.
+constexpr unsigned OUTSIDE = 0xFFFFFFF0u;
+struct Panel {
+    Buffer buf;
+    unsigned ld;                                              // bytes
+    __device__ __forceinline__ Panel(const void* base, long long ld_bytes, int row0, int rows, int height) : ld((unsigned)ld_bytes) {
+        buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + row0 * ld_bytes, 0, (unsigned)max(0, min(rows - row0, height)) * (unsigned)ld_bytes, 0x00020000);
+    }
+    __device__ __forceinline__ unsigned at(int r, unsigned byte, bool in) const { return in ? (unsigned)r * ld + byte : OUTSIDE; }
+    __device__ __forceinline__ void put(const u32x4 v, unsigned o) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 0); }
+    __device__ __forceinline__ u32x4 get(unsigned o) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, o, 0, 0); }
+};
+// block of rows `row` .. + 31 of the panel, columns col0 .. + 31 of which those below `cols` (a multiple of 16) exist
+template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
+    u32x4 a, b;
+    w.turn(pack8(v[0]), w.lh, pack8(v[1]), 2 + w.lh, a, b);
+    const int c = col0 + 8 * w.p4;
+    const unsigned o = out.at(row + w.r4, 2 * c, c < cols);
+    out.put(a, o);
+    out.put(b, c < cols ? o + 16 * out.ld : OUTSIDE);
+}
 // 24 bits of fp32 values: the upper three bytes, cut (off by 2^-15 of a value at most, where the gradients made from
 // them are rounded to bf16, 2^-8; rounding took four more instructions a value)
-template <class W> __device__ __forceinline__ void store_24(unsigned short* hi, unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, const float (&v)[2][8], const W& w) {
+template <class W> __device__ __forceinline__ void store_24(const Panel& hi, const Panel& lo, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
     u32x4 h[2], a, b;
     u32x2 l[2];
 #pragma unroll
@@ -426,20 +461,19 @@ template <class W> __device__ __forceinline__ void store_24(unsigned short* hi, 
     }
     w.turn(h[0], w.lh, h[1], 2 + w.lh, a, b);
     const u32x4 lv = w.turn2(l[0], l[1]);
-    const int c = col0 + 8 * w.p4, r = row0 + w.r4;           // (cols is a multiple of 16: whole pieces)
-    if (c < cols) {
-        if (r < rows) *reinterpret_cast<u32x4*>(hi + (long long)r * ld + c) = a;
-        if (r + 16 < rows) *reinterpret_cast<u32x4*>(hi + (long long)(r + 16) * ld + c) = b;
-    }
-    const int c2 = col0 + 16 * w.p2, r2 = row0 + w.r2;
-    if (c2 < cols && r2 < rows) *reinterpret_cast<u32x4*>(lo + (long long)r2 * ld + c2) = lv;
+    const int c = col0 + 8 * w.p4, c2 = col0 + 16 * w.p2;
+    const unsigned o = hi.at(row + w.r4, 2 * c, c < cols);
+    hi.put(a, o);
+    hi.put(b, c < cols ? o + 16 * hi.ld : OUTSIDE);
+    lo.put(lv, lo.at(row + w.r2, c2, c2 < cols));
 }
 struct Raw24 { u32x4 a, b, l; };
-template <class W> __device__ __forceinline__ void load_24(const unsigned short* hi, const unsigned char* lo, long long ld, int row0, int col0, int rows, int cols, Raw24& x, const W& w) {
-    const int c = min(col0 + 8 * w.p4, cols - 8), c2 = min(col0 + 16 * w.p2, cols - 16);
-    x.a = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4, rows - 1) * ld + c);
-    x.b = *reinterpret_cast<const u32x4*>(hi + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
-    x.l = *reinterpret_cast<const u32x4*>(lo + (long long)min(row0 + w.r2, rows - 1) * ld + c2);
+template <class W> __device__ __forceinline__ void load_24(const Panel& hi, const Panel& lo, int row, int col0, int cols, Raw24& x, const W& w) {
+    const int c = col0 + 8 * w.p4, c2 = col0 + 16 * w.p2;
+    const unsigned o = hi.at(row + w.r4, 2 * c, c < cols);
+    x.a = hi.get(o);
+    x.b = hi.get(c < cols ? o + 16 * hi.ld : OUTSIDE);
+    x.l = lo.get(lo.at(row + w.r2, c2, c2 < cols));
 }
 template <class W> __device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], const W& w) {
     u32x4 h[2];
@@ -897,6 +931,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
         } else if constexpr (GATED) {
             constexpr int HJ = NJ / 2;
             static_assert(HJ == 1, "");
+            const Panel out(p.C, 2 * p.ldc, row0, p.M, RW);   // (EP_GATED)
+            const Panel hi_a(p.gu, 2 * p.ldgu, row0, p.M, RW), hi_b(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, 2 * p.ldgu, row0, p.M, RW);
+            const Panel lo_a(p.gu_lo, p.ldgu, row0, p.M, RW), lo_b(p.gu_lo + p.gu_half, p.ldgu, row0, p.M, RW);
             float bg[2][8], bu[2][8];
             put_biases(bias_a, wh);
             bias_of(0, bg, wh);
@@ -926,10 +963,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r) acc[i][j][r] = h[r >> 3][r & 7];
                         } else if constexpr (EP == EP_GATED) {
-                            store_bf16(reinterpret_cast<unsigned short*>(p.C), p.ldc, r0, c, p.M, N16, h, wh);
+                            panel_bf16(out, i * 32, c, N16, h, wh);
                             if (p.gu) {
-                                store_24(reinterpret_cast<unsigned short*>(p.gu), p.gu_lo, p.ldgu, r0, c, p.M, N16, a, wh);
-                                store_24(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, p.gu_lo + p.gu_half, p.ldgu, r0, c, p.M, N16, b, wh);
+                                store_24(hi_a, lo_a, i * 32, c, N16, a, wh);
+                                store_24(hi_b, lo_b, i * 32, c, N16, b, wh);
                             }
                         } else {
                             if (p.gu) {
@@ -984,6 +1021,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
             }
         } else {
             const int col0 = n0 + wc * CW, strip = tile_m * WM + wr;
+            // (FAST: 24 bits)
+            const Panel out_a(p.C, 2 * p.ldc, row0, p.M, RW), out_b(reinterpret_cast<unsigned short*>(p.C) + p.gu_half, 2 * p.ldc, row0, p.M, RW);
+            const Panel hi_a(p.gu, 2 * p.ldgu, row0, p.M, RW), hi_b(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, 2 * p.ldgu, row0, p.M, RW);
+            const Panel lo_a(p.gu_lo, p.ldgu, row0, p.M, RW), lo_b(p.gu_lo + p.gu_half, p.ldgu, row0, p.M, RW);
+            Raw24 ra[MI], rb[MI];
+            auto load = [&](int i, int c) {
+                load_24(hi_a, lo_a, i * 32, c, p.gu_half, ra[i], wh);
+                load_24(hi_b, lo_b, i * 32, c, p.gu_half, rb[i], wh);
+            };
             auto gate = [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
@@ -1017,9 +1063,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             cs[16 + r] += db[r >> 3][r & 7];
                         }
                         if constexpr (FAST) {
-                            unsigned short* C = reinterpret_cast<unsigned short*>(p.C);
-                            store_bf16(C, p.ldc, r0, c, p.M, p.gu_half, da, wh);
-                            store_bf16(C + p.gu_half, p.ldc, r0, c, p.M, p.gu_half, db, wh);
+                            panel_bf16(out_a, i * 32, c, p.gu_half, da, wh);
+                            panel_bf16(out_b, i * 32, c, p.gu_half, db, wh);
                         } else {
                             store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, p.gu_half, da, wh);
                             store_split(reinterpret_cast<char*>(p.C) + split_at(p.gu_half, 0), p.ldc, r0, c, p.M, p.gu_half, db, wh);
@@ -1027,13 +1072,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                         __builtin_amdgcn_sched_barrier(0);
                     };
                     if constexpr (FAST) {
-                        const unsigned short* hi = reinterpret_cast<const unsigned short*>(p.gu);
-                        Raw24 ra[MI], rb[MI];
 #pragma unroll
-                        for (int i = 0; i < MI; ++i) {
-                            load_24(hi, p.gu_lo, p.ldgu, opaque(row0 + i * 32), c, p.M, p.gu_half, ra[i], wh);
-                            load_24(hi + p.gu_half, p.gu_lo + p.gu_half, p.ldgu, opaque(row0 + i * 32), c, p.M, p.gu_half, rb[i], wh);
-                        }
+                        for (int i = 0; i < MI; ++i) load(i, c);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int i = 0; i < MI; ++i) {
