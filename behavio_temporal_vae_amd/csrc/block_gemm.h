@@ -432,7 +432,7 @@ struct Panel {
     }
     __device__ __forceinline__ unsigned at(int r, unsigned byte, bool in) const { return in ? (unsigned)r * ld + byte : OUTSIDE; }
     __device__ __forceinline__ void put(const u32x4 v, unsigned o) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 0); }
-    __device__ __forceinline__ u32x4 get(unsigned o) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, o, 0, 0); }
+    __device__ __forceinline__ u32x4 get(unsigned o) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, o, 0, 2); }      // (nt: read once)
 };
 // block of rows `row` .. + 31 of the panel, columns col0 .. + 31 of which those below `cols` (a multiple of 16) exist
 template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
