@@ -169,13 +169,13 @@ class _Packer:
         nv.call("btvae_block_pack", (ctypes.c_longlong * len(jobs))(*jobs), len(self.todo))
 
 
-REPACK_READS = 1024        # rows or columns of a product from which a bf16 matrix with rows off 64-byte boundaries is copied first
+REPACK_READS = 2048        # rows or columns of a product from which a bf16 matrix with rows off 64-byte boundaries is copied first
 
 
 def _in_place(t, planes, reads):
-    """May a product read ``t`` where it is?  Rows that do not start on 64 bytes cost the copies to LDS twice the requests (measured:
-    65,536 x 1000 times 1000 x 1024, 2000-byte rows 200 us, 2048-byte rows 154; the copy 55), so a matrix that is read against
-    ``reads`` others is laid out anew from ``REPACK_READS`` on."""
+    """May a product read ``t`` where it is?  Rows that do not start on 64 bytes cost the copies to LDS more requests, so a matrix that
+    is read against ``reads`` others is laid out anew from ``REPACK_READS`` on (measured, 65,536 x 1000 times 1000 x N, in place
+    against the copy and the product: N 512 80 and 118 us, 1024 155 and 178, 2048 346 and 316, 4096 653 and 596)."""
     return planes == 1 and _fits(t) and (reads < REPACK_READS or (2 * _pitch(t) % 64 == 0 and t.data_ptr() % 64 == 0))
 
 

@@ -507,17 +507,17 @@ inline int row_splits(int T, int stages, int unit) {
 }
 
 struct ProductPlan { int z, kz; };
-// EP_LINEAR: splits of the reduction, each a multiple of `unit` stages
-static ProductPlan plan_product(int M, int N, int stages, int unit) {
+// EP_LINEAR: splits of the reduction, each a multiple of `unit` stages; tiles of 128 x `tn`
+static ProductPlan plan_product(int M, int N, int tn, int stages, int unit) {
     ProductPlan r;
-    r.kz = tiles(tiles(stages, row_splits(tiles(M, 128) * tiles(N, 128), stages, unit)), unit) * unit;
+    r.kz = tiles(tiles(stages, row_splits(tiles(M, 128) * tiles(N, tn), stages, unit)), unit) * unit;
     r.z = tiles(stages, r.kz);
     return r;
 }
 struct ColPlan { int big, z, rz; };
 static ColPlan plan_cols(int M, int N, int R, int planes) {
     ColPlan r;
-    // 256 x 256 tiles from where their splits fill the chip (measured at 65,536 rows, 4032 x 1000: bf16 773 us against 978 with 128 x 128 tiles)
+    // 256 x 256 tiles from where their splits fill the chip: see gemm_cols
     r.big = tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
     const int t = r.big ? 256 : 128;
     const int T = tiles(M, t) * tiles(N, t);
@@ -616,7 +616,7 @@ BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* W
 BTVAE_API int btvae_gated_proj_strips(int M) { return 2 * bk::tiles(M, 128); }
 
 BTVAE_API long long btvae_block_product_ws(int M, int N, int K, int planes) {
-    const bk::ProductPlan r = bk::plan_product(M, N, stages_of(K, planes), 1);
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tile_width(planes == 3), stages_of(K, planes), 1);
     return r.z > 1 ? (long long)r.z * M * N : 0;
 }
 BTVAE_API int btvae_block_product(const void* A, long long lda, const void* B, long long ldb, const void* bias, int bias_bf16, void* C, long long ldc, int c_bf16,
@@ -629,7 +629,7 @@ BTVAE_API int btvae_block_product(const void* A, long long lda, const void* B, l
     bk::Args p = {};
     p.A = (const char*)A; p.lda = lda; p.B = (const char*)B; p.ldb = ldb;
     p.M = M; p.N = N; p.K = K; p.ks = stages_of(K, planes);
-    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 1);
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tile_width(planes == 3), p.ks, 1);
     BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "block_product: workspace too small");
     p.kz = r.kz; p.slab = ws;
     p.bias = bias; p.bias_bf16 = bias_bf16;
@@ -775,7 +775,7 @@ static bool fp8_ok(const void* q, long long ldq, const void* sc, long long scp, 
     return bk::al16(q) && (ldq & 15) == 0 && ldq >= (long long)kb * 128 && ((uintptr_t)sc & 3) == 0 && (scp & 3) == 0 && scp >= kb;
 }
 BTVAE_API long long btvae_fp8_product_ws(int M, int N, int K) {
-    const bk::ProductPlan r = bk::plan_product(M, N, bk::tiles(K, 128), 4);
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tile_width(false), bk::tiles(K, 128), 4);
     return r.z > 1 ? (long long)r.z * M * N : 0;
 }
 BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, long long xsp, const void* W, long long ldw, const void* wsc, long long wscp, const float* bias,
@@ -788,7 +788,7 @@ BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, lo
     p.A = (const char*)X; p.lda = ldx; p.B = (const char*)W; p.ldb = ldw;
     p.M = M; p.N = N; p.K = K; p.ks = bk::tiles(K, 128);
     p.a_sc = (const unsigned char*)xs; p.a_scp = xsp; p.b_sc = (const unsigned*)wsc; p.b_scp = (int)(wscp / 4);
-    const bk::ProductPlan r = bk::plan_product(M, N, p.ks, 4);
+    const bk::ProductPlan r = bk::plan_product(M, N, bk::tile_width(false), p.ks, 4);
     BTVAE_REQUIRE(r.z == 1 || (ws && ws_floats >= (long long)r.z * M * N), "fp8_product: workspace too small");
     p.kz = r.kz; p.slab = ws; p.bias = bias;
     p.C = C; p.ldc = ldc; p.c_type = c_bf16 ? bk::T_BF16 : bk::T_F32;

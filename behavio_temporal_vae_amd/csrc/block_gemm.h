@@ -5,28 +5,32 @@
 //   gemm_cols:  C[m][n] = sum_r A[r][m] B[r][n]      both operands with the reduction across rows (weight gradients)
 //
 // fp32 operands.  A value x is the sum of three bf16 values x0 + x1 + x2 (round to nearest of x, of the rest, of the rest
-// of that: |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, nothing is lost).  Of the nine products of two such sums the six largest
-// are taken, smallest first, into the same fp32 accumulators; the dropped x1 y2, x2 y1 and x2 y2 are below 2^-26 of x y,
-// four times below an fp32 rounding.  A matrix of such values ("split") keeps, for every 16 columns, 16 x0, 16 x1 and 16 x2: 96
-// bytes in a row.  A stage of 16 reduction steps brings all three pieces of both operands, so that each piece read from LDS is
-// multiplied twice on average: this form waits for the matrix pipe alone.
+// of that: |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|, nothing is lost).  Of the nine products of two such sums the six largest
+// are taken; the dropped x1 y2, x2 y1 and x2 y2 are together below 2^-23 of x y and of random sign, about an fp32 rounding.  gemm_rows sums the
+// products of first pieces apart from the five small ones, so that a result is rounded once in 16 columns.  A matrix of such
+// values ("split") keeps, for every 16 columns, 16 x0, 16 x1 and 16 x2: 96 bytes in a row.  A stage of 16 reduction steps brings
+// all three pieces of both operands, so that each piece read from LDS is multiplied twice on average.
 //
-// Layout of the loop (both kernels).  Four waves compute a 256 x 256 tile (128 x 128 each), or 128 x 128 / 128 x 256 where
-// there are too few tiles to fill the chip; the reduction goes in stages of 128 bytes per row (64 bf16, 128 e4m3: whole lines,
-// which is what L2 serves at its full rate), copied global -> LDS without passing through registers, two stages deep.  A wave reads the operands of its next
-// step into a second set of registers while it multiplies the present one; once all waves have read a stage (one barrier a
-// stage) its slot is refilled with the stage after next.  A wave's 128 x 128
-// reads LDS half as often for a multiplication as its 64 x 128 would, which is what bounds the loop; it takes 256
-// accumulators and one wave to a SIMD.  gemm_rows goes through several tiles: the ring keeps filling with
-// the next tile's stages while the results of the last one are computed and stored from registers.  Pieces of 16 bytes past the
-// end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns; rows past
-// the end repeat the last row (gemm_rows, where they only reach outputs that are not stored) or are zeros (gemm_cols, where
-// rows are the reduction).
+// gemm_rows.  128 x 256 tiles, eight waves of 64 x 64 and one workgroup to a compute unit (split operands: 128 x 128, four waves, two
+// workgroups); the reduction goes in stages of 128 bytes per row (64 bf16, 128 e4m3: whole lines, which is what L2 serves at its full
+// rate; split: 96), copied global -> LDS without passing through registers, three stages deep.  A wave reads the operands of its
+// next step into a second set of registers while it multiplies the present one; one barrier a stage.  A workgroup goes
+// through several tiles: the next tile's stages are on their way while the results of the last one are stored.  Pieces of 16
+// bytes past the end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns;
+// rows past the end repeat the last row and only reach outputs that are not stored.
+//   Measured (one card, 1.75 to 2.0 GHz under these loads, which is its power limit; a large library product in bf16 reaches 1394 TFLOP/s):
+//   bf16 65,536 x 4000 x 1000 490 us, 1070 TFLOP/s (128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of eight
+//   waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
+//   713 us, the 1.05 GB that it stores being 210 us of it; its backward 645 us, 1.3 GB loaded and stored; split 16,384 x
+//   4000 x 1000 680 us, 193 TFLOP/s of fp32 or 1156 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
+//   397 us, 1320 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 us, 1417 TFLOP/s.
+//   What they wait for: operands on their way through L2 and LDS at a clock that falls with what is moved; skewing the
+//   workgroups against each other, giving them priorities, or letting a tile's stores pass its successor's first stage changed nothing.
 //
 // Results.  The weights are the MFMA's first operand, so a lane's 16 results of a 32 x 32 block are 16 columns of ONE row, and the
 // weight rows are laid into LDS with bits 2 and 3 of their index swapped, which makes them two runs of 8 consecutive
-// columns.  Bias, activation, product and rounding happen there; 2 KiB of LDS to a wave then turn each 64 bytes of 32 rows
-// over to four neighbouring lanes a row: stores of 16 bytes a lane whose neighbours do not continue them cost several
+// columns.  Bias, activation, product and rounding happen there; 2 KiB of LDS to a wave (or 1 KiB twice) then turn each 64 bytes of
+// 32 rows over to four neighbouring lanes a row: stores of 16 bytes a lane whose neighbours do not continue them cost several
 // times as much (measured: 150 cycles a store instruction instead of about 30).
 #pragma once
 #include "common.h"
@@ -536,7 +540,7 @@ template <class W> __device__ __forceinline__ void clear_beyond(float (&v)[2][8]
         if (col0 + 16 * (r >> 3) + 8 * w.lh + (r & 7) >= cols) v[r >> 3][r & 7] = 0.f;
 }
 
-// WM x WN waves of (32 MI) x (32 NJ) outputs each.
+// WM x WN waves of (32 MI) x (32 NJ) outputs each
 template <int FMT, int EP, int WM, int WN, int MI, int NJ>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
     constexpr bool GATED = is_gated(EP), FAST = EP != EP_GATED_3 && EP != EP_GATED_BWD_3;
@@ -1125,6 +1129,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 // reads 4 rows x 16 columns and lane i gets column i) deliver them.  A row of the image is whole multiples of 256 bytes, so
 // rows collide on the banks; the 32-byte granules of a row are therefore stored at granule ^ 2 (row & 3), which gives the four
 // rows x two granules (neighbours, or three apart in a split row) that 32 lanes read together eight different places.
+// Stages come through registers, two ahead (split: one), and are written to one of three LDS slots: the compiler waits for every copy
+// global -> LDS on its way before a transposing read, so that such copies would not overlap anything (768 us instead of 545 below).
+// Four waves, 256 x 256 tiles of one workgroup a compute unit where the splits of the rows fill the chip with them, else 128 x 128 and two.
+//   Measured, 256 / 128 tiles: bf16 65,536 rows, 4032 x 1000: 546 / 707 us (968 TFLOP/s; a library product of the shape 687), 16,384 rows
+//   1000 x 2000 86 / 94 us, 4096 rows 44 / 37 us, 65,536 rows 512 x 256 63 / 45 us; split 16,384 rows, 4032 x 1000: 608 / 717 us (217
+//   TFLOP/s of fp32, 1300 of the products done), 2048 rows 1024 x 1024 50 / 38 us.  What bounds it: the matrix pipe at the power limit's clock.
 struct ColArgs {
     const char* A; long long lda; int a_cols;                 // byte pitch; columns that may be read (a multiple of 8; split: of 16)
     const char* B; long long ldb; int b_cols;

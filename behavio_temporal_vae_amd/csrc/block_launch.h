@@ -8,17 +8,17 @@ namespace btvae_block {
 constexpr int CHIP = 256;                                             // compute units
 
 inline int tiles(int n, int t) { return (n + t - 1) / t; }
+constexpr int tile_width(bool split) { return split ? 128 : 256; }    // columns of gemm_rows' tiles (of 128 rows): see there
 inline bool al16(const void* q) { return ((uintptr_t)q & 15) == 0; }
 
 template <int FMT, int EP> int launch_rows(Args& p, int z, hipStream_t s, const char* what);
 int launch_cols(const ColArgs& p, int split, int big, int z, hipStream_t s);
 
 #ifdef BTVAE_BLOCK_KERNELS
-// As many workgroups as the chip holds at a time, each going through its items.  128 x 128 tiles, two workgroups to a compute unit;
-// quantised results: 128 x 256 and one, since a row's block of 128 columns of h has to lie in one workgroup.
+// As many workgroups as the chip holds at a time (one of eight waves to a compute unit, or two of four), each going through its items.
 template <int FMT, int EP>
 int launch_rows(Args& p, int z, hipStream_t s, const char* what) {
-    constexpr int WN = FMT == FMT_SPLIT ? 2 : 4;
+    constexpr int WN = tile_width(FMT == FMT_SPLIT) / 64;
     p.tiles_m = tiles(p.M, 128); p.tiles_n = tiles(p.N, 64 * WN / (is_gated(EP) ? 2 : 1)); p.splits = z;
     const long long items = (long long)p.tiles_m * p.tiles_n * z;
     if (items >= (1 << 29)) return btvae::set_error("%s: too many tiles", what);
