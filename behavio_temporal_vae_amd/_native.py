@@ -104,6 +104,7 @@ _SIGS = {
     "btvae_gated_proj_bwd": [P, LL, P, LL, P, P, LL, I, P, LL, P, I, I, I, I, I, P],
     "btvae_block_product": [P, LL, P, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],
     "btvae_block_wgrad": [P, LL, P, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
+    "btvae_block_wgrad_pair": [P, P, LL, I, I, I, P],
     "btvae_block_colsum": [P, I, LL, P, LL, P, I, I, I, I, P],
     "btvae_block_strip_sums": [P, I, I, P, P, I, I, P],
     "btvae_few_rows": [P, I, LL, P, P, I, LL, P, P, P, I, LL, I, I, I, I, P],
@@ -139,6 +140,7 @@ _RET = {
     "btvae_gated_proj_strips": (c_int, [I]),
     "btvae_block_product_ws": (c_longlong, [I, I, I, I]),
     "btvae_block_wgrad_ws": (c_longlong, [I, I, I, I]),
+    "btvae_block_wgrad_pair_ws": (c_longlong, [c_int] * 6),
     "btvae_block_colsum_ws": (c_longlong, [I, I]),
     "btvae_few_rows_max": (c_int, []),
     "btvae_fp8_product_ws": (c_longlong, [I, I, I]),

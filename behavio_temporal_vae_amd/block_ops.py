@@ -175,7 +175,8 @@ REPACK_READS = 2048        # rows or columns of a product from which a bf16 matr
 def _in_place(t, planes, reads):
     """May a product read ``t`` where it is?  Rows that do not start on 64 bytes cost the copies to LDS more requests, so a matrix that
     is read against ``reads`` others is laid out anew from ``REPACK_READS`` on (measured, 65,536 x 1000 times 1000 x N, in place
-    against the copy and the product: N 512 80 and 118 us, 1024 155 and 178, 2048 346 and 316, 4096 653 and 596)."""
+    against the copy and the product: N 512 80 and 118 us, 1024 155 and 178, 2048 346 and 316, 4096 653 and 596; never copying
+    costs a gated unit's training pass of 65,536 x 1000 x 2000 3 %)."""
     return planes == 1 and _fits(t) and (reads < REPACK_READS or (2 * _pitch(t) % 64 == 0 and t.data_ptr() % 64 == 0))
 
 
@@ -252,7 +253,7 @@ class GatedTape:
         dwg, dwu, dwd, dbg, dbu, dbd = outs
         acc = int(accumulate)
         packer = _Packer(planes, dev)
-        DY, WdT = _operand(dy, planes, F, packer), packer.add_transposed(w_down, width=_up(N, 32))
+        DY, WdT = _operand(dy, planes, 2 * F, packer), packer.add_transposed(w_down, width=_up(N, 32))
         WT = packer.add_transposed(w_gate, w_up, width=half) if need_input else None
         packer.run()
         dGU = _operand_buffer(M, 2 * _row_bytes(F, planes), 2 * half, dev)
@@ -266,11 +267,10 @@ class GatedTape:
             _product(dGU, WT, None, dx, planes, M, K, 2 * half)
         if not need_weights:
             return (dx,) + (None,) * 6
-        ws = _workspace(max(lib.btvae_block_wgrad_ws(2 * half, K, M, planes), lib.btvae_block_wgrad_ws(N, F, M, planes)), dev)
-        nv.call("btvae_block_wgrad", dGU.ptr(), dGU.ld, self.X.ptr(), self.X.ld, _p(ws), ws.numel(),
-                _p(dwg), F, _p(dwu), half, F, K, int(dwg.dtype == torch.bfloat16), acc, planes, 2 * half, K, M)
-        nv.call("btvae_block_wgrad", DY.ptr(), DY.ld, self.H.ptr(), self.H.ld, _p(ws), ws.numel(),
-                _p(dwd), N, None, 0, 0, F, int(dwd.dtype == torch.bfloat16), acc, planes, N, F, M)
+        ws = _workspace(lib.btvae_block_wgrad_pair_ws(2 * half, K, N, F, M, planes), dev)
+        jobs = (dGU.ptr(), dGU.ld, self.X.ptr(), self.X.ld, _p(dwg), F, _p(dwu), half, F, K, dwg.dtype == torch.bfloat16, 2 * half, K,
+                DY.ptr(), DY.ld, self.H.ptr(), self.H.ld, _p(dwd), N, 0, 0, 0, F, dwd.dtype == torch.bfloat16, N, F)
+        nv.call("btvae_block_wgrad_pair", (ctypes.c_longlong * 26)(*jobs), _p(ws), ws.numel(), planes, M, acc)
         if want_bias:
             first, second = (dbg, dbu) if dbg is not None else (torch.empty_like(dbu), dbu)
             nv.call("btvae_block_strip_sums", _p(colpart), strips, F, _p(first), _p(second), int(first.dtype == torch.bfloat16), acc)

@@ -66,10 +66,18 @@ template <bool SRC16, bool SPLIT>
 __device__ __forceinline__ void pack_transposed(const PackJob& p, unsigned block, float (*t)[65]) {
     const unsigned across = (unsigned)(p.dst_cols + 63) / 64;
     const int r0 = (int)(block % across) * 64, c0 = (int)(block / across) * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        t[i >> 6][i & 63] = r < p.rows && c < p.cols ? (SRC16 ? bf_load(p.src, (long long)r * p.ld + c) : reinterpret_cast<const float*>(p.src)[(long long)r * p.ld + c]) : 0.f;
+    float x[16];                                              // (all loads on their way together, from the first element where there is none)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int r = r0 + 4 * k + (int)(threadIdx.x >> 6), c = c0 + (int)(threadIdx.x & 63);
+        const bool in = r < p.rows && c < p.cols;
+        const long long o = in ? (long long)r * p.ld + c : 0;
+        x[k] = 0.f;
+        if (p.rows > 0) x[k] = SRC16 ? bf_load(p.src, o) : reinterpret_cast<const float*>(p.src)[o];
+        if (!in) x[k] = 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t[4 * k + (threadIdx.x >> 6)][threadIdx.x & 63] = x[k];
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
         const int c = i >> 3, rg = (i & 7) * 8;
@@ -100,28 +108,35 @@ __global__ __launch_bounds__(256) void pack(const PackJobs jobs) {
 
 // ---- partial results ------------------------------------------------------------------------------------------------
 // out(m, n) (+)= sum_z slab[z][m][n] (+ bias[n]), in the order of z.  Rows [0, rows0) go to out0, [off1, off1 + rows1) to out1.
-__global__ __launch_bounds__(256) void reduce_slabs(const float* __restrict__ slab, int nz, int M, int N, void* out0, long long ld, int rows0, void* out1, int off1, int rows1,
-                                                    const void* bias, int bias_bf16, int out_bf16, int accumulate) {
-    const long long total = (long long)M * N;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int m = (int)(i / N), n = (int)(i - (long long)m * N);
-        void* out = out0;
+struct SlabJob {
+    const float* slab; int nz, M, N;
+    void* out0; long long ld; int rows0; void* out1; int off1, rows1;
+    const void* bias; int bias_bf16, out_bf16, accumulate;
+    unsigned first, blocks;
+};
+struct SlabJobs { SlabJob j[2]; int n; };
+__global__ __launch_bounds__(256) void reduce_slabs(const SlabJobs jobs) {
+    const SlabJob& p = jobs.j[jobs.n > 1 && blockIdx.x >= jobs.j[1].first];
+    const long long total = (long long)p.M * p.N;
+    for (long long i = (long long)(blockIdx.x - p.first) * 256 + threadIdx.x; i < total; i += (long long)p.blocks * 256) {
+        const int m = (int)(i / p.N), n = (int)(i - (long long)m * p.N);
+        void* out = p.out0;
         int row = m;
-        if (m >= rows0) {
-            row = m - off1;
-            if (!out1 || row < 0 || row >= rows1) continue;
-            out = out1;
+        if (m >= p.rows0) {
+            row = m - p.off1;
+            if (!p.out1 || row < 0 || row >= p.rows1) continue;
+            out = p.out1;
         }
         float v = 0.f;
-        for (int z = 0; z < nz; ++z) v += slab[(long long)z * total + i];
-        if (bias) v += bias_bf16 ? bf_load(bias, n) : reinterpret_cast<const float*>(bias)[n];
-        const long long o = (long long)row * ld + n;
-        if (out_bf16) {
+        for (int z = 0; z < p.nz; ++z) v += p.slab[(long long)z * total + i];
+        if (p.bias) v += p.bias_bf16 ? bf_load(p.bias, n) : reinterpret_cast<const float*>(p.bias)[n];
+        const long long o = (long long)row * p.ld + n;
+        if (p.out_bf16) {
             unsigned short* d = reinterpret_cast<unsigned short*>(out);
-            d[o] = bf_bits(accumulate ? bf_load(d, o) + v : v);
+            d[o] = bf_bits(p.accumulate ? bf_load(d, o) + v : v);
         } else {
             float* d = reinterpret_cast<float*>(out);
-            d[o] = accumulate ? d[o] + v : v;
+            d[o] = p.accumulate ? d[o] + v : v;
         }
     }
 }
@@ -514,13 +529,25 @@ static ProductPlan plan_product(int M, int N, int tn, int stages, int unit) {
     r.z = tiles(stages, r.kz);
     return r;
 }
+// Launch of reduce_slabs over one or two results
+static int launch_reduce(SlabJobs& q, hipStream_t s, const char* what) {
+    unsigned blocks = 0;
+    for (int i = 0; i < q.n; ++i) {
+        q.j[i].first = blocks;
+        q.j[i].blocks = (unsigned)std::min<long long>(((long long)q.j[i].M * q.j[i].N + 255) / 256, 8192);
+        blocks += q.j[i].blocks;
+    }
+    hipLaunchKernelGGL(reduce_slabs, dim3(blocks), dim3(256), 0, s, q);
+    return btvae::check_launch(what);
+}
 struct ColPlan { int big, z, rz; };
-static ColPlan plan_cols(int M, int N, int R, int planes) {
+// `beside`: tiles of another product in the same launch
+static ColPlan plan_cols(int M, int N, int R, int beside = 0) {
     ColPlan r;
     // 256 x 256 tiles from where their splits fill the chip: see gemm_cols
-    r.big = tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
+    r.big = !beside && tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
     const int t = r.big ? 256 : 128;
-    const int T = tiles(M, t) * tiles(N, t);
+    const int T = tiles(M, t) * tiles(N, t) + beside;
     // fill the chip; a split has at least 256 rows, and multiples of eight splits keep one row range on one XCD
     const int fill = r.big ? CHIP : 2 * CHIP;
     int z = std::max(1, std::min((T >= fill ? 1 : fill / T), tiles(R, 256)));
@@ -637,38 +664,103 @@ BTVAE_API int btvae_block_product(const void* A, long long lda, const void* B, l
     ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
     const int rc = planes == 3 ? bk::launch_rows<bk::FMT_SPLIT, bk::EP_LINEAR>(p, r.z, s, "block_product") : bk::launch_rows<bk::FMT_BF16, bk::EP_LINEAR>(p, r.z, s, "block_product");
     if (rc || r.z == 1) return rc;
-    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0, bias, bias_bf16, c_bf16, 0);
-    return check_launch("block_product reduction");
+    bk::SlabJobs q = {};
+    q.n = 1;
+    q.j[0] = {ws, r.z, M, N, C, ldc, M, nullptr, 0, 0, bias, bias_bf16, c_bf16, 0, 0, 0};
+    return bk::launch_reduce(q, s, "block_product reduction");
 }
 
+namespace btvae_block {
+struct ColJob {
+    const void* A; long long lda; const void* B; long long ldb;
+    void* out0; long long rows0; void* out1; long long off1, rows1, ldo, out_bf16; long long M, N;
+};
+static int tiles128(const ColJob& j) { return tiles((int)j.M, 128) * tiles((int)j.N, 128); }
+// Two products in one launch where both are small enough for 128 x 128 tiles and all their splits are on the chip at a time (measured:
+// the three weight gradients of 203 x 531 from 1537 rows, fp32: 17 + 4 + 15 + 4 us in four launches, 18 + 5 in two)
+static bool side_by_side(const ColJob& a, const ColJob& b, int R) {
+    return !plan_cols((int)a.M, (int)a.N, R).big && !plan_cols((int)b.M, (int)b.N, R).big && tiles128(a) + tiles128(b) <= 2 * CHIP;
+}
+static long long cols_floats(const ColJob& j, int z) { return (long long)z * j.M * j.N; }
+static long long cols_ws(const ColJob* j, int n, int R) {
+    if (n == 2 && side_by_side(j[0], j[1], R)) {
+        const int z = plan_cols((int)j[0].M, (int)j[0].N, R, tiles128(j[1])).z;
+        return cols_floats(j[0], z) + cols_floats(j[1], z);
+    }
+    long long need = 0;
+    for (int i = 0; i < n; ++i) need = std::max(need, cols_floats(j[i], plan_cols((int)j[i].M, (int)j[i].N, R).z));
+    return need;
+}
+static int run_cols(const ColJob* j, int n, float* ws, int planes, int R, int accumulate, hipStream_t s) {
+    const int unit = planes == 3 ? 16 : 8;
+    const ColPlan r = n == 2 ? plan_cols((int)j[0].M, (int)j[0].N, R, tiles128(j[1])) : plan_cols((int)j[0].M, (int)j[0].N, R);
+    const int t = r.big ? 256 : 128;
+    ColPair q = {};
+    SlabJobs sums = {};
+    sums.n = n;
+    float* slab = ws;
+    double flops = 0;
+    for (int i = 0; i < n; ++i) {
+        ColArgs& p = q.a[i];
+        const int M = (int)j[i].M, N = (int)j[i].N;
+        p.A = (const char*)j[i].A; p.lda = j[i].lda; p.a_cols = tiles(M, unit) * unit; p.B = (const char*)j[i].B; p.ldb = j[i].ldb; p.b_cols = tiles(N, unit) * unit;
+        p.R = R; p.M = M; p.N = N; p.rz = r.rz; p.slab = slab; p.tiles_m = tiles(M, t); p.tiles_n = tiles(N, t);
+        if (i == 0) q.tiles0 = p.tiles_m * p.tiles_n;
+        q.tiles += p.tiles_m * p.tiles_n;
+        sums.j[i] = {slab, r.z, M, N, j[i].out0, j[i].ldo, (int)j[i].rows0, j[i].out1, (int)j[i].off1, (int)j[i].rows1, nullptr, 0, (int)j[i].out_bf16, accumulate, 0, 0};
+        slab += cols_floats(j[i], r.z);
+        flops += 2.0 * M * N * R;
+    }
+    {
+        ProfScope prof(PK_GEMM_WGRAD, s, flops, 0.0);
+        if (int rc = launch_cols(q, planes == 3, r.big, r.z, s)) return rc;
+    }
+    return launch_reduce(sums, s, "block_wgrad reduction");
+}
+}  // namespace btvae_block
+
+static int check_cols(const bk::ColJob& j, int planes, int R) {
+    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_wgrad: planes must be 1 or 3");
+    BTVAE_REQUIRE(j.M > 0 && j.N > 0 && j.M < (1 << 30) && j.N < (1 << 30) && R >= 0 && j.rows0 > 0 && j.rows0 <= j.M && j.ldo >= j.N && j.out0, "block_wgrad: bad sizes (M %lld, N %lld, R %d)", j.M, j.N, R);
+    const int unit = planes == 3 ? 16 : 8, M8 = bk::tiles((int)j.M, unit) * unit, N8 = bk::tiles((int)j.N, unit) * unit;
+    BTVAE_REQUIRE(!j.out1 || (j.off1 >= j.rows0 && j.rows1 >= 0 && j.off1 + j.rows1 <= j.M), "block_wgrad: bad row ranges");
+    BTVAE_REQUIRE(R == 0 || (operand_ok(j.A, j.lda, planes, M8) && operand_ok(j.B, j.ldb, planes, N8)), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of %d columns", unit);
+    BTVAE_REQUIRE(j.lda < (1 << 23) && j.ldb < (1 << 23), "block_wgrad: rows of more than 8 MiB");
+    return 0;
+}
 BTVAE_API long long btvae_block_wgrad_ws(int M, int N, int R, int planes) {
-    const bk::ColPlan r = bk::plan_cols(M, N, R, planes);
-    return (long long)r.z * M * N;
+    bk::ColJob j = {};
+    j.M = M; j.N = N;
+    return bk::cols_ws(&j, 1, R);
 }
 // out(m, n) (+)= sum_r A[r][m] B[r][n], m < M (rows [0, rows0) -> out0, [off1, off1 + rows1) -> out1), n < N
 BTVAE_API int btvae_block_wgrad(const void* A, long long lda, const void* B, long long ldb, float* ws, long long ws_floats,
                                 void* out0, int rows0, void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate, int planes, int M, int N, int R, void* stream) {
-    BTVAE_REQUIRE(planes == 1 || planes == 3, "block_wgrad: planes must be 1 or 3");
-    const int unit = planes == 3 ? 16 : 8, M8 = bk::tiles(M, unit) * unit, N8 = bk::tiles(N, unit) * unit;
-    BTVAE_REQUIRE(M > 0 && N > 0 && R >= 0 && rows0 > 0 && rows0 <= M && ldo >= N && out0, "block_wgrad: bad sizes (M %d, N %d, R %d)", M, N, R);
-    BTVAE_REQUIRE(!out1 || (off1 >= rows0 && off1 + rows1 <= M), "block_wgrad: bad row ranges");
-    BTVAE_REQUIRE(R == 0 || (operand_ok(A, lda, planes, M8) && operand_ok(B, ldb, planes, N8)), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of %d columns", unit);
-    BTVAE_REQUIRE(lda < (1 << 23) && ldb < (1 << 23), "block_wgrad: rows of more than 8 MiB");
+    const bk::ColJob j = {A, lda, B, ldb, out0, rows0, out1, off1, rows1, ldo, out_bf16, M, N};
+    if (int rc = check_cols(j, planes, R)) return rc;
+    BTVAE_REQUIRE(ws && ws_floats >= bk::cols_ws(&j, 1, R), "block_wgrad: workspace too small");
+    return bk::run_cols(&j, 1, ws, planes, R, accumulate, BLK_STREAM(stream));
+}
+// Two such sums over the same rows, in one launch where that pays: jobs of thirteen numbers (A, lda, B, ldb, out0, rows0, out1, off1, rows1, ldo, out_bf16, M, N)
+static void cols_jobs(const long long* a, bk::ColJob* j) {
+    for (int i = 0; i < 2; ++i, a += 13) j[i] = {(const void*)a[0], a[1], (const void*)a[2], a[3], (void*)a[4], a[5], (void*)a[6], a[7], a[8], a[9], a[10], a[11], a[12]};
+}
+BTVAE_API long long btvae_block_wgrad_pair_ws(int M0, int N0, int M1, int N1, int R, int planes) {
+    bk::ColJob j[2] = {};
+    j[0].M = M0; j[0].N = N0; j[1].M = M1; j[1].N = N1;
+    return bk::cols_ws(j, 2, R);
+}
+BTVAE_API int btvae_block_wgrad_pair(const long long* jobs, float* ws, long long ws_floats, int planes, int R, int accumulate, void* stream) {
+    BTVAE_REQUIRE(jobs, "block_wgrad: null jobs");
+    bk::ColJob j[2];
+    cols_jobs(jobs, j);
+    for (int i = 0; i < 2; ++i)
+        if (int rc = check_cols(j[i], planes, R)) return rc;
+    BTVAE_REQUIRE(ws && ws_floats >= bk::cols_ws(j, 2, R), "block_wgrad: workspace too small");
     hipStream_t s = BLK_STREAM(stream);
-    const bk::ColPlan r = bk::plan_cols(M, N, R, planes);
-    BTVAE_REQUIRE(ws && ws_floats >= (long long)r.z * M * N, "block_wgrad: workspace too small");
-    bk::ColArgs p = {};
-    p.A = (const char*)A; p.lda = lda; p.a_cols = M8; p.B = (const char*)B; p.ldb = ldb; p.b_cols = N8;
-    p.R = R; p.M = M; p.N = N; p.rz = r.rz; p.slab = ws;
-    const int t = r.big ? 256 : 128;
-    p.tiles_m = bk::tiles(M, t); p.tiles_n = bk::tiles(N, t);
-    {
-        ProfScope prof(PK_GEMM_WGRAD, s, 2.0 * M * N * R, 0.0);
-        if (int rc = bk::launch_cols(p, planes == 3, r.big, r.z, s)) return rc;
-    }
-    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, out0, ldo, rows0, out1, off1, rows1,
-                       (const void*)nullptr, 0, out_bf16, accumulate);
-    return check_launch("block_wgrad reduction");
+    if (bk::side_by_side(j[0], j[1], R)) return bk::run_cols(j, 2, ws, planes, R, accumulate, s);
+    if (int rc = bk::run_cols(j, 1, ws, planes, R, accumulate, s)) return rc;
+    return bk::run_cols(j + 1, 1, ws, planes, R, accumulate, s);
 }
 
 // out[n] (+)= sum_r src[r][n]; ws: btvae_block_colsum_ws floats
@@ -795,9 +887,10 @@ BTVAE_API int btvae_fp8_product(const void* X, long long ldx, const void* xs, lo
     ProfScope prof(PK_GEMM_FWD, s, 2.0 * M * N * K, 0.0);
     if (int rc = bk::launch_rows<bk::FMT_E4M3, bk::EP_LINEAR>(p, r.z, s, "fp8_product")) return rc;
     if (r.z == 1) return 0;
-    hipLaunchKernelGGL(bk::reduce_slabs, dim3((unsigned)std::min<long long>(((long long)M * N + 255) / 256, 8192)), dim3(256), 0, s, (const float*)ws, r.z, M, N, C, ldc, M, (void*)nullptr, 0, 0,
-                       (const void*)bias, 0, c_bf16, 0);
-    return check_launch("fp8_product reduction");
+    bk::SlabJobs q = {};
+    q.n = 1;
+    q.j[0] = {ws, r.z, M, N, C, ldc, M, nullptr, 0, 0, bias, 0, c_bf16, 0, 0, 0};
+    return bk::launch_reduce(q, s, "fp8_product reduction");
 }
 // H = act(x Wg^T + bg) (x Wu^T + bu), quantised again (q [M][ldh], scale bytes [M][hsp]) in the epilogue.  expanded: X, Wg, Wu hold bf16 (pitches in
 // elements, whole blocks of 128 columns) instead of e4m3 and scales.

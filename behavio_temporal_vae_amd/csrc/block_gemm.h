@@ -1144,9 +1144,12 @@ struct ColArgs {
     int tiles_m, tiles_n;
     float* slab;                                              // [z][M][N]
 };
+// One product, or two over the same rows and splits side by side (small ones do not fill the chip, and a launch less is most of their time)
+struct ColPair { ColArgs a[2]; int tiles0, tiles; };          // tiles of the first, of both
+
 
 template <bool SPLIT, int WM, int WN, int MI, int NJ>
-__global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols(const ColArgs p) {
+__global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols(const ColPair pair) {
     constexpr int NW = WM * WN, RW = MI * 32, CW = NJ * 32, TM = WM * RW, TN = WN * CW;
     constexpr int EB = SPLIT ? 6 : 2, SR = SPLIT ? 16 : 32, SLOTS = 3, SETS = SPLIT ? 1 : 2;        // bytes of a column, rows of a stage, stages in LDS and in registers
     constexpr int ARB = TM * EB, BRB = TN * EB;               // bytes of an image row
@@ -1159,7 +1162,7 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
     const int lh = lane >> 5;
     const Where<false> wh(smem + RING + wid * Where<false>::LDS_B);
     // Splits of the reduction first: all output tiles of one row range run together on one XCD and share its rows in L2.
-    const int T = p.tiles_m * p.tiles_n, nz = (int)gridDim.z;
+    const int T = pair.tiles, nz = (int)gridDim.z;
     int zz, tile;
     if ((nz & 7) == 0) {
         const int L = (int)blockIdx.x + T * (int)blockIdx.z, xcd = L & 7, idx = L >> 3;
@@ -1169,6 +1172,8 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
         zz = (int)blockIdx.z;
         tile = (int)blockIdx.x;
     }
+    const ColArgs& p = pair.a[tile >= pair.tiles0];
+    if (tile >= pair.tiles0) tile -= pair.tiles0;
     const int tile_m = tile / p.tiles_n, tile_n = tile % p.tiles_n;
     const int m0 = tile_m * TM, n0 = tile_n * TN;
     const int rbeg = zz * p.rz, rows = max(0, min(p.rz, p.R - rbeg));

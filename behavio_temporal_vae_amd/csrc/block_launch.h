@@ -12,7 +12,7 @@ constexpr int tile_width(bool split) { return split ? 128 : 256; }    // columns
 inline bool al16(const void* q) { return ((uintptr_t)q & 15) == 0; }
 
 template <int FMT, int EP> int launch_rows(Args& p, int z, hipStream_t s, const char* what);
-int launch_cols(const ColArgs& p, int split, int big, int z, hipStream_t s);
+int launch_cols(const ColPair& p, int split, int big, int z, hipStream_t s);
 
 #ifdef BTVAE_BLOCK_KERNELS
 // As many workgroups as the chip holds at a time (one of eight waves to a compute unit, or two of four), each going through its items.

@@ -410,6 +410,9 @@ int btvae_block_product(const void* A, long long lda, const void* B, long long l
 long long btvae_block_wgrad_ws(int M, int N, int R, int planes);
 int btvae_block_wgrad(const void* A, long long lda, const void* B, long long ldb, float* ws, long long ws_floats, void* out0, int rows0,
             void* out1, int off1, int rows1, long long ldo, int out_bf16, int accumulate, int planes, int M, int N, int R, void* stream);
+/* Two such sums over the same rows R, each described by thirteen numbers: A, lda, B, ldb, out0, rows0, out1, off1, rows1, ldo, out_bf16, M, N. */
+long long btvae_block_wgrad_pair_ws(int M0, int N0, int M1, int N1, int R, int planes);
+int btvae_block_wgrad_pair(const long long* jobs, float* ws, long long ws_floats, int planes, int R, int accumulate, void* stream);
 /* out[n] (+)= column sums of src [R, N]. */
 long long btvae_block_colsum_ws(int R, int N);
 int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, long long ws_floats, void* out, int out_bf16,

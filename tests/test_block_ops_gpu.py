@@ -926,3 +926,29 @@ def test_networks_gradients_accumulate(dev):
     assert grads[0]
     for k, g in grads[0].items():
         assert torch.equal(grads[1][k], 2 * g), k
+
+
+@pytest.mark.parametrize("planes", [1, 3])
+@pytest.mark.parametrize("R,shapes", [(1537, ((104, 203), (203, 53))), (70, ((1, 1), (9, 260))), (0, ((8, 8), (16, 5))), (3000, ((2000, 1000), (130, 40)))])
+def test_block_wgrad_pair(dev, planes, R, shapes):
+    """Two weight gradients in one call (one launch when both are small, two when not): each as by itself, to float32's accuracy, the
+    memory behind the workspace untouched, sums added to what was there."""
+    lib = nv.lib()
+    dtype = BF if planes == 1 else F32
+    mats, jobs, outs, refs = [], [], [], []
+    for i, (M, N) in enumerate(shapes):
+        a, b = rnd(dev, R, M, seed=101 + i, dtype=dtype), rnd(dev, R, N, seed=111 + i, dtype=dtype)
+        A, X = (B._operand(a, planes, 1 << 30), B._operand(b, planes, 1 << 30)) if R else (None, None)
+        out = torch.full((M, N), 2.0, device=dev)
+        mats += [A, X]
+        jobs += [A.ptr() if R else 0, A.ld if R else 0, X.ptr() if R else 0, X.ld if R else 0, out.data_ptr(), M, 0, 0, 0, N, 0, M, N]
+        outs.append(out)
+        refs.append(2.0 + d64(a).t() @ d64(b))
+    need = lib.btvae_block_wgrad_pair_ws(*shapes[0], *shapes[1], R, planes)
+    ws = torch.full((need + 64,), 7.0, device=dev)
+    nv.call("btvae_block_wgrad_pair", (nv.ctypes.c_longlong * 26)(*jobs), ws.data_ptr(), need, planes, R, 1)
+    for o, r, (M, N) in zip(outs, refs, shapes):
+        frob(o, r, E * (6 + math.sqrt(max(R, 1))), f"{M} x {N}")
+    assert bool((ws[need:] == 7.0).all())
+    with pytest.raises(RuntimeError, match="workspace"):
+        nv.call("btvae_block_wgrad_pair", (nv.ctypes.c_longlong * 26)(*jobs), ws.data_ptr(), need - 1, planes, R, 1)
