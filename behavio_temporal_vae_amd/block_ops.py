@@ -121,9 +121,14 @@ def _operand_buffer(rows, ld, width, device) -> _Operand:
     return _Operand(t.data_ptr(), ld, width, t)
 
 
+def _bytes(cols, planes):
+    return cols * (6 if planes == 3 else 2)
+
+
 def _row_bytes(cols, planes):
-    """Bytes of an operand row of ``cols`` columns (whole groups of 32, so that rows start on 64 bytes)."""
-    return _up(cols, 32) * (6 if planes == 3 else 2)
+    """Pitch of an operand of ``cols`` columns: whole groups of 32, bf16 rows on 128 bytes (rows on 64 of them cost a product of 65,536 x
+    2000 x 1000 391 us instead of 275)."""
+    return _bytes(_up(cols, 32 if planes == 3 else 64), planes)
 
 
 def _fits(t):
@@ -146,8 +151,8 @@ class _Packer:
 
     def add_transposed(self, *ts, width) -> _Operand:
         """[t0^T t1^T ..], ``width`` columns to each."""
-        cols, piece = ts[0].shape[1], _row_bytes(width, self.planes)
-        ld = piece * len(ts)
+        cols, piece = ts[0].shape[1], _bytes(width, self.planes)
+        ld = _up(piece * len(ts), 128 if self.planes == 1 else 96)
         op = _Operand(self.bytes, ld, width * len(ts))
         for i, t in enumerate(ts):
             self._job(t, op, i * piece, cols * ld if i == 0 else 0, width, 1)
@@ -214,9 +219,9 @@ def _product(a: _Operand, b: _Operand, bias, out, planes, M, N, K):
 class GatedTape:
     """What the backward pass of one ``gated_feed_forward`` needs: the inputs, both projections, h."""
 
-    def __init__(self, x, weights, biases, act, planes, X, H, GU, GU_lo, half):
+    def __init__(self, x, weights, biases, act, planes, X, H, kept):
         self.x, self.weights, self.biases, self.act, self.planes = x, weights, biases, act, planes
-        self.X, self.H, self.GU, self.GU_lo, self.half = X, H, GU, GU_lo, half
+        self.X, self.H, self.kept = X, H, kept
 
     def _check_outs(self, outs):
         if len(outs) != 6:
@@ -243,7 +248,7 @@ class GatedTape:
         nv.ensure_device(dev)
         dy = _rows(_tensor(dy, "the gradient"), "the gradient")
         _matrix(dy, "the gradient", (M, N), dy.dtype, dev)
-        lib, half = nv.lib(), self.half
+        lib, half = nv.lib(), _up(F, 32)
         if outs is None:
             outs = [torch.empty_like(w, memory_format=torch.contiguous_format) for w in self.weights] + \
                    [None if b is None else torch.empty_like(b, memory_format=torch.contiguous_format) for b in self.biases]
@@ -256,11 +261,11 @@ class GatedTape:
         DY, WdT = _operand(dy, planes, 2 * F, packer), packer.add_transposed(w_down, width=_up(N, 32))
         WT = packer.add_transposed(w_gate, w_up, width=half) if need_input else None
         packer.run()
-        dGU = _operand_buffer(M, 2 * _row_bytes(F, planes), 2 * half, dev)
+        dGU = _operand_buffer(M, _bytes(2 * half, planes), 2 * half, dev)
         want_bias = need_weights and (dbg is not None or dbu is not None)
         strips = lib.btvae_gated_proj_strips(M) if M else 0
         colpart = _workspace(strips * 2 * F, dev) if want_bias else None
-        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, WdT.ptr(), WdT.ld, _p(self.GU), _p(self.GU_lo), 2 * half, half, dGU.ptr(), dGU.ld, _p(colpart), planes, self.act, M, F, DY.width)
+        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, WdT.ptr(), WdT.ld, _p(self.kept), dGU.ptr(), dGU.ld, _p(colpart), planes, self.act, M, F, DY.width)
         dx = None
         if need_input:
             dx = torch.empty(M, K, dtype=x.dtype, device=dev)
@@ -307,21 +312,19 @@ def _ffn_forward(x2, weights, biases, act, planes, out_dtype, keep):
     w_gate, w_up, w_down = weights
     b_gate, b_up, b_down = biases
     dev, (M, K), F, N = x2.device, x2.shape, w_gate.shape[0], w_down.shape[0]
-    half = _up(F, 32)
     packer = _Packer(planes, dev)
     X = _operand(x2, planes, 2 * F, packer, apart=keep)
     Wg, Wu = _operand_pair(w_gate, w_up, planes, M, packer)
     Wd = _operand(w_down, planes, M, packer)
     packer.run()
     H = _operand_buffer(M, _row_bytes(F, planes), _up(F, 8), dev)
-    GU = torch.empty(M * 2 * half, dtype=torch.float32 if planes == 3 else torch.int16, device=dev) if keep else None
-    GU_lo = torch.empty(M * 2 * half, dtype=torch.uint8, device=dev) if keep and planes == 1 else None
+    kept = torch.empty(nv.lib().btvae_gated_kept_bytes(M, F, planes), dtype=torch.uint8, device=dev) if keep else None
     bias16 = int(any(b is not None and b.dtype == torch.bfloat16 for b in (b_gate, b_up)))
     nv.call("btvae_gated_proj_fwd", X.ptr(), X.ld, Wg.ptr(), Wu.ptr(), Wg.ld, _p(b_gate), _p(b_up), bias16,
-            H.ptr(), H.ld, _p(GU), _p(GU_lo), 2 * half, half, planes, act, M, F, X.width)
+            H.ptr(), H.ld, _p(kept), planes, act, M, F, X.width)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
     _product(H, Wd, b_down, y, planes, M, N, Wd.width)
-    return y, GatedTape(x2, weights, biases, act, planes, X, H, GU, GU_lo, half) if keep else None
+    return y, GatedTape(x2, weights, biases, act, planes, X, H, kept) if keep else None
 
 
 def _ffn_few(x2, weights, biases, act):
@@ -354,7 +357,7 @@ class _GatedNode(torch.autograd.Function):
         x2, w_gate, w_up, w_down, b_gate, b_up, b_down = ctx.saved_tensors
         need = ctx.needs_input_grad
         t = ctx.tape
-        tape = GatedTape(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], t.act, t.planes, t.X, t.H, t.GU, t.GU_lo, t.half)
+        tape = GatedTape(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], t.act, t.planes, t.X, t.H, t.kept)
         return (None, *tape.backward(dy, need_input=need[1], need_weights=any(need[2:])))
 
 

@@ -597,44 +597,44 @@ BTVAE_API int btvae_block_pack(const long long* jobs, int n, void* stream) {
     return check_launch("block_pack");
 }
 
-static bool kept_ok(const void* GU, const void* GU_lo, long long ldgu, int gu_half, int planes, int F) {
-    return bk::al16(GU) && (planes == 3 || (GU_lo && bk::al16(GU_lo))) && (ldgu & 15) == 0 && (gu_half & 31) == 0 && gu_half >= F && ldgu >= 2LL * gu_half && ldgu < (1 << 24);
+// Bytes of the kept projections: blocks of 32 x 32 values of a and of b, 24 bits a value for bf16 operands, else 32
+BTVAE_API long long btvae_gated_kept_bytes(int M, int F, int planes) {
+    return (long long)bk::tiles(M, 32) * bk::tiles(F, 32) * 2 * (planes == 3 ? bk::kept_bytes<false>() : bk::kept_bytes<true>());
 }
-
 BTVAE_API int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu, int bias_bf16,
-                                   void* H, long long ldh, void* GU, void* GU_lo, long long ldgu, int gu_half, int planes, int act, int M, int F, int K, void* stream) {
+                                   void* H, long long ldh, void* kept, int planes, int act, int M, int F, int K, void* stream) {
     BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_fwd: planes must be 1 or 3");
     BTVAE_REQUIRE(M >= 0 && F > 0 && K > 0 && (planes == 3 || (K & 7) == 0), "gated_proj_fwd: bad sizes (M %d, F %d, K %d)", M, F, K);
     BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_fwd: unknown activation %d", act);
     if (M == 0) return 0;
     BTVAE_REQUIRE(operand_ok(X, ldx, planes, K) && operand_ok(Wg, ldw, planes, K) && operand_ok(Wu, ldw, planes, K), "gated_proj_fwd: bad operand layout");
     BTVAE_REQUIRE(operand_ok(H, ldh, planes, bk::tiles(F, 16) * 16) && ldh < (1 << 24), "gated_proj_fwd: bad layout of H");
-    BTVAE_REQUIRE(!GU || kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_fwd: bad layout of the kept projections");
+    BTVAE_REQUIRE(bk::al16(kept), "gated_proj_fwd: the kept projections must start on 16 bytes");
     bk::Args p = {};
     p.A = (const char*)X; p.lda = ldx; p.B = (const char*)Wg; p.B2 = (const char*)Wu; p.ldb = ldw;
     p.M = M; p.N = F; p.K = K; p.ks = p.kz = stages_of(K, planes);
     p.bias = bg; p.bias2 = bu; p.bias_bf16 = bias_bf16;
     p.C = H; p.ldc = planes == 3 ? ldh : ldh / 2;
-    p.act = act; p.gu = GU; p.gu_lo = (unsigned char*)GU_lo; p.ldgu = ldgu; p.gu_half = gu_half;
+    p.act = act; p.kept = (char*)kept; p.half = bk::tiles(F, 32) * 32;
     ProfScope prof(PK_GEMM_FWD, BLK_STREAM(stream), 4.0 * M * F * K, 0.0);
     if (planes == 3) return bk::launch_rows<bk::FMT_SPLIT, bk::EP_GATED_3>(p, 1, BLK_STREAM(stream), "gated_proj_fwd");
     return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED>(p, 1, BLK_STREAM(stream), "gated_proj_fwd");
 }
 
-BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* GU, const void* GU_lo, long long ldgu, int gu_half,
-                                   void* dGU, long long ldd, float* colpart, int planes, int act, int M, int F, int N, void* stream) {
+BTVAE_API int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* kept, void* dGU, long long ldd, float* colpart, int planes, int act, int M, int F, int N, void* stream) {
     BTVAE_REQUIRE(planes == 1 || planes == 3, "gated_proj_bwd: planes must be 1 or 3");
     BTVAE_REQUIRE(M >= 0 && F > 0 && N > 0 && (planes == 3 || (N & 7) == 0), "gated_proj_bwd: bad sizes (M %d, F %d, N %d)", M, F, N);
     BTVAE_REQUIRE(act >= 0 && act <= 3, "gated_proj_bwd: unknown activation %d", act);
     if (M == 0) return 0;
     BTVAE_REQUIRE(operand_ok(dY, lddy, planes, N) && operand_ok(WdT, ldw, planes, N), "gated_proj_bwd: bad operand layout");
-    BTVAE_REQUIRE(kept_ok(GU, GU_lo, ldgu, gu_half, planes, F), "gated_proj_bwd: bad layout of the kept projections");
-    BTVAE_REQUIRE(operand_ok(dGU, ldd, planes, 2 * gu_half) && ldd < (1 << 26), "gated_proj_bwd: bad layout of the gradients");
+    const int half = bk::tiles(F, 32) * 32;
+    BTVAE_REQUIRE(kept && bk::al16(kept), "gated_proj_bwd: the kept projections must start on 16 bytes");
+    BTVAE_REQUIRE(operand_ok(dGU, ldd, planes, 2 * half) && ldd < (1 << 26), "gated_proj_bwd: bad layout of the gradients");
     bk::Args p = {};
     p.A = (const char*)dY; p.lda = lddy; p.B = (const char*)WdT; p.ldb = ldw;
     p.M = M; p.N = F; p.K = N; p.ks = p.kz = stages_of(N, planes);
     p.C = dGU; p.ldc = planes == 3 ? ldd : ldd / 2;
-    p.act = act; p.gu = const_cast<void*>(GU); p.gu_lo = (unsigned char*)const_cast<void*>(GU_lo); p.ldgu = ldgu; p.gu_half = gu_half; p.colpart = colpart;
+    p.act = act; p.kept = (char*)const_cast<void*>(kept); p.half = half; p.colpart = colpart;
     ProfScope prof(PK_GEMM_DGRAD, BLK_STREAM(stream), 2.0 * M * F * N, 0.0);
     if (planes == 3) return bk::launch_rows<bk::FMT_SPLIT, bk::EP_GATED_BWD_3>(p, 1, BLK_STREAM(stream), "gated_proj_bwd");
     return bk::launch_rows<bk::FMT_BF16, bk::EP_GATED_BWD>(p, 1, BLK_STREAM(stream), "gated_proj_bwd");

@@ -88,10 +88,10 @@ struct Args {
     void* C; long long ldc; int c_type;             // EP_LINEAR: T_F32 or T_BF16, pitch in elements; split results: pitch in bytes
     float* slab;                                    // splits > 1: fp32 partial results [z][M][N]
     int act;
-    // Gated: where a, b are kept for the backward pass (null: not); backward: read; b starts gu_half columns after a.  fp32, or (bf16
-    // operands) 24 bits: the upper two bytes here, the third in gu_lo -- 2^-15 instead of bf16's 2^-8, since these values are rounded again as part of
-    // the gradients
-    void* gu; unsigned char* gu_lo; long long ldgu; int gu_half;
+    // Gated: where a, b are kept for the backward pass (null: not), in the order in which the kernels' lanes hold them: for every 32 rows and
+    // 32 columns a block of a and one of b, 16 values to a lane, each fp32 or (bf16 operands) 24 bits -- 2^-15 instead of bf16's
+    // 2^-8, since these values are rounded again as part of the gradients.  Backward: `half` columns of da (a multiple of 32), then db
+    char* kept; int half;
     float* colpart;                                 // backward: column sums of (da, db) per wave's strip of rows [strips][2][N], or null
     unsigned char* q_sc; long long q_scp;           // EP_GATED_Q: scale bytes of the output [M][q_scp]
 };
@@ -350,16 +350,6 @@ template <bool HALF> struct Where {
         }
         fence();
     }
-    // ... and back
-    __device__ __forceinline__ void back(const u32x4 a, const u32x4 b, int c0, u32x4& x0, int c1, u32x4& x1) const {
-        static_assert(!HALF, "");
-        *at4(r4, p4) = a;
-        *at4(r4 + 16, p4) = b;
-        fence();
-        x0 = *at4(li, c0);
-        x1 = *at4(li, c1);
-        fence();
-    }
     // 8-byte pieces lh and 2 + lh of this lane's row of 32 bytes -> 16-byte piece p2 of row r2
     __device__ __forceinline__ u32x4 turn2(const u32x2 x0, const u32x2 x1) const {
         *reinterpret_cast<u32x2*>(at2(li) + ((8 * lh) ^ two(li))) = x0;
@@ -368,13 +358,6 @@ template <bool HALF> struct Where {
         const u32x4 a = *reinterpret_cast<const u32x4*>(at2(r2) + ((16 * p2) ^ two(r2)));
         fence();
         return a;
-    }
-    __device__ __forceinline__ void back2(const u32x4 a, u32x2& x0, u32x2& x1) const {
-        *reinterpret_cast<u32x4*>(at2(r2) + ((16 * p2) ^ two(r2))) = a;
-        fence();
-        x0 = *reinterpret_cast<const u32x2*>(at2(li) + ((8 * lh) ^ two(li)));
-        x1 = *reinterpret_cast<const u32x2*>(at2(li) + ((16 + 8 * lh) ^ two(li)));
-        fence();
     }
 };
 // 8 bf16 (a lane's 16 bytes) at columns c .. c + 7 of a row, those below n only
@@ -425,8 +408,7 @@ template <class W> __device__ __forceinline__ void store_split(char* base, long 
         if (r + 16 < rows) *reinterpret_cast<u32x4*>(d + 16 * ld) = b;
     }
 }
-// A wave's rows of a matrix of whole 16-byte pieces, through a buffer descriptor that ends behind the last row: pieces outside are loaded as
-// zeros and not stored.  No lane is masked, so that no wait has to allow for stores that were skipped.
+// A wave's rows of a matrix of whole 16-byte pieces, through a buffer descriptor that ends behind the last row: pieces outside are not stored.
 constexpr unsigned OUTSIDE = 0xFFFFFFF0u;
 struct Panel {
     Buffer buf;
@@ -436,7 +418,6 @@ struct Panel {
     }
     __device__ __forceinline__ unsigned at(int r, unsigned byte, bool in) const { return in ? (unsigned)r * ld + byte : OUTSIDE; }
     __device__ __forceinline__ void put(const u32x4 v, unsigned o) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 0); }
-    __device__ __forceinline__ u32x4 get(unsigned o) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, o, 0, 2); }      // (nt: read once)
 };
 // block of rows `row` .. + 31 of the panel, columns col0 .. + 31 of which those below `cols` (a multiple of 16) exist
 template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
@@ -447,69 +428,59 @@ template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, 
     out.put(a, o);
     out.put(b, c < cols ? o + 16 * out.ld : OUTSIDE);
 }
-// 24 bits of fp32 values: the upper three bytes, cut (off by 2^-15 of a value at most, where the gradients made from
-// them are rounded to bf16, 2^-8; rounding took four more instructions a value)
-template <class W> __device__ __forceinline__ void store_24(const Panel& hi, const Panel& lo, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
-    u32x4 h[2], a, b;
-    u32x2 l[2];
+// Kept projections: a block's bytes, and block (row0, col0) of a (0) or b (1); every store and load is 1 KiB in a row
+template <bool B24> constexpr int kept_bytes() { return B24 ? 3072 : 4096; }
+template <bool B24> __device__ __forceinline__ char* kept_at(const Args& p, int row0, int col0, int which) {
+    return p.kept + (((long long)(row0 >> 5) * (p.half >> 5) + (col0 >> 5)) * 2 + which) * kept_bytes<B24>() + (threadIdx.x & 63) * 16;
+}
+struct Raw24 { u32x4 h[2], l; };
+struct Raw32 { u32x4 x[4]; };
+// 24 bits: the upper three bytes, cut (off by 2^-15 of a value at most, where the gradients made from them are rounded to bf16, 2^-8;
+// rounding took four more instructions a value)
+__device__ __forceinline__ void keep_24(char* at, const float (&v)[2][8]) {
+    u32x4 l;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         unsigned u[8];
+        u32x4 h;
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[q][e]);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) h[q][d] = __builtin_amdgcn_perm(u[2 * d + 1], u[2 * d], 0x07060302u);
+        for (int d = 0; d < 4; ++d) h[d] = __builtin_amdgcn_perm(u[2 * d + 1], u[2 * d], 0x07060302u);
 #pragma unroll
         for (int d = 0; d < 2; ++d)                           // byte 1 of four values
-            l[q][d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0501u), __builtin_amdgcn_perm(u[4 * d + 1], u[4 * d], 0x0C0C0501u), 0x05040100u);
+            l[2 * q + d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0501u), __builtin_amdgcn_perm(u[4 * d + 1], u[4 * d], 0x0C0C0501u), 0x05040100u);
+        *reinterpret_cast<u32x4*>(at + q * 1024) = h;
     }
-    w.turn(h[0], w.lh, h[1], 2 + w.lh, a, b);
-    const u32x4 lv = w.turn2(l[0], l[1]);
-    const int c = col0 + 8 * w.p4, c2 = col0 + 16 * w.p2;
-    const unsigned o = hi.at(row + w.r4, 2 * c, c < cols);
-    hi.put(a, o);
-    hi.put(b, c < cols ? o + 16 * hi.ld : OUTSIDE);
-    lo.put(lv, lo.at(row + w.r2, c2, c2 < cols));
+    *reinterpret_cast<u32x4*>(at + 2048) = l;
 }
-struct Raw24 { u32x4 a, b, l; };
-template <class W> __device__ __forceinline__ void load_24(const Panel& hi, const Panel& lo, int row, int col0, int cols, Raw24& x, const W& w) {
-    const int c = col0 + 8 * w.p4, c2 = col0 + 16 * w.p2;
-    const unsigned o = hi.at(row + w.r4, 2 * c, c < cols);
-    x.a = hi.get(o);
-    x.b = hi.get(c < cols ? o + 16 * hi.ld : OUTSIDE);
-    x.l = lo.get(lo.at(row + w.r2, c2, c2 < cols));
+__device__ __forceinline__ u32x4 load_once(const char* at) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at)); }
+__device__ __forceinline__ void load_24(const char* at, Raw24& x) {
+    x.h[0] = load_once(at);
+    x.h[1] = load_once(at + 1024);
+    x.l = load_once(at + 2048);
 }
-template <class W> __device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8], const W& w) {
-    u32x4 h[2];
-    u32x2 l[2];
-    w.back(x.a, x.b, w.lh, h[0], 2 + w.lh, h[1]);
-    w.back2(x.l, l[0], l[1]);
+__device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8]) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             // bytes 3, 2: the half word, byte 1: the low byte, byte 0: zero
             const unsigned sel = (e & 1 ? 0x07060000u : 0x05040000u) | (unsigned)(e & 3) << 8 | 0x0Cu;
-            v[q][e] = __uint_as_float(__builtin_amdgcn_perm(h[q][e >> 1], l[q][e >> 2], sel));
+            v[q][e] = __uint_as_float(__builtin_amdgcn_perm(x.h[q][e >> 1], x.l[2 * q + (e >> 2)], sel));
         }
 }
-struct Raw32 { u32x4 a[2], b[2]; };
-template <class W> __device__ __forceinline__ void load_f32(const float* base, long long ld, int row0, int col0, int rows, int cols, Raw32& x, const W& w) {
+__device__ __forceinline__ void keep_32(char* at, const float (&v)[2][8]) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int c = min(col0 + 16 * q + 4 * w.p4, cols - 4);
-        x.a[q] = *reinterpret_cast<const u32x4*>(base + (long long)min(row0 + w.r4, rows - 1) * ld + c);
-        x.b[q] = *reinterpret_cast<const u32x4*>(base + (long long)min(row0 + w.r4 + 16, rows - 1) * ld + c);
-    }
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(at + k * 1024) = raw4(v[k >> 1] + 4 * (k & 1));
 }
-template <class W> __device__ __forceinline__ void unpack_f32(const Raw32& x, float (&v)[2][8], const W& w) {
+__device__ __forceinline__ void load_32(const char* at, Raw32& x) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        u32x4 p0, p1;
-        w.back(x.a[q], x.b[q], 2 * w.lh, p0, 2 * w.lh + 1, p1);
+    for (int k = 0; k < 4; ++k) x.x[k] = load_once(at + k * 1024);
+}
+__device__ __forceinline__ void unpack_32(const Raw32& x, float (&v)[2][8]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v[q][e] = __uint_as_float(p0[e]); v[q][4 + e] = __uint_as_float(p1[e]); }
-    }
+    for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = __uint_as_float(x.x[r >> 2][r & 3]);
 }
 // Biases are loaded once a tile, before its loop, a column to a lane (a load behind the results' stores would wait for them),
 // and read from the lanes: columns c .. c + 31 of what the lanes hold.
@@ -936,8 +907,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
             constexpr int HJ = NJ / 2;
             static_assert(HJ == 1, "");
             const Panel out(p.C, 2 * p.ldc, row0, p.M, RW);   // (EP_GATED)
-            const Panel hi_a(p.gu, 2 * p.ldgu, row0, p.M, RW), hi_b(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, 2 * p.ldgu, row0, p.M, RW);
-            const Panel lo_a(p.gu_lo, p.ldgu, row0, p.M, RW), lo_b(p.gu_lo + p.gu_half, p.ldgu, row0, p.M, RW);
             float bg[2][8], bu[2][8];
             put_biases(bias_a, wh);
             bias_of(0, bg, wh);
@@ -968,14 +937,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             for (int r = 0; r < 16; ++r) acc[i][j][r] = h[r >> 3][r & 7];
                         } else if constexpr (EP == EP_GATED) {
                             panel_bf16(out, i * 32, c, N16, h, wh);
-                            if (p.gu) {
-                                store_24(hi_a, lo_a, i * 32, c, N16, a, wh);
-                                store_24(hi_b, lo_b, i * 32, c, N16, b, wh);
+                            if (p.kept && r0 < p.M && c < p.half) {         // (uniform)
+                                keep_24(kept_at<true>(p, r0, c, 0), a);
+                                keep_24(kept_at<true>(p, r0, c, 1), b);
                             }
                         } else {
-                            if (p.gu) {
-                                store_f32(reinterpret_cast<float*>(p.gu), p.ldgu, r0, c, p.M, N16, a, wh);
-                                store_f32(reinterpret_cast<float*>(p.gu) + p.gu_half, p.ldgu, r0, c, p.M, N16, b, wh);
+                            if (p.kept && r0 < p.M && c < p.half) {         // (uniform)
+                                keep_32(kept_at<false>(p, r0, c, 0), a);
+                                keep_32(kept_at<false>(p, r0, c, 1), b);
                             }
                             __builtin_amdgcn_sched_barrier(0);
                             store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, N16, h, wh);
@@ -1025,20 +994,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
             }
         } else {
             const int col0 = n0 + wc * CW, strip = tile_m * WM + wr;
-            // (FAST: 24 bits)
-            const Panel out_a(p.C, 2 * p.ldc, row0, p.M, RW), out_b(reinterpret_cast<unsigned short*>(p.C) + p.gu_half, 2 * p.ldc, row0, p.M, RW);
-            const Panel hi_a(p.gu, 2 * p.ldgu, row0, p.M, RW), hi_b(reinterpret_cast<unsigned short*>(p.gu) + p.gu_half, 2 * p.ldgu, row0, p.M, RW);
-            const Panel lo_a(p.gu_lo, p.ldgu, row0, p.M, RW), lo_b(p.gu_lo + p.gu_half, p.ldgu, row0, p.M, RW);
-            Raw24 ra[MI], rb[MI];
-            auto load = [&](int i, int c) {
-                load_24(hi_a, lo_a, i * 32, c, p.gu_half, ra[i], wh);
-                load_24(hi_b, lo_b, i * 32, c, p.gu_half, rb[i], wh);
-            };
+            const Panel out_a(p.C, 2 * p.ldc, row0, p.M, RW), out_b(reinterpret_cast<unsigned short*>(p.C) + p.half,      // (FAST)
+                        2 * p.ldc, row0, p.M, RW);
             auto gate = [&](auto act) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const int c = opaque(col0 + j * 32);
-                    if (c >= p.gu_half) continue;             // (uniform)
+                    if (c >= p.half) continue;             // (uniform)
                     float cs[32];
 #pragma unroll
                     for (int k = 0; k < 32; ++k) cs[k] = 0.f;
@@ -1059,7 +1021,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r) da[r >> 3][r & 7] = db[r >> 3][r & 7] = 0.f;
                         }
-                        clear_beyond(da, c, p.N, wh);         // zeros from N to gu_half: both halves are one operand of the next product
+                        clear_beyond(da, c, p.N, wh);         // zeros from N to half: both halves are one operand of the next product
                         clear_beyond(db, c, p.N, wh);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
@@ -1067,23 +1029,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             cs[16 + r] += db[r >> 3][r & 7];
                         }
                         if constexpr (FAST) {
-                            panel_bf16(out_a, i * 32, c, p.gu_half, da, wh);
-                            panel_bf16(out_b, i * 32, c, p.gu_half, db, wh);
+                            panel_bf16(out_a, i * 32, c, p.half, da, wh);
+                            panel_bf16(out_b, i * 32, c, p.half, db, wh);
                         } else {
-                            store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, p.gu_half, da, wh);
-                            store_split(reinterpret_cast<char*>(p.C) + split_at(p.gu_half, 0), p.ldc, r0, c, p.M, p.gu_half, db, wh);
+                            store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, p.half, da, wh);
+                            store_split(reinterpret_cast<char*>(p.C) + split_at(p.half, 0), p.ldc, r0, c, p.M, p.half, db, wh);
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     };
                     if constexpr (FAST) {
+                        Raw24 ra[MI], rb[MI];
 #pragma unroll
-                        for (int i = 0; i < MI; ++i) load(i, c);
+                        for (int i = 0; i < MI; ++i) {
+                            const int rl = min(opaque(row0 + i * 32), (p.M - 1) & ~31);      // (a block that exists)
+                            load_24(kept_at<true>(p, rl, c, 0), ra[i]);
+                            load_24(kept_at<true>(p, rl, c, 1), rb[i]);
+                        }
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int i = 0; i < MI; ++i) {
                             float a[2][8], b[2][8];
-                            unpack_24(ra[i], a, wh);
-                            unpack_24(rb[i], b, wh);
+                            unpack_24(ra[i], a);
+                            unpack_24(rb[i], b);
                             one(i, a, b);
                         }
                     } else {
@@ -1091,11 +1058,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                         for (int i = 0; i < MI; ++i) {
                             float a[2][8], b[2][8];
                             Raw32 ra, rb;
-                            const int rl = opaque(row0 + i * 32);
-                            load_f32(reinterpret_cast<const float*>(p.gu), p.ldgu, rl, c, p.M, p.gu_half, ra, wh);
-                            load_f32(reinterpret_cast<const float*>(p.gu) + p.gu_half, p.ldgu, rl, c, p.M, p.gu_half, rb, wh);
-                            unpack_f32(ra, a, wh);
-                            unpack_f32(rb, b, wh);
+                            const int rl = min(opaque(row0 + i * 32), (p.M - 1) & ~31);
+                            load_32(kept_at<false>(p, rl, c, 0), ra);
+                            load_32(kept_at<false>(p, rl, c, 1), rb);
+                            unpack_32(ra, a);
+                            unpack_32(rb, b);
                             one(i, a, b);
                         }
                     }

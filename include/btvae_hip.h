@@ -390,16 +390,15 @@ int btvae_dirichlet_sample(const float* gamma, const long long* rows, float* out
 /* n <= 4 operands in one launch, each described by ten numbers: src [rows, cols] (pointer), src_bf16, ld, dst (pointer), planes,
  * dst_ld, rows, cols, dst_cols, transpose.  dst = src (transpose: its transpose), zeros up to dst_cols columns (a multiple of 16). */
 int btvae_block_pack(const long long* jobs, int n, void* stream);
-/* H [M] = h, an operand (zeros up to a multiple of 16 columns); GU [M][ldgu] (null: not kept): x Wg^T + bg at column 0, x Wu^T + bu at column gu_half, fp32 with three
- * planes, else the upper two bytes of fp32 there and the third in GU_lo [M][ldgu]. */
+/* H [M] = h, an operand (zeros up to a multiple of 16 columns); kept (null: not): x Wg^T + bg and x Wu^T + bu for the backward pass, in the
+ * kernels' own order, btvae_gated_kept_bytes(M, F, planes) bytes (24 bits a value with one plane, 32 with three). */
+long long btvae_gated_kept_bytes(int M, int F, int planes);
 int btvae_gated_proj_fwd(const void* X, long long ldx, const void* Wg, const void* Wu, long long ldw, const void* bg, const void* bu,
-            int bias_bf16, void* H, long long ldh, void* GU, void* GU_lo, long long ldgu, int gu_half, int planes, int act, int M, int F,
-            int K, void* stream);
-/* dGU [M], an operand of 2 gu_half columns: da at column 0, db at column gu_half (zeros between F and gu_half) from dh = dY WdT^T;
- * colpart: null, or [btvae_gated_proj_strips(M)][2][F] column sums of da and db. */
-int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* GU, const void* GU_lo,
-            long long ldgu, int gu_half, void* dGU, long long ldd, float* colpart, int planes, int act, int M, int F, int N,
-            void* stream);
+            int bias_bf16, void* H, long long ldh, void* kept, int planes, int act, int M, int F, int K, void* stream);
+/* dGU [M], an operand of 2 half columns, half = F rounded up to 32: da at column 0, db at column half (zeros between F and half) from
+ * dh = dY WdT^T; colpart: null, or [btvae_gated_proj_strips(M)][2][F] column sums of da and db. */
+int btvae_gated_proj_bwd(const void* dY, long long lddy, const void* WdT, long long ldw, const void* kept, void* dGU, long long ldd,
+            float* colpart, int planes, int act, int M, int F, int N, void* stream);
 int btvae_gated_proj_strips(int M);
 /* C [M, N] = A B^T + bias; workspace (floats) of btvae_block_product_ws, 0: none. */
 long long btvae_block_product_ws(int M, int N, int K, int planes);

@@ -160,15 +160,14 @@ def test_c_entry_points_refuse():
     refused("btvae_block_pack", "four", None, 1)
     refused("btvae_block_pack", "four", (ctypes.c_longlong * 50)(), 5)
 
-    refused("btvae_gated_proj_fwd", "planes", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 2, 0, 4, 64, 64)
-    refused("btvae_gated_proj_fwd", "sizes", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 0, 4, 64, 60)
-    refused("btvae_gated_proj_fwd", "activation", a, 128, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 4, 4, 64, 64)
-    refused("btvae_gated_proj_fwd", "operand", a, 112, a, a, 128, None, None, 0, a, 128, None, None, 0, 0, 1, 0, 4, 64, 64)
-    refused("btvae_gated_proj_fwd", "layout of H", a, 128, a, a, 128, None, None, 0, a, 112, None, None, 0, 0, 1, 0, 4, 64, 64)
-    refused("btvae_gated_proj_fwd", "kept", a, 128, a, a, 128, None, None, 0, a, 128, a, None, 128, 64, 1, 0, 4, 64, 64)
-    refused("btvae_gated_proj_fwd", "kept", a, 128, a, a, 128, None, None, 0, a, 128, a, a, 128, 32, 1, 0, 4, 64, 64)
-    refused("btvae_gated_proj_bwd", "kept", a, 128, a, 128, None, None, 128, 64, a, 256, None, 1, 0, 4, 64, 64)
-    refused("btvae_gated_proj_bwd", "gradients", a, 128, a, 128, a, a, 128, 64, a, 128, None, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "planes", a, 128, a, a, 128, None, None, 0, a, 128, None, 2, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "sizes", a, 128, a, a, 128, None, None, 0, a, 128, None, 1, 0, 4, 64, 60)
+    refused("btvae_gated_proj_fwd", "activation", a, 128, a, a, 128, None, None, 0, a, 128, None, 1, 4, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "operand", a, 112, a, a, 128, None, None, 0, a, 128, None, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "layout of H", a, 128, a, a, 128, None, None, 0, a, 112, None, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_fwd", "kept", a, 128, a, a, 128, None, None, 0, a, 128, a + 8, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_bwd", "kept", a, 128, a, 128, None, a, 256, None, 1, 0, 4, 64, 64)
+    refused("btvae_gated_proj_bwd", "gradients", a, 128, a, 128, a, a, 128, None, 1, 0, 4, 64, 64)
     refused("btvae_block_product", "sizes", a, 128, a, 128, None, 0, a, 60, 0, None, 0, 1, 4, 64, 64)
     refused("btvae_block_product", "operand", a, 128, a + 4, 128, None, 0, a, 64, 0, None, 0, 1, 4, 64, 64)
     need = lib.btvae_block_product_ws(64, 64, 4096, 1)
