@@ -19,11 +19,11 @@
 // bytes past the end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns;
 // rows past the end repeat the last row and only reach outputs that are not stored.
 //   Measured (one card, 1.75 to 2.0 GHz under these loads, which is its power limit; a large library product in bf16 reaches 1394 TFLOP/s):
-//   bf16 65,536 x 4000 x 1000 490 us, 1070 TFLOP/s (128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of eight
-//   waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
-//   713 us, the 1.05 GB that it stores being 210 us of it; its backward 645 us, 1.3 GB loaded and stored; split 16,384 x
-//   4000 x 1000 680 us, 193 TFLOP/s of fp32 or 1156 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
-//   397 us, 1320 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 us, 1417 TFLOP/s.
+//   bf16 65,536 x 4000 x 1000 490 to 540 us, 970 to 1070 TFLOP/s (128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of
+//   eight waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
+//   645 us, 813 TFLOP/s and 1.03 GB stored; its backward 480 us, 0.8 GB loaded and 0.6 stored; split 16,384 x 4000 x 1000 690 us,
+//   190 TFLOP/s of fp32 or 1140 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
+//   400 us, 1310 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
 //   What they wait for: operands on their way through L2 and LDS at a clock that falls with what is moved; skewing the
 //   workgroups against each other, giving them priorities, or letting a tile's stores pass its successor's first stage changed nothing.
 //
@@ -1128,17 +1128,12 @@ __global__ __launch_bounds__(64 * WM * WN, MI * NJ == 16 ? 1 : 2) void gemm_cols
     const int wr = wid / WN, wc = wid % WN;
     const int lh = lane >> 5;
     const Where<false> wh(smem + RING + wid * Where<false>::LDS_B);
-    // Splits of the reduction first: all output tiles of one row range run together on one XCD and share its rows in L2.
-    const int T = pair.tiles, nz = (int)gridDim.z;
-    int zz, tile;
-    if ((nz & 7) == 0) {
-        const int L = (int)blockIdx.x + T * (int)blockIdx.z, xcd = L & 7, idx = L >> 3;
-        zz = xcd * (nz >> 3) + idx / T;
-        tile = idx % T;
-    } else {
-        zz = (int)blockIdx.z;
-        tile = (int)blockIdx.x;
-    }
+    // Each XCD (every eighth workgroup) gets a contiguous run of the tiles of one row range after another: neighbouring tiles share that range's
+    // rows in its L2 (measured, 65,536 rows of 4032 x 1000 in four ranges: 2.4 -> 0.8 GB read beyond it, 585 -> 575 us)
+    const int T = pair.tiles, total = T * (int)gridDim.z, L = (int)blockIdx.x + T * (int)blockIdx.z, xcd = L & 7, q = total >> 3, rem = total & 7;
+    const int item = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + (L >> 3);
+    const int zz = item / T;
+    int tile = item % T;
     const ColArgs& p = pair.a[tile >= pair.tiles0];
     if (tile >= pair.tiles0) tile -= pair.tiles0;
     const int tile_m = tile / p.tiles_n, tile_n = tile % p.tiles_n;
