@@ -429,7 +429,7 @@ template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, 
     out.put(b, c < cols ? o + 16 * out.ld : OUTSIDE);
 }
 // Kept projections: a block's bytes, and block (row0, col0) of a (0) or b (1); every store and load is 1 KiB in a row
-template <bool B24> constexpr int kept_bytes() { return B24 ? 3072 : 4096; }
+template <bool B24> constexpr int kept_bytes() { return (B24 ? 3 : 4) * 1024; }
 template <bool B24> __device__ __forceinline__ char* kept_at(const Args& p, int row0, int col0, int which) {
     return p.kept + (((long long)(row0 >> 5) * (p.half >> 5) + (col0 >> 5)) * 2 + which) * kept_bytes<B24>() + (threadIdx.x & 63) * 16;
 }
