@@ -103,6 +103,9 @@ _SIGS = {
     "btvae_gated_proj_fwd": [P, LL, P, P, LL, P, P, I, P, LL, P, I, I, I, I, I, P],
     "btvae_gated_proj_bwd": [P, LL, P, LL, P, P, LL, P, I, I, I, I, I, P],
     "btvae_block_product": [P, LL, P, LL, P, I, P, LL, I, P, LL, I, I, I, I, P],
+    "btvae_gated_unit_bytes": [P, I, P],
+    "btvae_gated_unit_fwd": [P, P, LL, I, P, LL, P, LL, P],
+    "btvae_gated_unit_bwd": [P, P, P, LL, P, LL, P],
     "btvae_block_wgrad": [P, LL, P, LL, P, LL, P, I, P, I, I, LL, I, I, I, I, I, I, P],
     "btvae_block_wgrad_pair": [P, P, LL, I, I, I, P],
     "btvae_block_colsum": [P, I, LL, P, LL, P, I, I, I, I, P],
@@ -140,6 +143,7 @@ _RET = {
     "btvae_gated_proj_strips": (c_int, [I]),
     "btvae_block_product_ws": (c_longlong, [I, I, I, I]),
     "btvae_gated_kept_bytes": (c_longlong, [I, I, I]),
+    "btvae_gated_unit_bwd_bytes": (c_longlong, [P, P]),
     "btvae_block_wgrad_ws": (c_longlong, [I, I, I, I]),
     "btvae_block_wgrad_pair_ws": (c_longlong, [c_int] * 6),
     "btvae_block_colsum_ws": (c_longlong, [I, I]),

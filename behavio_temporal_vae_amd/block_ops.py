@@ -105,8 +105,7 @@ def _refuse_capture(what):
 
 class _Operand:
     """A matrix as the products read it: bf16 (``planes`` 1), or float32 values as three bf16 pieces each, 96 bytes for every 16
-    columns (``planes`` 3); ``ld`` bytes to a row, rows on 16 bytes, ``width`` columns of which those beyond the matrix's own are zeros.  A
-    bf16 matrix that is laid out so already is used in place."""
+    columns (``planes`` 3); ``ld`` bytes to a row, rows on 16 bytes, ``width`` columns of which those beyond the matrix's own are zeros."""
     __slots__ = ("at", "ld", "width", "t")
 
     def __init__(self, at, ld, width, t=None):
@@ -116,92 +115,15 @@ class _Operand:
         return self.at
 
 
-def _operand_buffer(rows, ld, width, device) -> _Operand:
-    t = torch.empty(rows * ld, dtype=torch.uint8, device=device)
-    return _Operand(t.data_ptr(), ld, width, t)
-
-
-def _bytes(cols, planes):
-    return cols * (6 if planes == 3 else 2)
-
-
-def _row_bytes(cols, planes):
-    """Pitch of an operand of ``cols`` columns: whole groups of 32, bf16 rows on 128 bytes (rows on 64 of them cost a product of 65,536 x
-    2000 x 1000 391 us instead of 275)."""
-    return _bytes(_up(cols, 32 if planes == 3 else 64), planes)
-
-
-def _fits(t):
-    return t.dtype == torch.bfloat16 and t.shape[1] % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0
-
-
-class _Packer:
-    """Matrices to be laid out as operands: noted one by one, written by one launch into one buffer."""
-
-    def __init__(self, planes, device):
-        self.planes, self.device, self.todo, self.bytes = planes, device, [], 0
-
-    def add(self, t, apart=False) -> _Operand:
-        """``apart``: in a buffer of its own, for what outlives the others."""
-        rows, cols = t.shape
-        ld = _row_bytes(cols, self.planes)
-        op = _operand_buffer(rows, ld, _up(cols, 8), self.device) if apart else _Operand(self.bytes, ld, _up(cols, 8))
-        self._job(t, op, 0, 0 if apart else rows * ld, _up(cols, 32), 0)
-        return op
-
-    def add_transposed(self, *ts, width) -> _Operand:
-        """[t0^T t1^T ..], ``width`` columns to each."""
-        cols, piece = ts[0].shape[1], _bytes(width, self.planes)
-        ld = _up(piece * len(ts), 128 if self.planes == 1 else 96)
-        op = _Operand(self.bytes, ld, width * len(ts))
-        for i, t in enumerate(ts):
-            self._job(t, op, i * piece, cols * ld if i == 0 else 0, width, 1)
-        return op
-
-    def _job(self, t, op, offset, size, dst_cols, transpose):
-        self.todo.append((op, offset, t, dst_cols, transpose))
-        self.bytes += _up(size, 256)
-
-    def run(self):
-        if not self.todo:
-            return
-        buf = torch.empty(self.bytes, dtype=torch.uint8, device=self.device)
-        base, jobs = buf.data_ptr(), []
-        for op, offset, t, dst_cols, transpose in self.todo:
-            if op.t is None:
-                op.at, op.t = base + op.at, buf
-            jobs += (t.data_ptr(), t.dtype == torch.bfloat16, _pitch(t), op.at + offset, self.planes, op.ld, *t.shape, dst_cols, transpose)
-        nv.call("btvae_block_pack", (ctypes.c_longlong * len(jobs))(*jobs), len(self.todo))
-
-
-REPACK_READS = 2048        # rows or columns of a product from which a bf16 matrix with rows off 64-byte boundaries is copied first
-
-
-def _in_place(t, planes, reads):
-    """May a product read ``t`` where it is?  Rows that do not start on 64 bytes cost the copies to LDS more requests, so a matrix that
-    is read against ``reads`` others is laid out anew from ``REPACK_READS`` on (measured, 65,536 x 1000 times 1000 x N, in place
-    against the copy and the product: N 512 80 and 118 us, 1024 155 and 178, 2048 346 and 316, 4096 653 and 596; never copying
-    costs a gated unit's training pass of 65,536 x 1000 x 2000 3 %)."""
-    return planes == 1 and _fits(t) and (reads < REPACK_READS or (2 * _pitch(t) % 64 == 0 and t.data_ptr() % 64 == 0))
-
-
-def _operand(t, planes, reads, packer=None, apart=False) -> _Operand:
-    """``t`` where it is, or laid out by ``packer`` (its ``run`` has to come before the operand is used; absent: at once)."""
-    if _in_place(t, planes, reads):
-        return _Operand(t.data_ptr(), 2 * _pitch(t), t.shape[1], t)
-    if packer is not None:
-        return packer.add(t, apart)
-    packer = _Packer(planes, t.device)
-    op = packer.add(t)
-    packer.run()
-    return op
-
-
-def _operand_pair(a, b, planes, reads, packer):
-    """Two matrices of one shape with a common pitch."""
-    if _in_place(a, planes, reads) and _in_place(b, planes, reads) and _pitch(a) == _pitch(b):
-        return _operand(a, planes, reads), _operand(b, planes, reads)
-    return packer.add(a), packer.add(b)
+def _operand(t, planes, reads=0) -> _Operand:
+    """``t`` laid out as an operand, or where it is: a bf16 matrix with whole 16-byte pieces that is read against few others."""
+    rows, cols = t.shape
+    if planes == 1 and t.dtype == torch.bfloat16 and cols % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0 and reads < 2048:
+        return _Operand(t.data_ptr(), 2 * _pitch(t), cols, t)
+    ld = _up(cols, 32) * 6 if planes == 3 else _up(cols, 64) * 2
+    buf = torch.empty(rows * ld, dtype=torch.uint8, device=t.device)
+    nv.call("btvae_block_pack", (ctypes.c_longlong * 10)(t.data_ptr(), t.dtype == torch.bfloat16, _pitch(t), buf.data_ptr(), planes, ld, rows, cols, _up(cols, 32), 0), 1)
+    return _Operand(buf.data_ptr(), ld, _up(cols, 8), buf)
 
 
 def _workspace(floats, device):
@@ -216,18 +138,29 @@ def _product(a: _Operand, b: _Operand, bias, out, planes, M, N, K):
 
 
 # ------------------------------------------------------------------------------------------------ gated feed-forward unit
-class GatedTape:
-    """What the backward pass of one ``gated_feed_forward`` needs: the inputs, both projections, h."""
+_Numbers = {n: ctypes.c_longlong * n for n in (3, 15, 20)}
 
-    def __init__(self, x, weights, biases, act, planes, X, H, kept):
-        self.x, self.weights, self.biases, self.act, self.planes = x, weights, biases, act, planes
-        self.X, self.H, self.kept = X, H, kept
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _weight_numbers(weights):
+    g, u, d = weights
+    return (g.data_ptr(), _pitch(g), u.data_ptr(), _pitch(u), d.data_ptr(), _pitch(d), g.dtype == torch.bfloat16)
+
+
+class GatedTape:
+    """What the backward pass of one ``gated_feed_forward`` needs: the inputs, and (``store``) x and h as operands and both projections."""
+
+    def __init__(self, x, weights, biases, unit, store, in_place):
+        self.x, self.weights, self.biases, self.unit, self.store, self.in_place = x, weights, biases, unit, store, in_place
 
     def _check_outs(self, outs):
         if len(outs) != 6:
             raise ValueError(f"outs must be six tensors, got {len(outs)}")
         names = ("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
-        for o, t, what in zip(outs, self.weights + self.biases, names):
+        for o, t, what in zip(outs, (*self.weights, *self.biases), names):
             if t is None or o is None:
                 if o is not None or what[0] == "w":
                     raise ValueError(f"outs: {what} " + ("is absent" if t is None else "is missing"))
@@ -243,46 +176,36 @@ class GatedTape:
         """Gradients (x, w_gate, w_up, w_down, b_gate, b_up, b_down) for the gradient ``dy`` of the result; entries that are
         not wanted, or belong to an absent bias, are None.  ``outs``: six tensors (float32 or bfloat16, contiguous, None for
         biases that are absent or not wanted) that the weights' and biases' gradients are written to, or added to with ``accumulate``."""
-        x, (w_gate, w_up, w_down), planes = self.x, self.weights, self.planes
-        dev, (M, K), (F, _), N = x.device, x.shape, w_gate.shape, w_down.shape[0]
+        x, weights = self.x, self.weights
+        dev, (M, K), N = x.device, x.shape, weights[2].shape[0]
         nv.ensure_device(dev)
         dy = _rows(_tensor(dy, "the gradient"), "the gradient")
         _matrix(dy, "the gradient", (M, N), dy.dtype, dev)
-        lib, half = nv.lib(), _up(F, 32)
-        if outs is None:
-            outs = [torch.empty_like(w, memory_format=torch.contiguous_format) for w in self.weights] + \
-                   [None if b is None else torch.empty_like(b, memory_format=torch.contiguous_format) for b in self.biases]
-            accumulate = False
-        else:
+        if outs is not None:
             self._check_outs(outs)
-        dwg, dwu, dwd, dbg, dbu, dbd = outs
-        acc = int(accumulate)
-        packer = _Packer(planes, dev)
-        DY, WdT = _operand(dy, planes, 2 * F, packer), packer.add_transposed(w_down, width=_up(N, 32))
-        WT = packer.add_transposed(w_gate, w_up, width=half) if need_input else None
-        packer.run()
-        dGU = _operand_buffer(M, _bytes(2 * half, planes), 2 * half, dev)
-        want_bias = need_weights and (dbg is not None or dbu is not None)
-        strips = lib.btvae_gated_proj_strips(M) if M else 0
-        colpart = _workspace(strips * 2 * F, dev) if want_bias else None
-        nv.call("btvae_gated_proj_bwd", DY.ptr(), DY.ld, WdT.ptr(), WdT.ld, _p(self.kept), dGU.ptr(), dGU.ld, _p(colpart), planes, self.act, M, F, DY.width)
-        dx = None
-        if need_input:
-            dx = torch.empty(M, K, dtype=x.dtype, device=dev)
-            _product(dGU, WT, None, dx, planes, M, K, 2 * half)
+        elif need_weights:
+            accumulate = False
+            outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (*weights, *self.biases)]
         if not need_weights:
-            return (dx,) + (None,) * 6
-        ws = _workspace(lib.btvae_block_wgrad_pair_ws(2 * half, K, N, F, M, planes), dev)
-        jobs = (dGU.ptr(), dGU.ld, self.X.ptr(), self.X.ld, _p(dwg), F, _p(dwu), half, F, K, dwg.dtype == torch.bfloat16, 2 * half, K,
-                DY.ptr(), DY.ld, self.H.ptr(), self.H.ld, _p(dwd), N, 0, 0, 0, F, dwd.dtype == torch.bfloat16, N, F)
-        nv.call("btvae_block_wgrad_pair", (ctypes.c_longlong * 26)(*jobs), _p(ws), ws.numel(), planes, M, acc)
-        if want_bias:
-            first, second = (dbg, dbu) if dbg is not None else (torch.empty_like(dbu), dbu)
-            nv.call("btvae_block_strip_sums", _p(colpart), strips, F, _p(first), _p(second), int(first.dtype == torch.bfloat16), acc)
-        if dbd is not None:
-            cs = _workspace(lib.btvae_block_colsum_ws(M, N), dev)
-            nv.call("btvae_block_colsum", _p(dy), int(dy.dtype == torch.bfloat16), max(_pitch(dy), N), _p(cs), cs.numel(), _p(dbd), int(dbd.dtype == torch.bfloat16), acc, M, N)
-        return (dx, dwg, dwu, dwd, dbg, dbu, dbd)
+            outs = (None,) * 6
+        dx = torch.empty(M, K, dtype=x.dtype, device=dev) if need_input else None
+        types = [o is not None and o.dtype == torch.bfloat16 for o in outs]
+        grads = _Numbers[15](dy.data_ptr(), dy.dtype == torch.bfloat16, max(_pitch(dy), N), _at(dx), *[_at(o) for o in outs],
+                             types[0], types[2], types[3] or types[4], types[5], accumulate)
+        unit = _Numbers[20](*self.unit)
+        unit[7:14] = _weight_numbers(weights)
+        if self.in_place and (x.data_ptr(), _pitch(x)) != (unit[0], unit[2]):
+            # not the tensor of the forward pass but what a hook on saved tensors made of it: rows that can be read in place again
+            moved = torch.empty(M, _up(K, 64), dtype=x.dtype, device=dev)[:, :K]
+            moved.copy_(x)
+            unit[0], unit[2] = moved.data_ptr(), _pitch(moved)
+        lib = nv.lib()
+        size = lib.btvae_gated_unit_bwd_bytes(unit, grads)
+        if size < 0:
+            raise RuntimeError(f"btvae_gated_unit_bwd_bytes: {nv.last_error()}")
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        nv.call("btvae_gated_unit_bwd", unit, grads, self.store.data_ptr(), self.store.numel(), scratch.data_ptr(), size)
+        return (dx, *outs)
 
 
 def _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
@@ -309,22 +232,17 @@ def _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
 
 def _ffn_forward(x2, weights, biases, act, planes, out_dtype, keep):
     """(y [M, N], tape or None): the tile kernels."""
-    w_gate, w_up, w_down = weights
-    b_gate, b_up, b_down = biases
-    dev, (M, K), F, N = x2.device, x2.shape, w_gate.shape[0], w_down.shape[0]
-    packer = _Packer(planes, dev)
-    X = _operand(x2, planes, 2 * F, packer, apart=keep)
-    Wg, Wu = _operand_pair(w_gate, w_up, planes, M, packer)
-    Wd = _operand(w_down, planes, M, packer)
-    packer.run()
-    H = _operand_buffer(M, _row_bytes(F, planes), _up(F, 8), dev)
-    kept = torch.empty(nv.lib().btvae_gated_kept_bytes(M, F, planes), dtype=torch.uint8, device=dev) if keep else None
-    bias16 = int(any(b is not None and b.dtype == torch.bfloat16 for b in (b_gate, b_up)))
-    nv.call("btvae_gated_proj_fwd", X.ptr(), X.ld, Wg.ptr(), Wu.ptr(), Wg.ld, _p(b_gate), _p(b_up), bias16,
-            H.ptr(), H.ld, _p(kept), planes, act, M, F, X.width)
+    dev, (M, K), (F, _), N = x2.device, x2.shape, weights[0].shape, weights[2].shape[0]
+    bias16 = any(b is not None and b.dtype == torch.bfloat16 for b in biases)
+    unit = _Numbers[20](x2.data_ptr(), x2.dtype == torch.bfloat16, _pitch(x2), M, K, F, N, *_weight_numbers(weights), *[_at(b) for b in biases], bias16, planes, act)
+    sizes = _Numbers[3]()
+    if nv.lib().btvae_gated_unit_bytes(unit, keep, sizes):
+        raise RuntimeError(f"btvae_gated_unit_bytes: {nv.last_error()}")
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
-    _product(H, Wd, b_down, y, planes, M, N, Wd.width)
-    return y, GatedTape(x2, weights, biases, act, planes, X, H, kept) if keep else None
+    store = torch.empty(sizes[0], dtype=torch.uint8, device=dev) if keep else None
+    scratch = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+    nv.call("btvae_gated_unit_fwd", unit, y.data_ptr(), N, out_dtype == torch.bfloat16, _p(store), sizes[0], scratch.data_ptr(), sizes[1])
+    return y, GatedTape(x2, weights, biases, unit, store, sizes[2]) if keep else None
 
 
 def _ffn_few(x2, weights, biases, act):
@@ -345,19 +263,17 @@ class _GatedNode(torch.autograd.Function):
     def forward(ctx, act, x2, w_gate, w_up, w_down, b_gate, b_up, b_down):
         planes = 3 if x2.dtype == torch.float32 else 1
         y, tape = _ffn_forward(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], act, planes, x2.dtype, True)
-        ctx.save_for_backward(x2, w_gate, w_up, w_down, b_gate, b_up, b_down)
-        ctx.tape = tape
-        tape.x = tape.weights = tape.biases = None          # held by the saved tensors, which notice changes in place
+        ctx.save_for_backward(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, tape.store)
+        ctx.unit, ctx.in_place = tape.unit, tape.in_place
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         _refuse_capture("gated_feed_forward")
-        x2, w_gate, w_up, w_down, b_gate, b_up, b_down = ctx.saved_tensors
+        x2, w_gate, w_up, w_down, b_gate, b_up, b_down, store = ctx.saved_tensors
         need = ctx.needs_input_grad
-        t = ctx.tape
-        tape = GatedTape(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], t.act, t.planes, t.X, t.H, t.kept)
+        tape = GatedTape(x2, (w_gate, w_up, w_down), (b_gate, b_up, b_down), ctx.unit, store, ctx.in_place)
         return (None, *tape.backward(dy, need_input=need[1], need_weights=any(need[2:])))
 
 

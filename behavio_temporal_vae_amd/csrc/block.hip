@@ -516,7 +516,7 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
 // Splits of a reduction of `stages` stages over fewer tiles than compute units: as many as fill the chip about once, each at least
 // 12 stages long (the ring's fill and the slab's write and read cost about that much).
 inline int row_splits(int T, int stages, int unit) {
-    if (T >= CHIP * 3 / 4) return 1;
+    if (T <= 0 || T >= CHIP * 3 / 4) return 1;
     int z = std::min(CHIP / T, stages / std::max(12, unit));
     return std::max(1, std::min(z, 32));
 }
@@ -524,6 +524,7 @@ inline int row_splits(int T, int stages, int unit) {
 struct ProductPlan { int z, kz; };
 // EP_LINEAR: splits of the reduction, each a multiple of `unit` stages; tiles of 128 x `tn`
 static ProductPlan plan_product(int M, int N, int tn, int stages, int unit) {
+    if (M <= 0 || N <= 0 || stages <= 0) return {1, std::max(1, stages)};
     ProductPlan r;
     r.kz = tiles(tiles(stages, row_splits(tiles(M, 128) * tiles(N, tn), stages, unit)), unit) * unit;
     r.z = tiles(stages, r.kz);
@@ -547,7 +548,7 @@ static ColPlan plan_cols(int M, int N, int R, int beside = 0) {
     // 256 x 256 tiles from where their splits fill the chip: see gemm_cols
     r.big = !beside && tiles(M, 256) * tiles(N, 256) * std::max(1, R / 1024) >= CHIP;
     const int t = r.big ? 256 : 128;
-    const int T = tiles(M, t) * tiles(N, t) + beside;
+    const int T = std::max(1, tiles(M, t) * tiles(N, t) + beside);
     // fill the chip; a split has at least 256 rows, and multiples of eight splits keep one row range on one XCD
     const int fill = r.big ? CHIP : 2 * CHIP;
     int z = std::max(1, std::min((T >= fill ? 1 : fill / T), tiles(R, 256)));
@@ -785,6 +786,187 @@ BTVAE_API int btvae_block_strip_sums(const float* part, int strips, int N, void*
     BTVAE_REQUIRE(strips >= 0 && N > 0 && out0, "block_strip_sums: bad sizes");
     hipLaunchKernelGGL(bk::strip_sums, dim3((unsigned)bk::tiles(2 * N, 32)), dim3(256), 0, BLK_STREAM(stream), part, strips, N, 2, out0, out1, out_bf16, accumulate);
     return check_launch("block_strip_sums");
+}
+
+// ---- the whole unit in one call: operands laid out, projections, products, in memory that the caller gives ----
+// (a unit of a few hundred rows is its host's work: six calls and eight allocations from Python cost more than its kernels)
+namespace btvae_block {
+struct Unit {
+    const void* x; int x16; long long ldx; int M, K, F, N;
+    const void *wg, *wu, *wd; long long ldg, ldu, ldd; int w16;
+    const void *bg, *bu, *bd; int b16, planes, act;
+};
+// Memory handed out piece by piece; without a base only counted
+struct Pieces {
+    char* base; long long used;
+    char* take(long long n) {
+        char* at = base ? base + used : nullptr;
+        used += (n + 255) / 256 * 256;
+        return at;
+    }
+};
+struct Operand { const void* at; long long ld; int width; bool pack; };
+// Rows or columns of a product from which a bf16 matrix whose rows do not start on 64 bytes is laid out anew: such rows cost the copies to LDS more
+// requests (measured, 65,536 x 1000 times 1000 x N, in place against the copy and the product: N 512 80 and 118 us, 1024 155
+// and 178, 2048 346 and 316, 4096 653 and 596; never copying costs a gated unit's training pass of 65,536 x 1000 x 2000 3 %)
+constexpr long long REPACK_READS = 2048;
+static bool in_place(const void* t, int t16, long long ld, int cols, int planes, long long reads) {
+    if (planes != 1 || !t16 || cols % 8 || ld % 8 || !al16(t)) return false;
+    return reads < REPACK_READS || (2 * ld % 64 == 0 && ((uintptr_t)t & 63) == 0);
+}
+static long long bytes_of(long long cols, int planes) { return cols * (planes == 3 ? 6 : 2); }
+// Pitch of an operand: whole groups of 32 columns, bf16 rows on 128 bytes (h with rows on 64 of them cost the product of 65,536 x 2000 x 1000 391 us
+// instead of 330)
+static long long row_pitch(int cols, int planes) { return planes == 3 ? bytes_of(tiles(cols, 32) * 32LL, 3) : bytes_of(tiles(cols, 64) * 64LL, 1); }
+static Operand operand(const void* t, int t16, long long ld, int rows, int cols, int planes, bool as_is, Pieces& home) {
+    if (as_is) return {t, 2 * ld, cols, false};
+    const long long pitch = row_pitch(cols, planes);
+    return {home.take(rows * pitch), pitch, tiles(cols, 8) * 8, true};
+}
+// One matrix to be laid out (transpose: its transpose, behind `offset` bytes of each row)
+static void add_job(long long* jobs, int& n, const void* t, int t16, long long ld, const void* at, long long pitch, int planes, int rows, int cols, int dst_cols, int transpose) {
+    long long* j = jobs + 10 * n++;
+    j[0] = (long long)t; j[1] = t16; j[2] = ld; j[3] = (long long)at; j[4] = planes; j[5] = pitch; j[6] = rows; j[7] = cols; j[8] = dst_cols; j[9] = transpose;
+}
+// What the backward pass reads: x as an operand, h, both projections.  The same order in both passes.
+struct Kept { Operand X; char* H; long long ldh; char* kept; };
+static Kept lay_out(const Unit& u, bool keep, Pieces& home) {
+    Kept k;
+    k.X = operand(u.x, u.x16, u.ldx, u.M, u.K, u.planes, in_place(u.x, u.x16, u.ldx, u.K, u.planes, 2LL * u.F), home);
+    k.ldh = row_pitch(u.F, u.planes);
+    k.H = home.take(u.M * k.ldh);
+    k.kept = keep ? home.take(btvae_gated_kept_bytes(u.M, u.F, u.planes)) : nullptr;
+    return k;
+}
+struct ForwardPlan { Kept k; Operand Wg, Wu, Wd; float* ws; long long ws_floats; };
+static ForwardPlan plan_forward(const Unit& u, bool keep, Pieces& store, Pieces& scratch) {
+    ForwardPlan p;
+    p.k = lay_out(u, keep, keep ? store : scratch);
+    const bool pair = u.ldg == u.ldu && in_place(u.wg, u.w16, u.ldg, u.K, u.planes, u.M) && in_place(u.wu, u.w16, u.ldu, u.K, u.planes, u.M);
+    p.Wg = operand(u.wg, u.w16, u.ldg, u.F, u.K, u.planes, pair, scratch);
+    p.Wu = operand(u.wu, u.w16, u.ldu, u.F, u.K, u.planes, pair, scratch);
+    p.Wd = operand(u.wd, u.w16, u.ldd, u.N, u.F, u.planes, in_place(u.wd, u.w16, u.ldd, u.F, u.planes, u.M), scratch);
+    p.ws_floats = btvae_block_product_ws(u.M, u.N, p.Wd.width, u.planes);
+    p.ws = (float*)scratch.take(4 * p.ws_floats);
+    return p;
+}
+// b: dy, dy_bf16, lddy, dx, dwg, dwu, dwd, dbg, dbu, dbd, their types (w_gate and w_up, w_down, b_gate and b_up, b_down: bf16), accumulate
+struct BackwardPlan {
+    Operand DY, WdT, WT;
+    char* dGU; long long ldd; int half;
+    float *colpart, *ws, *other;
+    long long dx_floats, w_floats, c_floats;
+};
+static BackwardPlan plan_backward(const Unit& u, const long long* b, Pieces& scratch) {
+    BackwardPlan p;
+    p.half = tiles(u.F, 32) * 32;
+    const int n32 = tiles(u.N, 32) * 32, unit = u.planes == 3 ? 96 : 128;
+    const auto up = [&](long long n) { return (n + unit - 1) / unit * unit; };
+    p.DY = operand((const void*)b[0], (int)b[1], b[2], u.M, u.N, u.planes, in_place((const void*)b[0], (int)b[1], b[2], u.N, u.planes, 2LL * u.F), scratch);
+    p.WdT = {nullptr, up(bytes_of(n32, u.planes)), n32, true};
+    p.WdT.at = scratch.take(u.F * p.WdT.ld);
+    p.WT = {nullptr, up(bytes_of(2LL * p.half, u.planes)), 2 * p.half, true};
+    p.WT.at = b[3] ? scratch.take(u.K * p.WT.ld) : nullptr;
+    p.ldd = bytes_of(2LL * p.half, u.planes);
+    p.dGU = scratch.take(u.M * p.ldd);
+    const bool weights = b[4] != 0;
+    p.colpart = weights && (b[7] || b[8]) ? (float*)scratch.take(4LL * btvae_gated_proj_strips(u.M) * 2 * u.F) : nullptr;
+    p.other = weights && !b[7] && b[8] ? (float*)scratch.take(4LL * u.F) : nullptr;      // (sums that nobody wants)
+    // one after the other, so one place
+    p.dx_floats = b[3] ? btvae_block_product_ws(u.M, u.K, 2 * p.half, u.planes) : 0;
+    p.w_floats = weights ? btvae_block_wgrad_pair_ws(2 * p.half, u.K, u.N, u.F, u.M, u.planes) : 0;
+    p.c_floats = weights && b[9] ? btvae_block_colsum_ws(u.M, u.N) : 0;
+    p.ws = (float*)scratch.take(4 * std::max({p.dx_floats, p.w_floats, p.c_floats}));
+    return p;
+}
+}  // namespace btvae_block
+
+// a: x, x_bf16, ldx, M, K, F, N, wg, ldg, wu, ldu, wd, ldd, weights bf16, bg, bu, bd, biases bf16, planes, act
+static int unit_of(const long long* a, bk::Unit& u) {
+    BTVAE_REQUIRE(a, "gated_unit: null description");
+    const long long big = 1LL << 30;
+    BTVAE_REQUIRE(a[3] >= 0 && a[3] < 2 * big && a[4] > 0 && a[4] < big && a[5] > 0 && a[5] < big && a[6] > 0 && a[6] < big, "gated_unit: bad sizes (M %lld, K %lld, F %lld, N %lld)", a[3], a[4], a[5], a[6]);
+    BTVAE_REQUIRE(a[2] >= a[4] && a[8] >= a[4] && a[10] >= a[4] && a[12] >= a[5], "gated_unit: rows overlap");
+    BTVAE_REQUIRE(a[18] == 1 || a[18] == 3, "gated_unit: planes must be 1 or 3");
+    BTVAE_REQUIRE(a[18] == 1 || (!a[1] && !a[13]), "gated_unit: three planes are for fp32 matrices");
+    BTVAE_REQUIRE(a[19] >= 0 && a[19] <= 3, "gated_unit: unknown activation %lld", a[19]);
+    BTVAE_REQUIRE((a[0] || a[3] == 0) && a[7] && a[9] && a[11], "gated_unit: null matrix");
+    u = {(const void*)a[0], a[1] != 0, a[2], (int)a[3], (int)a[4], (int)a[5], (int)a[6], (const void*)a[7], (const void*)a[9], (const void*)a[11], a[8], a[10], a[12], a[13] != 0,
+         (const void*)a[14], (const void*)a[15], (const void*)a[16], a[17] != 0, (int)a[18], (int)a[19]};
+    return 0;
+}
+// bytes[0]: what the backward pass needs kept (0 without `keep`), bytes[1]: scratch of the forward pass, bytes[2]: 1 if x is read where it is
+BTVAE_API int btvae_gated_unit_bytes(const long long* unit, int keep, long long* bytes) {
+    bk::Unit u;
+    if (int rc = unit_of(unit, u)) return rc;
+    bk::Pieces store = {nullptr, 0}, scratch = {nullptr, 0};
+    const bk::ForwardPlan p = bk::plan_forward(u, keep != 0, store, scratch);
+    bytes[0] = store.used; bytes[1] = scratch.used; bytes[2] = !p.k.X.pack;
+    return 0;
+}
+BTVAE_API int btvae_gated_unit_fwd(const long long* unit, void* y, long long ldy, int y_bf16, void* store, long long store_bytes, void* scratch, long long scratch_bytes, void* stream) {
+    bk::Unit u;
+    if (int rc = unit_of(unit, u)) return rc;
+    if (u.M == 0) return 0;
+    bk::Pieces kept = {(char*)store, 0}, spare = {(char*)scratch, 0};
+    const bk::ForwardPlan p = bk::plan_forward(u, store != nullptr, kept, spare);
+    BTVAE_REQUIRE(kept.used <= store_bytes && spare.used <= scratch_bytes && (scratch || spare.used == 0), "gated_unit: workspace too small");
+    long long jobs[40];
+    int n = 0;
+    const auto pack = [&](const bk::Operand& o, const void* t, int t16, long long ld, int rows, int cols) {
+        if (o.pack) bk::add_job(jobs, n, t, t16, ld, o.at, o.ld, u.planes, rows, cols, bk::tiles(cols, 32) * 32, 0);
+    };
+    pack(p.k.X, u.x, u.x16, u.ldx, u.M, u.K);
+    pack(p.Wg, u.wg, u.w16, u.ldg, u.F, u.K);
+    pack(p.Wu, u.wu, u.w16, u.ldu, u.F, u.K);
+    pack(p.Wd, u.wd, u.w16, u.ldd, u.N, u.F);
+    if (int rc = btvae_block_pack(jobs, n, stream)) return rc;
+    if (int rc = btvae_gated_proj_fwd(p.k.X.at, p.k.X.ld, p.Wg.at, p.Wu.at, p.Wg.ld, u.bg, u.bu, u.b16, p.k.H, p.k.ldh, p.k.kept, u.planes, u.act, u.M, u.F, p.k.X.width, stream)) return rc;
+    return btvae_block_product(p.k.H, p.k.ldh, p.Wd.at, p.Wd.ld, u.bd, u.b16, y, ldy, y_bf16, p.ws, p.ws_floats, u.planes, u.M, u.N, p.Wd.width, stream);
+}
+static int check_back(const bk::Unit& u, const long long* b) {
+    BTVAE_REQUIRE(b && (b[0] || u.M == 0) && b[2] >= u.N, "gated_unit: bad gradient of the result");
+    BTVAE_REQUIRE((b[4] != 0) == (b[5] != 0) && (b[4] != 0) == (b[6] != 0), "gated_unit: gradients of all weights or of none");
+    return 0;
+}
+BTVAE_API long long btvae_gated_unit_bwd_bytes(const long long* unit, const long long* grads) {
+    bk::Unit u;
+    if (unit_of(unit, u) || check_back(u, grads)) return -1;
+    bk::Pieces scratch = {nullptr, 0};
+    bk::plan_backward(u, grads, scratch);
+    return scratch.used;
+}
+BTVAE_API int btvae_gated_unit_bwd(const long long* unit, const long long* grads, const void* store, long long store_bytes, void* scratch, long long scratch_bytes, void* stream) {
+    bk::Unit u;
+    if (int rc = unit_of(unit, u)) return rc;
+    if (int rc = check_back(u, grads)) return rc;
+    const long long* b = grads;
+    bk::Pieces kept = {(char*)const_cast<void*>(store), 0}, spare = {(char*)scratch, 0};
+    const bk::Kept k = bk::lay_out(u, true, kept);
+    const bk::BackwardPlan p = bk::plan_backward(u, b, spare);
+    BTVAE_REQUIRE((store || u.M == 0) && kept.used <= store_bytes && scratch && spare.used <= scratch_bytes, "gated_unit: workspace too small");
+    long long jobs[40];
+    int n = 0;
+    if (p.DY.pack) bk::add_job(jobs, n, (const void*)b[0], (int)b[1], b[2], p.DY.at, p.DY.ld, u.planes, u.M, u.N, bk::tiles(u.N, 32) * 32, 0);
+    bk::add_job(jobs, n, u.wd, u.w16, u.ldd, p.WdT.at, p.WdT.ld, u.planes, u.N, u.F, p.WdT.width, 1);
+    if (b[3]) {
+        bk::add_job(jobs, n, u.wg, u.w16, u.ldg, p.WT.at, p.WT.ld, u.planes, u.F, u.K, p.half, 1);
+        bk::add_job(jobs, n, u.wu, u.w16, u.ldu, (const char*)p.WT.at + bk::bytes_of(p.half, u.planes), p.WT.ld, u.planes, u.F, u.K, p.half, 1);
+    }
+    if (int rc = btvae_block_pack(jobs, n, stream)) return rc;
+    if (int rc = btvae_gated_proj_bwd(p.DY.at, p.DY.ld, p.WdT.at, p.WdT.ld, k.kept, p.dGU, p.ldd, p.colpart, u.planes, u.act, u.M, u.F, p.DY.width, stream)) return rc;
+    if (b[3])
+        if (int rc = btvae_block_product(p.dGU, p.ldd, p.WT.at, p.WT.ld, nullptr, 0, (void*)b[3], u.K, u.x16, p.ws, p.dx_floats, u.planes, u.M, u.K, 2 * p.half, stream)) return rc;
+    if (!b[4]) return 0;
+    const int acc = b[14] != 0;
+    const long long w[26] = {(long long)p.dGU, p.ldd, (long long)k.X.at, k.X.ld, b[4], u.F, b[5], p.half, u.F, u.K, b[10], 2 * p.half, u.K,
+                             (long long)p.DY.at, p.DY.ld, (long long)k.H, k.ldh, b[6], u.N, 0, 0, 0, u.F, b[11], u.N, u.F};
+    if (int rc = btvae_block_wgrad_pair(w, p.ws, p.w_floats, u.planes, u.M, acc, stream)) return rc;
+    if (p.colpart)
+        if (int rc = btvae_block_strip_sums(p.colpart, u.M ? btvae_gated_proj_strips(u.M) : 0, u.F, b[7] ? (void*)b[7] : p.other, (void*)b[8], (int)b[12], acc, stream)) return rc;
+    if (b[9])
+        if (int rc = btvae_block_colsum((const void*)b[0], (int)b[1], std::max<long long>(b[2], u.N), p.ws, p.c_floats, (void*)b[9], (int)b[13], acc, u.M, u.N, stream)) return rc;
+    return 0;
 }
 
 // ---- few rows ----

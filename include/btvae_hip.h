@@ -418,6 +418,18 @@ int btvae_block_colsum(const void* src, int src_bf16, long long ld, float* ws, l
             int accumulate, int R, int N, void* stream);
 /* out0 / out1 [n] (+)= sums over strips of part[strip][0 / 1][n]. */
 int btvae_block_strip_sums(const float* part, int strips, int N, void* out0, void* out1, int out_bf16, int accumulate, void* stream);
+/* The whole unit y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd in one call.  unit: x, x_bf16, ldx, M, K, F, N, wg, ldg, wu, ldu, wd,
+ * ldd, weights bf16, bg, bu, bd, biases bf16, planes, act (pointers and sizes as numbers).  btvae_gated_unit_bytes: bytes[0] of `store`, which
+ * the backward pass reads (null: nothing is kept), bytes[1] of scratch, bytes[2] 1 if x itself is read (else store holds it; the backward pass
+ * wants the same x in the description all the same).  The backward pass reads x or store, and the weights.  grads:
+ * dy, dy_bf16, lddy, dx (of x's type, dense; null: not wanted), dwg, dwu, dwd (all or none), dbg, dbu, dbd (null: not wanted), bf16 flags of (dwg, dwu), dwd,
+ * (dbg, dbu), dbd, accumulate; its scratch has btvae_gated_unit_bwd_bytes (-1: refused). */
+int btvae_gated_unit_bytes(const long long* unit, int keep, long long* bytes);
+int btvae_gated_unit_fwd(const long long* unit, void* y, long long ldy, int y_bf16, void* store, long long store_bytes, void* scratch,
+            long long scratch_bytes, void* stream);
+long long btvae_gated_unit_bwd_bytes(const long long* unit, const long long* grads);
+int btvae_gated_unit_bwd(const long long* unit, const long long* grads, const void* store, long long store_bytes, void* scratch,
+            long long scratch_bytes, void* stream);
 /* Products of up to btvae_few_rows_max() rows: C = X W^T + bias, or with W2 act(X W^T + bias) (X W2^T + bias2).  Weights and biases are of
  * one type; X is of theirs, or (without W2) fp32. */
 int btvae_few_rows_max(void);

@@ -199,3 +199,50 @@ def test_c_entry_points_refuse():
     nfwd("outputs", out=None)
     nfwd("outputs", normed=None)
     nfwd("gate rows", gate=a, G=3)
+
+
+def test_workspace_sizes_of_nothing():
+    """The sizes of empty (or nonsensical) problems are numbers, not crashes."""
+    lib = nv.lib()
+    for m in (-1, 0, 1):
+        for n in (-1, 0, 1):
+            for k in (-1, 0, 1, 5000):
+                for planes in (1, 3):
+                    assert lib.btvae_block_product_ws(m, n, k, planes) >= 0
+                    assert lib.btvae_block_wgrad_ws(m, n, k, planes) >= 0 or m * n < 0
+                    lib.btvae_block_wgrad_pair_ws(m, n, n, m, k, planes)
+                lib.btvae_fp8_product_ws(m, n, k)
+            lib.btvae_block_colsum_ws(m, max(n, 0))
+            assert lib.btvae_gated_kept_bytes(max(m, 0), max(n, 0), 1) >= 0
+
+
+def unit(**kw):
+    u = dict(x=1 << 20, x16=0, ldx=8, M=5, K=8, F=12, N=6, wg=1 << 20, ldg=8, wu=1 << 20, ldu=8, wd=1 << 20, ldd=12, w16=0, bg=0, bu=0, bd=0, b16=0, planes=3, act=0)
+    u.update(kw)
+    return (ctypes.c_longlong * 20)(*u.values())
+
+
+def test_gated_unit_entry_points():
+    """Sizes of the whole unit's memory, and what its entry points refuse."""
+    lib = nv.lib()
+    sizes = (ctypes.c_longlong * 3)()
+    assert lib.btvae_gated_unit_bytes(unit(), 1, sizes) == 0
+    store, scratch, in_place = sizes
+    assert in_place == 0 and store >= 5 * 192 + 5 * 192 + lib.btvae_gated_kept_bytes(5, 12, 3) and scratch > 0
+    assert lib.btvae_gated_unit_bytes(unit(), 0, sizes) == 0 and sizes[0] == 0 and sizes[1] > scratch
+    assert lib.btvae_gated_unit_bytes(unit(x16=1, w16=1, planes=1, ldd=16, F=16), 1, sizes) == 0 and sizes[2] == 1
+    assert lib.btvae_gated_unit_bytes(unit(M=0), 1, sizes) == 0 and sizes[0] == 0
+    for bad, words in ((dict(K=0), "sizes"), (dict(M=-1), "sizes"), (dict(F=1 << 31), "sizes"), (dict(ldx=7), "overlap"), (dict(ldd=11), "overlap"), (dict(planes=2), "planes"),
+                       (dict(x16=1), "fp32"), (dict(act=9), "activation"), (dict(wu=0), "null"), (dict(x=0), "null")):
+        assert lib.btvae_gated_unit_bytes(unit(**bad), 1, sizes) != 0
+        assert words in nv.last_error(), (bad, nv.last_error())
+    a = 1 << 20
+    assert lib.btvae_gated_unit_fwd(unit(), a, 6, 0, a, store - 1, a, scratch, None) != 0 and "workspace" in nv.last_error()
+    assert lib.btvae_gated_unit_fwd(unit(), a, 6, 0, a, store, a, scratch - 1, None) != 0 and "workspace" in nv.last_error()
+    g = lambda **kw: (ctypes.c_longlong * 15)(*{**dict(dy=a, dy16=0, lddy=6, dx=a, dwg=a, dwu=a, dwd=a, dbg=0, dbu=0, dbd=0, w16=0, d16=0, b16=0, bd16=0, acc=0), **kw}.values())
+    need = lib.btvae_gated_unit_bwd_bytes(unit(), g())
+    assert need > 0 and lib.btvae_gated_unit_bwd_bytes(unit(), g(dwg=0, dwu=0, dwd=0, dx=0)) < need
+    assert lib.btvae_gated_unit_bwd_bytes(unit(), g(lddy=5)) == -1 and "gradient" in nv.last_error()
+    assert lib.btvae_gated_unit_bwd_bytes(unit(), g(dwu=0)) == -1 and "all weights" in nv.last_error()
+    assert lib.btvae_gated_unit_bwd(unit(), g(), a, store, a, need - 1, None) != 0 and "workspace" in nv.last_error()
+    assert lib.btvae_gated_unit_bwd(unit(), g(), None, 0, a, need, None) != 0 and "workspace" in nv.last_error()

@@ -952,3 +952,37 @@ def test_block_wgrad_pair(dev, planes, R, shapes):
     assert bool((ws[need:] == 7.0).all())
     with pytest.raises(RuntimeError, match="workspace"):
         nv.call("btvae_block_wgrad_pair", (nv.ctypes.c_longlong * 26)(*jobs), ws.data_ptr(), need - 1, planes, R, 1)
+
+
+@pytest.mark.parametrize("dtype,K", [(F32, 40), (BF, 64), (BF, 40), (BF, 41)])
+def test_ffn_saved_tensor_hooks_and_lifetime(dev, dtype, K):
+    """Saved tensors that a hook moves (as offloading does) give the same gradients to the last bit; they are let go with the backward pass; a
+    second pass over a kept graph repeats the first."""
+    M, F, N = 90, 48, 24
+    t = ffn_case(dev, M, K, F, N, dtype, True, seed=61)
+    dy = rnd(dev, M, N, seed=63, dtype=dtype)
+    leaves = [t[k].requires_grad_() for k in ("x", "wg", "wu", "wd", "bg", "bu", "bd")]
+    y = B.gated_feed_forward(*leaves)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    moved = []
+
+    def pack(s):
+        moved.append(s.numel())
+        return s.detach().cpu().clone()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda s: s.to(dev)):
+        y2 = B.gated_feed_forward(*leaves)
+    junk = [torch.randn(1 << 16, device=dev) for _ in range(8)]         # reuse what the hook let go
+    got = torch.autograd.grad(y2, leaves, dy)
+    for a, b, c in zip(want, again, got):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert len(moved) == 8 and junk
+    x2 = rnd(dev, 4096, 256, seed=64, dtype=dtype).requires_grad_()
+    big = [rnd(dev, 512, 256, seed=65, dtype=dtype), rnd(dev, 512, 256, seed=66, dtype=dtype), rnd(dev, 256, 512, seed=67, dtype=dtype)]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y3 = B.gated_feed_forward(x2, *big)
+    held = torch.cuda.memory_allocated() - before
+    torch.autograd.grad(y3, x2, torch.ones_like(y3))
+    assert torch.cuda.memory_allocated() - before <= held - 4096 * 512 * 3   # the kept projections, at least, are gone with y3 alive
