@@ -258,10 +258,17 @@ def _ffn_few(x2, weights, biases, act):
     return y
 
 
+def _planes(x2):
+    """Operands of a unit that keeps what its backward pass needs: float32 accuracy, or bfloat16 for more than a few bfloat16 rows.  Few
+    rows are a host's time: there neither h nor the projections' gradients are rounded on their way (error of two rows' gradients
+    1.7e-3, the rounding of the results, against 3.3e-3)."""
+    return 3 if x2.dtype == torch.float32 or x2.shape[0] <= nv.lib().btvae_few_rows_max() else 1
+
+
 class _GatedNode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, act, x2, w_gate, w_up, w_down, b_gate, b_up, b_down):
-        planes = 3 if x2.dtype == torch.float32 else 1
+        planes = _planes(x2)
         y, tape = _ffn_forward(x2, [w_gate, w_up, w_down], [b_gate, b_up, b_down], act, planes, x2.dtype, True)
         ctx.save_for_backward(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, tape.store)
         ctx.unit, ctx.in_place = tape.unit, tape.in_place
@@ -282,7 +289,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
 
     ``x`` [..., K], ``w_gate`` and ``w_up`` [F, K], ``w_down`` [N, F], all float32 or all bfloat16; result [..., N] of that type.
     ``activation``: "silu", "gelu" (erf form), "relu" or "sigmoid".  Differentiable in every tensor; for up to 32 rows without
-    a graph the weights are streamed once (the form for single profiles).  In float32 a row with an infinite input may
+    a graph the weights are streamed once (the form for single profiles).  bfloat16: h, and in the backward pass the gradients of
+    both projections, are rounded to bfloat16 as operands of the next product, but not for up to 32 rows.  In float32 a row with an infinite input may
     come out as NaN where float32 arithmetic would give an infinity."""
     x2, weights, biases, act = _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
@@ -300,7 +308,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
 def gated_feed_forward_tape(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu"):
     """``gated_feed_forward`` without autograd: (y, tape), ``tape.backward(dy)`` returns the gradients.  May be captured into a graph."""
     x2, weights, biases, act = _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-    y, tape = _ffn_forward(x2, weights, biases, act, 3 if x.dtype == torch.float32 else 1, x.dtype, True)
+    y, tape = _ffn_forward(x2, weights, biases, act, _planes(x2), x.dtype, True)
     return _shaped(y, (*x.shape[:-1], y.shape[1])), tape
 
 

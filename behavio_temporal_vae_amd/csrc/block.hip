@@ -888,7 +888,6 @@ static int unit_of(const long long* a, bk::Unit& u) {
     BTVAE_REQUIRE(a[3] >= 0 && a[3] < 2 * big && a[4] > 0 && a[4] < big && a[5] > 0 && a[5] < big && a[6] > 0 && a[6] < big, "gated_unit: bad sizes (M %lld, K %lld, F %lld, N %lld)", a[3], a[4], a[5], a[6]);
     BTVAE_REQUIRE(a[2] >= a[4] && a[8] >= a[4] && a[10] >= a[4] && a[12] >= a[5], "gated_unit: rows overlap");
     BTVAE_REQUIRE(a[18] == 1 || a[18] == 3, "gated_unit: planes must be 1 or 3");
-    BTVAE_REQUIRE(a[18] == 1 || (!a[1] && !a[13]), "gated_unit: three planes are for fp32 matrices");
     BTVAE_REQUIRE(a[19] >= 0 && a[19] <= 3, "gated_unit: unknown activation %lld", a[19]);
     BTVAE_REQUIRE((a[0] || a[3] == 0) && a[7] && a[9] && a[11], "gated_unit: null matrix");
     u = {(const void*)a[0], a[1] != 0, a[2], (int)a[3], (int)a[4], (int)a[5], (int)a[6], (const void*)a[7], (const void*)a[9], (const void*)a[11], a[8], a[10], a[12], a[13] != 0,
