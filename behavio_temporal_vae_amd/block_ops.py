@@ -26,6 +26,7 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
 FP8_BLOCK = 128
 _FLOATS = (torch.float32, torch.bfloat16)
+MAX_ROWS = 2 ** 31 - 2 ** 21            # row numbers, and those a few tiles or splits past them, are 32 bits
 
 
 # ------------------------------------------------------------------------------------------------ checks and layout
@@ -73,7 +74,7 @@ def _rows(t, what):
     rows = 1
     for n in t.shape[:-1]:
         rows *= n
-    if rows >= 2 ** 31 or t.shape[-1] >= 2 ** 30:
+    if rows > MAX_ROWS or t.shape[-1] >= 2 ** 30:
         raise ValueError(f"{what} is too large: {list(t.shape)}")
     if t.dim() != 2:
         t = t.reshape(rows, t.shape[-1])

@@ -727,6 +727,7 @@ static int check_cols(const bk::ColJob& j, int planes, int R) {
     BTVAE_REQUIRE(!j.out1 || (j.off1 >= j.rows0 && j.rows1 >= 0 && j.off1 + j.rows1 <= j.M), "block_wgrad: bad row ranges");
     BTVAE_REQUIRE(R == 0 || (operand_ok(j.A, j.lda, planes, M8) && operand_ok(j.B, j.ldb, planes, N8)), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of %d columns", unit);
     BTVAE_REQUIRE(j.lda < (1 << 23) && j.ldb < (1 << 23), "block_wgrad: rows of more than 8 MiB");
+    BTVAE_REQUIRE(R <= bk::MAX_ROWS, "block_wgrad: too many rows");
     return 0;
 }
 BTVAE_API long long btvae_block_wgrad_ws(int M, int N, int R, int planes) {
@@ -885,7 +886,7 @@ static BackwardPlan plan_backward(const Unit& u, const long long* b, Pieces& scr
 static int unit_of(const long long* a, bk::Unit& u) {
     BTVAE_REQUIRE(a, "gated_unit: null description");
     const long long big = 1LL << 30;
-    BTVAE_REQUIRE(a[3] >= 0 && a[3] < 2 * big && a[4] > 0 && a[4] < big && a[5] > 0 && a[5] < big && a[6] > 0 && a[6] < big, "gated_unit: bad sizes (M %lld, K %lld, F %lld, N %lld)", a[3], a[4], a[5], a[6]);
+    BTVAE_REQUIRE(a[3] >= 0 && a[3] <= bk::MAX_ROWS && a[4] > 0 && a[4] < big && a[5] > 0 && a[5] < big && a[6] > 0 && a[6] < big, "gated_unit: bad sizes (M %lld, K %lld, F %lld, N %lld)", a[3], a[4], a[5], a[6]);
     BTVAE_REQUIRE(a[2] >= a[4] && a[8] >= a[4] && a[10] >= a[4] && a[12] >= a[5], "gated_unit: rows overlap");
     BTVAE_REQUIRE(a[18] == 1 || a[18] == 3, "gated_unit: planes must be 1 or 3");
     BTVAE_REQUIRE(a[19] >= 0 && a[19] <= 3, "gated_unit: unknown activation %lld", a[19]);

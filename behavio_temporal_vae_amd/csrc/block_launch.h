@@ -6,6 +6,7 @@
 namespace btvae_block {
 
 constexpr int CHIP = 256;                                             // compute units
+constexpr int MAX_ROWS = 0x7FE00000;                                  // row numbers, and those a few tiles or splits past them, are 32 bits
 
 inline int tiles(int n, int t) { return (n + t - 1) / t; }
 constexpr int tile_width(bool split) { return split ? 128 : 256; }    // columns of gemm_rows' tiles (of 128 rows): see there
@@ -21,6 +22,7 @@ int launch_rows(Args& p, int z, hipStream_t s, const char* what) {
     constexpr int WN = tile_width(FMT == FMT_SPLIT) / 64;
     p.tiles_m = tiles(p.M, 128); p.tiles_n = tiles(p.N, 64 * WN / (is_gated(EP) ? 2 : 1)); p.splits = z;
     const long long items = (long long)p.tiles_m * p.tiles_n * z;
+    if (p.M > MAX_ROWS) return btvae::set_error("%s: too many rows", what);
     if (items >= (1 << 29)) return btvae::set_error("%s: too many tiles", what);
     if (p.lda >= (1 << 23) || p.ldb >= (1 << 23)) return btvae::set_error("%s: rows of more than 8 MiB", what);
     p.by_tiles = div_by(p.tiles_m * p.tiles_n); p.by_band = div_by(8 * p.tiles_n); p.by_last = div_by(p.tiles_m % 8 ? p.tiles_m % 8 : 8);

@@ -11,7 +11,7 @@
 // draws (draw s of profile b is row s B + b).  In the backward pass a group takes all (or one stretch) of the rows of one
 // gate row, so that gate row's gradient is a running sum in registers; the gradients of the row weights are running
 // sums too, joined over a workgroup's rows through LDS and over workgroups by a second launch, always in the same order.
-#include "block_gemm.h"
+#include "block_launch.h"
 #include <algorithm>
 
 using namespace btvae;
@@ -561,7 +561,8 @@ BTVAE_API int btvae_norm_max_columns(void) { return bn_::MAX_N; }
 // post / pre: 0 none, 1 rms, 2 layer.
 BTVAE_API int btvae_norm_gate_residual_fwd(const void* residual, const void* branch, const void* gate, int G, float scale, const float* scale_vec, const float* post_w, const float* post_b,
                                            const float* pre_w, const float* pre_b, int post, int pre, float eps, void* stream_out, void* normed, float* stats, int types, int M, int N, void* stream) {
-    BTVAE_REQUIRE(M >= 0 && N > 0 && N <= bn_::MAX_N, "norm_gate_residual: %d columns (1 to %d)", N, bn_::MAX_N);
+    BTVAE_REQUIRE(M >= 0 && M <= btvae_block::MAX_ROWS, "norm_gate_residual: too many rows");
+    BTVAE_REQUIRE(N > 0 && N <= bn_::MAX_N, "norm_gate_residual: %d columns (1 to %d)", N, bn_::MAX_N);
     BTVAE_REQUIRE(types == 0 || types == 2 || types == 3, "norm_gate_residual: a bf16 residual needs a bf16 branch");
     BTVAE_REQUIRE(post >= 0 && post <= 2 && pre >= 0 && pre <= 2 && eps >= 0.f, "norm_gate_residual: bad norm");
     if (M == 0) return 0;                                     // (empty matrices have no address to check)
@@ -593,7 +594,8 @@ BTVAE_API long long btvae_norm_gate_residual_ws(int M, int N, int G) {
 BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_normed, const void* residual, const void* branch, const void* gate, int G, float scale, const float* scale_vec,
                                            const float* post_w, const float* post_b, const float* pre_w, int post, int pre, const float* stats, void* d_residual, void* d_branch, void* d_gate,
                                            float* d_scale, float* d_post_w, float* d_post_b, float* d_pre_w, float* d_pre_b, float* ws, long long ws_floats, int types, int M, int N, void* stream) {
-    BTVAE_REQUIRE(M >= 0 && N > 0 && N <= bn_::MAX_N, "norm_gate_residual_bwd: %d columns (1 to %d)", N, bn_::MAX_N);
+    BTVAE_REQUIRE(M >= 0 && M <= btvae_block::MAX_ROWS, "norm_gate_residual_bwd: too many rows");
+    BTVAE_REQUIRE(N > 0 && N <= bn_::MAX_N, "norm_gate_residual_bwd: %d columns (1 to %d)", N, bn_::MAX_N);
     BTVAE_REQUIRE(types == 0 || types == 2 || types == 3, "norm_gate_residual_bwd: a bf16 residual needs a bf16 branch");
     BTVAE_REQUIRE(post >= 0 && post <= 2 && pre >= 0 && pre <= 2, "norm_gate_residual_bwd: bad norm");
     BTVAE_REQUIRE(M == 0 || !d_normed || pre, "norm_gate_residual_bwd: a gradient of a norm that was not asked for");

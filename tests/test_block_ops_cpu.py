@@ -29,6 +29,7 @@ def ffn(**kw):
     (ffn(x=torch.zeros(M, K, dtype=torch.float64)), TypeError, "x must be"),
     (ffn(x=torch.tensor(1.0)), ValueError, "at least one dimension"),
     (ffn(x=torch.zeros(M, 0), w_gate=torch.zeros(F, 0), w_up=torch.zeros(F, 0)), ValueError, "no columns"),
+    (ffn(x=torch.zeros(1, K).expand(2 ** 31 - 2 ** 20, K)), ValueError, "too large"),
     (ffn(x=torch.zeros(M, K + 1)), ValueError, "w_gate must have shape"),
     (ffn(x=torch.zeros(M, K, dtype=BF)), TypeError, "w_gate must be bfloat16"),
     (ffn(w_gate=torch.zeros(0, K), w_up=torch.zeros(0, K), w_down=torch.zeros(N, 0)), ValueError, "w_gate must be a matrix"),
@@ -193,6 +194,7 @@ def test_c_entry_points_refuse():
 
     nfwd("columns", N=limit + 1)
     nfwd("columns", N=0)
+    nfwd("rows", M=2 ** 31 - 2 ** 20)
     nfwd("bf16 branch", types=1)
     nfwd("bad norm", post=3)
     nfwd("bad norm", eps=-1.0)
@@ -232,7 +234,7 @@ def test_gated_unit_entry_points():
     assert lib.btvae_gated_unit_bytes(unit(), 0, sizes) == 0 and sizes[0] == 0 and sizes[1] > scratch
     assert lib.btvae_gated_unit_bytes(unit(x16=1, w16=1, planes=1, ldd=16, F=16), 1, sizes) == 0 and sizes[2] == 1
     assert lib.btvae_gated_unit_bytes(unit(M=0), 1, sizes) == 0 and sizes[0] == 0
-    for bad, words in ((dict(K=0), "sizes"), (dict(M=-1), "sizes"), (dict(F=1 << 31), "sizes"), (dict(ldx=7), "overlap"), (dict(ldd=11), "overlap"), (dict(planes=2), "planes"),
+    for bad, words in ((dict(K=0), "sizes"), (dict(M=-1), "sizes"), (dict(F=1 << 31), "sizes"), (dict(M=2 ** 31 - 2 ** 20), "sizes"), (dict(ldx=7), "overlap"), (dict(ldd=11), "overlap"), (dict(planes=2), "planes"),
                        (dict(act=9), "activation"), (dict(wu=0), "null"), (dict(x=0), "null")):
         assert lib.btvae_gated_unit_bytes(unit(**bad), 1, sizes) != 0
         assert words in nv.last_error(), (bad, nv.last_error())
