@@ -18,14 +18,16 @@
 // through several tiles: the next tile's stages are on their way while the results of the last one are stored.  Pieces of 16
 // bytes past the end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns;
 // rows past the end repeat the last row and only reach outputs that are not stored.
-//   Measured (one card, 1.75 to 2.0 GHz under these loads, which is its power limit; a large library product in bf16 reaches 1394 TFLOP/s):
-//   bf16 65,536 x 4000 x 1000 490 to 540 us, 970 to 1070 TFLOP/s (128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of
+//   Measured (one card, at 1.7 to 2.0 GHz under these loads; a large library product in bf16 reaches 1394 TFLOP/s):
+//   bf16 65,536 x 4000 x 1000 490 to 540 us, 970 to 1070 TFLOP/s (a library product of this shape 472; operands of zeros, which draw less
+//   power, 442 and 404; 128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of
 //   eight waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
 //   645 us, 813 TFLOP/s and 1.03 GB stored; its backward 480 us, 0.8 GB loaded and 0.6 stored; split 16,384 x 4000 x 1000 690 us,
 //   190 TFLOP/s of fp32 or 1140 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
 //   400 us, 1310 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
-//   What they wait for: operands on their way through L2 and LDS at a clock that falls with what is moved; skewing the
-//   workgroups against each other, giving them priorities, or letting a tile's stores pass its successor's first stage changed nothing.
+//   What they wait for: the matrix pipe is busy 48 to 66 % of the cycles (epilogues included), the rest are waits at a stage's barrier for operands from L2
+//   and LDS; skewing the workgroups against each other, giving waves priorities, or letting a tile's stores pass its successor's first
+//   stage changed nothing.
 //
 // Results.  The weights are the MFMA's first operand, so a lane's 16 results of a 32 x 32 block are 16 columns of ONE row, and the
 // weight rows are laid into LDS with bits 2 and 3 of their index swapped, which makes them two runs of 8 consecutive
@@ -1101,7 +1103,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 // Four waves, 256 x 256 tiles of one workgroup a compute unit where the splits of the rows fill the chip with them, else 128 x 128 and two.
 //   Measured, 256 / 128 tiles: bf16 65,536 rows, 4032 x 1000: 546 / 707 us (968 TFLOP/s; a library product of the shape 687), 16,384 rows
 //   1000 x 2000 86 / 94 us, 4096 rows 44 / 37 us, 65,536 rows 512 x 256 63 / 45 us; split 16,384 rows, 4032 x 1000: 608 / 717 us (217
-//   TFLOP/s of fp32, 1300 of the products done), 2048 rows 1024 x 1024 50 / 38 us.  What bounds it: the matrix pipe at the power limit's clock.
+//   TFLOP/s of fp32, 1300 of the products done), 2048 rows 1024 x 1024 50 / 38 us.  What bounds it: transposing reads (as many LDS
+//   cycles as matrix cycles) behind one wave to a SIMD; the matrix pipe is busy 52 % of the cycles, split 73 %.
 struct ColArgs {
     const char* A; long long lda; int a_cols;                 // byte pitch; columns that may be read (a multiple of 8; split: of 16)
     const char* B; long long ldb; int b_cols;
