@@ -410,6 +410,19 @@ template <class W> __device__ __forceinline__ void store_split(char* base, long 
         if (r + 16 < rows) *reinterpret_cast<u32x4*>(d + 16 * ld) = b;
     }
 }
+// 32 rows of 128 bytes, eight lanes to a row, through 4 KiB of LDS: a row's 16-byte piece `c` of row lane & 31 goes in with `put`, and piece lane & 7 of
+// rows 8 k + (lane >> 3) comes out
+struct Wide {
+    char* lds;
+    int li, r8, p8;
+    __device__ __forceinline__ explicit Wide(char* wave_lds) : lds(wave_lds) {
+        const int lane = threadIdx.x & 63;
+        li = lane & 31; r8 = lane >> 3; p8 = lane & 7;
+    }
+    __device__ __forceinline__ u32x4* at(int row, int piece) const { return reinterpret_cast<u32x4*>(lds + row * 128 + ((piece ^ (row & 7)) << 4)); }
+    __device__ __forceinline__ void put(int c, const u32x4 x) const { *at(li, c) = x; }
+    __device__ __forceinline__ u32x4 get(int k) const { return *at(8 * k + r8, p8); }
+};
 // A wave's rows of a matrix of whole 16-byte pieces, through a buffer descriptor that ends behind the last row: pieces outside are not stored.
 constexpr unsigned OUTSIDE = 0xFFFFFFF0u;
 struct Panel {
@@ -891,6 +904,62 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) bias_of(j * 32, b[j], wh);
             Turn::fence();
+            if constexpr (!SPLIT) {
+                // rows of 128 bytes through this wave's part of the slot that is filled next: all waves have read it, and only this wave's copies write there
+                static_assert(NB >= 4 && NJ == 2, "");
+                const Wide wide(smem + f_slot * STAGE + TM * ROWB + wid * NB * 1024);
+                const bool half = !to_slab && p.c_type == T_BF16;
+                float* const out = to_slab ? p.slab + (long long)zz * p.M * p.N : reinterpret_cast<float*>(p.C);
+                const long long ld = to_slab ? p.N : p.ldc;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    float v[2][2][8];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) v[j][r >> 3][r & 7] = acc[i][j][r] + b[j][r >> 3][r & 7];
+                    const int r0 = opaque(row0 + i * 32), c0 = opaque(col0);
+                    if (half) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) wide.put(2 * q + lh, pack8(v[q >> 1][q & 1]));
+                        Turn::fence();
+                        u32x4 x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = wide.get(k);
+                        Turn::fence();
+                        const int c = c0 + 8 * wide.p8, r = r0 + wide.r8;
+                        if (c < p.N) {
+                            unsigned short* d = reinterpret_cast<unsigned short*>(p.C) + (long long)r * p.ldc + c;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (r + 8 * k < p.M) put_bf16(d + 8 * k * p.ldc, x[k], c, p.N);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                wide.put(4 * q + 2 * lh, raw4(v[j][q]));
+                                wide.put(4 * q + 2 * lh + 1, raw4(v[j][q] + 4));
+                            }
+                            Turn::fence();
+                            u32x4 x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) x[k] = wide.get(k);
+                            Turn::fence();
+                            const int c = c0 + 32 * j + 4 * wide.p8, r = r0 + wide.r8;
+                            if (c < p.N) {
+                                float* d = out + (long long)r * ld + c;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (r + 8 * k < p.M) put_f32(d + 8 * k * ld, x[k], c, p.N);
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                wait_lds();                                   // (before this wave's copies into the same place)
+            } else
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
 #pragma unroll
