@@ -24,7 +24,7 @@
 //   eight waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
 //   645 us, 813 TFLOP/s and 1.03 GB stored; its backward 480 us, 0.8 GB loaded and 0.6 stored; split 16,384 x 4000 x 1000 690 us,
 //   190 TFLOP/s of fp32 or 1140 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
-//   400 us, 1310 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
+//   366 us, 1430 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
 //   What they wait for: the matrix pipe is busy 48 to 66 % of the cycles (epilogues included), the rest are waits at a stage's barrier for operands from L2
 //   and LDS; skewing the workgroups against each other, giving waves priorities, or letting a tile's stores pass its successor's first
 //   stage changed nothing.
@@ -34,6 +34,8 @@
 // columns.  Bias, activation, product and rounding happen there; 2 KiB of LDS to a wave (or 1 KiB twice) then turn each 64 bytes of
 // 32 rows over to four neighbouring lanes a row: stores of 16 bytes a lane whose neighbours do not continue them cost several
 // times as much (measured: 150 cycles a store instruction instead of about 30).
+// A plain product's results leave as whole 128 bytes of a row, through 4 KiB of the slot that is filled next (e4m3 131,072 x 1000 x 2000:
+// 366 us instead of 382 with 64 bytes; 240 with nothing stored, 315 with all stored to the same few rows: the rest is memory).
 #pragma once
 #include "common.h"
 #include <type_traits>
