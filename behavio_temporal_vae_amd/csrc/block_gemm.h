@@ -19,13 +19,13 @@
 // bytes past the end of a row read from a block of zeros instead, so operands need no padding beyond a multiple of 8 columns;
 // rows past the end repeat the last row and only reach outputs that are not stored.
 //   Measured (one card, at 1.7 to 2.0 GHz under these loads; a large library product in bf16 reaches 1394 TFLOP/s):
-//   bf16 65,536 x 4000 x 1000 490 to 540 us, 970 to 1070 TFLOP/s (a library product of this shape 472; operands of zeros, which draw less
+//   bf16 65,536 x 4000 x 1000 490 to 525 us, 1000 to 1070 TFLOP/s (a library product of this shape 472; operands of zeros, which draw less
 //   power, 442 and 404; 128 x 128 tiles of four waves, two stages: 550 us; 256 x 256 tiles of
 //   eight waves: 468 us, but their epilogues do not fit the registers); gated 65,536 x 1000 x 2 x 2000 with both projections kept
-//   645 us, 813 TFLOP/s and 1.03 GB stored; its backward 480 us, 0.8 GB loaded and 0.6 stored; split 16,384 x 4000 x 1000 690 us,
+//   600 to 625 us, 840 to 874 TFLOP/s and 1.03 GB stored; its backward 455 us, 0.8 GB loaded and 0.6 stored; split 16,384 x 4000 x 1000 690 us,
 //   190 TFLOP/s of fp32 or 1140 of the products done (a large library product in fp32: 154); e4m3 131,072 x 1000 x 2000
-//   366 us, 1430 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
-//   What they wait for: the matrix pipe is busy 48 to 66 % of the cycles (epilogues included), the rest are waits at a stage's barrier for operands from L2
+//   320 to 360 us, 1460 to 1640 TFLOP/s; e4m3 gated and quantised again 65,536 x 1000 x 2 x 2000 370 to 440 us, 1190 to 1417 TFLOP/s.
+//   What they wait for: the matrix pipe is busy 49 to 66 % of the cycles (epilogues included), the rest are waits at a stage's barrier for operands from L2
 //   and LDS; skewing the workgroups against each other, giving waves priorities, or letting a tile's stores pass its successor's first
 //   stage changed nothing.
 //
@@ -35,7 +35,8 @@
 // 32 rows over to four neighbouring lanes a row: stores of 16 bytes a lane whose neighbours do not continue them cost several
 // times as much (measured: 150 cycles a store instruction instead of about 30).
 // A plain product's results leave as whole 128 bytes of a row, through 4 KiB of the slot that is filled next (e4m3 131,072 x 1000 x 2000:
-// 366 us instead of 382 with 64 bytes; 240 with nothing stored, 315 with all stored to the same few rows: the rest is memory).
+// 366 us instead of 382 with 64 bytes; 240 with nothing stored, 268 of them turned but not stored).  Large ones are stored past L2, which keeps
+// the operands of the other tiles there (0.19 GB read beyond L2 instead of 0.47; 329 us): STREAM_BYTES has the rule.
 #pragma once
 #include "common.h"
 #include <type_traits>
@@ -90,6 +91,7 @@ struct Args {
     const unsigned* b_sc; const unsigned* b2_sc; int b_scp;     // e4m3: scale bytes of B's 128-row blocks, four to a word [blocks][b_scp words]
     const void* bias; const void* bias2; int bias_bf16;         // plain: bias; gated: gate and up
     void* C; long long ldc; int c_type;             // EP_LINEAR: T_F32 or T_BF16, pitch in elements; split results: pitch in bytes
+    int stream;                                     // bf16 and e4m3 operands: results are stored past L2
     float* slab;                                    // splits > 1: fp32 partial results [z][M][N]
     int act;
     // Gated: where a, b are kept for the backward pass (null: not), in the order in which the kernels' lanes hold them: for every 32 rows and
@@ -364,15 +366,20 @@ template <bool HALF> struct Where {
         return a;
     }
 };
+// STREAM: past L2, which holds the operands of other tiles
+template <bool STREAM, class T, class V> __device__ __forceinline__ void put_any(T* d, const V v) {
+    if constexpr (STREAM) __builtin_nontemporal_store((T)v, d);
+    else *d = v;
+}
 // 8 bf16 (a lane's 16 bytes) at columns c .. c + 7 of a row, those below n only
-__device__ __forceinline__ void put_bf16(unsigned short* d, const u32x4 v, int c, int n) {
-    if (c + 8 <= n) { *reinterpret_cast<u32x4_any*>(d) = v; return; }
+template <bool STREAM = false> __device__ __forceinline__ void put_bf16(unsigned short* d, const u32x4 v, int c, int n) {
+    if (c + 8 <= n) { put_any<STREAM>(reinterpret_cast<u32x4_any*>(d), v); return; }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (c + e < n) d[e] = (unsigned short)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
 }
-__device__ __forceinline__ void put_f32(float* d, const u32x4 u, int c, int n) {
-    if (c + 4 <= n) { *reinterpret_cast<f32x4_any*>(d) = __builtin_bit_cast(f32x4, u); return; }
+template <bool STREAM = false> __device__ __forceinline__ void put_f32(float* d, const u32x4 u, int c, int n) {
+    if (c + 4 <= n) { put_any<STREAM>(reinterpret_cast<f32x4_any*>(d), __builtin_bit_cast(f32x4, u)); return; }
 #pragma unroll
     for (int e = 0; e < 4; ++e) if (c + e < n) d[e] = __uint_as_float(u[e]);
 }
@@ -434,22 +441,29 @@ struct Panel {
         buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + row0 * ld_bytes, 0, (unsigned)max(0, min(rows - row0, height)) * (unsigned)ld_bytes, 0x00020000);
     }
     __device__ __forceinline__ unsigned at(int r, unsigned byte, bool in) const { return in ? (unsigned)r * ld + byte : OUTSIDE; }
-    __device__ __forceinline__ void put(const u32x4 v, unsigned o) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 0); }
+    __device__ __forceinline__ void put(const u32x4 v, unsigned o, bool stream) const {
+        if (stream) __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 2);       // (uniform; 2: non-temporal)
+        else __builtin_amdgcn_raw_buffer_store_b128(v, buf, o, 0, 0);
+    }
 };
 // block of rows `row` .. + 31 of the panel, columns col0 .. + 31 of which those below `cols` (a multiple of 16) exist
-template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, int row, int col0, int cols, const float (&v)[2][8], const W& w) {
+template <class W> __device__ __forceinline__ void panel_bf16(const Panel& out, int row, int col0, int cols, const float (&v)[2][8], const W& w, bool stream) {
     u32x4 a, b;
     w.turn(pack8(v[0]), w.lh, pack8(v[1]), 2 + w.lh, a, b);
     const int c = col0 + 8 * w.p4;
     const unsigned o = out.at(row + w.r4, 2 * c, c < cols);
-    out.put(a, o);
-    out.put(b, c < cols ? o + 16 * out.ld : OUTSIDE);
+    out.put(a, o, stream);
+    out.put(b, c < cols ? o + 16 * out.ld : OUTSIDE, stream);
 }
 // Kept projections: a block's bytes, and block (row0, col0) of a (0) or b (1); every store and load is 1 KiB in a row
 template <bool B24> constexpr int kept_bytes() { return (B24 ? 3 : 4) * 1024; }
 template <bool B24> __device__ __forceinline__ char* kept_at(const Args& p, int row0, int col0, int which) {
     return p.kept + (((long long)(row0 >> 5) * (p.half >> 5) + (col0 >> 5)) * 2 + which) * kept_bytes<B24>() + (threadIdx.x & 63) * 16;
 }
+// Kept projections are next read by the backward pass, long after caches have forgotten them: past L2 both ways (stores past it: a bf16
+// forward and backward pass of 4096 / 16,384 / 65,536 rows, 1000 -> 2000 -> 1000, 297 -> 291, 763 -> 747, 2770 -> 2742 us; fp32, 2048 / 16,384 rows: 517 -> 511,
+// 3154 -> 3125)
+__device__ __forceinline__ void keep_once(char* at, const u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(at)); }
 struct Raw24 { u32x4 h[2], l; };
 struct Raw32 { u32x4 x[4]; };
 // 24 bits: the upper three bytes, cut (off by 2^-15 of a value at most, where the gradients made from them are rounded to bf16, 2^-8;
@@ -467,9 +481,9 @@ __device__ __forceinline__ void keep_24(char* at, const float (&v)[2][8]) {
 #pragma unroll
         for (int d = 0; d < 2; ++d)                           // byte 1 of four values
             l[2 * q + d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0501u), __builtin_amdgcn_perm(u[4 * d + 1], u[4 * d], 0x0C0C0501u), 0x05040100u);
-        *reinterpret_cast<u32x4*>(at + q * 1024) = h;
+        keep_once(at + q * 1024, h);
     }
-    *reinterpret_cast<u32x4*>(at + 2048) = l;
+    keep_once(at + 2048, l);
 }
 __device__ __forceinline__ u32x4 load_once(const char* at) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at)); }
 __device__ __forceinline__ void load_24(const char* at, Raw24& x) {
@@ -489,7 +503,7 @@ __device__ __forceinline__ void unpack_24(const Raw24& x, float (&v)[2][8]) {
 }
 __device__ __forceinline__ void keep_32(char* at, const float (&v)[2][8]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(at + k * 1024) = raw4(v[k >> 1] + 4 * (k & 1));
+    for (int k = 0; k < 4; ++k) keep_once(at + k * 1024, raw4(v[k >> 1] + 4 * (k & 1)));
 }
 __device__ __forceinline__ void load_32(const char* at, Raw32& x) {
 #pragma unroll
@@ -934,7 +948,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             unsigned short* d = reinterpret_cast<unsigned short*>(p.C) + (long long)r * p.ldc + c;
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                if (r + 8 * k < p.M) put_bf16(d + 8 * k * p.ldc, x[k], c, p.N);
+                                if (r + 8 * k < p.M) {
+                                    if (p.stream) put_bf16<true>(d + 8 * k * p.ldc, x[k], c, p.N);
+                                    else put_bf16(d + 8 * k * p.ldc, x[k], c, p.N);
+                                }
                         }
                     } else {
 #pragma unroll
@@ -954,7 +971,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                                 float* d = out + (long long)r * ld + c;
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
-                                    if (r + 8 * k < p.M) put_f32(d + 8 * k * ld, x[k], c, p.N);
+                                    if (r + 8 * k < p.M) {
+                                        if (p.stream) put_f32<true>(d + 8 * k * ld, x[k], c, p.N);
+                                        else put_f32(d + 8 * k * ld, x[k], c, p.N);
+                                    }
                             }
                         }
                     }
@@ -1009,7 +1029,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r) acc[i][j][r] = h[r >> 3][r & 7];
                         } else if constexpr (EP == EP_GATED) {
-                            panel_bf16(out, i * 32, c, N16, h, wh);
+                            panel_bf16(out, i * 32, c, N16, h, wh, p.stream);
                             if (p.kept && r0 < p.M && c < p.half) {         // (uniform)
                                 keep_24(kept_at<true>(p, r0, c, 0), a);
                                 keep_24(kept_at<true>(p, r0, c, 1), b);
@@ -1102,8 +1122,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_rows(const Args p) {
                             cs[16 + r] += db[r >> 3][r & 7];
                         }
                         if constexpr (FAST) {
-                            panel_bf16(out_a, i * 32, c, p.half, da, wh);
-                            panel_bf16(out_b, i * 32, c, p.half, db, wh);
+                            panel_bf16(out_a, i * 32, c, p.half, da, wh, p.stream);
+                            panel_bf16(out_b, i * 32, c, p.half, db, wh, p.stream);
                         } else {
                             store_split(reinterpret_cast<char*>(p.C), p.ldc, r0, c, p.M, p.half, da, wh);
                             store_split(reinterpret_cast<char*>(p.C) + split_at(p.half, 0), p.ldc, r0, c, p.M, p.half, db, wh);
