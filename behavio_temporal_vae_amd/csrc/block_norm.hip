@@ -84,6 +84,8 @@ template <int T, int NV, bool VEC> struct Row {
                 v[8 * j + e] = col(t, j, VEC ? 0 : e) < N ? f : 0.f;
             }
     }
+    // bf16 rows leave past L2 in whole lines (8192 / 65,536 / 262,144 rows of 1000, forward and backward: 58 / 307 / 1212 us, through L2 60 / 326 / 1255; alone and
+    // with a kernel that reads `normed` the forward pass gains as well); fp32 rows, two stores of 16 in 32 bytes a lane, gain nothing by it (65,536 rows 236 us forward, past L2 245)
     template <bool H> __device__ __forceinline__ static void store(void* p, long long row0, int N, int t, const float (&v)[8 * NV]) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -94,7 +96,7 @@ template <int T, int NV, bool VEC> struct Row {
                     u32x4 q;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) q[e] = pack2(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
-                    *reinterpret_cast<u32x4*>(reinterpret_cast<unsigned short*>(p) + row0 + c) = q;
+                    __builtin_nontemporal_store(q, reinterpret_cast<u32x4*>(reinterpret_cast<unsigned short*>(p) + row0 + c));
                 } else {
                     float* d = reinterpret_cast<float*>(p) + row0 + c;
                     *reinterpret_cast<f32x4*>(d) = f32x4{v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]};
