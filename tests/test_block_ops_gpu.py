@@ -986,3 +986,36 @@ def test_ffn_saved_tensor_hooks_and_lifetime(dev, dtype, K):
     held = torch.cuda.memory_allocated() - before
     torch.autograd.grad(y3, x2, torch.ones_like(y3))
     assert torch.cuda.memory_allocated() - before <= held - 4096 * 512 * 3   # the kept projections, at least, are gone with y3 alive
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_results_stored_past_l2(out):
+    """More than 128 MiB of results, the last tile of rows and of columns ragged: sampled rows (the last among them) against 64 bits.  A result is off by
+    its own rounding (bf16: half a step, 2^-8) and by the sums': 2^-16 of the sum of magnitudes on the 8-bit pipe, K 2^-24 in fp32."""
+    M, K, N = 70001, 136, 1001
+    torch.manual_seed(5)
+    x = torch.randn(M, K, device="cuda")
+    w = B.fp8_weight(torch.randn(N, K, device="cuda") * K ** -0.5)
+    q = B.fp8_quantize(x)
+    y = B.fp8_linear(q, w, out_dtype=out)
+    rows = torch.cat([torch.arange(0, M, 997, device="cuda"), torch.arange(M - 130, M, device="cuda")])
+    a, b = q.dequantize()[rows].double(), w.dequantize().double()
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -16 * size if out == torch.bfloat16 else 2.0 ** -24 * want.abs() + K * 2.0 ** -24 * size
+    assert ((y[rows].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+def test_unit_whose_results_pass_l2():
+    """A bf16 unit with more than 128 MiB of h and of projection gradients, ragged in rows and columns, both ways against the same unit on 24,577 of
+    its rows, too few for that and enough that no reduction is split: y and dx of a row depend on that row alone, so they are equal."""
+    M, K, F, m = 68001, 64, 1010, 24577
+    torch.manual_seed(6)
+    make = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+    x, dy, wg, wu, wd = make(M, K), make(M, 64), make(F, K) * 0.125, make(F, K) * 0.125, make(64, F) * 0.03
+    y, tape = B.gated_feed_forward_tape(x, wg, wu, wd)
+    dx = tape.backward(dy)[0]
+    y2, tape2 = B.gated_feed_forward_tape(x[-m:].contiguous(), wg, wu, wd)
+    dx2 = tape2.backward(dy[-m:].contiguous())[0]
+    assert torch.equal(y[-m:], y2) and torch.equal(dx[-m:], dx2)
