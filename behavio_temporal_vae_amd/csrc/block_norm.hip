@@ -604,6 +604,7 @@ BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_n
     BTVAE_REQUIRE(M == 0 || !d_normed || pre, "norm_gate_residual_bwd: a gradient of a norm that was not asked for");
     BTVAE_REQUIRE(!gate || M == 0 || (branch && G > 0 && M % G == 0), "norm_gate_residual_bwd: %d rows are not a multiple of %d gate rows", M, G);
     BTVAE_REQUIRE(M == 0 || (!d_branch && !d_gate && !d_scale && !d_post_w && !d_post_b) || branch, "norm_gate_residual_bwd: gradients of an absent branch");
+    BTVAE_REQUIRE(!d_gate || (gate && G > 0), "norm_gate_residual_bwd: a gradient of an absent gate");
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     bn_::Args p = {};
     const int g = gate && G > 0 ? G : std::max(M, 1);
@@ -625,13 +626,14 @@ BTVAE_API int btvae_norm_gate_residual_bwd(const void* d_stream, const void* d_n
         else if (types == 2) bn_::launch<false, true, true>(p, vec, b.groups, s);
         else bn_::launch<true, true, true>(p, vec, b.groups, s);
         if (int rc = check_launch("norm_gate_residual_bwd")) return rc;
-        if (gp && d_gate) {
-            const long long total = (long long)g * N;
-            const unsigned grid = (unsigned)std::min<long long>((total + 255) / 256, 8192);
-            if (types & 2) hipLaunchKernelGGL((bn_::norm_gate_sum<true>), dim3(grid), dim3(256), 0, s, (const float*)p.dg_part, b.splits, total, d_gate);
-            else hipLaunchKernelGGL((bn_::norm_gate_sum<false>), dim3(grid), dim3(256), 0, s, (const float*)p.dg_part, b.splits, total, d_gate);
-            if (int rc = check_launch("norm_gate_residual_bwd gate")) return rc;
-        }
+    }
+    if (d_gate && (gp || M == 0)) {                           // (no rows: G x N sums of nothing)
+        const long long total = (long long)(M == 0 ? G : g) * N;
+        const int splits = M == 0 ? 0 : b.splits;
+        const unsigned grid = (unsigned)std::min<long long>((total + 255) / 256, 8192);
+        if (types & 2) hipLaunchKernelGGL((bn_::norm_gate_sum<true>), dim3(grid), dim3(256), 0, s, (const float*)p.dg_part, splits, total, d_gate);
+        else hipLaunchKernelGGL((bn_::norm_gate_sum<false>), dim3(grid), dim3(256), 0, s, (const float*)p.dg_part, splits, total, d_gate);
+        if (int rc = check_launch("norm_gate_residual_bwd gate")) return rc;
     }
     if (p.want) {
         hipLaunchKernelGGL(bn_::norm_columns, dim3((unsigned)((N + 31) / 32), 5), dim3(256), 0, s, f);

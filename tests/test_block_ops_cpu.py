@@ -248,3 +248,8 @@ def test_gated_unit_entry_points():
     assert lib.btvae_gated_unit_bwd_bytes(unit(), g(dwu=0)) == -1 and "all weights" in nv.last_error()
     assert lib.btvae_gated_unit_bwd(unit(), g(), a, store, a, need - 1, None) != 0 and "workspace" in nv.last_error()
     assert lib.btvae_gated_unit_bwd(unit(), g(), None, 0, a, need, None) != 0 and "workspace" in nv.last_error()
+
+
+def test_norm_gradient_of_absent_gate_is_refused():
+    assert nv.lib().btvae_norm_gate_residual_bwd(None, None, None, None, None, 3, 1.0, None, None, None, None, 0, 1, None, None, None, 1 << 20, None, None, None, None, None, None, 0, 0, 0, 8, None) != 0
+    assert "absent gate" in nv.last_error()

@@ -1019,3 +1019,24 @@ def test_unit_whose_results_pass_l2():
     y2, tape2 = B.gated_feed_forward_tape(x[-m:].contiguous(), wg, wu, wd)
     dx2 = tape2.backward(dy[-m:].contiguous())[0]
     assert torch.equal(y[-m:], y2) and torch.equal(dx[-m:], dx2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_norm_gradients_of_no_rows(dev, dtype):
+    """A batch without rows: the gradients of what its rows would share, gate rows and channel scale among them, are zeros, whatever the allocator's
+    memory held before."""
+    N, G = 40, 3
+    w = lambda: torch.ones(N, device=dev, requires_grad=True)
+    none = torch.empty(0, N, dtype=dtype, device=dev)
+    gate = torch.ones(G, N, dtype=dtype, device=dev, requires_grad=True)
+    shared = [gate, w(), w(), w(), w(), w()]
+    stream, normed = B.norm_gate_residual(none, none, gate=gate, scale=shared[1], post_norm="layer", post_weight=shared[2], post_bias=shared[3], pre_norm="layer",
+                                          pre_weight=shared[4], pre_bias=shared[5])
+    junk = [torch.full((G, N), float("nan"), dtype=dtype, device=dev) for _ in range(64)] + [torch.full((N,), float("nan"), device=dev) for _ in range(64)]
+    del junk
+    for t, g in zip(shared, torch.autograd.grad(stream.sum() + normed.sum(), shared)):
+        assert g.shape == t.shape and torch.equal(g, torch.zeros_like(t))
+    tape = B.norm_gate_residual_tape(none, none, gate=gate.detach())[2]
+    junk = [torch.full((G, N), float("nan"), dtype=dtype, device=dev) for _ in range(64)]
+    del junk
+    assert torch.equal(tape.backward(none, none)[2], torch.zeros_like(gate))
