@@ -813,14 +813,15 @@ def _block_precision():
     return (1, torch.bfloat16) if nv.lib().btvae_get_gemm_precision() == 1 else (3, torch.float32)
 
 
-def gated_forward(u: GatedUnit, x: torch.Tensor, saved: Optional[list]):
+def gated_forward(u: GatedUnit, x: torch.Tensor, train: bool, saved: Optional[list]):
     """x -> x + sum of the layers' branches; the stream between the layers is fp32, every addition and the next layer's norm
-    are one pass.  ``saved``: receives the layers' tapes as one entry."""
+    are one pass.  ``train``: the products of the pass that gradients are taken of, whether they are or not (``saved`` None): neither
+    8 bits nor the form for few rows.  ``saved``: receives the layers' tapes as one entry."""
     planes, btype = _block_precision()
     stream = x.detach()
     stream = (stream if stream.dtype == torch.float32 else stream.float()).contiguous()
     M = stream.shape[0]
-    few = saved is None and M <= nv.lib().btvae_few_rows_max()
+    few = not train and saved is None and M <= nv.lib().btvae_few_rows_max()
     if few:
         btype = torch.float32
     branch, scale, tapes = None, None, []
@@ -829,7 +830,7 @@ def gated_forward(u: GatedUnit, x: torch.Tensor, saved: Optional[list]):
         stream, n, ntape = B.norm_gate_residual_tape(stream, pre_weight=layer.norm.detach(), **add)
         weights, biases = [m.weight.detach() for m in (layer.gate, layer.up, layer.down)], [m.bias.detach() for m in (layer.gate, layer.up, layer.down)]
         act, ftape = B.ACTIVATIONS[layer.activation], None
-        if saved is None and layer.eval_fp8:
+        if not train and saved is None and layer.eval_fp8:
             # a copy of the weights as they are now, made per pass like the other products' images
             branch = B.fp8_gated_feed_forward(n, B.fp8_gated_weights(*weights, *biases), layer.activation)
         elif few:
@@ -921,7 +922,7 @@ def net_forward(plan: NetPlan, x: torch.Tensor, train: bool, tape: Optional[NetT
         # adds it in that format)
         pairs_ok = not train and (i + 1 < nt or all(len(units) > 1 for units in plan.heads.values()))
         if isinstance(u, GatedUnit):
-            h = gated_forward(u, h, tape.trunk if tape is not None else None)
+            h = gated_forward(u, h, train, tape.trunk if tape is not None else None)
             continue
         if i + 1 < nt and isinstance(plan.trunk[i + 1], GatedUnit):
             pairs_ok = False

@@ -1040,3 +1040,26 @@ def test_norm_gradients_of_no_rows(dev, dtype):
     junk = [torch.full((G, N), float("nan"), dtype=dtype, device=dev) for _ in range(64)]
     del junk
     assert torch.equal(tape.backward(none, none)[2], torch.zeros_like(gate))
+
+
+@pytest.mark.parametrize("prec", ["fp32_split2", "bf16"])
+@pytest.mark.parametrize("M", [20, 130])
+def test_gated_layers_of_a_training_network_without_gradients(dev, prec, M):
+    """A network in training mode has one forward pass: under no_grad it gives the head outputs and the BatchNorm statistics of the pass that
+    gradients are taken of, to the last bit; ``gated_eval_fp8`` changes neither, and changes the outputs in eval mode."""
+    runs = []
+    try:
+        for fp8, grad in ((False, True), (True, True), (True, False)):
+            m = gated_model(dev, prec, 1, 1, eval_fp8=fp8).train()
+            m._check_arena()
+            x = rnd(dev, M, 8 + conditions(prec), seed=91)
+            with torch.set_grad_enabled(grad):
+                out = m.decoder(x)
+            runs.append(({k: v.detach().clone() for k, v in out.items()}, {k: v.clone() for k, v in m.decoder.state_dict().items() if "running" in k}))
+        assert runs[0][1]
+        for got in runs[1:]:
+            for a, b in zip(runs[0], got):
+                for k in a:
+                    assert torch.equal(a[k], b[k]), k
+    finally:
+        nv.set_gemm_precision("fp32")
