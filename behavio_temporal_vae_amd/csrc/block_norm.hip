@@ -264,7 +264,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd(const Args p) 
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] += f[i] * x[i];
             R::template store<RH>(p.v, o, p.N, t, v);
-            if (p.stats && t == 0) { p.stats[row] = mean; p.stats[p.M + row] = q; }
+            if (p.stats && t == 0) { p.stats[row] = mean; p.stats[(long long)p.M + row] = q; }
         }
         if (p.n) {
             moments<T, NV, VEC>(v, p.pre, p.eps, p.N, t, red, turn, mean, q);
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd(const Args p) 
             R::template unpack<BH>(rn, p.N, t, e);
             R::template unpack<RH>(rr, p.N, t, h);
         }
-        const float mean = p.post != NONE ? p.stats[row] : 0.f, q = p.post != NONE ? p.stats[p.M + row] : 1.f;
+        const float mean = p.post != NONE ? p.stats[row] : 0.f, q = p.post != NONE ? p.stats[(long long)p.M + row] : 1.f;
         const float mean2 = p.dn ? p.stats[2LL * p.M + row] : 0.f, q2 = p.dn ? p.stats[3LL * p.M + row] : 0.f;
         bool last = ++at.s == at.end;                         // of its stretch
         if (last) {

@@ -1063,3 +1063,37 @@ def test_gated_layers_of_a_training_network_without_gradients(dev, prec, M):
                     assert torch.equal(a[k], b[k]), k
     finally:
         nv.set_gemm_precision("fp32")
+
+
+def test_norm_of_more_rows_than_half_the_numbers(dev):
+    """2^30 + 3 rows of one column: the statistics' four rows lie further apart than 32-bit indices reach.  The first, some middle and the last rows, both
+    ways, against 64 bits: a dozen float32 roundings (the bound of 16 2^-24 of what is added), each result rounded once, the stream's own rounding in front of its
+    norm's gradient (which the backward pass recomputes unrounded)."""
+    M, eps = 2 ** 30 + 3, 1.0
+    need = 20 * 2 * M + 16 * M
+    free = torch.cuda.mem_get_info()[0]
+    assert free > need, f"{need >> 30} GiB of device memory are needed, {free >> 30} are free"
+    torch.cuda.empty_cache()
+    base = torch.arange(M, dtype=torch.int32, device=dev)
+
+    def values(k):                                             # (bf16 holds them: 7 bits and a sign)
+        v = torch.empty(M, 1, dtype=BF, device=dev)
+        v[:, 0] = (base + k) % 251 - 125
+        return v.mul_(2.0 ** -5)
+
+    res, branch = values(0), values(77)
+    stream, normed, tape = B.norm_gate_residual_tape(res, branch, scale=0.5, post_norm="rms", pre_norm="rms", eps=eps)
+    dv, dn = values(13), values(101)
+    dres, dbranch = tape.backward(dv, dn, need=(True, True) + (False,) * 6)[:2]
+    at = torch.cat([torch.arange(0, 300), torch.arange(M // 2 - 150, M // 2 + 150), torch.arange(M - 300, M)]).to(dev)
+    r, y = (t[at].double().requires_grad_(True) for t in (res, branch))
+    norm = lambda t: t / torch.sqrt(t * t + eps)
+    rv = r + 0.5 * norm(y)
+    rn = norm(rv)
+    gr, gy = torch.autograd.grad([rv, rn], [r, y], [dv[at].double(), dn[at].double()])
+    f = 16 * E
+    within(stream[at], rv.detach(), U * rv.detach().abs() + f * (r.detach().abs() + 1), "stream")
+    within(normed[at], rn.detach(), U * rn.detach().abs() + 4 * f, "normed")
+    size = dv[at].double().abs() + dn[at].double().abs()
+    within(dres[at], gr, U * gr.abs() + 4 * f * size, "d residual")
+    within(dbranch[at], gy, U * gy.abs() + 4 * f * size, "d branch")
