@@ -164,7 +164,8 @@ __device__ __forceinline__ float exp_clamped(float x) {
     const float e = __builtin_amdgcn_exp2f(t);
     return __builtin_fmaf(e, r * 0.69314718f, e);
 }
-// 1 / x for 1 <= x (an infinity as 3e38): the approximate reciprocal and one Newton step
+// 1 / x for 1 <= x (an infinity as 3e38): the approximate reciprocal and one Newton step.  A result below 2^-126 is 0 (the instruction's, and so the
+// step's): the sigmoid below -87.3, whose product with a very negative a is 0 therefore.
 __device__ __forceinline__ float reciprocal(float x) {
     x = fminf(x, 3e38f);
     const float y = __builtin_amdgcn_rcpf(x);
@@ -184,7 +185,8 @@ __device__ __forceinline__ void act_value(int act, float a, float& v, float& d) 
             const float t = reciprocal(1.f + 0.5f * x);
             const float P = -1.26551223f + t * (1.00002368f + t * (0.37409196f + t * (0.09678418f + t * (-0.18628806f + t * (0.27886807f +
                             t * (-1.13520398f + t * (1.48851587f + t * (-0.82215223f + t * 0.17087277f))))))));
-            g = exp_clamped(-0.5f * a * a);
+            const float e = -0.5f * a * a;
+            g = e < -87.f ? 0.f : exp_clamped(e);             // (a times the clamped value would grow with a)
             half_erfc = 0.5f * t * g * exp_clamped(P);
         }
         const float phi = a < 0.f ? half_erfc : 1.f - half_erfc;

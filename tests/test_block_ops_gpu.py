@@ -1097,3 +1097,39 @@ def test_norm_of_more_rows_than_half_the_numbers(dev):
     size = dv[at].double().abs() + dn[at].double().abs()
     within(dres[at], gr, U * gr.abs() + 4 * f * size, "d residual")
     within(dbranch[at], gy, U * gy.abs() + 4 * f * size, "d branch")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M", [5, 60])
+def test_ffn_activation_of_large_values(dev, M, act):
+    """Gate pre-activations up to the largest finite magnitudes, float32: silu and gelu are 0 (their slope too) far below zero, the identity (slope 1) far above.
+    One up projection of 1 and a down weight of 1 hand act(a) and act'(a) out as they are: a product of one pair of values, exact but for three pieces' last bits.
+    Bounds: eight float32 roundings of the value, and what a sigmoid below the smallest normal number, 2^-126, loses: that times |a|, which is at most 104 before
+    e^a is no number at all."""
+    big = [88.0, 89.5, 1e2, 1e4, 1e10, 1e20, 1e30, 1e35, 1e37, 3e38]
+    vals = torch.tensor([-v for v in big] + big + [0.0, 1.0, -1.0, -20.0, 20.0] * 2 + [-87.0, 87.0] * 10 + [0.5] * 10, device=dev)[:, None]
+    vals = vals[:M] if M < 10 else vals
+    one = torch.ones(1, 1, device=dev)
+    zero, bu = torch.zeros(1, 1, device=dev), torch.ones(1, device=dev)
+    leaves = vals.clone().requires_grad_(True)
+    with torch.no_grad():
+        y = B.gated_feed_forward(vals, one, zero, one, None, bu, None, activation=act)
+    yg = B.gated_feed_forward(leaves, one, zero, one, None, bu, None, activation=act)
+    g, = torch.autograd.grad(yg.sum(), leaves)
+    a = vals.double().requires_grad_(True)
+    if act == "silu":
+        ref = a / (1 + torch.exp(-a))
+    else:
+        ref = torch.where(a < 0, 0.5 * a * torch.special.erfc(-a / math.sqrt(2)), a * (1 - 0.5 * torch.special.erfc(a / math.sqrt(2))))
+    s = torch.sigmoid(a.detach())
+    if act == "silu":
+        slope = s * (1 + torch.where(a.detach() > 700, torch.zeros_like(s), a.detach() * torch.sigmoid(-a.detach())))
+    else:
+        phi = torch.exp(-0.5 * a.detach() ** 2) / math.sqrt(2 * math.pi)
+        slope = 0.5 * torch.special.erfc(-a.detach() / math.sqrt(2)) + torch.where(phi == 0, phi, a.detach() * phi)
+    ref = ref.detach()
+    tiny = 2.0 ** -126 * 104
+    # erfc and exp are good to 1.2e-7 of a value of at most 1, the slope's terms are of size 1
+    within(y, ref, 8 * E * ref.abs() + 4 * E * (a.detach().abs() < 20) * (a.detach().abs() + 1) + tiny, "act, no graph")
+    within(yg, ref, 8 * E * ref.abs() + 4 * E * (a.detach().abs() < 20) * (a.detach().abs() + 1) + tiny, "act")
+    within(g, slope, 16 * E + 8 * E * slope.abs(), "slope")
