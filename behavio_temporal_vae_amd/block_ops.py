@@ -119,7 +119,7 @@ class _Operand:
 def _operand(t, planes, reads=0) -> _Operand:
     """``t`` laid out as an operand, or where it is: a bf16 matrix with whole 16-byte pieces that is read against few others."""
     rows, cols = t.shape
-    if planes == 1 and t.dtype == torch.bfloat16 and cols % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0 and reads < 2048:
+    if planes == 1 and t.dtype == torch.bfloat16 and cols % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0 and reads < 2048 and 2 * _pitch(t) < 2 ** 23:
         return _Operand(t.data_ptr(), 2 * _pitch(t), cols, t)
     ld = _up(cols, 32) * 6 if planes == 3 else _up(cols, 64) * 2
     buf = torch.empty(rows * ld, dtype=torch.uint8, device=t.device)

@@ -726,7 +726,7 @@ static int check_cols(const bk::ColJob& j, int planes, int R) {
     const int unit = planes == 3 ? 16 : 8, M8 = bk::tiles((int)j.M, unit) * unit, N8 = bk::tiles((int)j.N, unit) * unit;
     BTVAE_REQUIRE(!j.out1 || (j.off1 >= j.rows0 && j.rows1 >= 0 && j.off1 + j.rows1 <= j.M), "block_wgrad: bad row ranges");
     BTVAE_REQUIRE(R == 0 || (operand_ok(j.A, j.lda, planes, M8) && operand_ok(j.B, j.ldb, planes, N8)), "block_wgrad: operand rows must start on 16 bytes and hold whole groups of %d columns", unit);
-    BTVAE_REQUIRE(j.lda < (1 << 23) && j.ldb < (1 << 23), "block_wgrad: rows of more than 8 MiB");
+    BTVAE_REQUIRE(j.lda < bk::MAX_PITCH && j.ldb < bk::MAX_PITCH, "block_wgrad: rows of more than 8 MiB");
     BTVAE_REQUIRE(R <= bk::MAX_ROWS, "block_wgrad: too many rows");
     return 0;
 }
@@ -811,8 +811,9 @@ struct Operand { const void* at; long long ld; int width; bool pack; };
 // requests (measured, 65,536 x 1000 times 1000 x N, in place against the copy and the product: N 512 80 and 118 us, 1024 155
 // and 178, 2048 346 and 316, 4096 653 and 596; never copying costs a gated unit's training pass of 65,536 x 1000 x 2000 3 %)
 constexpr long long REPACK_READS = 2048;
+// Rows MAX_PITCH bytes apart and more are beyond the products' offsets, and are laid out side by side.
 static bool in_place(const void* t, int t16, long long ld, int cols, int planes, long long reads) {
-    if (planes != 1 || !t16 || cols % 8 || ld % 8 || !al16(t)) return false;
+    if (planes != 1 || !t16 || cols % 8 || ld % 8 || !al16(t) || 2 * ld >= MAX_PITCH) return false;
     return reads < REPACK_READS || (2 * ld % 64 == 0 && ((uintptr_t)t & 63) == 0);
 }
 static long long bytes_of(long long cols, int planes) { return cols * (planes == 3 ? 6 : 2); }

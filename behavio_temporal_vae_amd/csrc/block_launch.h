@@ -6,6 +6,7 @@
 namespace btvae_block {
 
 constexpr int CHIP = 256;                                             // compute units
+constexpr int MAX_PITCH = 1 << 23;                                    // bytes from row to row of an operand: a tile's rows are found with 32-bit offsets
 constexpr int MAX_ROWS = 0x7FE00000;                                  // row numbers, and those a few tiles or splits past them, are 32 bits
 
 inline int tiles(int n, int t) { return (n + t - 1) / t; }
@@ -31,7 +32,7 @@ int launch_rows(Args& p, int z, hipStream_t s, const char* what) {
     const long long items = (long long)p.tiles_m * p.tiles_n * z;
     if (p.M > MAX_ROWS) return btvae::set_error("%s: too many rows", what);
     if (items >= (1 << 29)) return btvae::set_error("%s: too many tiles", what);
-    if (p.lda >= (1 << 23) || p.ldb >= (1 << 23)) return btvae::set_error("%s: rows of more than 8 MiB", what);
+    if (p.lda >= MAX_PITCH || p.ldb >= MAX_PITCH) return btvae::set_error("%s: rows of more than 8 MiB", what);
     p.stream = z == 1 && (long long)p.M * (EP == EP_GATED_BWD ? 2 * p.half : p.N) * (EP == EP_LINEAR && p.c_type == T_F32 ? 4 : 2) > STREAM_BYTES;
     p.by_tiles = div_by(p.tiles_m * p.tiles_n); p.by_band = div_by(8 * p.tiles_n); p.by_last = div_by(p.tiles_m % 8 ? p.tiles_m % 8 : 8);
     const dim3 grid((unsigned)std::min<long long>(items, FMT == FMT_SPLIT ? 2 * CHIP : CHIP));

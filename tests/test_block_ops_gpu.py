@@ -1133,3 +1133,28 @@ def test_ffn_activation_of_large_values(dev, M, act):
     within(y, ref, 8 * E * ref.abs() + 4 * E * (a.detach().abs() < 20) * (a.detach().abs() + 1) + tiny, "act, no graph")
     within(yg, ref, 8 * E * ref.abs() + 4 * E * (a.detach().abs() < 20) * (a.detach().abs() + 1) + tiny, "act")
     within(g, slope, 16 * E + 8 * E * slope.abs(), "slope")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_ffn_rows_far_apart(dev, dtype):
+    """x, the result's gradient and a weight whose rows are 8 MiB and more apart (the last position of every long sequence, a slice of a large buffer): the
+    results of the same values side by side, to the last bit."""
+    M, K, F, N = 40, 64, 48, 64
+    t = ffn_case(dev, M, K, F, N, dtype, True, seed=17)
+    dy = rnd(dev, M, N, seed=18, dtype=dtype)
+    pitch = 2 ** 22 + 64                                       # elements: past 8 MiB in bf16, 16 MiB in fp32
+    room = torch.empty(48, pitch, dtype=dtype, device=dev)     # (F rows, the most of the three)
+    want_y, want = ffn_grads(t, "silu", dy)
+    with torch.no_grad():
+        plain = call_ffn(t, "silu")
+    for k in ("x", "dy", "wg", "wd"):
+        src = dy if k == "dy" else t[k]
+        far = room[:src.shape[0], :src.shape[1]] if src.shape[0] <= 48 else torch.empty(src.shape[0], pitch, dtype=dtype, device=dev)[:, :src.shape[1]]
+        far.copy_(src)
+        u = t if k == "dy" else {**t, k: far}
+        with torch.no_grad():
+            assert torch.equal(call_ffn(u, "silu"), plain), k
+        y, tape = B.gated_feed_forward_tape(u["x"], u["wg"], u["wu"], u["wd"], u["bg"], u["bu"], u["bd"])
+        assert torch.equal(y, want_y), k
+        for name, g in zip(("x", "wg", "wu", "wd", "bg", "bu", "bd"), tape.backward(far if k == "dy" else dy)):
+            assert torch.equal(g, want[name]), (k, name)
