@@ -431,7 +431,7 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
         for (int kb = wid; kb < kbn; kb += NWV) {
             const i32x4 a0 = *reinterpret_cast<const i32x4*>(w + kb * 128 + kq * 32), a1 = *reinterpret_cast<const i32x4*>(w + kb * 128 + kq * 32 + 16);
             const i32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-            const float sw = pow2i((int)wsc[kb] - 127);
+            const int ew = (int)wsc[kb] - 127;
             bf16x8 wa[4];
             expand32(a, wa);
 #pragma unroll
@@ -479,8 +479,9 @@ __global__ __launch_bounds__(512) void gemm_few(const FewArgs p) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa[g], xb[g], d, 0, 0, 0);
                 // a lane's four results: x row lane & 15, the row it quantised; weight rows of one block (GATED: lanes 0-31 gate, 32-63 up)
+                // (both scales at once: one after the other a sum may leave float32's range on its way)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][i] += (d[i] * pow2i(ex)) * sw;
+                for (int i = 0; i < 4; ++i) acc[t][i] += __builtin_amdgcn_ldexpf(d[i], ex + ew);
             }
         }
     }

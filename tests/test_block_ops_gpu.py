@@ -1158,3 +1158,19 @@ def test_ffn_rows_far_apart(dev, dtype):
         assert torch.equal(y, want_y), k
         for name, g in zip(("x", "wg", "wu", "wd", "bg", "bu", "bd"), tape.backward(far if k == "dy" else dy)):
             assert torch.equal(g, want[name]), (k, name)
+
+
+@pytest.mark.parametrize("M", [3, 20])
+@pytest.mark.parametrize("big,small", [(1e35, 2.0 ** -20), (2.0 ** -110, 2.0 ** 70)])
+def test_fp8_few_rows_of_large_and_small_values(dev, M, big, small):
+    """Rows and weights whose scales are far from 1 in opposite directions: a block's sum times one scale alone would leave float32's range, the result does
+    not.  Few rows are held to the float32 sums of their definition, as many rows are."""
+    K, N = 256, 40
+    x, w = rnd(dev, M, K, seed=1).abs() * big, rnd(dev, N, K, seed=2).abs() * small
+    xq, wq = e4m3_64(x, 1, 128), e4m3_64(w, 128, 128)
+    ref = xq @ wq.t()
+    W = B.fp8_weight(w)
+    lim = (K + 8) * E * (xq.abs() @ wq.abs().t()) + 2 * E * ref.abs()
+    assert ref.abs().max() < 1e38
+    within(B.fp8_linear(x, W), ref, lim, "few rows")
+    within(B.fp8_linear(x.repeat(40, 1), W)[:M], ref, lim, "many rows")
