@@ -172,11 +172,16 @@ class GatedTape:
         for a, b in ((0, 1), (3, 4)):
             if outs[a] is not None and outs[b] is not None and outs[a].dtype != outs[b].dtype:
                 raise TypeError(f"outs: {names[a]} and {names[b]} must be of one type")
+        spans = sorted((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size(), what) for o, what in zip(outs, names) if o is not None)
+        for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
+            if start < end:                                    # one launch writes several of them
+                raise ValueError(f"outs: {a} and {b} share memory")
 
     def backward(self, dy, need_input=True, need_weights=True, outs=None, accumulate=False):
         """Gradients (x, w_gate, w_up, w_down, b_gate, b_up, b_down) for the gradient ``dy`` of the result; entries that are
         not wanted, or belong to an absent bias, are None.  ``outs``: six tensors (float32 or bfloat16, contiguous, None for
-        biases that are absent or not wanted) that the weights' and biases' gradients are written to, or added to with ``accumulate``."""
+        biases that are absent or not wanted; no two in the same memory) that the weights' and biases' gradients are written to, or added to
+        with ``accumulate``."""
         x, weights = self.x, self.weights
         dev, (M, K), N = x.device, x.shape, weights[2].shape[0]
         nv.ensure_device(dev)

@@ -253,3 +253,29 @@ def test_gated_unit_entry_points():
 def test_norm_gradient_of_absent_gate_is_refused():
     assert nv.lib().btvae_norm_gate_residual_bwd(None, None, None, None, None, 3, 1.0, None, None, None, None, 0, 1, None, None, None, 1 << 20, None, None, None, None, None, None, 0, 0, 0, 8, None) != 0
     assert "absent gate" in nv.last_error()
+
+
+def test_ffn_outs_that_share_memory_are_refused():
+    """Gradients that one launch writes: tied weights, or slices of one buffer that overlap, would race."""
+    w = [torch.zeros(8, 8) for _ in range(3)]
+    tape = B.GatedTape(torch.zeros(5, 8), w, [torch.zeros(8)] * 3, None, None, False)
+    outs = lambda: [torch.zeros(8, 8) for _ in range(3)] + [torch.zeros(8) for _ in range(3)]
+    tape._check_outs(outs())
+    whole = torch.zeros(6 * 64)
+    tape._check_outs([whole[64 * i:64 * i + 64].view(8, 8) for i in range(3)] + [whole[192 + 8 * i:200 + 8 * i] for i in range(3)])
+    for i, j in ((0, 1), (0, 2), (1, 2), (3, 4), (3, 5), (4, 5)):
+        o = outs()
+        o[j] = o[i]
+        with pytest.raises(ValueError, match="share memory"):
+            tape._check_outs(o)
+    o = outs()
+    room = torch.zeros(100)
+    o[0], o[1] = room[:64].view(8, 8), room[36:].view(8, 8)
+    with pytest.raises(ValueError, match="w_gate and w_up share memory"):
+        tape._check_outs(o)
+    o = outs()
+    o[4] = o[0].view(-1)[60:64].repeat(2)                      # (a copy)
+    tape._check_outs(o)
+    o[4] = o[0].view(-1)[56:]
+    with pytest.raises(ValueError, match="w_gate and b_up share memory"):
+        tape._check_outs(o)
