@@ -569,14 +569,15 @@ def _fp8_product(x: Fp8Rows, w: Fp8Weight, bias, out):
 
 def fp8_linear(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype] = None):
     """x weight^T + bias with x quantised by ``fp8_quantize`` (or given as ``Fp8Rows``).  ``out_dtype``: float32 or
-    bfloat16, by default x's (float32 for ``Fp8Rows``).  Float32 results, and those of up to 32 rows of x, come from float32 sums; bfloat16 results from the
-    8-bit matrix pipe, whose own sums are off by about 2^-16 of a result.  Evaluation only: no backward pass."""
+    bfloat16, by default x's (float32 for ``Fp8Rows``).  Float32 results, and those of up to 32 rows that are quantised here, come from float32 sums; other
+    bfloat16 results from the 8-bit matrix pipe, whose own sums are off by about 2^-16 of a result.  Evaluation only: no backward pass, and what
+    wants a gradient is refused."""
     if not isinstance(weight, Fp8Weight):
         raise TypeError("weight must come from fp8_weight")
     packed = isinstance(x, Fp8Rows) and not isinstance(x, Fp8Weight)
     if not packed:
         _tensor(x, "x")
-        _no_graph("fp8_linear", x, bias)
+    _no_graph("fp8_linear", None if packed else x, bias)
     N, K = weight.shape
     if len(x.shape) < 1 or x.shape[-1] != K:
         raise ValueError(f"x must have {K} columns, got {list(x.shape)}")

@@ -279,3 +279,13 @@ def test_ffn_outs_that_share_memory_are_refused():
     o[4] = o[0].view(-1)[56:]
     with pytest.raises(ValueError, match="w_gate and b_up share memory"):
         tape._check_outs(o)
+
+
+def test_fp8_bias_that_wants_a_gradient_is_refused_beside_quantised_rows():
+    rows = B.Fp8Rows(torch.zeros(M, 128, dtype=torch.uint8), torch.zeros(M, 4, dtype=torch.uint8), (M, K))
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        B.fp8_linear(rows, weight(), torch.zeros(N, requires_grad=True))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="MI355X only"):
+        B.fp8_linear(rows, weight(), torch.zeros(N, requires_grad=True))
+    with pytest.raises(TypeError, match="x must be a tensor"):
+        B.fp8_linear([1.0], weight(), torch.zeros(N, requires_grad=True))

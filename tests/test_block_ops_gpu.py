@@ -1174,3 +1174,14 @@ def test_fp8_few_rows_of_large_and_small_values(dev, M, big, small):
     assert ref.abs().max() < 1e38
     within(B.fp8_linear(x, W), ref, lim, "few rows")
     within(B.fp8_linear(x.repeat(40, 1), W)[:M], ref, lim, "many rows")
+
+
+def test_fp8_bias_that_wants_a_gradient_is_refused(dev):
+    """Also beside rows that are quantised already: a result without a graph would drop the bias's gradient in silence."""
+    W, bias = B.fp8_weight(rnd(dev, 12, 8)), torch.zeros(12, device=dev, requires_grad=True)
+    q = B.fp8_quantize(rnd(dev, 40, 8))
+    for x in (q, rnd(dev, 40, 8)):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            B.fp8_linear(x, W, bias)
+    with torch.no_grad():
+        assert B.fp8_linear(q, W, bias).shape == (40, 12)
