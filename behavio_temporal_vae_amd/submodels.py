@@ -38,6 +38,10 @@ class GatedLayer(torch.nn.Module):
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"unknown gated_activation {activation!r}; choose from {list(ACTIVATIONS)}")
+        if width > nv.lib().btvae_norm_max_columns():
+            raise ValueError(f"gated_layers: networks of up to {nv.lib().btvae_norm_max_columns()} neurons, got {width}")
+        if not isinstance(hidden, int) or hidden < 1:
+            raise ValueError(f"gated_hidden must be a number of units, got {hidden!r}")
         self.activation, self.eval_fp8 = activation, bool(eval_fp8)
         self.norm = torch.nn.Parameter(torch.ones(width))
         self.gate, self.up, self.down = torch.nn.Linear(width, hidden), torch.nn.Linear(width, hidden), torch.nn.Linear(hidden, width)
@@ -60,6 +64,8 @@ class NNBlock(torch.nn.Module):
         S, L = torch.nn.Sequential, torch.nn.Linear
         self.input_layer = S(L(input_dim, num_neurons), ACTIVATION)
         self.middle_layers = torch.nn.ModuleList(S(L(num_neurons, num_neurons), ACTIVATION) for _ in range(num_hidden_layers))
+        if gated_layers is not None and (not isinstance(gated_layers, int) or gated_layers < 0):
+            raise ValueError(f"gated_layers must be a number of layers, got {gated_layers!r}")
         if gated_layers:
             self.gated_layers = torch.nn.ModuleList(GatedLayer(num_neurons, gated_hidden or 2 * num_neurons, gated_activation, gated_eval_fp8)
                                                     for _ in range(gated_layers))

@@ -289,3 +289,25 @@ def test_fp8_bias_that_wants_a_gradient_is_refused_beside_quantised_rows():
         B.fp8_linear(rows, weight(), torch.zeros(N, requires_grad=True))
     with pytest.raises(TypeError, match="x must be a tensor"):
         B.fp8_linear([1.0], weight(), torch.zeros(N, requires_grad=True))
+
+
+@pytest.mark.parametrize("config,words", [(dict(gated_layers=-1), "gated_layers"), (dict(gated_layers=1.5), "gated_layers"), (dict(gated_layers="2"), "gated_layers"),
+                                          (dict(gated_layers=1, gated_hidden=-4), "gated_hidden"), (dict(gated_layers=1, gated_hidden=2.5), "gated_hidden"),
+                                          (dict(gated_layers=1, num_neurons=8193), "up to 8192 neurons"), (dict(gated_layers=2, gated_activation="tanh"), "gated_activation")])
+def test_gated_layers_of_a_configuration_are_checked(config, words):
+    """What the layers cannot be is refused where the network is built, not in its first forward pass."""
+    from behavio_temporal_vae_amd.submodels import GaussianNN, NNBlock
+    common = dict(num_neurons=16, num_hidden_layers=0, **config) if "num_neurons" not in config else dict(num_hidden_layers=0, **config)
+    with pytest.raises(ValueError, match=words):
+        NNBlock(3, 4, **common)
+    with pytest.raises(ValueError, match=words):
+        GaussianNN(3, 4, **common)
+
+
+def test_gated_layers_of_a_configuration():
+    from behavio_temporal_vae_amd.submodels import NNBlock
+    for none in (0, None):
+        assert not hasattr(NNBlock(3, 4, num_neurons=16, gated_layers=none), "gated_layers")
+    block = NNBlock(3, 4, num_neurons=16, gated_layers=2)
+    assert [tuple(g.gate.weight.shape) for g in block.gated_layers] == [(32, 16)] * 2
+    assert NNBlock(3, 4, num_neurons=16, gated_layers=1, gated_hidden=5).gated_layers[0].down.weight.shape == (16, 5)
