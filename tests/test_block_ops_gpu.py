@@ -1185,3 +1185,81 @@ def test_fp8_bias_that_wants_a_gradient_is_refused(dev):
             B.fp8_linear(x, W, bias)
     with torch.no_grad():
         assert B.fp8_linear(q, W, bias).shape == (40, 12)
+
+
+# ---- kernels that only large sizes, or widths between the others, reach --------------------------------------------------------
+@pytest.mark.parametrize("planes", [1, 3])
+@pytest.mark.parametrize("M,N,R", [(2050, 1001, 9001), (1062, 203, 66000), (4001, 4100, 1025)])
+def test_block_wgrad_large_tiles(dev, planes, M, N, R):
+    """Weight gradients that fill the chip with 256 x 256 tiles (tiles times rows / 1024 of 256 and more), ragged in columns and rows, every element against
+    64 bits; sums added to what was there."""
+    assert -(-M // 256) * -(-N // 256) * (R // 1024) >= 256
+    dt = F32 if planes == 3 else BF
+    a, b = rnd(dev, R, M, seed=1, dtype=dt), rnd(dev, R, N, seed=2, dtype=dt)
+    A, X = B._operand(a, planes, 1 << 30), B._operand(b, planes, 1 << 30)
+    need = nv.lib().btvae_block_wgrad_ws(M, N, R, planes)
+    ws = torch.full((need + 64,), 7.0, device=dev)
+    out = torch.full((M, N), 2.0, device=dev)
+    ref = a.double().t() @ b.double()
+    for acc in (1, 0):
+        nv.call("btvae_block_wgrad", A.ptr(), A.ld, X.ptr(), X.ld, ws.data_ptr(), need, out.data_ptr(), M, None, 0, 0, N, 0, acc, planes, M, N, R)
+        frob(out, ref + 2.0 * acc, E * (6 + math.sqrt(R)), "sum" if acc else "result")
+        # no element is further off than its own terms allow: R roundings of partial sums below the sum of magnitudes
+        within(out, ref + 2.0 * acc, (4 + math.sqrt(R)) * 4 * E * (a.double().abs().t() @ b.double().abs()) / math.sqrt(R) + 8 * E * (ref.abs() + 2), "element")
+    assert bool((ws[need:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_ffn_of_many_tiles(dev, dtype):
+    """A unit whose gated products, forward and backward, are several tiles to every workgroup, and whose weight gradients take the large tiles: the result and
+    every gradient against 64 bits.  float32: the bounds of the small sizes.  bfloat16: the operands' roundings (h, da, db: 2^-8 each) and the result's own are
+    independent from element to element, so a gradient's Frobenius error stays below 2^-8 of its terms' root sum of squares, which for sums of
+    independent terms is the result's norm: 2^-8 for each of at most three roundings."""
+    M, K, F, N = 8200, 264, 2010, 264
+    t = ffn_case(dev, M, K, F, N, dtype, True, seed=23)
+    dy = rnd(dev, M, N, seed=24, dtype=dtype)
+    y, got = ffn_grads(t, "silu", dy)
+    assert -(-M // 128) * -(-F // 128) > 2 * 512 and -(-2 * F // 256) * -(-K // 256) * (M // 1024) >= 256 and -(-N // 256) * -(-F // 256) * (M // 1024) < 256
+    ref = ffn_grads64(t, "silu", dy)
+    yr = ffn64({k: d64(v) for k, v in t.items()}, "silu")[3]
+    if dtype == F32:
+        check_ffn_forward(y, t, "silu")
+        for k, v in got.items():
+            n = {"x": 2 * F}.get(k, M)
+            frob(v, ref[k], 3 * E * ((4 + math.sqrt(K)) + (4 + math.sqrt(N)) + (4 + math.sqrt(n))), f"d{k}")
+        return
+    frob(y, yr, 2 * U, "y")
+    for k, v in got.items():
+        frob(v, ref[k], 3 * U, f"d{k}")
+
+
+@pytest.mark.parametrize("case", [(70, 1025, 35, F32, F32, "layer", "rms", True, True), (96, 1032, 32, BF, BF, "layer", "layer", True, True), (40, 1500, 1, F32, BF, "rms", "layer", False, True),
+                                  (2500, 2048, 500, BF, BF, "rms", "rms", False, True), (33, 2047, 11, F32, F32, "rms", "rms", False, False), (24, 1288, 0, F32, BF, None, "rms", True, True),
+                                  (9, 1096, 3, F32, F32, "layer", None, False, True)], ids=lambda c: f"{c[0]}x{c[1]}g{c[2]}")
+def test_norm_of_four_waves_a_row(dev, case):
+    """Widths from 1025 to 2048, where a row belongs to four waves: vector and scalar, all types, both kinds of column sums."""
+    test_norm_gate_residual(dev, case)
+
+
+def test_ffn_kept_projections_hold_24_bits(dev):
+    """bfloat16: the projections kept for the backward pass are good to 2^-15, not only to a bfloat16 rounding.  With one row that has a gradient the bias
+    gradients are that row's da and db as they were before any rounding, in float32: db = dh act(a), da = dh b act'(a), off by 2^-15 of a and of b through
+    the functions' slopes (|act''| <= 0.5 for silu), and by float32's sums and the fast exp (2^-18, generously).  A kept bfloat16 would be off by up to 2^-8 of a."""
+    M, K, F, N = 40, 64, 300, 24
+    t = ffn_case(dev, M, K, F, N, BF, True, seed=29)
+    dy = torch.zeros(M, N, dtype=BF, device=dev)
+    dy[33] = rnd(dev, N, seed=30, dtype=BF)
+    y, tape = B.gated_feed_forward_tape(*[t[k] for k in ("x", "wg", "wu", "wd", "bg", "bu", "bd")])
+    outs = [torch.empty(v.shape, device=dev) for v in (t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])]
+    tape.backward(dy, outs=outs)
+    r = {k: d64(v)[33:34] if k == "x" else d64(v) for k, v in t.items()}
+    a, b, _, _ = ffn64(r, "silu")
+    a, b = a[0], b[0]
+    s = torch.sigmoid(a)
+    v, d = a * s, s * (1 + a * (1 - s))
+    dh = dy[33].double() @ r["wd"]
+    cut, small = 2.0 ** -15, 2.0 ** -18
+    sums = (K + 4) * E * (r["x"][0].abs() @ r["wg"].abs().t() + r["x"][0].abs() @ r["wu"].abs().t() + 1) + small
+    dhe = (N + 4) * E * (dy[33].double().abs() @ r["wd"].abs()) + small * dh.abs()
+    within(outs[4], dh * v, dh.abs() * (cut * a.abs() * 1.1 + 1.1 * sums) + dhe * (v.abs() + 1), "db")
+    within(outs[3], dh * b * d, dh.abs() * ((cut * a.abs() * 0.5 + 1.1 * sums) * b.abs() + (cut * b.abs() + sums) * 1.1) + dhe * (1.1 * b.abs() + 1), "da")
