@@ -1263,3 +1263,56 @@ def test_ffn_kept_projections_hold_24_bits(dev):
     dhe = (N + 4) * E * (dy[33].double().abs() @ r["wd"].abs()) + small * dh.abs()
     within(outs[4], dh * v, dh.abs() * (cut * a.abs() * 1.1 + 1.1 * sums) + dhe * (v.abs() + 1), "db")
     within(outs[3], dh * b * d, dh.abs() * ((cut * a.abs() * 0.5 + 1.1 * sums) * b.abs() + (cut * b.abs() + sums) * 1.1) + dhe * (1.1 * b.abs() + 1), "da")
+
+
+@pytest.mark.parametrize("prec,width,bn", [("fp32_split2", 50, True), ("fp32_split2", 41, True), ("fp32_split", 41, False), ("fp32", 50, True), ("bf16", 50, True)])
+@pytest.mark.parametrize("M", [20, 200])
+def test_network_with_gated_layers_of_odd_widths(dev, prec, width, bn, M):
+    """Trunks whose rows are no whole groups of four or eight columns: head outputs and every gradient against 64 bits, bounds as above."""
+    m = gated_model(dev, prec, 1, 1, bn, width=width).train()
+    m._check_arena()
+    net = m.decoder
+    x = rnd(dev, M, 8 + conditions(prec), seed=51)
+    wmu, wsg = rnd(dev, M, 24, seed=52), rnd(dev, M, 24, seed=53)
+    try:
+        for p in net.parameters():
+            p.grad.zero_()
+        out = net(x)
+        ((out["mu"] * wmu).sum() + (out["sigma"] * wsg).sum()).backward()
+        wide = {k: p.detach().double().requires_grad_() for k, p in net.named_parameters()}
+        ref = net64(net, x.double(), True, wide)
+        ((ref["mu"] * wmu.double()).sum() + (ref["sigma"] * wsg.double()).sum()).backward()
+        tol = 40 * U if prec == "bf16" else 2000 * E
+        for k in ("mu", "sigma"):
+            frob(out[k], ref[k].detach(), tol, k)
+        whole = math.sqrt(sum(float(w.grad.norm()) ** 2 for w in wide.values()))
+        for k, p in net.named_parameters():
+            assert ((p.grad.double() - wide[k].grad).norm().item()) <= tol * whole, k
+    finally:
+        nv.set_gemm_precision("fp32")
+
+
+@pytest.mark.parametrize("N", [3, 60])
+def test_scoring_of_a_model_with_gated_layers(dev, N):
+    """Importance-weighted log-likelihoods through encoder and decoder with gated layers, few rows and many, against 64 bits.  Both networks' errors
+    (2000 2^-24 of a tensor's norm) enter a row's log-density times its residual over the deviation (sums of 24 terms of a few units each): 0.1 of a row's
+    terms' size at most is allowed for, relative 2^-10."""
+    from behavio_temporal_vae_amd.testing_lib import iw_loglikelihood_device
+    K, L, D = 7, 8, 24
+    m = gated_model(dev, "fp32_split2", 1, 1).eval()
+    x, c, eps = rnd(dev, N, D, seed=1, scale=0.3), rnd(dev, N, conditions("fp32_split2"), seed=2), rnd(dev, K, N, L, seed=3)
+    try:
+        with torch.no_grad():
+            ll, rlls, _ = iw_loglikelihood_device(m, x, c, K, mc_sample_batch_size=4, eps=eps, return_rlls=True)
+        wide = lambda net: {k: p.detach().double() for k, p in net.named_parameters()}
+        q = net64(m.encoder, torch.cat([x, c], 1).double(), False, wide(m.encoder))
+        z = q["mu"] + q["sigma"] * eps.double()
+        p = net64(m.decoder, torch.cat([z.reshape(K * N, L), c.double().repeat(K, 1)], 1), False, wide(m.decoder))
+        normal = lambda t, mu, sd: (-0.5 * ((t - mu) / sd) ** 2 - torch.log(sd) - 0.5 * math.log(2 * math.pi)).sum(-1)
+        r = normal(x.double().repeat(K, 1), p["mu"], p["sigma"]).view(K, N)
+        ref = torch.logsumexp(r + normal(z, torch.zeros_like(z), torch.ones_like(z)) - normal(z, q["mu"], q["sigma"]), 0) - math.log(K)
+        size = ((x.double().repeat(K, 1) - p["mu"]) / p["sigma"]).pow(2).sum(-1).view(K, N) + 60
+        within(rlls, r, size * 2.0 ** -10, "log-densities")
+        within(ll, ref, size.amax(0) * 2.0 ** -10, "scores")
+    finally:
+        nv.set_gemm_precision("fp32")
