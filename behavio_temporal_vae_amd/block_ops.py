@@ -257,7 +257,7 @@ def _ffn_few(x2, weights, biases, act):
     if _pitch(w_up) != _pitch(w_gate):
         w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     bf = int(x2.dtype == torch.bfloat16)
-    h = torch.empty(M, F, device=x2.device)                  # float32: few rows cost nothing to keep unrounded
+    h = torch.empty(M, F, dtype=torch.float32, device=x2.device)         # few rows cost nothing to keep unrounded
     y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
     nv.call("btvae_few_rows", _p(x2), bf, _pitch(x2), _p(w_gate), _p(w_up), bf, _pitch(w_gate), _p(biases[0]), _p(biases[1]), _p(h), 0, F, act, M, F, K)
     nv.call("btvae_few_rows", _p(h), 0, F, _p(w_down), None, bf, _pitch(w_down), _p(biases[2]), None, _p(y), bf, N, act, M, N, F)
@@ -491,7 +491,7 @@ class Fp8Rows:
         """The values held, as float32."""
         nv.ensure_device(self.device)
         rows, K = self.q.shape[0], self.shape[-1]
-        out = torch.empty(rows, K, device=self.device)
+        out = torch.empty(rows, K, dtype=torch.float32, device=self.device)
         nv.call("btvae_fp8_dequantize", _p(self.q), self.q.shape[1], _p(self.scales), self.scales.shape[1], self.blocks, _p(out), rows, K)
         return out.view(self.shape)
 
@@ -642,7 +642,7 @@ def fp8_gated_feed_forward(x, weights: Fp8GatedWeights, activation="silu", out_d
     nv.ensure_device(dev)
     y = torch.empty(M, N, dtype=dtype, device=dev)
     if M <= nv.lib().btvae_few_rows_max():
-        h = torch.empty(M, F, device=dev)
+        h = torch.empty(M, F, dtype=torch.float32, device=dev)
         nv.call("btvae_fp8_few_rows", _p(x2), int(x.dtype == torch.bfloat16), _pitch(x2), _p(w.gate.q), _p(w.gate.scales), _p(w.up.q), _p(w.up.scales), w.gate.q.shape[1],
                 w.gate.scales.shape[1], _p(w.b_gate), _p(w.b_up), _p(h), F, 0, act, M, F, K)
         nv.call("btvae_fp8_few_rows", _p(h), 0, F, _p(w.down.q), _p(w.down.scales), None, None, w.down.q.shape[1], w.down.scales.shape[1], _p(w.b_down), None,

@@ -311,3 +311,13 @@ def test_gated_layers_of_a_configuration():
     block = NNBlock(3, 4, num_neurons=16, gated_layers=2)
     assert [tuple(g.gate.weight.shape) for g in block.gated_layers] == [(32, 16)] * 2
     assert NNBlock(3, 4, num_neurons=16, gated_layers=1, gated_hidden=5).gated_layers[0].down.weight.shape == (16, 5)
+
+
+def test_tensors_are_made_with_a_type_of_their_own():
+    """Memory that kernels write as float32 is not made with torch's default type, which a program may have set to bfloat16."""
+    import ast
+    import inspect
+    makers = {"empty", "zeros", "ones", "full", "tensor", "arange"}
+    for call in ast.walk(ast.parse(inspect.getsource(B))):
+        if isinstance(call, ast.Call) and isinstance(call.func, ast.Attribute) and call.func.attr in makers and ast.unparse(call.func.value) == "torch":
+            assert any(k.arg == "dtype" for k in call.keywords), ast.unparse(call)

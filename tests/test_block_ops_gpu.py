@@ -1316,3 +1316,30 @@ def test_scoring_of_a_model_with_gated_layers(dev, N):
         within(ll, ref, size.amax(0) * 2.0 ** -10, "scores")
     finally:
         nv.set_gemm_precision("fp32")
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_results_under_another_default_type(dev, default):
+    """A program that builds its model under torch.set_default_dtype calls the operators under it too: the same results, nothing written past its memory."""
+    out = []
+    for kind in (F32, default):
+        t = {d: ffn_case(dev, M, 136, 264, 72, d, True, seed=41) for M, d in ((9, F32), (10, BF))}
+        t |= {(M, d): ffn_case(dev, M, 136, 264, 72, d, True, seed=43) for M in (60,) for d in (F32, BF)}
+        n = norm_case(dev, 24, 40, 8, F32, F32, "layer", "rms", True, True, seed=3)
+        ups = rnd(dev, 24, 40, seed=5)
+        torch.set_default_dtype(kind)
+        try:
+            got = []
+            for c in t.values():
+                P, W = B.fp8_gated_weights(c["wg"], c["wu"], c["wd"], c["bg"], c["bu"], c["bd"]), B.fp8_weight(c["wg"])
+                y, tape = B.gated_feed_forward_tape(*[c[k] for k in ("x", "wg", "wu", "wd", "bg", "bu", "bd")])
+                got += [call_ffn(c, "silu"), y, *tape.backward(y), B.fp8_linear(c["x"], W), B.fp8_linear(c["x"], W, out_dtype=F32), B.fp8_gated_feed_forward(c["x"], P),
+                        B.fp8_gated_feed_forward(c["x"], P, out_dtype=F32), W.dequantize(), B.fp8_quantize(c["x"]).dequantize()]
+            s, v, tape = B.norm_gate_residual_tape(n["residual"], n["branch"], gate=n["gate"], scale=n["scale"], post_norm="layer", post_weight=n["post_weight"],
+                                                   post_bias=n["post_bias"], pre_weight=n["pre_weight"], pre_bias=n["pre_bias"])
+            got += [s, v, *tape.backward(ups, ups)]
+        finally:
+            torch.set_default_dtype(F32)
+        out.append(got)
+    for a, b in zip(*out):
+        assert a.dtype == b.dtype and torch.equal(a, b)
