@@ -1343,3 +1343,134 @@ def test_results_under_another_default_type(dev, default):
         out.append(got)
     for a, b in zip(*out):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("planes", [1, 3])
+@pytest.mark.parametrize("M,N,K", [(9000, 2056, 8), (70000, 72, 24)])
+def test_block_product_of_short_reductions(dev, planes, M, N, K):
+    """One stage to a tile and several tiles to a workgroup: every copy is for a later tile."""
+    dt = F32 if planes == 3 else BF
+    a, b, bias = rnd(dev, M, K, seed=1, dtype=dt), rnd(dev, N, K, seed=2, dtype=dt), rnd(dev, N, seed=3)
+    A, W = B._operand(a, planes, N), B._operand(b, planes, 1 << 30)
+    ref = a.double() @ b.double().t() + bias.double()
+    size = a.double().abs() @ b.double().abs().t() + bias.double().abs()
+    within(B._product(A, W, bias, torch.empty(M, N, device=dev), planes, M, N, A.width), ref, (K + 4) * E * size, "fp32 result")
+
+
+@pytest.mark.parametrize("M,K,F,N", [(9000, 8, 2010, 8), (40000, 16, 300, 24)])
+def test_ffn_of_short_reductions(dev, M, K, F, N):
+    """The same for the gated products both ways: one or two stages to a tile."""
+    t = ffn_case(dev, M, K, F, N, F32, True, seed=23)
+    dy = rnd(dev, M, N, seed=24)
+    y, got = ffn_grads(t, "gelu", dy)
+    check_ffn_forward(y, t, "gelu")
+    ref = ffn_grads64(t, "gelu", dy)
+    for k, v in got.items():
+        n = {"x": 2 * F}.get(k, M)
+        frob(v, ref[k], 3 * E * ((4 + math.sqrt(K)) + (4 + math.sqrt(N)) + (4 + math.sqrt(n))), f"d{k}")
+    b16 = {k: v.to(BF) for k, v in t.items()}
+    check_ffn_forward(call_ffn(b16, "gelu"), b16, "gelu")
+
+
+def test_fp8_linear_of_short_reductions(dev):
+    M, K, N = 40000, 8, 600
+    x, w = rnd(dev, M, K, seed=1), rnd(dev, N, K, seed=2)
+    W = B.fp8_weight(w)
+    xq, wq = e4m3_64(x, 1, 128), e4m3_64(w, 128, 128)
+    ref = xq @ wq.t()
+    lim = (K + 8) * E * (xq.abs() @ wq.abs().t()) + 2 * E * ref.abs()
+    within(B.fp8_linear(x, W), ref, lim, "fp32 result")
+    pipe = math.sqrt(K) * 2.0 ** -13 * xq.abs().amax(1, keepdim=True) * wq.abs().amax(1)
+    within(B.fp8_linear(x, W, out_dtype=BF), ref, lim + pipe + U * ref.abs() * 1.01, "bf16 result")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_one_dimension_and_the_same_tensor_twice(dev, dtype):
+    """A single row without leading dimensions; one tensor in two places, whose gradient is the sum of both places'."""
+    K, F = 40, 56
+    t = ffn_case(dev, 1, K, F, K, dtype, True, seed=3)
+    x = t["x"][0]
+    for grad in (False, True):
+        y = call_ffn({**t, "x": x.clone().requires_grad_(grad)}, "silu")
+        assert y.shape == (K,)
+        check_ffn_forward(y[None], t, "silu")
+    s, n = B.norm_gate_residual(x, y.detach(), gate=t["bd"], post_norm="rms")
+    s2, n2 = B.norm_gate_residual(t["x"], y.detach()[None], gate=t["bd"][None], post_norm="rms")
+    assert s.shape == n.shape == (K,) and torch.equal(s, s2[0]) and torch.equal(n, n2[0])
+    W = B.fp8_weight(t["wg"])
+    assert B.fp8_linear(x, W).shape == (F,) and torch.equal(B.fp8_linear(x, W), B.fp8_linear(t["x"], W)[0])
+    for M in (7, 60):
+        a, w, wd = (rnd(dev, *sh, seed=i, scale=0.2, dtype=dtype) for i, sh in enumerate(((M, K), (F, K), (K, F))))
+        dy = rnd(dev, M, K, seed=5, dtype=dtype)
+        wl = w.clone().requires_grad_()
+        tied, = torch.autograd.grad(B.gated_feed_forward(a, wl, wl, wd), wl, dy)
+        w1, w2 = w.clone().requires_grad_(), w.clone().requires_grad_()
+        g1, g2 = torch.autograd.grad(B.gated_feed_forward(a, w1, w2, wd), (w1, w2), dy)
+        assert torch.equal(tied, g1 + g2)
+        al = a.clone().requires_grad_()
+        both, = torch.autograd.grad(B.norm_gate_residual(al, al, post_norm="rms")[1], al, dy)
+        a1, a2 = a.clone().requires_grad_(), a.clone().requires_grad_()
+        g1, g2 = torch.autograd.grad(B.norm_gate_residual(a1, a2, post_norm="rms")[1], (a1, a2), dy)
+        assert torch.equal(both, g1 + g2)
+
+
+def test_two_threads_and_streams_at_once(dev):
+    """Forward and backward passes, norms and 8-bit units from two threads on streams of their own, at the same time: every result is the one of the
+    same call alone."""
+    import threading
+    cases = [(ffn_case(dev, M, 136, 264, 72, d, True, seed=s), rnd(dev, M, 72, seed=s, dtype=d)) for M, d, s in ((300, F32, 1), (300, BF, 2), (9, BF, 3), (2000, F32, 4))]
+    packs = [B.fp8_gated_weights(*[t[k] for k in ("wg", "wu", "wd", "bg", "bu", "bd")]) for t, _ in cases]
+
+    def work(t, dy, P):
+        y, g = ffn_grads(t, "silu", dy)
+        s, n = B.norm_gate_residual(dy, y.detach(), gate=dy[:1], post_norm="rms")
+        return [y.detach(), *g.values(), s, n, B.fp8_gated_feed_forward(t["x"], P)]
+
+    alone = [work(*c, P) for c, P in zip(cases, packs)]
+    torch.cuda.synchronize()
+    errors = []
+
+    def run(first):
+        try:
+            torch.cuda.set_device(dev)
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for rep in range(6):
+                    i = (first + rep) % len(cases)
+                    got = work(*cases[i], packs[i])
+                    st.synchronize()
+                    for a, b in zip(got, alone[i]):
+                        assert torch.equal(a, b), (first, rep)
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in (0, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_forms_for_few_rows_are_captured(dev):
+    """The forms for up to 32 rows in a graph: replays after new inputs equal the eager results."""
+    for dtype in (F32, BF):
+        t = ffn_case(dev, 7, 136, 264, 72, dtype, True, seed=5)
+        P = B.fp8_gated_weights(t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])
+        x = t["x"].clone()
+
+        def step(x):
+            y = B.gated_feed_forward(x, t["wg"], t["wu"], t["wd"], t["bg"], t["bu"], t["bd"])
+            return [y, *B.norm_gate_residual(y, y, post_norm="layer"), B.fp8_gated_feed_forward(x, P), B.fp8_linear(x, P.gate)]
+
+        step(x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step(x)
+        for rep in range(4):
+            x.copy_(rnd(dev, 7, 136, seed=60 + rep, dtype=dtype))
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs, step(x.clone())):
+                assert torch.equal(a, b), rep
