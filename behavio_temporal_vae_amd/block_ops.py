@@ -296,8 +296,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     ``x`` [..., K], ``w_gate`` and ``w_up`` [F, K], ``w_down`` [N, F], all float32 or all bfloat16; result [..., N] of that type.
     ``activation``: "silu", "gelu" (erf form), "relu" or "sigmoid".  Differentiable in every tensor; for up to 32 rows without
     a graph the weights are streamed once (the form for single profiles).  bfloat16: h, and in the backward pass the gradients of
-    both projections, are rounded to bfloat16 as operands of the next product, but not for up to 32 rows.  In float32 a row with an infinite input may
-    come out as NaN where float32 arithmetic would give an infinity."""
+    both projections, are rounded to bfloat16 as operands of the next product, but not for up to 32 rows.  In float32 a row with an infinite input, or
+    whose hidden values pass float32's range, may come out as NaN where float32 arithmetic would give an infinity."""
     x2, weights, biases, act = _ffn_inputs(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
     if grad:

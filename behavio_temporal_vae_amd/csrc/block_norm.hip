@@ -526,8 +526,14 @@ inline int waves_for(int N) { return N <= 512 ? 1 : N <= 1024 ? 2 : N <= 2048 ? 
 struct BwdPlan { int groups, splits; };
 static BwdPlan bwd_plan(int M, int N, int G) {
     const int W = waves_for(N), rpb = W == 1 ? 4 : 1;
-    // row groups in flight: a few waves to a SIMD, fewer and each column sum is shorter (65,536 x 1000 bf16: 1024 groups 217 us with the sums,
-    // 1366 202, 2048 241)
+    // row groups in flight: a few waves to a SIMD, fewer and each column sum is shorter.  Measured, us with the sums, at 512 / 768 / 1024 / 1366 / 2048 / 2732 groups:
+    //   one wave a row: 500 columns bf16, 65,536 rows 513 / 393 / 271 / 274 / 158 / 163; 200 columns, 200,000 rows 838 / 628 / 425 / 325 / 222 / 230
+    //   two: 1000 columns bf16, 65,536 rows of 4096 gate rows 320 / 252 / 190 / 176 / 216 / 184, 50,001 of 16,667 258 / 187 / 158 / 144 / 173 / 155,
+    //     60,000 of 3000 299 / 213 / 174 / 189 / 156 / 173; fp32, no gate, 65,536 rows 535 / 400 / 326 / 451 / 435 / 379
+    //   four: 1500 columns bf16, 65,536 rows 608 / 721 / 617 / 685 / 632 / 681; 2048 fp32, 32,768 rows 336 / 432 / 346 / 384 / 360 / 397
+    //   eight (256 / 384 / 512 / 768): 4000 columns bf16, 16,384 rows 209 / 253 / 215 / 219; 8000 fp32, 10,000 rows 857 / 1038 / 863 / 890
+    // What decides is how many of a kernel's workgroups a compute unit holds, which its types change: one number a width cannot suit all, and
+    // those for four and eight waves lose a sixth to 512 and 256
     const int units = W == 1 ? 2048 : W == 2 ? 1366 : W == 4 ? 768 : 384;
     const int share = M / std::max(G, 1);
     BwdPlan b;
