@@ -117,7 +117,8 @@ class _Operand:
 
 
 def _operand(t, planes, reads=0) -> _Operand:
-    """``t`` laid out as an operand, or where it is: a bf16 matrix with whole 16-byte pieces that is read against few others."""
+    """``t`` laid out as an operand of the products that are called one by one (a whole unit lays out its own), or where it is: a bf16 matrix
+    with whole 16-byte pieces that is read against few others."""
     rows, cols = t.shape
     if planes == 1 and t.dtype == torch.bfloat16 and cols % 8 == 0 and _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0 and reads < 2048 and 2 * _pitch(t) < 2 ** 23:
         return _Operand(t.data_ptr(), 2 * _pitch(t), cols, t)

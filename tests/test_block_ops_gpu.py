@@ -1474,3 +1474,16 @@ def test_forms_for_few_rows_are_captured(dev):
             torch.cuda.synchronize()
             for a, b in zip(outs, step(x.clone())):
                 assert torch.equal(a, b), rep
+
+
+def test_weight_gradients_of_a_unit_whose_results_pass_l2(dev):
+    """The weight and bias gradients of a bfloat16 unit with more than 128 MiB of h and of projection gradients against 64 bits: three operand roundings of
+    2^-8 at most, independent from element to element (the bound of a unit of many tiles)."""
+    M, K, F, N = 68001, 64, 1010, 64
+    t = ffn_case(dev, M, K, F, N, BF, True, seed=47)
+    dy = rnd(dev, M, N, seed=48, dtype=BF)
+    y, tape = B.gated_feed_forward_tape(*[t[k] for k in ("x", "wg", "wu", "wd", "bg", "bu", "bd")])
+    got = dict(zip(("x", "wg", "wu", "wd", "bg", "bu", "bd"), tape.backward(dy)))
+    ref = ffn_grads64(t, "silu", dy)
+    for k, v in got.items():
+        frob(v, ref[k], 3 * U, f"d{k}")
